@@ -48,6 +48,11 @@ class _Group(C.Structure):
                 ("accumulate", C.c_int), ("act", C.c_int), ("out_cols", C.POINTER(C.c_void_p))]
 
 
+class _Dropout(C.Structure):
+    _fields_ = [("p", C.c_float), ("seed", C.c_uint64), ("offset", C.c_uint64),
+                ("step", C.c_void_p)]
+
+
 def lib_path() -> str:
     return _LIB_PATH
 
@@ -109,6 +114,21 @@ def lib():
                                                vp, i64, i64, cf, vp, i64, i64, vp, i64, i64, vp, vp,
                                                vp, vp]
     L.ginn_b200_attention_forward.restype = L.ginn_b200_attention_backward.restype = ci
+    dp = C.POINTER(_Dropout)
+    L.ginn_b200_layer_norm_forward.argtypes = [ci, vp, ci, i64, i64, vp, i64, vp, vp, cf, vp, i64, vp,
+                                               vp]
+    L.ginn_b200_layer_norm_backward.argtypes = [ci, vp, ci, i64, i64, vp, i64, vp, vp, vp, vp, i64, vp,
+                                                i64, vp, vp, ci]
+    L.ginn_b200_dropout_forward.argtypes = [ci, vp, ci, i64, i64, vp, i64, vp, i64, dp, vp, i64]
+    L.ginn_b200_dropout_backward.argtypes = [ci, vp, ci, i64, i64, vp, i64, dp, vp, i64, ci]
+    L.ginn_b200_residual_norm_forward.argtypes = [ci, vp, ci, i64, i64, vp, i64, vp, i64, dp, vp, vp,
+                                                  cf, vp, i64, vp, i64, vp, vp]
+    L.ginn_b200_residual_norm_backward.argtypes = [ci, vp, ci, i64, i64, vp, i64, vp, vp, vp, vp, i64,
+                                                   vp, i64, dp, vp, i64, vp, i64, vp, vp, ci]
+    for name in ("ginn_b200_layer_norm_forward", "ginn_b200_layer_norm_backward",
+                 "ginn_b200_dropout_forward", "ginn_b200_dropout_backward",
+                 "ginn_b200_residual_norm_forward", "ginn_b200_residual_norm_backward"):
+        getattr(L, name).restype = ci
     L.ginn_b200_conv2d_workspace.argtypes = [ci] + [i64] * 9
     L.ginn_b200_conv2d_workspace.restype = C.c_size_t
     L.ginn_b200_conv2d_forward.argtypes = [ci, vp, ci] + [i64] * 9 + [vp, vp, vp, vp]
@@ -409,6 +429,110 @@ def softmax_backward(y: torch.Tensor, dy: torch.Tensor, dx: torch.Tensor, accumu
     _check(lib().ginn_b200_softmax_backward(_dev(y), _stream(y), _dtype_of(y), rows, cols,
                                             y.data_ptr(), _ld(y), dy.data_ptr(), _ld(dy),
                                             dx.data_ptr(), _ld(dx), int(accumulate)))
+
+
+def _matrix(t: torch.Tensor, name: str, like: torch.Tensor) -> tuple:
+    """(pointer, leading dimension) of a column-major matrix with the shape, type and device of
+    `like`."""
+    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+        raise GinnB200Error(1, f"{name}: shape, type or device differs from the other operands'")
+    if t.dim() != 2 or (t.shape[0] > 1 and t.stride(0) != 1) or (t.shape[1] > 1 and t.stride(1) < max(t.shape[0], 1)):
+        raise GinnB200Error(1, f"{name}: matrix must be column-major")
+    return t.data_ptr(), _ld(t)
+
+
+def _opt_matrix(t: Optional[torch.Tensor], name: str, like: torch.Tensor) -> tuple:
+    return (None, 0) if t is None else _matrix(t, name, like)
+
+
+def _vector(t: Optional[torch.Tensor], name: str, n: int, dtype, device) -> Optional[int]:
+    if t is None:
+        return None
+    if t.numel() != n or t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise GinnB200Error(1, f"{name}: expected {n} contiguous elements of {dtype} on {device}")
+    return t.data_ptr()
+
+
+def _dropout(p: float, seed: int, offset: int, step: Optional[torch.Tensor], device):
+    if not 0 <= seed < 1 << 64 or not 0 <= offset < 1 << 64:
+        raise GinnB200Error(1, "seed and offset are unsigned 64-bit numbers")
+    return C.byref(_Dropout(p, seed, offset, _vector(step, "step", 1, torch.int64, device)))
+
+
+def layer_norm_forward(x, gain, bias, y, mean=None, rstd=None, eps: float = 1e-5) -> None:
+    """y = gain * (x - mean) * rstd + bias, column by column (ginn_b200_layer_norm_forward).
+    gain, bias: (rows,) of x's type or None; mean, rstd: (cols,) fp32 for the backward pass."""
+    xp, yp = _matrix(x, "x", x), _matrix(y, "y", x)
+    rows, cols = x.shape
+    _check(lib().ginn_b200_layer_norm_forward(
+        _dev(x), _stream(x), _dtype_of(x), rows, cols, *xp, _vector(gain, "gain", rows, x.dtype, x.device),
+        _vector(bias, "bias", rows, x.dtype, x.device), eps, *yp,
+        _vector(mean, "mean", cols, torch.float32, x.device),
+        _vector(rstd, "rstd", cols, torch.float32, x.device)))
+
+
+def layer_norm_backward(x, gain, mean, rstd, dy, dx=None, dgain=None, dbias=None,
+                        accumulate: bool = True) -> None:
+    """Gradients of layer_norm_forward, added to dx / dgain / dbias or (accumulate=False) assigned
+    (ginn_b200_layer_norm_backward)."""
+    rows, cols = x.shape
+    _check(lib().ginn_b200_layer_norm_backward(
+        _dev(x), _stream(x), _dtype_of(x), rows, cols, *_matrix(x, "x", x),
+        _vector(gain, "gain", rows, x.dtype, x.device),
+        _vector(mean, "mean", cols, torch.float32, x.device),
+        _vector(rstd, "rstd", cols, torch.float32, x.device), *_matrix(dy, "dy", x),
+        *_opt_matrix(dx, "dx", x), _vector(dgain, "dgain", rows, x.dtype, x.device),
+        _vector(dbias, "dbias", rows, x.dtype, x.device), int(accumulate)))
+
+
+def dropout_forward(x, y, p: float, seed: int, offset: int = 0, residual=None, step=None) -> None:
+    """y = (residual +) drop(x) with the counter-based mask of (seed, offset)
+    (ginn_b200_dropout_forward); step: one int64 on the device that is added to the offset."""
+    rows, cols = x.shape
+    _check(lib().ginn_b200_dropout_forward(
+        _dev(x), _stream(x), _dtype_of(x), rows, cols, *_matrix(x, "x", x),
+        *_opt_matrix(residual, "residual", x), _dropout(p, seed, offset, step, x.device),
+        *_matrix(y, "y", x)))
+
+
+def dropout_backward(dy, dx, p: float, seed: int, offset: int = 0, step=None,
+                     accumulate: bool = True) -> None:
+    """dx (+)= dy through the mask of the same (p, seed, offset) (ginn_b200_dropout_backward)."""
+    rows, cols = dy.shape
+    _check(lib().ginn_b200_dropout_backward(
+        _dev(dy), _stream(dy), _dtype_of(dy), rows, cols, *_matrix(dy, "dy", dy),
+        _dropout(p, seed, offset, step, dy.device), *_matrix(dx, "dx", dy), int(accumulate)))
+
+
+def residual_norm_forward(x, residual, gain, bias, h, y, mean=None, rstd=None, p: float = 0.0,
+                          seed: int = 0, offset: int = 0, step=None, eps: float = 1e-5) -> None:
+    """h = residual + drop(x), y = normalisation of h, in one pass
+    (ginn_b200_residual_norm_forward)."""
+    rows, cols = x.shape
+    _check(lib().ginn_b200_residual_norm_forward(
+        _dev(x), _stream(x), _dtype_of(x), rows, cols, *_matrix(x, "x", x),
+        *_opt_matrix(residual, "residual", x), _dropout(p, seed, offset, step, x.device),
+        _vector(gain, "gain", rows, x.dtype, x.device), _vector(bias, "bias", rows, x.dtype, x.device),
+        eps, *_matrix(h, "h", x), *_matrix(y, "y", x),
+        _vector(mean, "mean", cols, torch.float32, x.device),
+        _vector(rstd, "rstd", cols, torch.float32, x.device)))
+
+
+def residual_norm_backward(h, gain, mean, rstd, dy, dh=None, dx=None, dres=None, dgain=None,
+                           dbias=None, p: float = 0.0, seed: int = 0, offset: int = 0, step=None,
+                           accumulate: bool = True) -> None:
+    """Gradients of residual_norm_forward; dh is what reaches h along the residual connection
+    (ginn_b200_residual_norm_backward)."""
+    rows, cols = h.shape
+    _check(lib().ginn_b200_residual_norm_backward(
+        _dev(h), _stream(h), _dtype_of(h), rows, cols, *_matrix(h, "h", h),
+        _vector(gain, "gain", rows, h.dtype, h.device),
+        _vector(mean, "mean", cols, torch.float32, h.device),
+        _vector(rstd, "rstd", cols, torch.float32, h.device), *_matrix(dy, "dy", h),
+        *_opt_matrix(dh, "dh", h), _dropout(p, seed, offset, step, h.device),
+        *_opt_matrix(dx, "dx", h), *_opt_matrix(dres, "dres", h),
+        _vector(dgain, "dgain", rows, h.dtype, h.device),
+        _vector(dbias, "dbias", rows, h.dtype, h.device), int(accumulate)))
 
 
 def lstm_cell_forward(gates, c_prev, c, h, xh_next=None, n_next=0) -> None:

@@ -1591,6 +1591,184 @@ int ginn_b200_conv2d_backward(int device, void* stream_, int dtype, int64_t C, i
   return status;
 }
 
+namespace {
+// A rows x cols matrix argument: present, and its columns do not overlap.
+int check_matrix(const char* name, const void* p, int64_t ld, int64_t rows) {
+  if (!p) return fail(GINN_B200_BAD_ARGUMENT, "%s is a null pointer", name);
+  if (ld < rows)
+    return fail(GINN_B200_BAD_ARGUMENT, "leading dimension %lld of %s is smaller than its %lld rows",
+                (long long)ld, name, (long long)rows);
+  return GINN_B200_OK;
+}
+
+int check_dropout(const ginn_b200_dropout* d, gb::Dropout* out) {
+  *out = gb::Dropout();
+  if (!d) return fail(GINN_B200_BAD_ARGUMENT, "null dropout description");
+  if (!(d->p >= 0.f) || !(d->p < 1.f))
+    return fail(GINN_B200_BAD_ARGUMENT, "dropout probability %g is not in [0, 1)", (double)d->p);
+  const double t = static_cast<double>(d->p) * 65536.0 + 0.5;
+  const uint32_t threshold = static_cast<uint32_t>(t);
+  if (threshold >= 65536u)
+    return fail(GINN_B200_BAD_ARGUMENT, "dropout probability %g rounds to 1 in steps of 2^-16", (double)d->p);
+  out->seed_lo = static_cast<uint32_t>(d->seed);
+  out->seed_hi = static_cast<uint32_t>(d->seed >> 32);
+  out->offset = d->offset;
+  out->step = reinterpret_cast<const unsigned long long*>(d->step);
+  out->threshold = threshold;
+  out->factor = static_cast<float>(65536.0 / (65536 - threshold));
+  return GINN_B200_OK;
+}
+
+int norm_forward(int device, void* stream, int dtype, const gb::NormArgs& a) {
+  if (!(a.eps > 0.f)) return fail(GINN_B200_BAD_ARGUMENT, "eps must be positive (got %g)", (double)a.eps);
+  DevCtx* ctx;
+  if (int s = get_ctx(device, &ctx)) return s;
+  CU_TRY(gb::launch_norm_forward(dtype, a, static_cast<cudaStream_t>(stream)));
+  g_launches.fetch_add(1);
+  return GINN_B200_OK;
+}
+
+int norm_backward(int device, void* stream_, int dtype, const gb::NormGradArgs& a) {
+  const bool weights = a.dgain != nullptr || a.dbias != nullptr;
+  if (!a.dres && !a.dx && !weights) return GINN_B200_OK;
+  if (a.rows == 0 || (a.cols == 0 && (!weights || a.accumulate))) return GINN_B200_OK;
+  DevCtx* ctx;
+  if (int s = get_ctx(device, &ctx)) return s;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  const int parts = gb::norm_backward_parts(a.rows, a.cols, ctx->num_sms);
+  void* partial = nullptr;
+  if (weights && parts > 0)
+    CU_TRY(cudaMallocAsync(&partial, static_cast<size_t>(parts) * 2 * a.rows * sizeof(float), stream));
+  const cudaError_t e = gb::launch_norm_backward(dtype, a, parts, static_cast<float*>(partial), stream);
+  if (partial) cudaFreeAsync(partial, stream);
+  if (e != cudaSuccess)
+    return fail(GINN_B200_CUDA_ERROR, "layer norm backward launch failed: %s", cudaGetErrorString(e));
+  g_launches.fetch_add((a.cols > 0 && (a.rows <= gb::kNormRegisterRows || a.dres || a.dx)) +
+                       (weights && a.cols > 0 && a.rows > gb::kNormRegisterRows) + weights);
+  return GINN_B200_OK;
+}
+}  // namespace
+
+int ginn_b200_layer_norm_forward(int device, void* stream, int dtype, int64_t rows, int64_t cols,
+                                 const void* x, int64_t ldx, const void* gain, const void* bias,
+                                 float eps, void* y, int64_t ldy, float* mean, float* rstd) {
+  if (int s = check_common(dtype, rows, cols, 0)) return s;
+  if (rows == 0 || cols == 0) return GINN_B200_OK;
+  if (int s = check_matrix("x", x, ldx, rows)) return s;
+  if (int s = check_matrix("y", y, ldy, rows)) return s;
+  gb::NormArgs a = {};
+  a.x = x; a.gain = gain; a.bias = bias; a.y = y; a.mean = mean; a.rstd = rstd;
+  a.ldx = ldx; a.ldy = ldy; a.rows = rows; a.cols = cols;
+  a.eps = eps;
+  return norm_forward(device, stream, dtype, a);
+}
+
+int ginn_b200_layer_norm_backward(int device, void* stream, int dtype, int64_t rows, int64_t cols,
+                                  const void* x, int64_t ldx, const void* gain, const float* mean,
+                                  const float* rstd, const void* dy, int64_t lddy, void* dx,
+                                  int64_t lddx, void* dgain, void* dbias, int accumulate) {
+  if (int s = check_common(dtype, rows, cols, 0)) return s;
+  if (rows > 0 && cols > 0) {
+    if (int s = check_matrix("x", x, ldx, rows)) return s;
+    if (int s = check_matrix("dy", dy, lddy, rows)) return s;
+    if (dx)
+      if (int s = check_matrix("dx", dx, lddx, rows)) return s;
+    if (!mean || !rstd) return fail(GINN_B200_BAD_ARGUMENT, "mean and rstd of the forward pass are needed");
+  }
+  gb::NormGradArgs a = {};
+  a.h = x; a.gain = gain; a.mean = mean; a.rstd = rstd; a.dy = dy; a.dres = dx; a.dgain = dgain; a.dbias = dbias;
+  a.ldh = ldx; a.lddy = lddy; a.lddres = lddx; a.rows = rows; a.cols = cols;
+  a.accumulate = accumulate ? 1 : 0;
+  return norm_backward(device, stream, dtype, a);
+}
+
+int ginn_b200_dropout_forward(int device, void* stream, int dtype, int64_t rows, int64_t cols,
+                              const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                              const ginn_b200_dropout* drop, void* y, int64_t ldy) {
+  if (int s = check_common(dtype, rows, cols, 0)) return s;
+  gb::Dropout d;
+  if (int s = check_dropout(drop, &d)) return s;
+  if (rows == 0 || cols == 0) return GINN_B200_OK;
+  if (int s = check_matrix("x", x, ldx, rows)) return s;
+  if (int s = check_matrix("y", y, ldy, rows)) return s;
+  if (residual)
+    if (int s = check_matrix("residual", residual, ldr, rows)) return s;
+  DevCtx* ctx;
+  if (int s = get_ctx(device, &ctx)) return s;
+  CU_TRY(gb::launch_dropout(dtype, x, ldx, residual, ldr, y, ldy, rows, cols, d, ctx->num_sms,
+                            static_cast<cudaStream_t>(stream)));
+  g_launches.fetch_add(1);
+  return GINN_B200_OK;
+}
+
+int ginn_b200_dropout_backward(int device, void* stream, int dtype, int64_t rows, int64_t cols,
+                               const void* dy, int64_t lddy, const ginn_b200_dropout* drop, void* dx,
+                               int64_t lddx, int accumulate) {
+  if (int s = check_common(dtype, rows, cols, 0)) return s;
+  gb::Dropout d;
+  if (int s = check_dropout(drop, &d)) return s;
+  if (rows == 0 || cols == 0) return GINN_B200_OK;
+  if (int s = check_matrix("dy", dy, lddy, rows)) return s;
+  if (int s = check_matrix("dx", dx, lddx, rows)) return s;
+  DevCtx* ctx;
+  if (int s = get_ctx(device, &ctx)) return s;
+  CU_TRY(gb::launch_dropout(dtype, dy, lddy, accumulate ? dx : nullptr, lddx, dx, lddx, rows, cols, d,
+                            ctx->num_sms, static_cast<cudaStream_t>(stream)));
+  g_launches.fetch_add(1);
+  return GINN_B200_OK;
+}
+
+int ginn_b200_residual_norm_forward(int device, void* stream, int dtype, int64_t rows, int64_t cols,
+                                    const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                                    const ginn_b200_dropout* drop, const void* gain,
+                                    const void* bias, float eps, void* h, int64_t ldh, void* y,
+                                    int64_t ldy, float* mean, float* rstd) {
+  if (int s = check_common(dtype, rows, cols, 0)) return s;
+  gb::NormArgs a = {};
+  if (int s = check_dropout(drop, &a.drop)) return s;
+  if (rows == 0 || cols == 0) return GINN_B200_OK;
+  if (int s = check_matrix("x", x, ldx, rows)) return s;
+  if (int s = check_matrix("h", h, ldh, rows)) return s;
+  if (int s = check_matrix("y", y, ldy, rows)) return s;
+  if (residual)
+    if (int s = check_matrix("residual", residual, ldr, rows)) return s;
+  if (y == h || y == x || y == residual)
+    return fail(GINN_B200_BAD_ARGUMENT, "y must be storage of its own");
+  a.x = x; a.res = residual; a.gain = gain; a.bias = bias; a.h = h; a.y = y; a.mean = mean; a.rstd = rstd;
+  a.ldx = ldx; a.ldres = ldr; a.ldh = ldh; a.ldy = ldy; a.rows = rows; a.cols = cols;
+  a.eps = eps;
+  return norm_forward(device, stream, dtype, a);
+}
+
+int ginn_b200_residual_norm_backward(int device, void* stream, int dtype, int64_t rows,
+                                     int64_t cols, const void* h, int64_t ldh, const void* gain,
+                                     const float* mean, const float* rstd, const void* dy,
+                                     int64_t lddy, const void* dh, int64_t lddh,
+                                     const ginn_b200_dropout* drop, void* dx, int64_t lddx,
+                                     void* dres, int64_t lddres, void* dgain, void* dbias,
+                                     int accumulate) {
+  if (int s = check_common(dtype, rows, cols, 0)) return s;
+  gb::NormGradArgs a = {};
+  if (int s = check_dropout(drop, &a.drop)) return s;
+  if (rows > 0 && cols > 0) {
+    if (int s = check_matrix("h", h, ldh, rows)) return s;
+    if (int s = check_matrix("dy", dy, lddy, rows)) return s;
+    if (dh)
+      if (int s = check_matrix("dh", dh, lddh, rows)) return s;
+    if (dx)
+      if (int s = check_matrix("dx", dx, lddx, rows)) return s;
+    if (dres)
+      if (int s = check_matrix("dres", dres, lddres, rows)) return s;
+    if (dx && dx == dres) return fail(GINN_B200_BAD_ARGUMENT, "dx and dres are the same tensor");
+    if (!mean || !rstd) return fail(GINN_B200_BAD_ARGUMENT, "mean and rstd of the forward pass are needed");
+  }
+  a.h = h; a.gain = gain; a.mean = mean; a.rstd = rstd; a.dy = dy; a.dh = dh; a.dx = dx; a.dres = dres;
+  a.dgain = dgain; a.dbias = dbias;
+  a.ldh = ldh; a.lddy = lddy; a.lddh = lddh; a.lddx = lddx; a.lddres = lddres; a.rows = rows; a.cols = cols;
+  a.accumulate = accumulate ? 1 : 0;
+  return norm_backward(device, stream, dtype, a);
+}
+
 int ginn_b200_fill(int device, void* stream, int dtype, int64_t n, void* x, float value) {
   if (dtype != GINN_B200_F32 && dtype != GINN_B200_F16)
     return fail(GINN_B200_UNSUPPORTED, "dtype %d is not fp32 (0) or fp16 (1)", dtype);

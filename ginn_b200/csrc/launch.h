@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include "problem.h"
+#include "dropout.cuh"
 
 struct CUtensorMap_st;  // CUDA driver tensor-map descriptor (cuda.h)
 
@@ -147,6 +148,48 @@ cudaError_t launch_attention_fwd(const AttentionArgs& a, cudaStream_t stream, in
 // row > column (keys after the query) become -inf.
 cudaError_t launch_scale_mask_f32(float* s, long long ld, long long stride, int T, int batches,
                                   float scale, int causal, cudaStream_t stream);
+
+// --- layer normalisation, dropout, and both behind a residual connection (norm_ops.cu) ---
+struct NormArgs {
+  const void* x;
+  const void* res;   // residual added to drop(x); may be null
+  const void* gain;  // may be null (1)
+  const void* bias;  // may be null (0)
+  void* h;           // residual + drop(x) as stored; null: x itself is normalised, `drop` and `res` unused
+  void* y;
+  float* mean;       // may be null
+  float* rstd;       // may be null
+  long long ldx, ldres, ldh, ldy, rows, cols;
+  float eps;
+  Dropout drop;
+};
+struct NormGradArgs {
+  const void* h;
+  const void* gain;
+  const float* mean;
+  const float* rstd;
+  const void* dy;
+  const void* dh;  // gradient that reaches h from elsewhere; may be null
+  void* dres;      // gradient of h (and of the residual); may be null
+  void* dx;        // that gradient through the dropout; may be null
+  void* dgain;     // may be null
+  void* dbias;     // may be null
+  long long ldh, lddy, lddh, lddres, lddx, rows, cols;
+  int accumulate;
+  Dropout drop;
+};
+// Longest column whose backward pass keeps it in registers.
+constexpr long long kNormRegisterRows = 8192;
+// Partial vectors (2 x rows floats each) the weight gradients of a backward pass need.
+int norm_backward_parts(long long rows, long long cols, int num_sms);
+cudaError_t launch_norm_forward(int dtype, const NormArgs& a, cudaStream_t stream);
+// `partial`: norm_backward_parts(...) x 2 x rows floats, null when neither dgain nor dbias is set.
+cudaError_t launch_norm_backward(int dtype, const NormGradArgs& a, int parts, float* partial,
+                                 cudaStream_t stream);
+// y = drop(x) (+ add); `add` may be y itself.
+cudaError_t launch_dropout(int dtype, const void* x, long long ldx, const void* add, long long lda,
+                           void* y, long long ldy, long long rows, long long cols,
+                           const Dropout& drop, int num_sms, cudaStream_t stream);
 
 // --- Conv2d as patch extraction + matrix products (conv.cu) ---
 struct ConvShape {

@@ -1,0 +1,709 @@
+// Layer normalisation, dropout and the two fused behind a residual connection, on column-major
+// matrices (a column = one token's features).  All of it is bound by HBM bandwidth: each kernel
+// reads its operands once and keeps a column in registers between the reduction and the result.
+//
+//   norm forward  : h = residual + drop(x)  (plain normalisation: h = x)
+//                   mu = mean(h), r = 1 / sqrt(mean((h - mu)^2) + eps), y = gain (h - mu) r + bias
+//   norm backward : xh = (h - mu) r, G = gain dy
+//                   dh' = r (G - mean(G) - xh mean(G xh)) + dh,   dres (+)= dh',  dx (+)= drop'(dh')
+//                   dgain (+)= sum over columns of dy xh,  dbias (+)= sum over columns of dy
+//   dropout       : y = residual + drop(x),  dx (+)= drop'(dy)
+//
+// Statistics, sums and weight gradients are fp32 whatever the storage type; each result is rounded
+// once.  Weight gradients: every CTA adds its columns in registers and leaves one vector of
+// partial sums; a second small kernel adds those in a fixed order, so a call's result does not
+// depend on which CTA finishes first.
+#include <cuda_fp16.h>
+#include "math.cuh"
+#include "ptx.cuh"
+#include "launch.h"
+
+namespace gb {
+
+namespace {
+
+constexpr int kEl = 8;  // elements a thread handles together: one generator block
+
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __half* p, float (&x)[8]) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(__half* p, const float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<__half2*>(&w[i]) = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Rows of a column that a thread of a group of G threads handles.  VEC: eight consecutive rows
+// (16-byte accesses).  Otherwise a warp covers 256 consecutive rows, its lanes side by side, so
+// that accesses of any alignment coalesce.  `piece` counts the group's sweeps of 8 G rows.
+template <bool VEC>
+__device__ __forceinline__ long long first_row(long long piece, int G, int t) {
+  if (VEC) return (piece * G + t) * kEl;
+  return (piece * G + (t & ~31)) * kEl + (t & 31);
+}
+template <bool VEC>
+__device__ __forceinline__ constexpr int row_step() { return VEC ? 1 : 32; }
+
+// The thread's eight elements of one column, zero behind the last row.
+template <bool VEC, typename T>
+__device__ __forceinline__ void load_piece(const T* col, long long r0, long long rows, float (&x)[8]) {
+  if (VEC) {
+    if (r0 < rows) {
+      load8(col + r0, x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const long long r = r0 + 32 * e;
+      x[e] = r < rows ? to_f(col[r]) : 0.f;
+    }
+  }
+}
+template <bool VEC, typename T>
+__device__ __forceinline__ void store_piece(T* col, long long r0, long long rows, const float (&x)[8]) {
+  if (VEC) {
+    if (r0 < rows) store8(col + r0, x);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const long long r = r0 + 32 * e;
+      if (r < rows) col[r] = from_f<T>(x[e]);
+    }
+  }
+}
+// Keep bits of those eight elements (the whole warp calls it).
+template <bool VEC>
+__device__ __forceinline__ uint32_t keep_piece(const Philox& gen, long long col, long long rows,
+                                               long long r0, int lane) {
+  const unsigned long long e0 = static_cast<unsigned long long>(col) * rows;
+  if (VEC) return gen.keep8((e0 + r0) >> 3);  // rows % 8 == 0: r0 starts a block
+  return gen.keep_strided(e0 + (r0 - lane), lane);
+}
+__device__ __forceinline__ void drop8(float (&x)[8], uint32_t keep, float factor) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = (keep >> e) & 1u ? x[e] * factor : 0.f;
+}
+
+// Sum over the G threads (a multiple of 32) that share a column; `slot` holds one value per warp
+// of the CTA and alternates between two buffers, so one barrier per reduction is enough.
+__device__ __forceinline__ float group_sum(float v, int G, int t, float* slot) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (G == 32) return v;
+  const int warp = threadIdx.x >> 5, first = warp - (t >> 5);
+  if ((t & 31) == 0) slot[warp] = v;
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / G), "r"(G) : "memory");
+  float s = 0.f;
+  for (int w = 0; w < G / 32; ++w) s += slot[first + w];
+  return s;
+}
+// Two sums at once.
+__device__ __forceinline__ float2 group_sum2(float2 v, int G, int t, float2* slot) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  }
+  if (G == 32) return v;
+  const int warp = threadIdx.x >> 5, first = warp - (t >> 5);
+  if ((t & 31) == 0) slot[warp] = v;
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / G), "r"(G) : "memory");
+  float2 s = make_float2(0.f, 0.f);
+  for (int w = 0; w < G / 32; ++w) {
+    s.x += slot[first + w].x;
+    s.y += slot[first + w].y;
+  }
+  return s;
+}
+
+template <typename T>
+struct NormFwd {
+  const T* x;
+  const T* res;   // may be null
+  const T* gain;  // may be null: 1
+  const T* bias;  // may be null: 0
+  T* h;           // null: plain normalisation of x
+  T* y;
+  float* mean;    // may be null
+  float* rstd;    // may be null
+  long long ldx, ldres, ldh, ldy, rows, cols;
+  float eps;
+  Dropout drop;
+};
+
+// h of the thread's eight elements: the residual sum as it is stored.
+template <bool VEC, typename T>
+__device__ __forceinline__ void form_h(const NormFwd<T>& p, const Philox& gen, long long col,
+                                       long long r0, int lane, float (&v)[8]) {
+  load_piece<VEC>(p.x + col * p.ldx, r0, p.rows, v);
+  if (p.h == nullptr) return;
+  if (p.drop.threshold != 0) drop8(v, keep_piece<VEC>(gen, col, p.rows, r0, lane), p.drop.factor);
+  if (p.res != nullptr) {
+    float q[8];
+    load_piece<VEC>(p.res + col * p.ldres, r0, p.rows, q);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += q[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = to_f(from_f<T>(v[e]));
+  store_piece<VEC>(p.h + col * p.ldh, r0, p.rows, v);
+}
+
+template <bool VEC, typename T>
+__device__ __forceinline__ void write_y(const NormFwd<T>& p, long long col, long long r0, float mean,
+                                        float rstd, float (&v)[8]) {
+  float g[8], b[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    g[e] = 1.f;
+    b[e] = 0.f;
+  }
+  if (p.gain != nullptr) load_piece<VEC>(p.gain, r0, p.rows, g);
+  if (p.bias != nullptr) load_piece<VEC>(p.bias, r0, p.rows, b);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (v[e] - mean) * rstd * g[e] + b[e];
+  store_piece<VEC>(p.y + col * p.ldy, r0, p.rows, v);
+}
+
+// One group of G threads per column, the column in registers (8 NV elements per thread): the
+// variance is formed from the differences to the mean, not from a difference of squares.
+template <typename T, bool VEC, int NV>
+__global__ void __launch_bounds__(512)
+norm_forward_kernel(const NormFwd<T> p, int G) {
+  __shared__ float slot[2][16];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int t = threadIdx.x % G, lane = threadIdx.x & 31;
+  const long long col = static_cast<long long>(blockIdx.x) * (blockDim.x / G) + threadIdx.x / G;
+  if (col >= p.cols) return;  // uniform over the group
+  const Philox gen(p.drop);
+  float v[NV][8];
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    form_h<VEC>(p, gen, col, first_row<VEC>(i, G, t), lane, v[i]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += v[i][e];
+  }
+  const float mean = group_sum(s, G, t, slot[0]) / static_cast<float>(p.rows);
+  float q = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const long long r0 = first_row<VEC>(i, G, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float d = v[i][e] - mean;
+      if (VEC ? r0 < p.rows : r0 + 32 * e < p.rows) q += d * d;
+    }
+  }
+  const float rstd = 1.f / sqrtf(group_sum(q, G, t, slot[1]) / static_cast<float>(p.rows) + p.eps);
+  if (t == 0) {
+    if (p.mean != nullptr) p.mean[col] = mean;
+    if (p.rstd != nullptr) p.rstd[col] = rstd;
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) write_y<VEC>(p, col, first_row<VEC>(i, G, t), mean, rstd, v[i]);
+}
+
+// Columns too long for the registers of one CTA: three sweeps over the column, the later ones
+// from cache.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(512)
+norm_forward_long_kernel(const NormFwd<T> p) {
+  __shared__ float slot[2][16];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int G = blockDim.x, t = threadIdx.x, lane = t & 31;
+  const long long col = blockIdx.x, pieces = (p.rows + 8LL * G - 1) / (8LL * G);
+  const Philox gen(p.drop);
+  // the second and third sweep read what the first one wrote, each thread its own elements
+  const T* src = p.h != nullptr ? p.h + col * p.ldh : p.x + col * p.ldx;
+  float s = 0.f;
+  for (long long i = 0; i < pieces; ++i) {
+    float v[8];
+    form_h<VEC>(p, gen, col, first_row<VEC>(i, G, t), lane, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += v[e];
+  }
+  const float mean = group_sum(s, G, t, slot[0]) / static_cast<float>(p.rows);
+  float q = 0.f;
+  for (long long i = 0; i < pieces; ++i) {
+    const long long r0 = first_row<VEC>(i, G, t);
+    float v[8];
+    load_piece<VEC>(src, r0, p.rows, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float d = v[e] - mean;
+      if (VEC ? r0 < p.rows : r0 + 32 * e < p.rows) q += d * d;
+    }
+  }
+  const float rstd = 1.f / sqrtf(group_sum(q, G, t, slot[1]) / static_cast<float>(p.rows) + p.eps);
+  if (t == 0) {
+    if (p.mean != nullptr) p.mean[col] = mean;
+    if (p.rstd != nullptr) p.rstd[col] = rstd;
+  }
+  for (long long i = 0; i < pieces; ++i) {
+    const long long r0 = first_row<VEC>(i, G, t);
+    float v[8];
+    load_piece<VEC>(src, r0, p.rows, v);
+    write_y<VEC>(p, col, r0, mean, rstd, v);
+  }
+}
+
+template <typename T>
+struct NormBwd {
+  const T* h;
+  const T* gain;  // may be null: 1
+  const float* mean;
+  const float* rstd;
+  const T* dy;
+  const T* dh;    // gradient that reaches h from elsewhere; may be null
+  T* dres;        // may be null
+  T* dx;          // may be null
+  float* partial; // gridDim.x x 2 x rows sums (dgain, dbias); null when neither is wanted
+  long long ldh, lddy, lddh, lddres, lddx, rows, cols;
+  int accumulate;
+  Dropout drop;
+};
+
+// Gradient of the normalisation's input from the column sums, and its two destinations.
+template <bool VEC, typename T>
+__device__ __forceinline__ void write_dh(const NormBwd<T>& p, const Philox& gen, long long col,
+                                         long long r0, int lane, float rstd, float2 m,
+                                         const float (&xh)[8], const float (&g)[8]) {
+  float d[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) d[e] = rstd * (g[e] - m.x - xh[e] * m.y);
+  if (p.dh != nullptr) {
+    float q[8];
+    load_piece<VEC>(p.dh + col * p.lddh, r0, p.rows, q);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d[e] += q[e];
+  }
+  float o[8];
+  if (p.dres != nullptr) {
+    T* c = p.dres + col * p.lddres;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = 0.f;
+    if (p.accumulate) load_piece<VEC>(c, r0, p.rows, o);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] += d[e];
+    store_piece<VEC>(c, r0, p.rows, o);
+  }
+  if (p.dx != nullptr) {
+    T* c = p.dx + col * p.lddx;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = 0.f;
+    if (p.accumulate) load_piece<VEC>(c, r0, p.rows, o);
+    if (p.drop.threshold != 0) drop8(d, keep_piece<VEC>(gen, col, p.rows, r0, lane), p.drop.factor);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] += d[e];
+    store_piece<VEC>(c, r0, p.rows, o);
+  }
+}
+
+// Groups of G threads walk the columns; a thread meets the same rows in every column, so the
+// weight gradients stay in its registers until the end, where the groups of the CTA add theirs
+// through shared memory (2 x rows floats).
+template <typename T, bool VEC, int NV>
+__global__ void __launch_bounds__(512, 1)
+norm_backward_kernel(const NormBwd<T> p, int G) {
+  __shared__ float2 slot[2][16];
+  extern __shared__ float sums[];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int groups = blockDim.x / G, group = threadIdx.x / G;
+  const int t = threadIdx.x % G, lane = threadIdx.x & 31;
+  const Philox gen(p.drop);
+  float dg[NV][8], db[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dg[i][e] = db[i][e] = 0.f;
+  const float inv = 1.f / static_cast<float>(p.rows);
+  int turn = 0;
+  for (long long col = static_cast<long long>(blockIdx.x) * groups + group; col < p.cols;
+       col += static_cast<long long>(gridDim.x) * groups, turn ^= 1) {
+    float xh[NV][8], g[NV][8];
+    const float mean = p.mean[col], rstd = p.rstd[col];
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const long long r0 = first_row<VEC>(i, G, t);
+      load_piece<VEC>(p.h + col * p.ldh, r0, p.rows, xh[i]);
+      load_piece<VEC>(p.dy + col * p.lddy, r0, p.rows, g[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const long long r0 = first_row<VEC>(i, G, t);
+      float w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = 1.f;
+      if (p.gain != nullptr) load_piece<VEC>(p.gain, r0, p.rows, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        xh[i][e] = (xh[i][e] - mean) * rstd;
+        dg[i][e] += g[i][e] * xh[i][e];  // dy is zero behind the last row
+        db[i][e] += g[i][e];
+        g[i][e] *= w[e];
+        s.x += g[i][e];
+        s.y += g[i][e] * xh[i][e];
+      }
+    }
+    s = group_sum2(s, G, t, slot[turn]);
+    s.x *= inv;
+    s.y *= inv;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      write_dh<VEC>(p, gen, col, first_row<VEC>(i, G, t), lane, rstd, s, xh[i], g[i]);
+  }
+  if (p.partial == nullptr) return;
+  // the groups take turns, in order
+  for (int k = 0; k < groups; ++k) {
+    __syncthreads();
+    if (group != k) continue;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const long long r0 = first_row<VEC>(i, G, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const long long r = r0 + row_step<VEC>() * e;
+        if (r < p.rows) {
+          sums[r] = (k ? sums[r] : 0.f) + dg[i][e];
+          sums[p.rows + r] = (k ? sums[p.rows + r] : 0.f) + db[i][e];
+        }
+      }
+    }
+  }
+  __syncthreads();
+  float* out = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.rows;
+  for (long long r = threadIdx.x; r < 2 * p.rows; r += blockDim.x) out[r] = sums[r];
+}
+
+// Long columns: the column sums and the input's gradient in two sweeps, one CTA per column.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(512)
+norm_backward_long_kernel(const NormBwd<T> p) {
+  __shared__ float2 slot[16];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int G = blockDim.x, t = threadIdx.x, lane = t & 31;
+  const long long col = blockIdx.x, pieces = (p.rows + 8LL * G - 1) / (8LL * G);
+  const Philox gen(p.drop);
+  const float mean = p.mean[col], rstd = p.rstd[col];
+  float2 s = make_float2(0.f, 0.f);
+  auto fetch = [&](long long r0, float (&xh)[8], float (&g)[8]) {
+    load_piece<VEC>(p.h + col * p.ldh, r0, p.rows, xh);
+    load_piece<VEC>(p.dy + col * p.lddy, r0, p.rows, g);
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = 1.f;
+    if (p.gain != nullptr) load_piece<VEC>(p.gain, r0, p.rows, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      xh[e] = (xh[e] - mean) * rstd;
+      g[e] *= w[e];
+    }
+  };
+  for (long long i = 0; i < pieces; ++i) {
+    float xh[8], g[8];
+    fetch(first_row<VEC>(i, G, t), xh, g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      s.x += g[e];
+      s.y += g[e] * xh[e];
+    }
+  }
+  s = group_sum2(s, G, t, slot);
+  s.x /= static_cast<float>(p.rows);
+  s.y /= static_cast<float>(p.rows);
+  for (long long i = 0; i < pieces; ++i) {
+    const long long r0 = first_row<VEC>(i, G, t);
+    float xh[8], g[8];
+    fetch(r0, xh, g);
+    write_dh<VEC>(p, gen, col, r0, lane, rstd, s, xh, g);
+  }
+}
+
+// Weight gradients of long columns: a thread owns a row, a CTA a range of columns.
+template <typename T>
+__global__ void __launch_bounds__(256)
+norm_weight_grad_kernel(const NormBwd<T> p, long long cols_per_part) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const long long r = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (r >= p.rows) return;
+  const long long c0 = blockIdx.y * cols_per_part;
+  const long long c1 = c0 + cols_per_part < p.cols ? c0 + cols_per_part : p.cols;
+  float dg = 0.f, db = 0.f;
+  for (long long c = c0; c < c1; ++c) {
+    const float d = to_f(p.dy[c * p.lddy + r]);
+    dg += d * ((to_f(p.h[c * p.ldh + r]) - p.mean[c]) * p.rstd[c]);
+    db += d;
+  }
+  float* out = p.partial + static_cast<long long>(blockIdx.y) * 2 * p.rows;
+  out[r] = dg;
+  out[p.rows + r] = db;
+}
+
+// dgain / dbias (+)= the sum over `parts` partial vectors, always in the same order.  A CTA serves
+// 32 rows; its eight warps take every eighth vector.
+template <typename T>
+__global__ void __launch_bounds__(256)
+norm_weight_sum_kernel(const float* __restrict__ partial, int parts, long long rows,
+                       T* __restrict__ dgain, T* __restrict__ dbias, int accumulate) {
+  __shared__ float red[8][32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long r = static_cast<long long>(blockIdx.x) * 32 + lane;
+  T* out = blockIdx.y ? dbias : dgain;
+  if (out == nullptr) return;
+  float s = 0.f;
+  if (r < rows)
+    for (int k = warp; k < parts; k += 8) s += partial[(2LL * k + blockIdx.y) * rows + r];
+  red[warp][lane] = s;
+  __syncthreads();
+  if (warp != 0 || r >= rows) return;
+  float a = accumulate ? to_f(out[r]) : 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) a += red[w][lane];
+  out[r] = from_f<T>(a);
+}
+
+// y = (add) + drop(x): eight elements per thread and pass.  `add` is the residual forward and the
+// gradient itself when it accumulates; VEC as above, with col_len the length of one contiguous run
+// (the whole matrix when nothing lies between its columns).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+dropout_kernel(const T* x, long long ldx, const T* add, long long lda, T* y, long long ldy,
+               long long rows, long long cols, Dropout drop) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const Philox gen(drop);
+  const long long per_col = (rows + 7) / 8, n = VEC ? per_col * cols : rows * cols;
+  const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
+  for (long long q = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; q < n; q += stride) {
+    if (VEC) {
+      const long long col = cols == 1 ? 0 : q / per_col, r0 = (q - col * per_col) * 8;
+      const T* xp = x + col * ldx + r0;
+      const T* ap = add + col * lda + r0;
+      T* yp = y + col * ldy + r0;
+      float v[8], a[8];
+      const bool full = r0 + 8 <= rows;  // only the last run of a flat matrix may be short
+      if (full) {
+        load8(xp, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = r0 + e < rows ? to_f(xp[e]) : 0.f;
+      }
+      if (drop.threshold != 0)
+        drop8(v, gen.keep8((static_cast<unsigned long long>(col) * rows + r0) >> 3), drop.factor);
+      if (add != nullptr) {
+        if (full) {
+          load8(ap, a);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) a[e] = r0 + e < rows ? to_f(ap[e]) : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += a[e];
+      }
+      if (full) {
+        store8(yp, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (r0 + e < rows) yp[e] = from_f<T>(v[e]);
+      }
+    } else {
+      const long long col = q / rows, r = q - col * rows;
+      float v = to_f(x[col * ldx + r]);
+      if (drop.threshold != 0)
+        v = (gen.keep8(static_cast<unsigned long long>(q) >> 3) >> (q & 7)) & 1u ? v * drop.factor : 0.f;
+      if (add != nullptr) v += to_f(add[col * lda + r]);
+      y[col * ldy + r] = from_f<T>(v);
+    }
+  }
+}
+
+// Every column of a matrix starts on a 16-byte boundary.
+bool cols16(const void* p, long long ld, int es, long long cols) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (cols <= 1 || (ld * es) % 16 == 0);
+}
+
+// Threads per column (32 at least) such that 8 * nv elements per thread cover it; 0 = too long.
+int group_size(long long rows, int nv) {
+  for (int g = 32; g <= 512; g *= 2)
+    if (rows <= 8LL * nv * g) return g;
+  return 0;
+}
+
+template <typename T, bool VEC>
+cudaError_t forward_tv(const NormFwd<T>& p, cudaStream_t stream) {
+  int nv = 1, G = 32;
+  if (p.rows > 256) nv = p.rows <= 512 ? 2 : 4;
+  G = group_size(p.rows, nv);
+  if (G == 0) {
+    if (p.cols > 0x7fffffffLL) return cudaErrorInvalidValue;
+    return launch_kernel(norm_forward_long_kernel<T, VEC>, dim3(static_cast<unsigned>(p.cols)), dim3(512), 0,
+                         stream, pdl_enabled(), p);
+  }
+  const int threads = G > 256 ? G : 256;
+  const long long per = threads / G, grid = (p.cols + per - 1) / per;
+  if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
+  auto kern = nv == 1 ? norm_forward_kernel<T, VEC, 1> : nv == 2 ? norm_forward_kernel<T, VEC, 2> : norm_forward_kernel<T, VEC, 4>;
+  return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(threads), 0, stream, pdl_enabled(), p, G);
+}
+
+template <typename T>
+cudaError_t forward_t(const NormArgs& a, cudaStream_t stream) {
+  NormFwd<T> p;
+  p.x = static_cast<const T*>(a.x);
+  p.res = static_cast<const T*>(a.res);
+  p.gain = static_cast<const T*>(a.gain);
+  p.bias = static_cast<const T*>(a.bias);
+  p.h = static_cast<T*>(a.h);
+  p.y = static_cast<T*>(a.y);
+  p.mean = a.mean;
+  p.rstd = a.rstd;
+  p.ldx = a.ldx; p.ldres = a.ldres; p.ldh = a.ldh; p.ldy = a.ldy;
+  p.rows = a.rows; p.cols = a.cols;
+  p.eps = a.eps;
+  p.drop = a.drop;
+  const int es = sizeof(T);
+  const bool vec = a.rows % 8 == 0 && cols16(a.x, a.ldx, es, a.cols) && cols16(a.y, a.ldy, es, a.cols) &&
+                   cols16(a.res, a.ldres, es, a.cols) && cols16(a.h, a.ldh, es, a.cols) &&
+                   cols16(a.gain, 0, es, 1) && cols16(a.bias, 0, es, 1);
+  return vec ? forward_tv<T, true>(p, stream) : forward_tv<T, false>(p, stream);
+}
+
+template <typename T, bool VEC>
+cudaError_t backward_tv(const NormBwd<T>& p, const NormGradArgs& a, int parts, cudaStream_t stream) {
+  if (a.rows > kNormRegisterRows) {
+    if (p.cols > 0x7fffffffLL) return cudaErrorInvalidValue;
+    if (p.dres != nullptr || p.dx != nullptr) {
+      cudaError_t e = launch_kernel(norm_backward_long_kernel<T, VEC>, dim3(static_cast<unsigned>(p.cols)),
+                                    dim3(512), 0, stream, pdl_enabled(), p);
+      if (e != cudaSuccess) return e;
+    }
+    if (p.partial == nullptr) return cudaSuccess;
+    const long long per = (p.cols + parts - 1) / parts;
+    return launch_kernel(norm_weight_grad_kernel<T>,
+                         dim3(static_cast<unsigned>((p.rows + 255) / 256), static_cast<unsigned>(parts)), dim3(256), 0,
+                         stream, pdl_enabled(), p, per);
+  }
+  const int nv = p.rows <= 256 ? 1 : 2;
+  const int G = group_size(p.rows, nv);
+  auto kern = nv == 1 ? norm_backward_kernel<T, VEC, 1> : norm_backward_kernel<T, VEC, 2>;
+  const int smem = p.partial != nullptr ? static_cast<int>(2 * p.rows * sizeof(float)) : 0;
+  static unsigned long long smem_set[2] = {0, 0};  // per template instantiation
+  cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern),
+                                      2 * kNormRegisterRows * static_cast<int>(sizeof(float)), &smem_set[nv - 1]);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(kern, dim3(static_cast<unsigned>(parts)), dim3(512), smem, stream, pdl_enabled(), p, G);
+}
+
+template <typename T>
+cudaError_t backward_t(const NormGradArgs& a, int parts, float* partial, cudaStream_t stream) {
+  NormBwd<T> p;
+  p.h = static_cast<const T*>(a.h);
+  p.gain = static_cast<const T*>(a.gain);
+  p.mean = a.mean;
+  p.rstd = a.rstd;
+  p.dy = static_cast<const T*>(a.dy);
+  p.dh = static_cast<const T*>(a.dh);
+  p.dres = static_cast<T*>(a.dres);
+  p.dx = static_cast<T*>(a.dx);
+  p.partial = partial;
+  p.ldh = a.ldh; p.lddy = a.lddy; p.lddh = a.lddh; p.lddres = a.lddres; p.lddx = a.lddx;
+  p.rows = a.rows; p.cols = a.cols;
+  p.accumulate = a.accumulate;
+  p.drop = a.drop;
+  const int es = sizeof(T);
+  const bool vec = a.rows % 8 == 0 && cols16(a.h, a.ldh, es, a.cols) && cols16(a.dy, a.lddy, es, a.cols) &&
+                   cols16(a.dh, a.lddh, es, a.cols) && cols16(a.dres, a.lddres, es, a.cols) &&
+                   cols16(a.dx, a.lddx, es, a.cols) && cols16(a.gain, 0, es, 1);
+  if (a.cols > 0) {
+    cudaError_t e = vec ? backward_tv<T, true>(p, a, parts, stream) : backward_tv<T, false>(p, a, parts, stream);
+    if (e != cudaSuccess) return e;
+  }
+  if (a.dgain == nullptr && a.dbias == nullptr) return cudaSuccess;
+  return launch_kernel(norm_weight_sum_kernel<T>, dim3(static_cast<unsigned>((a.rows + 31) / 32), 2), dim3(256), 0, stream,
+                       pdl_enabled(), static_cast<const float*>(partial), a.cols > 0 ? parts : 0, a.rows,
+                       static_cast<T*>(a.dgain), static_cast<T*>(a.dbias), a.accumulate);
+}
+
+template <typename T>
+cudaError_t dropout_t(const void* x, long long ldx, const void* add, long long lda, void* y, long long ldy,
+                      long long rows, long long cols, const Dropout& drop, int num_sms, cudaStream_t stream) {
+  if (cols > 1 && ldx == rows && ldy == rows && (add == nullptr || lda == rows)) {
+    rows *= cols;  // nothing between the columns: one run, whatever its length
+    cols = 1;
+  }
+  const int es = sizeof(T);
+  const bool vec = (cols == 1 || rows % 8 == 0) && cols16(x, ldx, es, cols) && cols16(y, ldy, es, cols) &&
+                   cols16(add, lda, es, cols);
+  const long long work = vec ? (rows + 7) / 8 * cols : rows * cols;
+  const long long want = (work + 255) / 256, most = static_cast<long long>(num_sms) * 8;
+  const unsigned grid = static_cast<unsigned>(want < most ? want : most);
+  auto kern = vec ? dropout_kernel<T, true> : dropout_kernel<T, false>;
+  return launch_kernel(kern, dim3(grid), dim3(256), 0, stream, pdl_enabled(), static_cast<const T*>(x), ldx,
+                       static_cast<const T*>(add), lda, static_cast<T*>(y), ldy, rows, cols, drop);
+}
+
+}  // namespace
+
+int norm_backward_parts(long long rows, long long cols, int num_sms) {
+  if (cols <= 0) return 0;
+  if (rows > kNormRegisterRows) {
+    // enough CTAs to fill the device with 256 rows each, at most 64 partial vectors
+    const long long row_blocks = (rows + 255) / 256;
+    long long parts = (4LL * num_sms + row_blocks - 1) / row_blocks;
+    parts = parts > 64 ? 64 : parts;
+    parts = parts > cols ? cols : parts;
+    const long long per = (cols + parts - 1) / parts;
+    return static_cast<int>((cols + per - 1) / per);
+  }
+  const int groups = 512 / group_size(rows, rows <= 256 ? 1 : 2);
+  const long long want = (cols + groups - 1) / groups;
+  return static_cast<int>(want < num_sms ? want : num_sms);
+}
+
+cudaError_t launch_norm_forward(int dtype, const NormArgs& a, cudaStream_t stream) {
+  return dtype == 0 ? forward_t<float>(a, stream) : forward_t<__half>(a, stream);
+}
+
+cudaError_t launch_norm_backward(int dtype, const NormGradArgs& a, int parts, float* partial,
+                                 cudaStream_t stream) {
+  return dtype == 0 ? backward_t<float>(a, parts, partial, stream) : backward_t<__half>(a, parts, partial, stream);
+}
+
+cudaError_t launch_dropout(int dtype, const void* x, long long ldx, const void* add, long long lda, void* y,
+                           long long ldy, long long rows, long long cols, const Dropout& drop, int num_sms,
+                           cudaStream_t stream) {
+  return dtype == 0 ? dropout_t<float>(x, ldx, add, lda, y, ldy, rows, cols, drop, num_sms, stream)
+                    : dropout_t<__half>(x, ldx, add, lda, y, ldy, rows, cols, drop, num_sms, stream);
+}
+
+}  // namespace gb

@@ -342,6 +342,74 @@ int ginn_b200_attention_backward(int device, void* stream, int dtype, int64_t t,
                                  int64_t ldp, int64_t stride_p, const void* d_o, int64_t ldo,
                                  int64_t stride_o, void* ds, void* dk, void* dq, void* dv);
 
+/* ---- Layer normalisation and dropout -------------------------------------------------------- */
+
+/* Normalisation of every column of x (rows x cols), the work of ginn's LayerNorm node
+ * (ginn/node/layernorm.h) with a learned gain and bias per row:
+ *   mu = mean(x_j),  r = 1 / sqrt(mean((x_j - mu)^2) + eps),  y_j = gain (.) (x_j - mu) r + bias.
+ * gain / bias: `rows` elements of type `dtype`, NULL = 1 / 0.  mean / rstd: `cols` floats each that
+ * the backward pass reads, NULL when none follows.  y may be x itself (same leading dimension).
+ * eps must be positive. */
+int ginn_b200_layer_norm_forward(int device, void* stream, int dtype, int64_t rows, int64_t cols,
+                                 const void* x, int64_t ldx, const void* gain, const void* bias,
+                                 float eps, void* y, int64_t ldy, float* mean, float* rstd);
+
+/* Gradients of the above, `+=` when accumulate != 0 and `=` otherwise; each may be NULL:
+ *   dx_j (+)= r (G - mean(G) - xh mean(G (.) xh))  with  xh = (x_j - mu) r,  G = gain (.) dy_j;
+ *   dgain (+)= sum_j dy_j (.) xh_j;   dbias (+)= sum_j dy_j   (type `dtype`, summed in fp32 in a
+ * fixed order).  The weight gradients take at most 2 * rows * 148 floats of stream-ordered scratch.
+ * dx may be dy itself. */
+int ginn_b200_layer_norm_backward(int device, void* stream, int dtype, int64_t rows, int64_t cols,
+                                  const void* x, int64_t ldx, const void* gain, const float* mean,
+                                  const float* rstd, const void* dy, int64_t lddy, void* dx,
+                                  int64_t lddx, void* dgain, void* dbias, int accumulate);
+
+/* The random numbers of a dropout: the mask is a function of (seed, offset, element) and is never
+ * stored; the backward call takes the same values.  Element (i, j) of a rows x cols matrix is
+ * number e = i + rows * j whatever the leading dimension; it takes 16-bit number e % 8 (low halves
+ * first) of Philox4x32-10 block e / 8 -- counter words (block low, block high, offset low, offset
+ * high), key (seed low, seed high) -- and is kept when that is not below round(65536 p).  Kept
+ * elements are multiplied by 65536 / (65536 - round(65536 p)).  p: 0 <= p, round(65536 p) < 65536.
+ * `step`, when not NULL, points to a device counter that is added to `offset`: a captured training
+ * step that advances it draws a new mask at every replay. */
+typedef struct {
+  float p;
+  uint64_t seed;
+  uint64_t offset;
+  const uint64_t* step;
+} ginn_b200_dropout;
+
+/* y = residual + drop(x); residual may be NULL.  The work of ginn's Dropout node
+ * (ginn/node/common.h), which draws and keeps a mask tensor, and of the Add behind it.
+ * y may be x or residual. */
+int ginn_b200_dropout_forward(int device, void* stream, int dtype, int64_t rows, int64_t cols,
+                              const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                              const ginn_b200_dropout* drop, void* y, int64_t ldy);
+/* dx (+)= dy on the kept elements times their factor, 0 on the others. */
+int ginn_b200_dropout_backward(int device, void* stream, int dtype, int64_t rows, int64_t cols,
+                               const void* dy, int64_t lddy, const ginn_b200_dropout* drop, void* dx,
+                               int64_t lddx, int accumulate);
+
+/* Both in one pass, the seam between two sublayers of a transformer block:
+ *   h = residual + drop(x)  (stored, rounded to `dtype`),   y = normalisation of h as above.
+ * residual may be NULL.  h may be residual or x; y must be storage of its own. */
+int ginn_b200_residual_norm_forward(int device, void* stream, int dtype, int64_t rows, int64_t cols,
+                                    const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                                    const ginn_b200_dropout* drop, const void* gain,
+                                    const void* bias, float eps, void* h, int64_t ldh, void* y,
+                                    int64_t ldy, float* mean, float* rstd);
+/* Its gradients: with g = (gradient of the normalisation's input) + dh, dh (may be NULL) being what
+ * reaches h along the residual connection:
+ *   dres (+)= g,   dx (+)= g on the kept elements times their factor,   dgain, dbias as above.
+ * Each result may be NULL.  dres or dx may be dh or dy, but not each other. */
+int ginn_b200_residual_norm_backward(int device, void* stream, int dtype, int64_t rows,
+                                     int64_t cols, const void* h, int64_t ldh, const void* gain,
+                                     const float* mean, const float* rstd, const void* dy,
+                                     int64_t lddy, const void* dh, int64_t lddh,
+                                     const ginn_b200_dropout* drop, void* dx, int64_t lddx,
+                                     void* dres, int64_t lddres, void* dgain, void* dbias,
+                                     int accumulate);
+
 /* ---- Conv2d through the same products ------------------------------------------------------ */
 
 /* 2-d convolution with "SAME" padding, as Conv2dNode computes it (ginn/node/conv.h:28-79 over

@@ -230,6 +230,55 @@ def attention_backward(k, q, v, p, d_o, scale=1.0):
     return dk.astype(dt), dq.astype(dt), dv.astype(dt)
 
 
+def philox4x32(counter, key, rounds: int = 10):
+    """Philox4x32 (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3", SC 2011): counter
+    (4, n) and key (2,) of 32-bit words -> (4, n) output words."""
+    c = np.array(counter, dtype=np.uint64)
+    k = [int(x) for x in key]
+    low, s32 = np.uint64(0xFFFFFFFF), np.uint64(32)
+    for _ in range(rounds):
+        p0, p1 = np.uint64(0xD2511F53) * c[0], np.uint64(0xCD9E8D57) * c[2]
+        c = np.stack([(p1 >> s32) ^ c[1] ^ np.uint64(k[0]), p1 & low,
+                      (p0 >> s32) ^ c[3] ^ np.uint64(k[1]), p0 & low])
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return c
+
+
+def dropout_mask(rows: int, cols: int, p: float, seed: int, offset: int) -> np.ndarray:
+    """rows x cols factors: 0 where element row + rows * col is dropped, else the inverse of the
+    keep probability, which is a multiple of 2^-16."""
+    n = rows * cols
+    block = np.arange((n + 7) // 8, dtype=np.uint64)
+    ctr = np.stack([block & np.uint64(0xFFFFFFFF), block >> np.uint64(32),
+                    np.full_like(block, offset & 0xFFFFFFFF), np.full_like(block, offset >> 32)])
+    w = philox4x32(ctr, (seed & 0xFFFFFFFF, seed >> 32))
+    numbers = np.stack([h for x in w for h in (x & np.uint64(0xFFFF), x >> np.uint64(16))], 1).reshape(-1)[:n]
+    threshold = int(np.floor(float(np.float32(p)) * 65536 + 0.5))
+    return np.where(numbers >= threshold, 65536.0 / (65536 - threshold), 0.0).reshape(cols, rows).T
+
+
+def layer_norm_forward(x, gain=None, bias=None, eps=1e-5):
+    """(y, mean, rstd) of the column normalisation."""
+    x = f64(x)
+    mean = x.mean(0)
+    rstd = 1.0 / np.sqrt(((x - mean) ** 2).mean(0) + eps)
+    y = (x - mean) * rstd
+    if gain is not None:
+        y = y * f64(gain)[:, None]
+    if bias is not None:
+        y = y + f64(bias)[:, None]
+    return y, mean, rstd
+
+
+def layer_norm_backward(x, gain, mean, rstd, dy):
+    """(dx, dgain, dbias) without what they are added to."""
+    x, dy = f64(x), f64(dy)
+    xh = (x - f64(mean)) * f64(rstd)
+    g = dy if gain is None else dy * f64(gain)[:, None]
+    dx = f64(rstd) * (g - g.mean(0) - xh * (g * xh).mean(0))
+    return dx, (dy * xh).sum(1), dy.sum(1)
+
+
 def conv2d_geometry(rows, cols, krows, kcols, row_stride, col_stride):
     """Output extents and leading padding of Eigen's PADDING_SAME (eigen_conv.h:40-47 and the
     patch extraction it calls): out = ceil(in / stride), total padding max(0, (out - 1) stride
