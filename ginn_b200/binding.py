@@ -53,6 +53,27 @@ class _Dropout(C.Structure):
                 ("step", C.c_void_p)]
 
 
+class _RelativeAttention(C.Structure):
+    _fields_ = ([(n, C.c_int64) for n in ("tq", "tk", "head_size", "heads", "kv_heads", "batch")]
+                + [(n, t) for x in "qkv" for n, t in ((x, C.c_void_p), ("ld" + x, C.c_int64),
+                                                      (f"stride_{x}_head", C.c_int64),
+                                                      (f"stride_{x}_batch", C.c_int64))]
+                + [("table", C.c_void_p), ("ldt", C.c_int64), ("buckets", C.c_int64),
+                   ("map", C.c_void_p), ("reach", C.c_int64), ("scale", C.c_float),
+                   ("causal", C.c_int), ("q_offset", C.c_int64), ("q_offsets", C.c_void_p),
+                   ("q_lengths", C.c_void_p), ("k_lengths", C.c_void_p), ("o", C.c_void_p),
+                   ("ldo", C.c_int64), ("stride_o_head", C.c_int64), ("stride_o_batch", C.c_int64),
+                   ("lse", C.c_void_p)])
+
+
+class _RelativeAttentionGrad(C.Structure):
+    _fields_ = ([(n, t) for x in ("d_o", "dq", "dk", "dv")
+                 for n, t in ((x, C.c_void_p), ("ld" + x.replace("_", ""), C.c_int64),
+                              (f"stride_{x.replace('_', '')}_head", C.c_int64),
+                              (f"stride_{x.replace('_', '')}_batch", C.c_int64))]
+                + [("dtable", C.c_void_p), ("lddt", C.c_int64), ("accumulate", C.c_int)])
+
+
 def lib_path() -> str:
     return _LIB_PATH
 
@@ -128,6 +149,13 @@ def lib():
     for name in ("ginn_b200_layer_norm_forward", "ginn_b200_layer_norm_backward",
                  "ginn_b200_dropout_forward", "ginn_b200_dropout_backward",
                  "ginn_b200_residual_norm_forward", "ginn_b200_residual_norm_backward"):
+        getattr(L, name).restype = ci
+    L.ginn_b200_relative_attention_forward.argtypes = [ci, vp, ci, C.POINTER(_RelativeAttention)]
+    L.ginn_b200_relative_attention_backward.argtypes = [ci, vp, ci, C.POINTER(_RelativeAttention),
+                                                        C.POINTER(_RelativeAttentionGrad)]
+    L.ginn_b200_relative_buckets.argtypes = [ci, ci, ci, i64, vp]
+    for name in ("ginn_b200_relative_attention_forward", "ginn_b200_relative_attention_backward",
+                 "ginn_b200_relative_buckets"):
         getattr(L, name).restype = ci
     L.ginn_b200_conv2d_workspace.argtypes = [ci] + [i64] * 9
     L.ginn_b200_conv2d_workspace.restype = C.c_size_t
@@ -533,6 +561,82 @@ def residual_norm_backward(h, gain, mean, rstd, dy, dh=None, dx=None, dres=None,
         *_opt_matrix(dx, "dx", h), *_opt_matrix(dres, "dres", h),
         _vector(dgain, "dgain", rows, h.dtype, h.device),
         _vector(dbias, "dbias", rows, h.dtype, h.device), int(accumulate)))
+
+
+def relative_buckets(buckets: int, max_distance: int, bidirectional: bool,
+                     reach: Optional[int] = None) -> torch.Tensor:
+    """Bucket of every distance key - query from -reach to reach (max_distance when not given), as a
+    host int32 tensor (ginn_b200_relative_buckets)."""
+    reach = max_distance if reach is None else reach
+    out = torch.empty(2 * max(reach, 0) + 1, dtype=torch.int32)
+    _check(lib().ginn_b200_relative_buckets(buckets, max_distance, int(bidirectional), reach,
+                                            out.data_ptr()))
+    return out
+
+
+def _heads(t: torch.Tensor, name: str, shape, like: torch.Tensor) -> tuple:
+    """(pointer, ld, head stride, batch stride) of a (head size, time, heads, batch) tensor."""
+    if tuple(t.shape) != tuple(shape) or t.dtype != like.dtype or t.device != like.device:
+        raise GinnB200Error(1, f"{name}: expected {tuple(shape)} of {like.dtype} on {like.device}")
+    if t.shape[0] > 1 and t.stride(0) != 1:
+        raise GinnB200Error(1, f"{name}: the elements of a head must be contiguous")
+    return t.data_ptr(), t.stride(1), t.stride(2), t.stride(3)
+
+
+def _relative_attention(q, k, v, table, bucket_map, o, lse, scale, causal, q_offset, q_offsets,
+                        q_lengths, k_lengths):
+    for name, t in (("q", q), ("k", k)):
+        if t.dim() != 4:
+            raise GinnB200Error(1, f"{name}: expected (head size, time, heads, batch)")
+    hs, tq, heads, batch = q.shape
+    tk, kv = k.shape[1], k.shape[2]
+    tab, ldt, buckets, reach, bmap = None, 0, 0, 0, None
+    if table is not None:
+        if table.dim() != 2 or table.shape[1] != heads or table.dtype != q.dtype or table.device != q.device:
+            raise GinnB200Error(1, f"table: expected buckets x {heads} of {q.dtype} on {q.device}")
+        if bucket_map is None or bucket_map.dim() != 1 or bucket_map.numel() % 2 == 0:
+            raise GinnB200Error(1, "bucket_map: expected 2 * reach + 1 ints")
+        buckets, reach = table.shape[0], bucket_map.numel() // 2
+        tab, ldt = _matrix(table, "table", table)
+        bmap = _vector(bucket_map, "bucket_map", 2 * reach + 1, torch.int32, q.device)
+    return _RelativeAttention(
+        tq, tk, hs, heads, kv, batch, *_heads(q, "q", (hs, tq, heads, batch), q),
+        *_heads(k, "k", (hs, tk, kv, batch), q), *_heads(v, "v", (hs, tk, kv, batch), q), tab, ldt,
+        buckets, bmap, reach, scale, int(causal), q_offset,
+        _vector(q_offsets, "q_offsets", batch, torch.int32, q.device),
+        _vector(q_lengths, "q_lengths", batch, torch.int32, q.device),
+        _vector(k_lengths, "k_lengths", batch, torch.int32, q.device),
+        *_heads(o, "o", (hs, tq, heads, batch), q),
+        _vector(lse, "lse", tq * heads * batch, torch.float32, q.device))
+
+
+def relative_attention_forward(q, k, v, table, bucket_map, o, lse, scale: float,
+                               causal: bool = False, q_offset: int = 0, q_offsets=None,
+                               q_lengths=None, k_lengths=None) -> None:
+    """Attention with a relative position bias (ginn_b200_relative_attention_forward).  q, o: (head
+    size, tq, heads, batch), k, v: (head size, tk, kv heads, batch), any strides with contiguous
+    heads; table: (buckets, heads) or None; bucket_map: int32 from relative_buckets, on the device;
+    lse: batch * heads * tq contiguous floats."""
+    a = _relative_attention(q, k, v, table, bucket_map, o, lse, scale, causal, q_offset, q_offsets,
+                            q_lengths, k_lengths)
+    _check(lib().ginn_b200_relative_attention_forward(_dev(q), _stream(q), _dtype_of(q), C.byref(a)))
+
+
+def relative_attention_backward(q, k, v, table, bucket_map, o, lse, d_o, dq=None, dk=None, dv=None,
+                                dtable=None, scale: float = 1.0, causal: bool = False,
+                                q_offset: int = 0, q_offsets=None, q_lengths=None, k_lengths=None,
+                                accumulate: bool = True) -> None:
+    """Gradients of relative_attention_forward from its o and lse, added to dq / dk / dv / dtable or
+    (accumulate=False) assigned (ginn_b200_relative_attention_backward)."""
+    a = _relative_attention(q, k, v, table, bucket_map, o, lse, scale, causal, q_offset, q_offsets,
+                            q_lengths, k_lengths)
+    out = [(None, 0, 0, 0) if t is None else _heads(t, n, x.shape, q)
+           for n, t, x in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v))]
+    dt = (None, 0) if dtable is None else _matrix(dtable, "dtable", dtable if table is None else table)
+    g = _RelativeAttentionGrad(*_heads(d_o, "d_o", q.shape, q), *out[0], *out[1], *out[2], *dt,
+                               int(accumulate))
+    _check(lib().ginn_b200_relative_attention_backward(_dev(q), _stream(q), _dtype_of(q),
+                                                       C.byref(a), C.byref(g)))
 
 
 def lstm_cell_forward(gates, c_prev, c, h, xh_next=None, n_next=0) -> None:

@@ -1,9 +1,12 @@
 // extern "C" layer: argument validation, path selection, per-device state.
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -1767,6 +1770,433 @@ int ginn_b200_residual_norm_backward(int device, void* stream, int dtype, int64_
   a.ldh = ldh; a.lddy = lddy; a.lddh = lddh; a.lddx = lddx; a.lddres = lddres; a.rows = rows; a.cols = cols;
   a.accumulate = accumulate ? 1 : 0;
   return norm_backward(device, stream, dtype, a);
+}
+
+// ---- attention with a relative position bias --------------------------------------------------
+namespace {
+
+struct RelStrides {
+  int64_t ld, head, batch;
+};
+
+// Stream-ordered scratch of one call, handed back to the pool on every path out.
+struct Scratch {
+  cudaStream_t stream;
+  void* held[16];
+  int count = 0;
+  explicit Scratch(cudaStream_t s) : stream(s) {}
+  ~Scratch() {
+    for (int i = 0; i < count; ++i) cudaFreeAsync(held[i], stream);
+  }
+  cudaError_t take(float** out, long long n) {
+    void* p = nullptr;
+    if (count == 16) return cudaErrorMemoryAllocation;
+    const cudaError_t e = cudaMallocAsync(&p, static_cast<size_t>(n > 0 ? n : 1) * sizeof(float), stream);
+    if (e == cudaSuccess) held[count++] = p;
+    *out = static_cast<float*>(p);
+    return e;
+  }
+};
+
+int check_heads(const char* name, const void* p, const RelStrides& s) {
+  if (!p) return fail(GINN_B200_BAD_ARGUMENT, "%s is a null pointer", name);
+  if (s.ld < 0 || s.head < 0 || s.batch < 0)
+    return fail(GINN_B200_BAD_ARGUMENT, "%s has a negative stride", name);
+  return GINN_B200_OK;
+}
+// An output: its elements must be places of their own.
+int check_heads_out(const char* name, const void* p, const RelStrides& s, int64_t hs, int64_t t, int64_t heads, int64_t batch) {
+  if (int e = check_heads(name, p, s)) return e;
+  struct Dim {
+    int64_t n, stride;
+  } d[3] = {{t, s.ld}, {heads, s.head}, {batch, s.batch}};
+  for (int i = 0; i < 2; ++i)  // by stride
+    for (int j = 0; j < 2 - i; ++j)
+      if (d[j].stride > d[j + 1].stride) std::swap(d[j], d[j + 1]);
+  int64_t span = hs;  // elements covered by the dimensions inside
+  for (const Dim& x : d) {
+    if (x.n <= 1) continue;
+    if (x.stride < span)
+      return fail(GINN_B200_BAD_ARGUMENT, "the strides of %s make its elements overlap", name);
+    span = (x.n - 1) * x.stride + span;
+  }
+  return GINN_B200_OK;
+}
+
+int check_relative(int dtype, const ginn_b200_relative_attention* a) {
+  if (dtype != GINN_B200_F32 && dtype != GINN_B200_F16)
+    return fail(GINN_B200_UNSUPPORTED, "dtype %d is not fp32 (0) or fp16 (1)", dtype);
+  if (!a) return fail(GINN_B200_BAD_ARGUMENT, "null attention description");
+  constexpr int64_t kMost = 1 << 29;
+  if (a->tq < 0 || a->tk < 0 || a->batch < 0 || a->heads < 0 || a->tq >= kMost || a->tk >= kMost ||
+      a->batch > 0x7fffffffLL || a->heads > 65535)
+    return fail(GINN_B200_BAD_ARGUMENT, "bad extents tq=%lld tk=%lld heads=%lld batch=%lld", (long long)a->tq,
+                (long long)a->tk, (long long)a->heads, (long long)a->batch);
+  if (a->head_size < 1 || a->head_size > 256)
+    return fail(GINN_B200_UNSUPPORTED, "head size %lld is not in 1..256", (long long)a->head_size);
+  if (a->heads > 0 && (a->kv_heads < 1 || a->heads % a->kv_heads != 0))
+    return fail(GINN_B200_BAD_ARGUMENT, "%lld query heads cannot share %lld key / value heads", (long long)a->heads,
+                (long long)a->kv_heads);
+  if (a->batch * a->heads > 0x7fffffffLL)
+    return fail(GINN_B200_BAD_ARGUMENT, "more than 2^31-1 heads in all");
+  if (!(a->scale > -INFINITY && a->scale < INFINITY))
+    return fail(GINN_B200_BAD_ARGUMENT, "the scale is not finite");
+  if (a->q_offset < -(1 << 30) || a->q_offset > (1 << 30))
+    return fail(GINN_B200_BAD_ARGUMENT, "query offset %lld is not within 2^30", (long long)a->q_offset);
+  if (a->table) {
+    if (a->buckets < 1 || a->buckets > 65536)
+      return fail(GINN_B200_BAD_ARGUMENT, "bucket count %lld is not in 1..65536", (long long)a->buckets);
+    if (a->ldt < a->buckets)
+      return fail(GINN_B200_BAD_ARGUMENT, "leading dimension %lld of the table is smaller than its %lld buckets",
+                  (long long)a->ldt, (long long)a->buckets);
+    if (!a->map) return fail(GINN_B200_BAD_ARGUMENT, "a bias table needs its bucket map");
+    if (a->reach < 0 || a->reach > (1 << 24))
+      return fail(GINN_B200_BAD_ARGUMENT, "reach %lld is not in 0..2^24", (long long)a->reach);
+  }
+  if (a->tq == 0 || a->heads == 0 || a->batch == 0) return GINN_B200_OK;
+  const RelStrides q = {a->ldq, a->stride_q_head, a->stride_q_batch}, k = {a->ldk, a->stride_k_head, a->stride_k_batch},
+                   v = {a->ldv, a->stride_v_head, a->stride_v_batch}, o = {a->ldo, a->stride_o_head, a->stride_o_batch};
+  if (int s = check_heads("q", a->q, q)) return s;
+  if (a->tk > 0) {
+    if (int s = check_heads("k", a->k, k)) return s;
+    if (int s = check_heads("v", a->v, v)) return s;
+  }
+  if (int s = check_heads_out("o", a->o, o, a->head_size, a->tq, a->heads, a->batch)) return s;
+  if (!a->lse) return fail(GINN_B200_BAD_ARGUMENT, "lse is a null pointer");
+  return GINN_B200_OK;
+}
+
+// An operand of the composed path: fp32, its heads equally spaced over all sequences.
+struct RelDense {
+  const float* p = nullptr;
+  long long ld = 0, stride = 0;
+};
+
+// `src` as it is when it already has that form and no length cuts it, else a packed copy.
+int rel_dense_in(Scratch* scratch, int dtype, const void* src, const RelStrides& s, int64_t hs, int64_t t, int64_t heads,
+                 int64_t batch, const int* lengths, RelDense* out) {
+  const bool even = batch == 1 || s.batch == heads * s.head;
+  if (dtype == GINN_B200_F32 && even && lengths == nullptr && s.ld >= hs) {
+    out->p = static_cast<const float*>(src);
+    out->ld = s.ld;
+    out->stride = s.head;
+    return GINN_B200_OK;
+  }
+  const int hsp = static_cast<int>((hs + 3) & ~int64_t(3));
+  float* p;
+  CU_TRY(scratch->take(&p, hsp * t * heads * batch));
+  CU_TRY(gb::launch_rel_pack(dtype, src, s.ld, s.head, s.batch, (int)hs, hsp, (int)t, (int)heads, (int)batch, lengths, p,
+                             scratch->stream));
+  g_launches.fetch_add(1);
+  out->p = p;
+  out->ld = hsp;
+  out->stride = hsp * t;
+  return GINN_B200_OK;
+}
+
+// Where a result's products go: the result itself, or a packed fp32 copy that finish() hands over.
+struct RelOut {
+  float* p = nullptr;
+  long long ld = 0, stride = 0;
+  bool packed = false;
+};
+int rel_dense_out(Scratch* scratch, int dtype, void* dst, const RelStrides& s, int64_t hs, int64_t t, int64_t heads,
+                  int64_t batch, RelOut* out) {
+  const bool even = batch == 1 || s.batch == heads * s.head;
+  if (dtype == GINN_B200_F32 && even && s.ld >= hs) {
+    out->p = static_cast<float*>(dst);
+    out->ld = s.ld;
+    out->stride = s.head;
+    return GINN_B200_OK;
+  }
+  const long long hsp = (hs + 3) & ~int64_t(3);
+  CU_TRY(scratch->take(&out->p, hsp * t * heads * batch));
+  out->ld = hsp;
+  out->stride = hsp * t;
+  out->packed = true;
+  return GINN_B200_OK;
+}
+int rel_finish_out(cudaStream_t stream, int dtype, const RelOut& o, void* dst, const RelStrides& s, int64_t hs, int64_t t,
+                   int64_t heads, int64_t batch, int accumulate) {
+  if (!o.packed) return GINN_B200_OK;
+  CU_TRY(gb::launch_rel_unpack(dtype, o.p, (int)hs, (int)o.ld, (int)t, (int)heads, (int)batch, accumulate, dst, s.ld, s.head,
+                               s.batch, stream));
+  g_launches.fetch_add(1);
+  return GINN_B200_OK;
+}
+
+// The composed path, forward (g null) or backward: per chunk of heads whose scores stay in the L2
+// cache, the fp32 products with the passes of relative_attention.cu between them.  Half operands
+// are widened first, so scores and probabilities are fp32 whatever the type.
+int relative_composed(int device, cudaStream_t stream, int dtype, const ginn_b200_relative_attention& a,
+                      const ginn_b200_relative_attention_grad* g) {
+  Scratch scratch(stream);
+  // A contraction split over CTAs adds its parts with atomics, in whatever order they finish: the
+  // products here are not split, so that a call gives the same bits every time.
+  struct NoSplit {
+    int old = t_max_split;
+    NoSplit() { t_max_split = 1; }
+    ~NoSplit() { t_max_split = old; }
+  } no_split;
+  const int64_t hs = a.head_size, tq = a.tq, tk = a.tk, kv = a.kv_heads, group = a.heads / kv, units = kv * a.batch;
+  const RelStrides sq = {a.ldq, a.stride_q_head, a.stride_q_batch}, sk = {a.ldk, a.stride_k_head, a.stride_k_batch},
+                   sv = {a.ldv, a.stride_v_head, a.stride_v_batch}, so = {a.ldo, a.stride_o_head, a.stride_o_batch};
+  RelDense q, k, v, d_o;
+  if (int s = rel_dense_in(&scratch, dtype, a.q, sq, hs, tq, a.heads, a.batch, a.q_lengths, &q)) return s;
+  if (int s = rel_dense_in(&scratch, dtype, a.k, sk, hs, tk, kv, a.batch, a.k_lengths, &k)) return s;
+  if (int s = rel_dense_in(&scratch, dtype, a.v, sv, hs, tk, kv, a.batch, a.k_lengths, &v)) return s;
+  float* bias = nullptr;
+  if (a.table) {
+    CU_TRY(scratch.take(&bias, (2 * a.reach + 1) * a.heads));
+    CU_TRY(gb::launch_rel_bias_expand(dtype, a.table, a.ldt, a.map, (int)a.buckets, a.reach, (int)a.heads, 1.f, bias, stream));
+    g_launches.fetch_add(1);
+  }
+  gb::RelScores sc;
+  sc.ld = (tk + 3) & ~int64_t(3);
+  sc.tq = (int)tq; sc.tk = (int)tk; sc.heads = (int)a.heads;
+  sc.scale = a.scale; sc.causal = a.causal ? 1 : 0;
+  sc.q_offset = a.q_offset; sc.q_offsets = a.q_offsets; sc.q_lengths = a.q_lengths; sc.k_lengths = a.k_lengths;
+  sc.reach = a.table ? a.reach : 0;
+
+  // Chunks: as many shared heads as keep the scores within 64 MiB (half the L2 cache), one at least;
+  // the queries of a head in pieces where its scores alone pass 512 MiB.
+  const int64_t head_bytes = tq * sc.ld * 4;
+  int64_t nq = tq;
+  if (group * head_bytes > (int64_t(512) << 20)) {
+    nq = (int64_t(512) << 20) / (group * sc.ld * 4) / gb::kRelDiagonal * gb::kRelDiagonal;
+    nq = nq < gb::kRelDiagonal ? gb::kRelDiagonal : nq;
+    nq = nq > tq ? tq : nq;
+  }
+  int64_t per = (int64_t(g ? 32 : 64) << 20) / (group * nq * sc.ld * 4);
+  per = per < 1 ? 1 : per > units ? units : per;
+  per = per * group > 65535 ? (65535 / group > 0 ? 65535 / group : 1) : per;
+  float *p, *dp = nullptr;
+  CU_TRY(scratch.take(&p, per * group * nq * sc.ld));
+
+  RelOut o, dq, dk, dv;
+  const bool want_dq = g && g->dq, want_dk = g && g->dk, want_dv = g && g->dv, want_dt = g && g->dtable && a.table;
+  const RelStrides sdo = g ? RelStrides{g->lddo, g->stride_do_head, g->stride_do_batch} : RelStrides{0, 0, 0};
+  const RelStrides sdq = g ? RelStrides{g->lddq, g->stride_dq_head, g->stride_dq_batch} : RelStrides{0, 0, 0};
+  const RelStrides sdk = g ? RelStrides{g->lddk, g->stride_dk_head, g->stride_dk_batch} : RelStrides{0, 0, 0};
+  const RelStrides sdv = g ? RelStrides{g->lddv, g->stride_dv_head, g->stride_dv_batch} : RelStrides{0, 0, 0};
+  float* diagonal = nullptr;
+  const int64_t qblocks = (tq + gb::kRelDiagonal - 1) / gb::kRelDiagonal;
+  if (g) {
+    if (int s = rel_dense_in(&scratch, dtype, g->d_o, sdo, hs, tq, a.heads, a.batch, a.q_lengths, &d_o)) return s;
+    CU_TRY(scratch.take(&dp, per * group * nq * sc.ld));
+    if (want_dq)
+      if (int s = rel_dense_out(&scratch, dtype, g->dq, sdq, hs, tq, a.heads, a.batch, &dq)) return s;
+    if (want_dk)
+      if (int s = rel_dense_out(&scratch, dtype, g->dk, sdk, hs, tk, kv, a.batch, &dk)) return s;
+    if (want_dv)
+      if (int s = rel_dense_out(&scratch, dtype, g->dv, sdv, hs, tk, kv, a.batch, &dv)) return s;
+    if (want_dt) CU_TRY(scratch.take(&diagonal, a.heads * a.batch * qblocks * (tq + tk - 1)));
+  } else {
+    if (int s = rel_dense_out(&scratch, dtype, a.o, so, hs, tq, a.heads, a.batch, &o)) return s;
+  }
+  auto product = [&](int ta, int tb, int64_t m, int64_t n, int64_t kk, const float* x, long long ldx, long long sx,
+                     const float* y, long long ldy, long long sy, float* c, long long ldc, long long strc, int64_t count,
+                     int accumulate) {
+    return gemm_impl(device, stream, GINN_B200_F32, ta, tb, m, n, kk, x, ldx, sx, y, ldy, sy, c, ldc, strc, count, accumulate);
+  };
+  for (int64_t u0 = 0; u0 < units; u0 += per) {
+    const int64_t nu = units - u0 < per ? units - u0 : per;
+    for (int64_t i0 = 0; i0 < tq; i0 += nq) {
+      const int64_t n = tq - i0 < nq ? tq - i0 : nq;
+      const long long ms = n * sc.ld;  // one head's scores
+      sc.s = p;
+      sc.nq = (int)n; sc.q0 = (int)i0;
+      sc.matrices = nu * group; sc.matrix0 = u0 * group;
+      for (int64_t r = 0; r < group; ++r)  // S (tk x n) = K^T Q
+        if (int s = product(1, 0, tk, n, hs, k.p + u0 * k.stride, k.ld, k.stride, q.p + (u0 * group + r) * q.stride + i0 * q.ld,
+                            q.ld, group * q.stride, p + r * ms, sc.ld, group * ms, nu, 0))
+          return s;
+      CU_TRY(gb::launch_rel_softmax(sc, bias, g ? a.lse : nullptr, a.lse, stream));
+      g_launches.fetch_add(1);
+      for (int64_t r = 0; r < group && !g; ++r)  // O (hs x n) = V P
+        if (int s = product(0, 0, hs, n, tk, v.p + u0 * v.stride, v.ld, v.stride, p + r * ms, sc.ld, group * ms,
+                            o.p + (u0 * group + r) * o.stride + i0 * o.ld, o.ld, group * o.stride, nu, 0))
+          return s;
+      if (!g) continue;
+      const float* dop = d_o.p + u0 * group * d_o.stride + i0 * d_o.ld;
+      for (int64_t r = 0; r < group; ++r) {
+        const int add = dv.packed || !want_dv ? (r > 0 || i0 > 0) : (g->accumulate || r > 0 || i0 > 0);
+        if (want_dv)  // dV (hs x tk) += dO P^T
+          if (int s = product(0, 1, hs, tk, n, dop + r * d_o.stride, d_o.ld, group * d_o.stride, p + r * ms, sc.ld, group * ms,
+                              dv.p + u0 * dv.stride, dv.ld, dv.stride, nu, add))
+            return s;
+        if (want_dq || want_dk || want_dt)  // dP (tk x n) = V^T dO
+          if (int s = product(1, 0, tk, n, hs, v.p + u0 * v.stride, v.ld, v.stride, dop + r * d_o.stride, d_o.ld,
+                              group * d_o.stride, dp + r * ms, sc.ld, group * ms, nu, 0))
+            return s;
+      }
+      if (!want_dq && !want_dk && !want_dt) continue;
+      // the scale goes with the scores' gradient, but not into the table's: there the pass that
+      // sums the diagonals leaves the scaled values behind
+      CU_TRY(gb::launch_rel_softmax_grad(sc, p, dp, want_dt ? 1.f : a.scale, stream));
+      g_launches.fetch_add(1);
+      if (want_dt) {
+        CU_TRY(gb::launch_rel_diagonal(sc, dp, a.scale, diagonal, (int)qblocks, stream));
+        g_launches.fetch_add(1);
+      }
+      for (int64_t r = 0; r < group; ++r) {
+        if (want_dk) {  // dK (hs x tk) += Q dS^T
+          const int add = dk.packed ? (r > 0 || i0 > 0) : (g->accumulate || r > 0 || i0 > 0);
+          if (int s = product(0, 1, hs, tk, n, q.p + (u0 * group + r) * q.stride + i0 * q.ld, q.ld, group * q.stride, dp + r * ms,
+                              sc.ld, group * ms, dk.p + u0 * dk.stride, dk.ld, dk.stride, nu, add))
+            return s;
+        }
+        if (want_dq)  // dQ (hs x n) = K dS
+          if (int s = product(0, 0, hs, n, tk, k.p + u0 * k.stride, k.ld, k.stride, dp + r * ms, sc.ld, group * ms,
+                              dq.p + (u0 * group + r) * dq.stride + i0 * dq.ld, dq.ld, group * dq.stride, nu,
+                              dq.packed ? 0 : g->accumulate))
+            return s;
+      }
+    }
+  }
+  if (!g) return rel_finish_out(stream, dtype, o, a.o, so, hs, tq, a.heads, a.batch, 0);
+  if (want_dq)
+    if (int s = rel_finish_out(stream, dtype, dq, g->dq, sdq, hs, tq, a.heads, a.batch, g->accumulate)) return s;
+  if (want_dk)
+    if (int s = rel_finish_out(stream, dtype, dk, g->dk, sdk, hs, tk, kv, a.batch, g->accumulate)) return s;
+  if (want_dv)
+    if (int s = rel_finish_out(stream, dtype, dv, g->dv, sdv, hs, tk, kv, a.batch, g->accumulate)) return s;
+  if (want_dt) {
+    CU_TRY(gb::launch_rel_table_grad(dtype, sc, diagonal, (int)qblocks, a.heads * a.batch, a.map, (int)a.buckets,
+                                     (int)a.heads, g->accumulate, g->dtable, g->lddt, stream));
+    g_launches.fetch_add(1);
+  }
+  return GINN_B200_OK;
+}
+
+}  // namespace
+
+int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, const ginn_b200_relative_attention* a) {
+  if (int s = check_relative(dtype, a)) return s;
+  if (a->tq == 0 || a->heads == 0 || a->batch == 0) return GINN_B200_OK;
+  DevCtx* ctx;
+  if (int s = get_ctx(device, &ctx)) return s;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (a->tk == 0) {  // nothing to see for anyone
+    CU_TRY(gb::launch_rel_unpack(dtype, nullptr, (int)a->head_size, 0, (int)a->tq, (int)a->heads, (int)a->batch, 0, a->o, a->ldo,
+                                 a->stride_o_head, a->stride_o_batch, stream));
+    CU_TRY(gb::launch_fill(GINN_B200_F32, a->lse, a->tq * a->heads * a->batch, -INFINITY, ctx->num_sms, stream));
+    g_launches.fetch_add(2);
+    return GINN_B200_OK;
+  }
+  return relative_composed(device, stream, dtype, *a, nullptr);
+}
+
+int ginn_b200_relative_attention_backward(int device, void* stream_, int dtype, const ginn_b200_relative_attention* a,
+                                          const ginn_b200_relative_attention_grad* g) {
+  if (int s = check_relative(dtype, a)) return s;
+  if (!g) return fail(GINN_B200_BAD_ARGUMENT, "null gradient description");
+  if (g->dtable && !a->table) return fail(GINN_B200_BAD_ARGUMENT, "dtable without a bias table");
+  if (g->dtable && g->lddt < a->buckets)
+    return fail(GINN_B200_BAD_ARGUMENT, "leading dimension %lld of dtable is smaller than its %lld buckets", (long long)g->lddt,
+                (long long)a->buckets);
+  if (a->heads == 0 || !(g->dq || g->dk || g->dv || g->dtable)) return GINN_B200_OK;
+  const int64_t hs = a->head_size, tq = a->batch ? a->tq : 0, tk = a->batch ? a->tk : 0;
+  const bool none = tq == 0 || tk == 0;
+  if (!none)
+    if (int s = check_heads("d_o", g->d_o, {g->lddo, g->stride_do_head, g->stride_do_batch})) return s;
+  if (g->dq && tq)
+    if (int s = check_heads_out("dq", g->dq, {g->lddq, g->stride_dq_head, g->stride_dq_batch}, hs, tq, a->heads, a->batch)) return s;
+  if (g->dk && tk)
+    if (int s = check_heads_out("dk", g->dk, {g->lddk, g->stride_dk_head, g->stride_dk_batch}, hs, tk, a->kv_heads, a->batch)) return s;
+  if (g->dv && tk)
+    if (int s = check_heads_out("dv", g->dv, {g->lddv, g->stride_dv_head, g->stride_dv_batch}, hs, tk, a->kv_heads, a->batch)) return s;
+  if (none && g->accumulate) return GINN_B200_OK;
+  DevCtx* ctx;
+  if (int s = get_ctx(device, &ctx)) return s;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (!none) return relative_composed(device, stream, dtype, *a, g);
+  // no pairs: the results that exist are zero
+  if (g->dq && tq)
+    CU_TRY(gb::launch_rel_unpack(dtype, nullptr, (int)hs, 0, (int)tq, (int)a->heads, (int)a->batch, 0, g->dq, g->lddq,
+                                 g->stride_dq_head, g->stride_dq_batch, stream));
+  if (g->dk && tk)
+    CU_TRY(gb::launch_rel_unpack(dtype, nullptr, (int)hs, 0, (int)tk, (int)a->kv_heads, (int)a->batch, 0, g->dk, g->lddk,
+                                 g->stride_dk_head, g->stride_dk_batch, stream));
+  if (g->dv && tk)
+    CU_TRY(gb::launch_rel_unpack(dtype, nullptr, (int)hs, 0, (int)tk, (int)a->kv_heads, (int)a->batch, 0, g->dv, g->lddv,
+                                 g->stride_dv_head, g->stride_dv_batch, stream));
+  if (g->dtable)
+    CU_TRY(gb::launch_rel_table_grad(dtype, gb::RelScores(), nullptr, 0, 0, a->map, (int)a->buckets, (int)a->heads, 0, g->dtable,
+                                     g->lddt, stream));
+  g_launches.fetch_add((g->dq && tq) + (g->dk && tk) + (g->dv && tk) + (g->dtable != nullptr));
+  return GINN_B200_OK;
+}
+
+namespace {
+// Natural numbers as 32-bit digits, lowest first: just enough to compare products of powers.
+using Digits = std::vector<uint32_t>;
+void times(Digits* n, uint32_t f) {
+  uint64_t carry = 0;
+  for (uint32_t& d : *n) {
+    carry += static_cast<uint64_t>(d) * f;
+    d = static_cast<uint32_t>(carry);
+    carry >>= 32;
+  }
+  if (carry) n->push_back(static_cast<uint32_t>(carry));
+}
+bool not_above(const Digits& a, const Digits& b) {
+  if (a.size() != b.size()) return a.size() < b.size();
+  for (size_t i = a.size(); i-- > 0;)
+    if (a[i] != b[i]) return a[i] < b[i];
+  return true;
+}
+}  // namespace
+
+int ginn_b200_relative_buckets(int buckets, int max_distance, int bidirectional, int64_t reach, int* map) {
+  if (buckets < (bidirectional ? 4 : 2) || buckets > 512)
+    return fail(GINN_B200_BAD_ARGUMENT, "%d buckets: 2 .. 512 (4 at least when bidirectional)", buckets);
+  if (max_distance < 1 || max_distance > (1 << 20))
+    return fail(GINN_B200_BAD_ARGUMENT, "max_distance %d is not in 1..2^20", max_distance);
+  if (reach < 0 || reach > (1 << 24)) return fail(GINN_B200_BAD_ARGUMENT, "reach %lld is not in 0..2^24", (long long)reach);
+  if (!map) return fail(GINN_B200_BAD_ARGUMENT, "null map");
+  const int side = bidirectional ? buckets / 2 : buckets;  // buckets of one direction
+  try {
+    const int near = side / 2, steps = side - near;
+    // first[e]: smallest distance >= near in logarithmic bucket e, the smallest d with
+    //   max_distance^e near^(steps - e) <= d^steps;  found near its floating-point value, decided exactly
+    std::vector<int64_t> first(steps, near);
+    for (int e = 1; e < steps; ++e) {
+      Digits limit(1, 1);
+      for (int i = 0; i < e; ++i) times(&limit, static_cast<uint32_t>(max_distance));
+      for (int i = e; i < steps; ++i) times(&limit, static_cast<uint32_t>(near));
+      auto reaches = [&](int64_t d) {
+        Digits p(1, 1);
+        for (int i = 0; i < steps; ++i) times(&p, static_cast<uint32_t>(d));
+        return not_above(limit, p);
+      };
+      const double guess = near * std::pow(static_cast<double>(max_distance) / near, static_cast<double>(e) / steps);
+      int64_t d = static_cast<int64_t>(guess);
+      d = d < near ? near : d;
+      while (d > near && reaches(d - 1)) --d;
+      while (!reaches(d)) ++d;
+      first[e] = d;
+    }
+    for (int64_t at = 0; at <= 2 * reach; ++at) {
+      const int64_t rel = at - reach;
+      int base = 0;
+      int64_t d = rel < 0 ? -rel : rel;
+      if (bidirectional) {
+        if (rel > 0) base = side;
+      } else if (rel > 0) {
+        d = 0;
+      }
+      int b = static_cast<int>(d);
+      if (d >= near) {
+        int e = static_cast<int>(std::upper_bound(first.begin(), first.end(), d) - first.begin()) - 1;
+        b = near + e;
+      }
+      map[at] = base + b;
+    }
+  } catch (const std::bad_alloc&) {  // nothing may leave a C entry point but a status
+    return fail(GINN_B200_CUDA_ERROR, "out of host memory");
+  }
+  return GINN_B200_OK;
 }
 
 int ginn_b200_fill(int device, void* stream, int dtype, int64_t n, void* x, float value) {

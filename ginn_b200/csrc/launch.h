@@ -5,6 +5,7 @@
 #include <stddef.h>
 #include "problem.h"
 #include "dropout.cuh"
+#include "relative_attention.cuh"
 
 struct CUtensorMap_st;  // CUDA driver tensor-map descriptor (cuda.h)
 
@@ -190,6 +191,32 @@ cudaError_t launch_norm_backward(int dtype, const NormGradArgs& a, int parts, fl
 cudaError_t launch_dropout(int dtype, const void* x, long long ldx, const void* add, long long lda,
                            void* y, long long ldy, long long rows, long long cols,
                            const Dropout& drop, int num_sms, cudaStream_t stream);
+
+// --- attention with a relative position bias: passes of the composed path (relative_attention.cu) ---
+// out[head][reach + d] = factor * table[map[reach + d], head] (0 where the bucket does not exist).
+cudaError_t launch_rel_bias_expand(int dtype, const void* table, long long ldt, const int* map,
+                                   int buckets, long long reach, int heads, float factor, float* out,
+                                   cudaStream_t stream);
+// dst[b][head][t][hsp] = src(h, t, head, b) in fp32, zero behind hs and behind the lengths.
+cudaError_t launch_rel_pack(int dtype, const void* src, long long ld, long long sh, long long sb,
+                            int hs, int hsp, int t_len, int heads, int batch, const int* lengths,
+                            float* dst, cudaStream_t stream);
+cudaError_t launch_rel_unpack(int dtype, const float* src, int hs, int hsp, int t_len, int heads,
+                              int batch, int accumulate, void* dst, long long ld, long long sh,
+                              long long sb, cudaStream_t stream);
+// Scores to probabilities in place; lse_in null: the statistics are formed and written to lse_out.
+cudaError_t launch_rel_softmax(const RelScores& s, const float* bias, const float* lse_in,
+                               float* lse_out, cudaStream_t stream);
+// dp = factor * p (.) (dp - colsum(p (.) dp)).
+cudaError_t launch_rel_softmax_grad(const RelScores& s, const float* p, float* dp, float factor,
+                                    cudaStream_t stream);
+// Diagonal sums of ds per block of kRelDiagonal queries: out[matrix][block][tq + tk - 1]; ds is left
+// multiplied by `factor`.
+cudaError_t launch_rel_diagonal(const RelScores& s, float* ds, float factor, float* out, int blocks,
+                                cudaStream_t stream);
+cudaError_t launch_rel_table_grad(int dtype, const RelScores& s, const float* diagonal, int blocks,
+                                  long long matrices, const int* map, int buckets, int heads,
+                                  int accumulate, void* dtable, long long lddt, cudaStream_t stream);
 
 // --- Conv2d as patch extraction + matrix products (conv.cu) ---
 struct ConvShape {

@@ -1,0 +1,57 @@
+// Shared description of attention with a relative position bias: which pairs of query and key
+// take part, and at which distance.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace gb {
+
+constexpr int kRelDiagonal = 256;  // queries whose diagonal sums are formed together
+
+// Scores of `matrices` (sequence, head) pairs from pair number `matrix0` on, queries q0 .. q0 + nq - 1
+// of tq: s[matrix][query][ld], keys contiguous.
+struct RelScores {
+  float* s = nullptr;
+  long long ld = 0, matrices = 0, matrix0 = 0;
+  int nq = 0, q0 = 0, tq = 0, tk = 0, heads = 1;
+  float scale = 1.f;
+  int causal = 0;
+  long long q_offset = 0;           // position of query 0, in keys
+  const int* q_offsets = nullptr;   // per sequence instead
+  const int* q_lengths = nullptr;   // queries / keys behind these take no part
+  const int* k_lengths = nullptr;
+  long long reach = 0;
+};
+
+__device__ __forceinline__ int rel_length(const int* lengths, int batch, int t) {
+  if (lengths == nullptr) return t;
+  const int n = lengths[batch];
+  return n < 0 ? 0 : n < t ? n : t;
+}
+__device__ __forceinline__ long long rel_offset(long long offset, const int* offsets, int batch) {
+  return offsets != nullptr ? offsets[batch] : offset;
+}
+// Number of keys 0 .. n - 1 the query at position `pos` sees.
+__device__ __forceinline__ int rel_visible(int causal, long long pos, int klen) {
+  if (!causal || pos >= klen - 1) return klen;
+  return pos < 0 ? 0 : static_cast<int>(pos) + 1;
+}
+
+// The query of score column `col` of a RelScores.
+struct RelQuery {
+  long long matrix, local;  // within the scores of this call
+  int batch, head, query, visible;
+  long long pos;            // its position in keys
+  __device__ __forceinline__ RelQuery(const RelScores& s, long long col) {
+    matrix = col / s.nq;
+    local = col - matrix * s.nq;
+    query = s.q0 + static_cast<int>(local);
+    batch = static_cast<int>((s.matrix0 + matrix) / s.heads);
+    head = static_cast<int>((s.matrix0 + matrix) % s.heads);
+    pos = query + rel_offset(s.q_offset, s.q_offsets, batch);
+    const int klen = rel_length(s.k_lengths, batch, s.tk);
+    visible = query < rel_length(s.q_lengths, batch, s.tq) ? rel_visible(s.causal, pos, klen) : 0;
+  }
+};
+
+}  // namespace gb

@@ -342,6 +342,84 @@ int ginn_b200_attention_backward(int device, void* stream, int dtype, int64_t t,
                                  int64_t ldp, int64_t stride_p, const void* d_o, int64_t ldo,
                                  int64_t stride_o, void* ds, void* dk, void* dq, void* dv);
 
+/* ---- Attention with a learned relative position bias ----------------------------------------- */
+
+/* Operands of attention over `batch` sequences of tq queries and tk keys.  Element (h, t, head, b)
+ * of q, k, v, o lies at base + h + t * ld + head * stride_head + b * stride_batch: the heads of one
+ * packed projection, heads as matrices of their own, or any other order.  `heads` query heads share
+ * `kv_heads` key / value heads (heads % kv_heads == 0; head n reads kv head n * kv_heads / heads).
+ *
+ *   s[j, i] = scale * k_j . q_i + table[map[reach + d], head],   d = clamp(j - (i + offset), -reach, reach)
+ *   p[:, i] = softmax of s[:, i] over the keys query i sees,   o_i = sum_j p[j, i] v_j,
+ *   lse[i] = log sum_j exp s[j, i]
+ *
+ * Query i sees key j when j < k_lengths[b], with `causal` also j <= i + offset, and i < q_lengths[b].
+ * A query that sees nothing gives o = 0 and lse = -inf.  What k, v, q and d_o hold behind the lengths
+ * is not looked at (NaN included); o and the gradients are zero there.
+ *   table      buckets x heads of type `dtype`, leading dimension ldt; NULL = no bias
+ *   map        2 * reach + 1 ints on the device: bucket of distance -reach .. reach (see
+ *              ginn_b200_relative_buckets); an entry outside [0, buckets) gives no bias
+ *   offset     position of query 0 among the keys: q_offset, or per sequence q_offsets[b] (device
+ *              ints, within +-2^30) when that is not NULL
+ *   *_lengths  device ints, one per sequence, NULL = all of tq / tk; clamped to the tensor
+ *   lse        tq x heads x batch floats, dense (i + tq * (head + heads * b)); the backward pass reads it
+ * head_size 1 .. 256; tq, tk < 2^29. */
+typedef struct {
+  int64_t tq, tk, head_size, heads, kv_heads, batch;
+  const void* q;
+  int64_t ldq, stride_q_head, stride_q_batch;
+  const void* k;
+  int64_t ldk, stride_k_head, stride_k_batch;
+  const void* v;
+  int64_t ldv, stride_v_head, stride_v_batch;
+  const void* table;
+  int64_t ldt, buckets;
+  const int* map;
+  int64_t reach;
+  float scale;
+  int causal;
+  int64_t q_offset;
+  const int* q_offsets;
+  const int* q_lengths;
+  const int* k_lengths;
+  void* o;
+  int64_t ldo, stride_o_head, stride_o_batch;
+  float* lse;
+} ginn_b200_relative_attention;
+
+/* Upstream gradient and results of the backward pass; each result may be NULL.  `+=` when accumulate
+ * != 0, `=` otherwise.  dk and dv are summed over the query heads that share them; dtable (buckets x
+ * heads, type `dtype`) over all sequences, in a fixed order. */
+typedef struct {
+  const void* d_o;
+  int64_t lddo, stride_do_head, stride_do_batch;
+  void* dq;
+  int64_t lddq, stride_dq_head, stride_dq_batch;
+  void* dk;
+  int64_t lddk, stride_dk_head, stride_dk_batch;
+  void* dv;
+  int64_t lddv, stride_dv_head, stride_dv_batch;
+  void* dtable;
+  int64_t lddt;
+  int accumulate;
+} ginn_b200_relative_attention_grad;
+
+int ginn_b200_relative_attention_forward(int device, void* stream, int dtype,
+                                         const ginn_b200_relative_attention* a);
+/* Reads a->o and a->lse of the forward call with the same operands. */
+int ginn_b200_relative_attention_backward(int device, void* stream, int dtype,
+                                          const ginn_b200_relative_attention* a,
+                                          const ginn_b200_relative_attention_grad* g);
+
+/* Host helper (no GPU work): map[reach + d] = bucket of distance d = key - query for |d| <= reach, on
+ * the usual scheme: half of the buckets (of each direction, when bidirectional; keys ahead of the
+ * query take the upper half of the numbers) one to a distance, the others logarithmic from there up to
+ * max_distance.  Without `bidirectional` keys ahead of the query share bucket 0.  Borders are decided
+ * in whole numbers.  buckets 2 .. 512 (>= 4 when bidirectional), max_distance 1 .. 2^20,
+ * reach 0 .. 2^24. */
+int ginn_b200_relative_buckets(int buckets, int max_distance, int bidirectional, int64_t reach,
+                               int* map);
+
 /* ---- Layer normalisation and dropout -------------------------------------------------------- */
 
 /* Normalisation of every column of x (rows x cols), the work of ginn's LayerNorm node

@@ -230,6 +230,73 @@ def attention_backward(k, q, v, p, d_o, scale=1.0):
     return dk.astype(dt), dq.astype(dt), dv.astype(dt)
 
 
+def relative_bucket(d: int, buckets: int, max_distance: int, bidirectional: bool) -> int:
+    """Bucket of distance d = key - query: half of the buckets of a direction one to a distance, the
+    rest logarithmic up to max_distance, borders compared as whole numbers."""
+    base = 0
+    if bidirectional:
+        buckets //= 2
+        base, d = (buckets if d > 0 else 0), abs(d)
+    else:
+        d = max(-d, 0)
+    near = buckets // 2
+    if d < near:
+        return base + d
+    steps, e = buckets - near, 0
+    while e + 1 < steps and max_distance ** (e + 1) * near ** (steps - e - 1) <= d ** steps:
+        e += 1
+    return base + near + e
+
+
+def relative_attention(q, k, v, table, bmap, scale, causal=False, offsets=None, q_lengths=None,
+                       k_lengths=None, d_o=None):
+    """Attention with a relative position bias over (head size, time, heads, batch) arrays: o and lse
+    (batch, heads, tq); with d_o also dq, dk, dv, dtable.  Pairs behind the lengths take no part;
+    offsets: position of query 0 per sequence."""
+    q, k, v = f64(q), f64(k), f64(v)
+    hs, tq, heads, batch = q.shape
+    tk, kv = k.shape[1], k.shape[2]
+    group, reach = heads // kv, len(bmap) // 2
+    o, lse = np.zeros(q.shape), np.full((batch, heads, tq), -np.inf)
+    out = {"dq": np.zeros(q.shape), "dk": np.zeros(k.shape), "dv": np.zeros(k.shape),
+           "dtable": None if table is None else np.zeros(np.shape(table))}
+    for b in range(batch):
+        nq = tq if q_lengths is None else max(0, min(tq, int(q_lengths[b])))
+        nk = tk if k_lengths is None else max(0, min(tk, int(k_lengths[b])))
+        if nq == 0 or nk == 0:
+            continue
+        off = 0 if offsets is None else int(offsets[b])
+        d = np.arange(nk)[:, None] - (np.arange(nq)[None] + off)
+        kind = np.asarray(bmap)[np.clip(d, -reach, reach) + reach]
+        ok = (kind >= 0) & (kind < (0 if table is None else len(table)))
+        for h in range(heads):
+            K, V, Q = k[:, :nk, h // group, b], v[:, :nk, h // group, b], q[:, :nq, h, b]
+            s = scale * (K.T @ Q)
+            if table is not None:
+                s = s + np.where(ok, f64(table)[np.where(ok, kind, 0), h], 0.0)
+            if causal:
+                s = np.where(d <= 0, s, -np.inf)
+            m = s.max(0)
+            m = np.where(np.isfinite(m), m, 0.0)
+            e = np.exp(s - m)
+            z = e.sum(0)
+            p = np.divide(e, z, out=np.zeros_like(e), where=z > 0)
+            with np.errstate(divide="ignore"):
+                lse[b, h, :nq] = np.log(z) + m
+            o[:, :nq, h, b] = V @ p
+            if d_o is None:
+                continue
+            g = f64(d_o)[:, :nq, h, b]
+            dp = V.T @ g
+            ds = p * (dp - (p * dp).sum(0))
+            out["dq"][:, :nq, h, b] = scale * (K @ ds)
+            out["dk"][:, :nk, h // group, b] += scale * (Q @ ds.T)
+            out["dv"][:, :nk, h // group, b] += g @ p.T
+            if table is not None:
+                np.add.at(out["dtable"][:, h], kind[ok], ds[ok])
+    return {"o": o, "lse": lse, **(out if d_o is not None else {})}
+
+
 def philox4x32(counter, key, rounds: int = 10):
     """Philox4x32 (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3", SC 2011): counter
     (4, n) and key (2,) of 32-bit words -> (4, n) output words."""

@@ -1,4 +1,5 @@
-"""What the transformer-block operators (layer norm, dropout, residual norm) promise without a GPU: the
+"""What the transformer-block operators (layer norm, dropout, residual norm,
+attention with a relative position bias) promise without a GPU: the
 oracle's formulas against differences and published numbers, and the refusals of the C ABI, which
 come before any GPU call."""
 import numpy as np
@@ -99,3 +100,90 @@ def test_refused_probabilities(p):
 def test_empty_matrices_need_no_gpu():
     assert norm_fwd(rows=0) == 0 and norm_fwd(cols=0) == 0 and norm_bwd(cols=0) == 0
     assert B.lib().ginn_b200_dropout_forward(0, None, 0, 0, 4, None, 8, None, 0, drop(), None, 8) == 0
+
+
+# ---- attention with a relative position bias ----
+
+@pytest.mark.parametrize("causal,lengths", [(False, None), (True, None), (True, ([3, 0, 5], [2, 4, 6]))])
+def test_relative_attention_gradient_against_differences(causal, lengths):
+    rng = np.random.default_rng(3)
+    q, k, v = rng.standard_normal((4, 5, 4, 3)), rng.standard_normal((4, 6, 2, 3)), rng.standard_normal((4, 6, 2, 3))
+    table, d_o = rng.standard_normal((6, 4)), rng.standard_normal(q.shape)
+    bmap = [orc.relative_bucket(d, 6, 4, True) for d in range(-4, 5)]
+    kw = dict(scale=0.7, causal=causal, offsets=[1, -2, 0])
+    if lengths:
+        kw |= dict(q_lengths=lengths[0], k_lengths=lengths[1])
+    got = orc.relative_attention(q, k, v, table, bmap, d_o=d_o, **kw)
+    at = {"dq": q, "dk": k, "dv": v, "dtable": table}
+    e = 1e-6
+    for name, x in at.items():
+        for i in list(np.ndindex(x.shape))[::7]:
+            old, x[i] = x[i], x[i] + e
+            hi = (orc.relative_attention(q, k, v, table, bmap, **kw)["o"] * d_o).sum()
+            x[i] = old - e
+            lo = (orc.relative_attention(q, k, v, table, bmap, **kw)["o"] * d_o).sum()
+            x[i] = old
+            # central difference: truncation of order e^2, rounding 2^-52 * |loss| / e
+            assert abs(got[name][i] - (hi - lo) / (2 * e)) < 1e-7, (name, i)
+
+
+@pytest.mark.parametrize("buckets,max_distance,both,reach", [
+    (32, 128, True, 300), (32, 128, False, 300), (2, 1, False, 5), (4, 7, True, 20), (65, 32, True, 40), (65, 32, False, 40),
+    (16, 3, True, 30), (40, 1000, False, 1200), (64, 4096, True, 5000), (12, 729, False, 800), (32, 128, True, 0), (512, 1 << 20, False, 3000),
+])
+def test_relative_buckets(buckets, max_distance, both, reach):
+    """Against the definition in Python's whole numbers; (12, 729) has borders that are distances
+    exactly, where a logarithm in floating point may fall on either side."""
+    got = B.relative_buckets(buckets, max_distance, both, reach).tolist()
+    step = 1 if buckets < 512 else 97
+    for at in range(0, 2 * reach + 1, step):
+        assert got[at] == orc.relative_bucket(at - reach, buckets, max_distance, both), at - reach
+
+
+@pytest.mark.parametrize("args", [(1, 8, 0, 4), (3, 8, 1, 4), (513, 8, 0, 4), (8, 0, 0, 4), (8, (1 << 20) + 1, 0, 4), (8, 8, 0, -1), (8, 8, 0, (1 << 24) + 1)])
+def test_refused_bucket_maps(args):
+    out = np.zeros(16, np.int32)
+    assert B.lib().ginn_b200_relative_buckets(*args, out.ctypes.data) == BAD
+    assert (out == 0).all()
+
+
+def described(**change):
+    """A valid description of 3 sequences, 4 heads over 2, 5 queries, 6 keys of size 8, changed."""
+    d = dict(tq=5, tk=6, head_size=8, heads=4, kv_heads=2, batch=3, q=P, ldq=8, stride_q_head=40, stride_q_batch=160, k=P, ldk=8,
+             stride_k_head=48, stride_k_batch=96, v=P, ldv=8, stride_v_head=48, stride_v_batch=96, table=P, ldt=32, buckets=32, map=P,
+             reach=16, scale=1.0, causal=0, q_offset=0, o=P, ldo=8, stride_o_head=40, stride_o_batch=160, lse=P)
+    return B._RelativeAttention(**{**d, **change})
+
+
+def forward(dtype=0, **change):
+    import ctypes
+    return B.lib().ginn_b200_relative_attention_forward(0, None, dtype, ctypes.byref(described(**change)))
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(dtype=3), UNSUPPORTED), (dict(tq=-1), BAD), (dict(tk=1 << 29), BAD), (dict(heads=65536), BAD), (dict(head_size=0), UNSUPPORTED),
+    (dict(head_size=257), UNSUPPORTED), (dict(kv_heads=3), BAD), (dict(kv_heads=0), BAD), (dict(scale=float("inf")), BAD),
+    (dict(scale=float("nan")), BAD), (dict(q_offset=1 << 31), BAD), (dict(buckets=0), BAD), (dict(ldt=31), BAD), (dict(map=None), BAD),
+    (dict(reach=-1), BAD), (dict(q=None), BAD), (dict(k=None), BAD), (dict(v=None), BAD), (dict(o=None), BAD), (dict(lse=None), BAD),
+    (dict(ldq=-8), BAD), (dict(ldo=7), BAD), (dict(stride_o_head=39), BAD), (dict(stride_o_batch=0), BAD), (dict(batch=1 << 20, heads=1 << 12, kv_heads=1), BAD),
+])
+def test_refused_attention(change, status):
+    assert forward(**change) == status
+    assert B.lib().ginn_b200_last_error()
+
+
+@pytest.mark.parametrize("change,grad", [
+    ({}, dict(d_o=None)), (dict(table=None), dict(dtable=P, lddt=32)), ({}, dict(dtable=P, lddt=31)), ({}, dict(dk=P, lddk=8, stride_dk_head=47)),
+    ({}, dict(lddo=-1)),
+])
+def test_refused_attention_gradient(change, grad):
+    import ctypes
+    g = dict(d_o=P, lddo=8, stride_do_head=40, stride_do_batch=160, dq=P, lddq=8, stride_dq_head=40, stride_dq_batch=160)
+    call = lambda g: B.lib().ginn_b200_relative_attention_backward(  # noqa: E731
+        0, None, 0, ctypes.byref(described(**change)), None if g is None else ctypes.byref(B._RelativeAttentionGrad(**g)))
+    assert call({**g, **grad}) == BAD
+    assert call(None) == BAD
+
+
+def test_attention_without_queries_needs_no_gpu():
+    assert forward(tq=0) == 0 and forward(batch=0) == 0
