@@ -14,7 +14,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libginn_b200.so")
-SOURCES = ["api.cu", "grouped_static.cu", "hgemm_tma.cu", "hgemm_pair.cu", "hgemm_gather.cu", "sgemm3x_tma.cu", "small.cu", "step_ops.cu", "conv.cu", "attention.cu", "norm_ops.cu", "relative_attention.cu"]
+SOURCES = ["api.cu", "grouped_static.cu", "hgemm_tma.cu", "hgemm_pair.cu", "hgemm_gather.cu", "sgemm3x_tma.cu", "small.cu", "step_ops.cu", "conv.cu", "attention.cu", "norm_ops.cu", "relative_attention.cu", "flash_attention.cu"]
 HEADERS = ["ptx.cuh", "math.cuh", "problem.h", "launch.h", "dropout.cuh", "relative_attention.cuh", os.path.join("..", "..", "include", "ginn_b200.h")]
 
 

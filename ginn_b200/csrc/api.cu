@@ -2071,6 +2071,35 @@ int relative_composed(int device, cudaStream_t stream, int dtype, const ginn_b20
 
 }  // namespace
 
+namespace {
+gb::FlashArgs flash_args(const ginn_b200_relative_attention& a) {
+  gb::FlashArgs f = {};
+  f.q = {a.q, a.ldq, a.stride_q_head, a.stride_q_batch};
+  f.k = {a.k, a.ldk, a.stride_k_head, a.stride_k_batch};
+  f.v = {a.v, a.ldv, a.stride_v_head, a.stride_v_batch};
+  f.o = {a.o, a.ldo, a.stride_o_head, a.stride_o_batch};
+  f.lse = a.lse;
+  f.tq = (int)a.tq; f.tk = (int)a.tk; f.hs = (int)a.head_size; f.heads = (int)a.heads; f.kv_heads = (int)a.kv_heads;
+  f.batch = (int)a.batch;
+  f.reach = a.table ? a.reach : 0;
+  f.q_offset = a.q_offset; f.q_offsets = a.q_offsets; f.q_lengths = a.q_lengths; f.k_lengths = a.k_lengths;
+  f.scale = a.scale;
+  f.causal = a.causal ? 1 : 0;
+  return f;
+}
+// Bias of every distance and head, times log2(e), for the flash kernels.
+int flash_bias(Scratch* scratch, int dtype, const ginn_b200_relative_attention& a, gb::FlashArgs* f) {
+  if (!a.table) return GINN_B200_OK;
+  float* bias;
+  CU_TRY(scratch->take(&bias, (2 * a.reach + 1) * a.heads));
+  CU_TRY(gb::launch_rel_bias_expand(dtype, a.table, a.ldt, a.map, (int)a.buckets, a.reach, (int)a.heads, 1.44269504f, bias,
+                                    scratch->stream));
+  g_launches.fetch_add(1);
+  f->bias = bias;
+  return GINN_B200_OK;
+}
+}  // namespace
+
 int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, const ginn_b200_relative_attention* a) {
   if (int s = check_relative(dtype, a)) return s;
   if (a->tq == 0 || a->heads == 0 || a->batch == 0) return GINN_B200_OK;
@@ -2082,6 +2111,14 @@ int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, c
                                  a->stride_o_head, a->stride_o_batch, stream));
     CU_TRY(gb::launch_fill(GINN_B200_F32, a->lse, a->tq * a->heads * a->batch, -INFINITY, ctx->num_sms, stream));
     g_launches.fetch_add(2);
+    return GINN_B200_OK;
+  }
+  gb::FlashArgs f = flash_args(*a);
+  if (dtype == GINN_B200_F16 && t_force_path == PATH_AUTO && gb::flash_supported(f)) {
+    Scratch scratch(stream);
+    if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
+    CU_TRY(gb::launch_flash_forward(f, stream, ctx->d_status));
+    g_launches.fetch_add(1);
     return GINN_B200_OK;
   }
   return relative_composed(device, stream, dtype, *a, nullptr);

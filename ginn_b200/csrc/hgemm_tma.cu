@@ -415,6 +415,24 @@ bool encode_tmap(CUtensorMap* out, int esize, const void* ptr, unsigned long lon
   return true;
 }
 
+bool encode_heads_tmap(CUtensorMap* out, const void* ptr, int hs, long long t, long long heads, long long batch,
+                       long long ld, long long sh, long long sb, int box_rows) {
+  EncodeFn enc = get_encode();
+  if (!enc) return false;
+  // strides of dimensions with one entry are never used, but have to be well formed
+  const long long s1 = t > 1 ? ld : (hs + 7) / 8 * 8;
+  const long long s2 = heads > 1 ? sh : s1 * t;
+  const long long s3 = batch > 1 ? sb : s2 * heads;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(hs), static_cast<cuuint64_t>(t), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(batch)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(s1) * 2, static_cast<cuuint64_t>(s2) * 2,
+                                 static_cast<cuuint64_t>(s3) * 2};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1}, estr[4] = {1, 1, 1, 1};
+  return enc(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool tmap_encoder_available() { return get_encode() != nullptr; }
 
 namespace {

@@ -94,6 +94,10 @@ cudaError_t launch_hgemm_gather_grouped(const Problem* dprobs, int nprobs, int t
 bool encode_tmap(::CUtensorMap_st* out, int esize, const void* ptr, unsigned long long d0,
                  unsigned long long d1, unsigned long long d2, unsigned long long ld,
                  unsigned long long batch_stride, unsigned b0, unsigned b1, bool swizzle128);
+// Half attention operand (head size, time, heads, batch): boxes of 64 head elements x box_rows
+// positions of one head, 128-byte swizzle, zero outside.
+bool encode_heads_tmap(::CUtensorMap_st* out, const void* ptr, int hs, long long t, long long heads,
+                       long long batch, long long ld, long long sh, long long sb, int box_rows);
 bool tmap_encoder_available();
 
 // --- TMA-fed fp32 (3xTF32) kernel (sgemm3x_tma.cu) ---
@@ -217,6 +221,28 @@ cudaError_t launch_rel_diagonal(const RelScores& s, float* ds, float factor, flo
 cudaError_t launch_rel_table_grad(int dtype, const RelScores& s, const float* diagonal, int blocks,
                                   long long matrices, const int* map, int buckets, int heads,
                                   int accumulate, void* dtable, long long lddt, cudaStream_t stream);
+
+// --- the same attention without the scores in memory, fp16 (flash_attention.cu) ---
+struct FlashOperand {
+  const void* p;
+  long long ld, head, batch;
+};
+struct FlashArgs {
+  FlashOperand q, k, v, o;
+  float* lse;
+  const float* bias;  // [head][2 * reach + 1], times log2(e); null = none
+  int tq, tk, hs, heads, kv_heads, batch;
+  long long reach, q_offset;
+  const int* q_offsets;
+  const int* q_lengths;
+  const int* k_lengths;
+  float scale;
+  int causal;
+};
+// True when the operands can be described by tensor maps: fp16, head size a multiple of 8 up to
+// 128, 16-byte aligned bases and strides.
+bool flash_supported(const FlashArgs& a);
+cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* status);
 
 // --- Conv2d as patch extraction + matrix products (conv.cu) ---
 struct ConvShape {
