@@ -2147,7 +2147,37 @@ int ginn_b200_relative_attention_backward(int device, void* stream_, int dtype, 
   DevCtx* ctx;
   if (int s = get_ctx(device, &ctx)) return s;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  if (!none) return relative_composed(device, stream, dtype, *a, g);
+  if (!none) {
+    gb::FlashArgs f = flash_args(*a);
+    gb::FlashGradArgs fg = {};
+    fg.d_o = {g->d_o, g->lddo, g->stride_do_head, g->stride_do_batch};
+    fg.dq = {g->dq, g->lddq, g->stride_dq_head, g->stride_dq_batch};
+    fg.dk = {g->dk, g->lddk, g->stride_dk_head, g->stride_dk_batch};
+    fg.dv = {g->dv, g->lddv, g->stride_dv_head, g->stride_dv_batch};
+    fg.dtable = g->dtable;
+    fg.lddt = g->lddt;
+    fg.map = a->map;
+    fg.buckets = (int)a->buckets;
+    fg.accumulate = g->accumulate ? 1 : 0;
+    if (dtype != GINN_B200_F16 || t_force_path != PATH_AUTO || !gb::flash_backward_supported(f, fg))
+      return relative_composed(device, stream, dtype, *a, g);
+    Scratch scratch(stream);
+    if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
+    const gb::FlashScratch need = gb::flash_backward_scratch(f, g->dtable != nullptr);
+    float *stats, *norms, *dist = nullptr, *sums = nullptr;
+    CU_TRY(scratch.take(&stats, need.stats));
+    CU_TRY(scratch.take(&norms, need.norms));
+    if (g->dtable) {
+      CU_TRY(scratch.take(&dist, need.dist));
+      CU_TRY(scratch.take(&sums, need.sums));
+    }
+    int launches = 0;
+    const cudaError_t e = gb::launch_flash_backward(f, fg, stats, norms, dist, sums, &launches, stream, ctx->d_status);
+    g_launches.fetch_add(launches);
+    if (e != cudaSuccess)
+      return fail(GINN_B200_CUDA_ERROR, "attention backward launch failed: %s", cudaGetErrorString(e));
+    return GINN_B200_OK;
+  }
   // no pairs: the results that exist are zero
   if (g->dq && tq)
     CU_TRY(gb::launch_rel_unpack(dtype, nullptr, (int)hs, 0, (int)tq, (int)a->heads, (int)a->batch, 0, g->dq, g->lddq,

@@ -395,6 +395,539 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
   }
 }
 
+// ---- backward -----------------------------------------------------------------------------------
+//
+// Two kernels of one shape: a CTA keeps 128 rows of two operands (A1, A2) in shared memory, streams
+// tiles of 64 rows of two others (B1, B2), and holds up to two results in tensor memory.
+//   rows = keys    : A1 = K, A2 = V, B1 = Q, B2 = dO;  X = K Q^T, Y = V dO^T;
+//                    dV += P dO,  dK += dS Q   (over all query heads that share the keys)
+//   rows = queries : A1 = Q, A2 = dO, B1 = K, B2 = V;  X = Q K^T, Y = dO V^T;  dQ += dS K,
+//                    and the sums of dS by distance for the bias table
+// with P = exp(X - lse), dS = P (Y - delta).  X and Y are formed twice in all (seven products instead of
+// five), which keeps every sum inside one CTA: no atomics on dQ, the same bits every time.
+// Two groups of 128 threads (a thread per row) take the streamed tiles in turn; X and Y of the next
+// tile are formed while they work.  Tensor memory: per group X (64 columns) and Y (64), overwritten
+// by P and dS as fp16 left operands; the results behind them.
+//
+// Range: P enters its product times 2^12 (probabilities down to 2^-26 stay normal numbers).  dS
+// enters times a power of two that brings its bound 2 max|dO| max|v| (Cauchy-Schwarz, per sequence
+// and key head) to 2^14, so neither large nor small upstream gradients leave a Half's range.
+constexpr int BN = 64;             // rows of a streamed tile
+constexpr int BCHUNK = BN * 128;   // bytes of 64 rows x 64 halves
+constexpr int BSTAGES = 4;
+constexpr int kDistSmem = 1024;    // distances whose sums fit in shared memory (per group)
+
+struct FlashBwdParams {
+  CUtensorMap tmQ, tmK, tmV, tmDO;      // boxes of 128 rows
+  CUtensorMap tmQ64, tmK64, tmV64, tmDO64;
+  __half *dq, *dk, *dv;
+  long long lddq, shdq, sbdq, lddk, shdk, sbdk, lddv, shdv, sbdv;
+  const float2* stats;        // [batch][heads][tq_pad]: lse * log2(e) (+inf = empty), delta
+  const unsigned* norms;      // [2][batch][kv heads]: bits of max |dO|^2, max |v|^2
+  float* dist;                // [batch][heads][query tile][2][width] sums of dS by distance; null = not wanted
+  const float* bias;
+  int tq, tk, hs, heads, kv_heads, group, batch, tq_pad, row_tiles, width;
+  long long reach, q_offset;
+  const int* q_offsets;
+  const int* q_lengths;
+  const int* k_lengths;
+  float scale, c1;
+  int causal, accumulate;
+};
+
+__device__ __forceinline__ float ds_scale(const FlashBwdParams& p, int batch, int kv) {
+  const int at = batch * p.kv_heads + kv;
+  const float b = 2.f * sqrtf(__uint_as_float(p.norms[at])) * sqrtf(__uint_as_float(p.norms[p.batch * p.kv_heads + at]));
+  if (!(b > 1e-30f && b < 1e30f)) return 1.f;
+  return exp2f(floorf(14.f - log2f(b)));
+}
+// First distance (clamped to the reach) that query tile i0 .. i0 + 127 keeps a sum of.
+__device__ __forceinline__ long long dist_low(long long reach, long long off, int i0) {
+  const long long d = -(i0 + FT - 1 + off);
+  return d > reach ? reach : d > -reach ? d : -reach;
+}
+
+// delta and lse of every query, and the largest norms of dO and v rows per key head.  Sixteen threads
+// per row; a CTA takes 64 rows of one head, of dO (first `qparts` parts) or of v.
+__global__ void __launch_bounds__(256)
+flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long long sbdo, const __half* o, long long ldo,
+                     long long sho, long long sbo, const __half* v, long long ldv, long long shv, long long sbv,
+                     const float* __restrict__ lse, const FlashBwdParams p, float2* __restrict__ stats,
+                     unsigned* __restrict__ norms, int qparts, long long qblocks) {
+  __shared__ float red[16];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int sub = threadIdx.x & 15, row16 = threadIdx.x >> 4;
+  const bool queries = blockIdx.x < qblocks;
+  const long long at = queries ? blockIdx.x : blockIdx.x - qblocks;
+  const int parts = queries ? qparts : (p.tk + 63) / 64;
+  const int hb = static_cast<int>(at / parts), part = static_cast<int>(at % parts);
+  const int heads = queries ? p.heads : p.kv_heads;
+  const int batch = hb / heads, head = hb - batch * heads;
+  const int kv = queries ? head / p.group : head;
+  const int len = queries ? rel_length(p.q_lengths, batch, p.tq) : rel_length(p.k_lengths, batch, p.tk);
+  auto load = [&](const __half* x, float (&f)[8]) {
+    const uint4 w = *reinterpret_cast<const uint4*>(x);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
+      f[2 * e] = q.x;
+      f[2 * e + 1] = q.y;
+    }
+  };
+  float most = 0.f;
+  for (int k = 0; k < 4; ++k) {
+    const int i = part * 64 + k * 16 + row16;
+    const bool real = i < len && sub * 8 < p.hs;
+    float norm = 0.f, dot = 0.f;
+    if (real) {
+      float a[8];
+      load(queries ? d_o + i * lddo + head * shdo + batch * sbdo + sub * 8 : v + i * ldv + head * shv + batch * sbv + sub * 8, a);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) norm += a[e] * a[e];
+      if (queries) {
+        float b[8];
+        load(o + i * ldo + head * sho + batch * sbo + sub * 8, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot += a[e] * b[e];
+      }
+    }
+#pragma unroll
+    for (int s = 8; s > 0; s >>= 1) {
+      norm += __shfl_xor_sync(0xffffffffu, norm, s);
+      dot += __shfl_xor_sync(0xffffffffu, dot, s);
+    }
+    // a row that is not a number or infinite makes the bound so (the integer order puts both last)
+    most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(norm)));
+    if (queries && sub == 0 && i < p.tq_pad) {
+      const long long row = static_cast<long long>(hb) * p.tq + i;
+      float2 s = make_float2(INFINITY, 0.f);
+      if (i < len) {
+        const float x = lse[row];
+        if (x > -INFINITY) s = make_float2(x * kLog2e, dot);
+      }
+      stats[static_cast<long long>(hb) * p.tq_pad + i] = s;
+    }
+  }
+  if (sub == 0) red[row16] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    unsigned m = 0;
+    for (int k = 0; k < 16; ++k) m = max(m, __float_as_uint(red[k]));
+    // a maximum of non-negative floats: the order of the updates does not matter
+    atomicMax(norms + (queries ? 0 : p.batch * p.kv_heads) + batch * p.kv_heads + kv, m);
+  }
+}
+
+template <int HS, bool KEYS>
+__global__ void __launch_bounds__(384, 1)
+flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict__ status) {
+  constexpr int ROWS = FCHUNK * (HS / 64);   // bytes of a resident operand
+  constexpr int TILE = BCHUNK * (HS / 64);   // bytes of a streamed tile
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t rows_full, b_full[BSTAGES], b_empty[BSTAGES], x_full[2], p_full[2], acc_full;
+  __shared__ uint32_t tmem_slot;
+  __shared__ float window[2][2][256];
+  __shared__ __align__(16) float2 colstats[KEYS ? 2 : 1][2][BN];
+  __shared__ float diag[KEYS ? 1 : 8][96];
+  __shared__ float dist_s[KEYS ? 1 : 2][KEYS ? 1 : kDistSmem];
+  __shared__ float far_s[2][2][4];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t a1_s = base, a2_s = base + ROWS, b_s = base + 2 * ROWS;  // stage: B1, B2
+
+  if (warp == 1) {
+    if (lane == 0) {
+      mbar_init(smem_u32(&rows_full), 1);
+      mbar_init(smem_u32(&acc_full), 1);
+      for (int s = 0; s < BSTAGES; ++s) {
+        mbar_init(smem_u32(&b_full[s]), 1);
+        mbar_init(smem_u32(&b_empty[s]), 1);
+      }
+      for (int g = 0; g < 2; ++g) {
+        mbar_init(smem_u32(&x_full[g]), 1);
+        mbar_init(smem_u32(&p_full[g]), 128);
+      }
+      fence_mbar_init();
+    }
+    __syncwarp();
+    tmem_alloc(smem_u32(&tmem_slot), 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // the CTAs with the most work first: under a causal mask the first keys and the last queries
+  const int heads = KEYS ? p.kv_heads : p.heads;
+  const int hbs = heads * p.batch, hb = static_cast<int>(blockIdx.x) % hbs;
+  const int tile = KEYS ? static_cast<int>(blockIdx.x) / hbs : p.row_tiles - 1 - static_cast<int>(blockIdx.x) / hbs;
+  const int batch = hb / heads, head = hb - batch * heads, kv = KEYS ? head : head / p.group;
+  const int r0 = tile * FT;  // first row
+  const int qlen = rel_length(p.q_lengths, batch, p.tq), klen = rel_length(p.k_lengths, batch, p.tk);
+  const long long off = rel_offset(p.q_offset, p.q_offsets, batch);
+  // streamed tiles: first .. first + per - 1, for every query head of the group
+  int first = 0, per = 0;
+  if (KEYS) {
+    if (r0 < klen && qlen > 0) {
+      long long i = p.causal ? r0 - off : 0;  // the first query that sees key r0
+      i = i < 0 ? 0 : i;
+      if (i < qlen) {
+        first = static_cast<int>(i / BN);
+        per = (qlen + BN - 1) / BN - first;
+      }
+    }
+  } else if (r0 < qlen) {
+    const int last = r0 + FT - 1 < qlen - 1 ? r0 + FT - 1 : qlen - 1;
+    per = (rel_visible(p.causal, last + off, klen) + BN - 1) / BN;
+  }
+  const int n = per * (KEYS ? p.group : 1);
+
+  if (warp == 0) {
+    // ===================== TMA producer =====================
+    if (n > 0 && elect_one()) {
+      mbar_arrive_expect_tx(smem_u32(&rows_full), 2 * ROWS);
+      for (int c = 0; c < HS / 64; ++c) {
+        tma_load_4d(a1_s + c * FCHUNK, KEYS ? &p.tmK : &p.tmQ, smem_u32(&rows_full), 64 * c, r0, head, batch);
+        tma_load_4d(a2_s + c * FCHUNK, KEYS ? &p.tmV : &p.tmDO, smem_u32(&rows_full), 64 * c, r0, head, batch);
+      }
+      for (int it = 0; it < n; ++it) {
+        const int s = it % BSTAGES;
+        if (!mbar_wait(smem_u32(&b_empty[s]), ((it / BSTAGES) & 1) ^ 1u, status, DEV_TIMEOUT_EMPTY, 0xd00)) break;
+        const uint32_t bar = smem_u32(&b_full[s]), dst = b_s + s * 2 * TILE;
+        const int at = (first + it % per) * BN, h = KEYS ? head * p.group + it / per : kv;
+        mbar_arrive_expect_tx(bar, 2 * TILE);
+        for (int c = 0; c < HS / 64; ++c) {
+          tma_load_4d(dst + c * BCHUNK, KEYS ? &p.tmQ64 : &p.tmK64, bar, 64 * c, at, h, batch);
+          tma_load_4d(dst + TILE + c * BCHUNK, KEYS ? &p.tmDO64 : &p.tmV64, bar, 64 * c, at, h, batch);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ===================== MMA issuer =====================
+    constexpr uint32_t IDESC_X = make_idesc(0, 0, 0, FT, BN);
+    constexpr uint32_t IDESC_ACC = make_idesc(0, 0, 1, FT, HS);
+    const bool leader = elect_one();
+    const int blen = KEYS ? qlen : klen, bt = KEYS ? p.tq : p.tk;
+    bool ok = n == 0 || warp_wait(&rows_full, 0, status, DEV_TIMEOUT_FULL, 0xe00);
+    auto scores = [&](int it) {
+      const int s = it % BSTAGES, at = (first + it % per) * BN;
+      ok = warp_wait(&b_full[s], (it / BSTAGES) & 1, status, DEV_TIMEOUT_FULL, 0xe01);
+      if (!ok) return;
+      tc_fence_after();
+      if (blen < bt && at + BN > blen) {
+        // rows behind the sequence's end may hold anything: the second products meet them with
+        // zeros, and so they have to be zero
+        uint8_t* stage = base_ptr + (b_s - base) + s * 2 * TILE;
+        const int from = blen - at;  // > 0: tiles behind the end are not streamed
+        for (int x = lane * 16; x < (BN - from) * 128; x += 512)
+          for (int c = 0; c < 2 * (HS / 64); ++c)
+            *reinterpret_cast<uint4*>(stage + c * BCHUNK + from * 128 + x) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (leader) {
+        const uint32_t b = b_s + s * 2 * TILE, d = tmem + (it & 1) * FT;
+#pragma unroll
+        for (int ks = 0; ks < HS / 16; ++ks) {
+          const uint32_t aa = (ks / 4) * FCHUNK + (ks % 4) * 32, bb = (ks / 4) * BCHUNK + (ks % 4) * 32;
+          mma_f16(d, make_smem_desc(a1_s + aa, 16, 1024), make_smem_desc(b + bb, 16, 1024), IDESC_X, ks > 0);
+        }
+#pragma unroll
+        for (int ks = 0; ks < HS / 16; ++ks) {
+          const uint32_t aa = (ks / 4) * FCHUNK + (ks % 4) * 32, bb = (ks / 4) * BCHUNK + (ks % 4) * 32;
+          mma_f16(d + BN, make_smem_desc(a2_s + aa, 16, 1024), make_smem_desc(b + TILE + bb, 16, 1024), IDESC_X, ks > 0);
+        }
+        tc_commit(smem_u32(&x_full[it & 1]));
+      }
+    };
+    if (n > 0 && ok) scores(0);
+    for (int it = 0; it < n && ok; ++it) {
+      const int s = it % BSTAGES, g = it & 1;
+      if (it + 1 < n) scores(it + 1);  // overwrites P and dS of tile it - 1, whose products are issued
+      ok = ok && warp_wait(&p_full[g], (it >> 1) & 1, status, DEV_TIMEOUT_FULL, 0xe02);
+      if (!ok) break;
+      tc_fence_after();
+      if (leader) {
+        const uint32_t b = b_s + s * 2 * TILE, a = tmem + g * FT;
+#pragma unroll
+        for (int ks = 0; ks < BN / 16; ++ks) {
+          if (KEYS)  // dV += P dO
+            mma_f16_ts(tmem + 2 * FT + HS, a + ks * 8, make_smem_desc(b + TILE + ks * 2048, BCHUNK, 1024), IDESC_ACC,
+                       (it > 0 || ks > 0) ? 1u : 0u);
+        }
+#pragma unroll
+        for (int ks = 0; ks < BN / 16; ++ks)  // dK += dS Q,  dQ += dS K
+          mma_f16_ts(tmem + 2 * FT, a + BN + ks * 8, make_smem_desc(b + ks * 2048, BCHUNK, 1024), IDESC_ACC,
+                     (it > 0 || ks > 0) ? 1u : 0u);
+        tc_commit(smem_u32(&b_empty[s]));
+        if (it == n - 1) tc_commit(smem_u32(&acc_full));
+      }
+      __syncwarp();
+    }
+  } else if (warp >= 4) {
+    // ===================== probabilities and their gradient =====================
+    const int g = (warp - 4) >> 2, r = threadIdx.x & 127;
+    const int row = r0 + r;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t x_col = lanes + g * FT, y_col = x_col + BN;
+    const float c1 = p.c1;
+    const float up = ds_scale(p, batch, kv);
+    const float f = up * (1.f / 4096.f);  // on P, which is formed times 2^12
+    const bool dist_on = !KEYS && p.dist != nullptr;
+    float2 mine = make_float2(INFINITY, 0.f);
+    int vis = 0;
+    if (!KEYS && row < p.tq) {
+      mine = p.stats[(static_cast<long long>(batch) * p.heads + head) * p.tq_pad + row];
+      vis = row < qlen ? rel_visible(p.causal, row + off, klen) : 0;
+    }
+    const long long low = KEYS ? 0 : dist_low(p.reach, off, r0);
+    float* dist = nullptr;
+    float far_lo = 0.f, far_hi = 0.f;
+    if (dist_on) {
+      float* out = p.dist + (((static_cast<long long>(batch) * p.heads + head) * p.row_tiles + tile) * 2 + g) * p.width;
+      dist = p.width <= kDistSmem ? dist_s[g] : out;
+      for (int e = r; e < p.width; e += 128) dist[e] = 0.f;
+      group_barrier(1 + g);
+    }
+    bool ok = true;
+    for (int it = g; it < n; it += 2) {
+      const int at = (first + it % per) * BN, turn = (it >> 1) & 1;
+      const int h = KEYS ? head * p.group + it / per : head;
+      const float* bias = p.bias != nullptr ? p.bias + h * (2 * p.reach + 1) : nullptr;
+      // distances of the tile's pairs: dlo .. dlo + 190
+      const long long dlo = KEYS ? r0 - (at + BN - 1 + off) : at - (r0 + FT - 1 + off);
+      bool flat = bias == nullptr;
+      float value = 0.f;
+      float* win = window[g][turn];
+      if (bias != nullptr) {
+        if (dlo >= p.reach || dlo + FT + BN - 2 <= -p.reach) {
+          flat = true;
+          value = __ldg(bias + (dlo >= p.reach ? 2 * p.reach : 0));
+        } else {
+          for (int w = r; w < FT + BN; w += 128) {
+            long long d = dlo + w;
+            d = d > p.reach ? p.reach : d < -p.reach ? -p.reach : d;
+            win[w] = __ldg(bias + d + p.reach);
+          }
+        }
+      }
+      if (KEYS && r < BN)
+        colstats[KEYS ? g : 0][turn][r] = p.stats[(static_cast<long long>(batch) * p.heads + h) * p.tq_pad + at + r];
+      if (KEYS || !flat) group_barrier(1 + g);
+      // window[c - r + 127] for query rows, window[r - c + 63] for key rows
+      const float* wrow = KEYS ? win + (BN - 1) + r : win + (FT - 1) - r;
+      ok = ok && warp_wait(&x_full[g], turn, status, DEV_TIMEOUT_ACCUM, 0xf00 + g);
+      // columns lo .. hi - 1 of this row take part
+      int lo = 0, hi = BN;
+      if (KEYS) {
+        hi = row < klen ? BN : 0;
+        if (p.causal) {
+          const long long from = row - off - at;
+          lo = from < 0 ? 0 : from > BN ? BN : static_cast<int>(from);
+        }
+      } else {
+        hi = vis - at;
+      }
+      const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < BN);
+      float run = 0.f, all = 0.f;
+      if (ok) {
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) {
+          uint32_t x[32], y[32];
+          tmem_ld32(x_col + c, x);
+          tmem_ld32(y_col + c, y);
+          tmem_ld_wait();
+          uint32_t pw[16], dw[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float pr[2], ds[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int col = c + e + k;
+              const float2 st = KEYS ? colstats[KEYS ? g : 0][turn][col] : mine;
+              const float b = flat ? value : KEYS ? wrow[-col] : wrow[col];
+              const float q = ex2(fmaf(__uint_as_float(x[e + k]), c1, (b + 12.f) - st.x));
+              const float d = q * ((__uint_as_float(y[e + k]) - st.y) * f);
+              const bool in = !masked || (col >= lo && col < hi);
+              pr[k] = in ? q : 0.f;
+              ds[k] = in ? d : 0.f;
+              if (dist_on) {
+                if (flat || p.reach == 0) {
+                  all += ds[k];
+                } else {
+                  // the running sum of a diagonal moves down one lane per column; lane 31 ends it
+                  run = __shfl_up_sync(0xffffffffu, run, 1);
+                  run = (lane == 0 ? 0.f : run) + ds[k];
+                  if (lane == 31) diag[KEYS ? 0 : warp - 4][col] = run;
+                }
+              }
+            }
+            pw[e / 2] = pack_half2(pr[0], pr[1]);
+            dw[e / 2] = pack_half2(ds[0], ds[1]);
+          }
+          if (KEYS) tmem_st16(x_col + c / 2, pw);
+          tmem_st16(y_col + c / 2, dw);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&p_full[g]));
+      }
+      if (dist_on) {
+        if (flat || p.reach == 0) {
+          // one side of the reach (no bias window without a table: then dist is off)
+          if (dlo >= p.reach) far_hi += all;
+          else far_lo += all;
+        } else {
+          // diag[warp][c - 31 + 31]: lane 31 left diagonals -31 .. 32 at 0 .. 63; the others end here
+          if (lane < 31) diag[KEYS ? 0 : warp - 4][64 + lane] = run;  // diagonal 63 - lane
+          group_barrier(1 + g);
+          for (int w = r; w < FT + BN - 1; w += 128) {
+            float sum = 0.f;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              // column - row = w - 127, row = 32 q + lane: diagonal w - 127 + 32 q of that warp
+              const int dg = w - (FT - 1) + 32 * q;
+              if (dg >= -31 && dg <= 63) sum += diag[KEYS ? 0 : g * 4 + q][dg <= 32 ? dg + 31 : 64 + 63 - dg];
+            }
+            const long long d = dlo + w;
+            if (d >= p.reach) far_hi += sum;
+            else if (d <= -p.reach) far_lo += sum;
+            else if (d - low < p.width) dist[d - low] += sum;  // behind the last key: nothing, and no place
+          }
+          group_barrier(1 + g);
+        }
+      }
+    }
+    // ---- sums by distance ----
+    if (dist_on) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        far_lo += __shfl_xor_sync(0xffffffffu, far_lo, o);
+        far_hi += __shfl_xor_sync(0xffffffffu, far_hi, o);
+      }
+      if (lane == 0) {
+        far_s[g][0][warp & 3] = far_lo;
+        far_s[g][1][warp & 3] = far_hi;
+      }
+      group_barrier(1 + g);
+      if (r == 0) {
+        float s[2];
+        for (int k = 0; k < 2; ++k) s[k] = (far_s[g][k][0] + far_s[g][k][1]) + (far_s[g][k][2] + far_s[g][k][3]);
+        if (-p.reach - low >= 0 && -p.reach - low < p.width) dist[-p.reach - low] += s[0];
+        if (p.reach - low >= 0 && p.reach - low < p.width) dist[p.reach - low] += s[1];
+      }
+      group_barrier(1 + g);
+      if (p.width <= kDistSmem) {
+        float* out = p.dist + (((static_cast<long long>(batch) * p.heads + head) * p.row_tiles + tile) * 2 + g) * p.width;
+        for (int e = r; e < p.width; e += 128) out[e] = dist[e];
+      }
+    }
+    // ---- results: group 0 writes dK, group 1 dV; the two share dQ's columns ----
+    if (n > 0 && ok) {
+      ok = warp_wait(&acc_full, 0, status, DEV_TIMEOUT_ACCUM, 0xf10 + g);
+      tc_fence_after();
+    }
+    __half* out = KEYS ? (g == 0 ? p.dk : p.dv) : p.dq;
+    const bool real = row < (KEYS ? p.tk : p.tq);
+    if (ok && out != nullptr && (n > 0 || !p.accumulate)) {
+      const long long ld = KEYS ? (g == 0 ? p.lddk : p.lddv) : p.lddq, sh = KEYS ? (g == 0 ? p.shdk : p.shdv) : p.shdq,
+                      sb = KEYS ? (g == 0 ? p.sbdk : p.sbdv) : p.sbdq;
+      out += row * ld + head * sh + batch * sb;
+      const float factor = KEYS && g == 1 ? 1.f / 4096.f : p.scale / up;
+      const uint32_t col0 = lanes + 2 * FT + (KEYS && g == 1 ? HS : 0);
+      const int c_from = KEYS ? 0 : g * (HS / 2), c_to = KEYS ? HS : c_from + HS / 2;
+      for (int c = c_from; c < c_to; c += 16) {
+        uint32_t w[16];
+        if (n > 0) {
+          tmem_ld16(col0 + c, w);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (!real || c + 8 * half >= p.hs) continue;
+          uint4* dst = reinterpret_cast<uint4*>(out + c + 8 * half);
+          uint32_t old[4] = {0, 0, 0, 0}, res[4];
+          if (p.accumulate) {
+            const uint4 q = *dst;
+            old[0] = q.x; old[1] = q.y; old[2] = q.z; old[3] = q.w;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&old[e]));
+            const float a = n > 0 ? __uint_as_float(w[8 * half + 2 * e]) * factor : 0.f;
+            const float b = n > 0 ? __uint_as_float(w[8 * half + 2 * e + 1]) * factor : 0.f;
+            res[e] = p.accumulate ? pack_half2(a + q.x, b + q.y) : pack_half2(a, b);
+          }
+          *dst = make_uint4(res[0], res[1], res[2], res[3]);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// sums[head][reach + d] = the query tiles' sums of dS at distance d over all sequences, in order; a CTA
+// serves 32 distances, its eight warps every eighth (sequence, tile).
+__global__ void __launch_bounds__(256)
+flash_dist_sum_kernel(const __grid_constant__ FlashBwdParams p, float* __restrict__ sums) {
+  __shared__ float red[8][32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y;
+  const long long at = static_cast<long long>(blockIdx.x) * 32 + lane, d = at - p.reach;
+  float s = 0.f;
+  for (int k = warp; k < p.batch * p.row_tiles; k += 8) {
+    const int batch = k / p.row_tiles, tile = k - batch * p.row_tiles;
+    const long long e = d - dist_low(p.reach, rel_offset(p.q_offset, p.q_offsets, batch), tile * FT);
+    if (d > p.reach || e < 0 || e >= p.width) continue;
+    const float* q = p.dist + ((static_cast<long long>(batch) * p.heads + head) * p.row_tiles + tile) * 2 * p.width + e;
+    s += (q[0] + q[p.width]) / ds_scale(p, batch, head / p.group);
+  }
+  red[warp][lane] = s;
+  __syncthreads();
+  if (warp != 0 || d > p.reach) return;
+  float a = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) a += red[w][lane];
+  sums[head * (2 * p.reach + 1) + at] = a;
+}
+
+// dtable[bucket, head] (+)= the sums of the distances that map to it; one warp per (bucket, head).
+__global__ void __launch_bounds__(256)
+flash_table_kernel(const float* __restrict__ sums, const int* __restrict__ map, long long reach, int buckets, int heads,
+                   int accumulate, __half* __restrict__ dtable, long long lddt) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const long long at = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (at >= static_cast<long long>(buckets) * heads) return;
+  const int head = static_cast<int>(at / buckets), bucket = static_cast<int>(at % buckets);
+  const float* s = sums + head * (2 * reach + 1);
+  float sum = 0.f;
+  for (long long d = lane; d < 2 * reach + 1; d += 32)
+    if (map[d] == bucket) sum += s[d];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane != 0) return;
+  __half* out = dtable + head * lddt + bucket;
+  *out = __float2half_rn(accumulate ? __half2float(*out) + sum : sum);
+}
+
 bool heads_aligned(const FlashOperand& x, long long t, long long heads, long long batch) {
   if ((reinterpret_cast<uintptr_t>(x.p) & 15u) != 0) return false;
   const long long n[3] = {t, heads, batch}, s[3] = {x.ld, x.head, x.batch};
@@ -434,6 +967,19 @@ cudaError_t forward_hs(FlashParams& p, cudaStream_t stream, int* status) {
   return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(384), smem, stream, pdl_enabled(), p, status);
 }
 
+template <int HS, bool KEYS>
+cudaError_t backward_hs(const FlashBwdParams& p, cudaStream_t stream, int* status) {
+  const int smem = 2 * FCHUNK * (HS / 64) + BSTAGES * 2 * BCHUNK * (HS / 64) + 1024;
+  static unsigned long long smem_set = 0;  // per template instantiation
+  auto kern = flash_backward_kernel<HS, KEYS>;
+  cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern), smem, &smem_set);
+  if (e != cudaSuccess) return e;
+  FlashBwdParams q = p;
+  q.row_tiles = ((KEYS ? p.tk : p.tq) + FT - 1) / FT;
+  const long long grid = static_cast<long long>(q.row_tiles) * (KEYS ? p.kv_heads : p.heads) * p.batch;
+  return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(384), smem, stream, pdl_enabled(), q, status);
+}
+
 }  // namespace
 
 bool flash_supported(const FlashArgs& a) {
@@ -447,6 +993,96 @@ cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* s
   FlashParams p;
   if (!fill_params(a, &p)) return cudaErrorInvalidValue;
   return a.hs <= 64 ? forward_hs<64, 3>(p, stream, status) : forward_hs<128, 2>(p, stream, status);
+}
+
+bool flash_backward_supported(const FlashArgs& a, const FlashGradArgs& g) {
+  const auto fits = [](long long parts, long long heads, long long batch) { return parts * heads * batch <= 0x3fffffffLL; };
+  return flash_supported(a) && heads_aligned(g.d_o, a.tq, a.heads, a.batch) &&
+         (g.dq.p == nullptr || heads_aligned(g.dq, a.tq, a.heads, a.batch)) &&
+         (g.dk.p == nullptr || heads_aligned(g.dk, a.tk, a.kv_heads, a.batch)) &&
+         (g.dv.p == nullptr || heads_aligned(g.dv, a.tk, a.kv_heads, a.batch)) &&
+         fits((a.tq + 127) / 128 * 2, a.heads, a.batch) && fits((a.tk + 63) / 64, a.kv_heads, a.batch);
+}
+
+FlashScratch flash_backward_scratch(const FlashArgs& a, bool table) {
+  FlashScratch s;
+  const long long rows = static_cast<long long>(a.heads) * a.batch, tiles = (a.tq + FT - 1) / FT;
+  s.stats = rows * tiles * FT * 2;
+  s.norms = 2LL * a.batch * a.kv_heads;
+  const long long width = 2 * a.reach + 1 < a.tk + FT - 1 ? 2 * a.reach + 1 : a.tk + FT - 1;
+  s.dist = table ? rows * tiles * 2 * width : 0;
+  s.sums = table ? (2 * a.reach + 1) * a.heads : 0;
+  return s;
+}
+
+cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, float* stats, float* norms, float* dist,
+                                  float* sums, int* launches, cudaStream_t stream, int* status) {
+  FlashBwdParams p;
+  std::memset(&p, 0, sizeof(p));
+  const struct {
+    CUtensorMap* map;
+    const FlashOperand* x;
+    int t, heads, rows;
+  } maps[] = {{&p.tmQ, &a.q, a.tq, a.heads, FT},   {&p.tmDO, &g.d_o, a.tq, a.heads, FT},
+              {&p.tmK, &a.k, a.tk, a.kv_heads, FT}, {&p.tmV, &a.v, a.tk, a.kv_heads, FT},
+              {&p.tmQ64, &a.q, a.tq, a.heads, BN},   {&p.tmDO64, &g.d_o, a.tq, a.heads, BN},
+              {&p.tmK64, &a.k, a.tk, a.kv_heads, BN}, {&p.tmV64, &a.v, a.tk, a.kv_heads, BN}};
+  for (const auto& m : maps)
+    if (!encode_heads_tmap(m.map, m.x->p, a.hs, m.t, m.heads, a.batch, m.x->ld, m.x->head, m.x->batch, m.rows))
+      return cudaErrorInvalidValue;
+  p.dq = static_cast<__half*>(const_cast<void*>(g.dq.p));
+  p.dk = static_cast<__half*>(const_cast<void*>(g.dk.p));
+  p.dv = static_cast<__half*>(const_cast<void*>(g.dv.p));
+  p.lddq = g.dq.ld; p.shdq = g.dq.head; p.sbdq = g.dq.batch;
+  p.lddk = g.dk.ld; p.shdk = g.dk.head; p.sbdk = g.dk.batch;
+  p.lddv = g.dv.ld; p.shdv = g.dv.head; p.sbdv = g.dv.batch;
+  p.stats = reinterpret_cast<const float2*>(stats);
+  p.norms = reinterpret_cast<const unsigned*>(norms);
+  p.dist = dist;
+  p.bias = a.bias;
+  p.tq = a.tq; p.tk = a.tk; p.hs = a.hs; p.heads = a.heads; p.kv_heads = a.kv_heads; p.group = a.heads / a.kv_heads;
+  p.batch = a.batch;
+  const int qtiles = (a.tq + FT - 1) / FT;
+  p.tq_pad = qtiles * FT;
+  p.reach = a.reach; p.q_offset = a.q_offset;
+  p.q_offsets = a.q_offsets; p.q_lengths = a.q_lengths; p.k_lengths = a.k_lengths;
+  p.scale = a.scale;
+  p.c1 = a.scale * kLog2e;
+  p.causal = a.causal;
+  p.accumulate = g.accumulate;
+  p.width = static_cast<int>(2 * a.reach + 1 < a.tk + FT - 1 ? 2 * a.reach + 1 : a.tk + FT - 1);
+  cudaError_t e = cudaMemsetAsync(norms, 0, sizeof(unsigned) * 2 * a.batch * a.kv_heads, stream);
+  if (e != cudaSuccess) return e;
+  const int qparts = qtiles * 2;
+  const long long qblocks = static_cast<long long>(qparts) * a.heads * a.batch,
+                  blocks = qblocks + static_cast<long long>((a.tk + 63) / 64) * a.kv_heads * a.batch;
+  e = launch_kernel(flash_prepare_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, pdl_enabled(),
+                    static_cast<const __half*>(g.d_o.p), g.d_o.ld, g.d_o.head, g.d_o.batch, static_cast<const __half*>(a.o.p),
+                    a.o.ld, a.o.head, a.o.batch, static_cast<const __half*>(a.v.p), a.v.ld, a.v.head, a.v.batch,
+                    static_cast<const float*>(a.lse), p, reinterpret_cast<float2*>(stats), reinterpret_cast<unsigned*>(norms),
+                    qparts, qblocks);
+  *launches = 1;
+  if (e != cudaSuccess) return e;
+  if (p.dk != nullptr || p.dv != nullptr) {
+    e = a.hs <= 64 ? backward_hs<64, true>(p, stream, status) : backward_hs<128, true>(p, stream, status);
+    ++*launches;
+    if (e != cudaSuccess) return e;
+  }
+  if (p.dq != nullptr || dist != nullptr) {
+    e = a.hs <= 64 ? backward_hs<64, false>(p, stream, status) : backward_hs<128, false>(p, stream, status);
+    ++*launches;
+    if (e != cudaSuccess) return e;
+  }
+  if (dist == nullptr) return cudaSuccess;
+  p.row_tiles = qtiles;
+  const long long n = 2 * a.reach + 1;
+  e = launch_kernel(flash_dist_sum_kernel, dim3(static_cast<unsigned>((n + 31) / 32), static_cast<unsigned>(a.heads)), dim3(256), 0,
+                    stream, pdl_enabled(), p, sums);
+  if (e != cudaSuccess) return e;
+  *launches += 2;
+  return launch_kernel(flash_table_kernel, dim3(static_cast<unsigned>((static_cast<long long>(g.buckets) * a.heads + 7) / 8)), dim3(256), 0,
+                       stream, pdl_enabled(), static_cast<const float*>(sums), g.map, a.reach, g.buckets, a.heads, g.accumulate,
+                       static_cast<__half*>(g.dtable), g.lddt);
 }
 
 }  // namespace gb

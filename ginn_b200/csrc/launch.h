@@ -243,6 +243,23 @@ struct FlashArgs {
 // 128, 16-byte aligned bases and strides.
 bool flash_supported(const FlashArgs& a);
 cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* status);
+struct FlashGradArgs {
+  FlashOperand d_o, dq, dk, dv;  // results: p null = not wanted
+  void* dtable;
+  long long lddt;
+  const int* map;
+  int buckets, accumulate;
+};
+bool flash_backward_supported(const FlashArgs& a, const FlashGradArgs& g);
+// Scratch of the backward pass, in floats; dist and sums only when the table's gradient is wanted.
+struct FlashScratch {
+  long long stats, norms, dist, sums;
+};
+FlashScratch flash_backward_scratch(const FlashArgs& a, bool table);
+// `launches`: kernels launched.
+cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, float* stats, float* norms,
+                                  float* dist, float* sums, int* launches, cudaStream_t stream,
+                                  int* status);
 
 // --- Conv2d as patch extraction + matrix products (conv.cu) ---
 struct ConvShape {

@@ -5,6 +5,13 @@ rounding, and for Half operands that of the probabilities and of the scores' gra
 into the second products, and of the stored output in delta).  E = 2^-17: what a product may be off
 relative to the product of the magnitudes (fp32 accumulation of exact Half products, or three
 TF32 products per term), which also covers the exponentials and the statistics.
+
+Floors of the Half operands inside the backward products, where a relative bound ends: below a Half's
+normal range a rounding is off by half a subnormal step, 2^-25, whatever the value.  P is formed times
+2^12: 2^-37 each.  dS is formed times 2^floor(14 - log2 B) with B = 2 max|d_o row| max|v row| per
+sequence and key head, which is more than 2^13 / B: less than 2^-38 B each.  A key that no query
+attends to (p < 1e-8) has a gradient of that size, 3e-8 in the peaked case with B = 2^8, so there the
+floor and not u decides whether the result rounds to 0 or to the smallest Half.
 """
 import numpy as np
 import pytest
@@ -108,11 +115,13 @@ class Case:
                 ds = p * (dp - delta)
                 edelta = (np.abs(G) * (eo + u * np.abs(o))).sum(0)
                 exact = ep * np.abs(dp - delta) + p * (E * (np.abs(V).T @ np.abs(G)) + edelta) + E * np.abs(ds)  # of ds before it is rounded
-                eds = exact + ui * np.abs(ds)
+                bound = 2 * np.sqrt((G ** 2).sum(0).max() * (V ** 2).sum(0).max()) if group == 1 else \
+                    2 * np.sqrt((g[:, :nq, h // group * group:(h // group + 1) * group, b] ** 2).sum(0).max() * (V ** 2).sum(0).max())
+                eds = exact + ui * np.abs(ds) + (2.0 ** -38 * bound if ui else 0)
                 a = abs(self.scale)
                 tol["dq"][:, :nq, h, b] += a * (np.abs(K) @ (eds + E * np.abs(ds)))
                 tol["dk"][:, :nk, h // group, b] += a * (np.abs(Q) @ (eds + E * np.abs(ds)).T)
-                tol["dv"][:, :nk, h // group, b] += np.abs(G) @ (ep + (ui + E) * p).T
+                tol["dv"][:, :nk, h // group, b] += np.abs(G) @ (ep + (ui + E) * p + (2.0 ** -37 if ui else 0)).T
                 if self.table is not None:
                     np.add.at(tol["dtable"][:, h], kind, exact + E * np.abs(ds))
         for n in ("dq", "dk", "dv", "dtable"):
