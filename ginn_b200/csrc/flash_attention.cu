@@ -41,6 +41,28 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two fp32 values at a time (one instruction each).
+struct F2 {
+  unsigned long long v;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -277,7 +299,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
     bool ok = true;
     for (int j = 0; j < nt; ++j) {
       const TileBias tb(bias, p.reach, static_cast<long long>(j) * FT - (i0 + t * FT + FT - 1 + hd.off), r, -1,
-                        window[t][j & 1], c1 >= 0.f);
+                        window[t][j & 1], c1 > 0.f);
       if (tb.near) group_barrier(1 + t);
       // a group that gave up still meets its barriers
       ok = ok && warp_wait(&s_full[t], j & 1, status, DEV_TIMEOUT_ACCUM, 0xc00 + t);
@@ -285,38 +307,39 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
       tc_fence_after();
       const int lim = vis - j * FT;  // columns below it are seen
       const bool masked = __any_sync(0xffffffffu, lim < FT);
-      float top = -INFINITY;
-      uint32_t v[32];
-#pragma unroll
-      for (int c = 0; c < FT; c += 32) {
-        tmem_ld32(s_col + c, v);
+      // 64 scores at a time: raw with a flat bias, finished with a window
+      uint32_t v[64];
+      auto fetch = [&](int c0) {
+        tmem_ld32(s_col + c0, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+        tmem_ld32(s_col + c0 + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
         tmem_ld_wait();
         if (tb.near) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float x = fmaf(__uint_as_float(v[e]), c1, tb.row[c + e]);
-            top = fmaxf(top, !masked || c + e < lim ? x : -INFINITY);
-          }
-        } else {
-          float raw = -INFINITY;
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) raw = fmaxf(raw, c + e < lim ? __uint_as_float(v[e]) : -INFINITY);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) raw = fmaxf(raw, __uint_as_float(v[e]));
-          }
-          if (raw != -INFINITY) top = fmaxf(top, fmaf(raw, c1, tb.value));
+          for (int c = 0; c < 64; ++c) v[c] = __float_as_uint(fmaf(__uint_as_float(v[c]), c1, tb.row[c0 + c]));
         }
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c) v[c] = c0 + c < lim ? v[c] : 0xff800000u;  // -inf
+        }
+      };
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c0 = 0; c0 < FT; c0 += 64) {
+        fetch(c0);
+#pragma unroll
+        for (int c = 0; c < 64; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            top[e] = fmaxf(top[e], fmaxf(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])));
       }
-      const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
-      if (__any_sync(0xffffffffu, grow)) {
-        // O exists from the second tile on; what it holds for a row without keys so far is zero
-        const float mn = fmaxf(m, top);
+      float mn = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      if (!tb.near && mn > -INFINITY) mn = fmaf(mn, c1, tb.value);
+      if (__any_sync(0xffffffffu, mn > m + 8.f)) {  // also a row's first visible key (m = -inf)
+        mn = fmaxf(m, mn);
         const float a = mn == -INFINITY ? 1.f : ex2(m - mn);
         l *= a;
         m = mn;
-        if (j > 0) {
+        if (j > 0) {  // O exists from the second tile on
 #pragma unroll
           for (int c = 0; c < HS; c += 16) {
             uint32_t w[16];
@@ -329,31 +352,30 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
         }
       }
       const float mu = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const float ca = tb.near ? 1.f : c1, cb = tb.value - mu;
+      const F2 ca2(ca, ca), cb2(cb, cb);
+      F2 sum[2] = {F2(0.f, 0.f), F2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < FT; c += 32) {
-        tmem_ld32(s_col + c, v);
-        tmem_ld_wait();
-        float pr[32];
-        const float shift = tb.value - mu;
+      for (int c0 = 0; c0 < FT; c0 += 64) {
+        fetch(c0);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float x = tb.near ? fmaf(__uint_as_float(v[e]), c1, tb.row[c + e] - mu) : fmaf(__uint_as_float(v[e]), c1, shift);
-          pr[e] = ex2(x);
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x, y;
+            fma2(F2(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])), ca2, cb2).get(x, y);
+            x = ex2(x);
+            y = ex2(y);
+            sum[e & 1] = add2(sum[e & 1], F2(x, y));
+            w[e] = pack_half2(x, y);
+          }
+          tmem_st16(s_col + (c0 + c) / 2, w);
         }
-        if (masked) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) pr[e] = c + e < lim ? pr[e] : 0.f;
-        }
-        uint32_t w[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          sum[e & 3] += pr[2 * e] + pr[2 * e + 1];
-          w[e] = pack_half2(pr[2 * e], pr[2 * e + 1]);
-        }
-        tmem_st16(s_col + c / 2, w);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      float sa, sb;
+      add2(sum[0], sum[1]).get(sa, sb);
+      l += sa + sb;
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(smem_u32(&p_full[t]));
@@ -466,8 +488,7 @@ flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long lon
   const int batch = hb / heads, head = hb - batch * heads;
   const int kv = queries ? head / p.group : head;
   const int len = queries ? rel_length(p.q_lengths, batch, p.tq) : rel_length(p.k_lengths, batch, p.tk);
-  auto load = [&](const __half* x, float (&f)[8]) {
-    const uint4 w = *reinterpret_cast<const uint4*>(x);
+  auto widen = [&](uint4 w, float (&f)[8]) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -476,36 +497,50 @@ flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long lon
       f[2 * e + 1] = q.y;
     }
   };
-  float most = 0.f;
-  for (int k = 0; k < 4; ++k) {
-    const int i = part * 64 + k * 16 + row16;
-    const bool real = i < len && sub * 8 < p.hs;
-    float norm = 0.f, dot = 0.f;
-    if (real) {
-      float a[8];
-      load(queries ? d_o + i * lddo + head * shdo + batch * sbdo + sub * 8 : v + i * ldv + head * shv + batch * sbv + sub * 8, a);
+  float norm[4], dot[4];
+  {
+    uint4 wa[4], wb[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) norm += a[e] * a[e];
-      if (queries) {
-        float b[8];
-        load(o + i * ldo + head * sho + batch * sbo + sub * 8, b);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dot += a[e] * b[e];
+    for (int k = 0; k < 4; ++k) {  // all loads before the first sum
+      const int i = part * 64 + k * 16 + row16;
+      wa[k] = wb[k] = make_uint4(0, 0, 0, 0);
+      if (i < len && sub * 8 < p.hs) {
+        wa[k] = *reinterpret_cast<const uint4*>(queries ? d_o + i * lddo + head * shdo + batch * sbdo + sub * 8
+                                                        : v + i * ldv + head * shv + batch * sbv + sub * 8);
+        if (queries) wb[k] = *reinterpret_cast<const uint4*>(o + i * ldo + head * sho + batch * sbo + sub * 8);
       }
     }
 #pragma unroll
-    for (int s = 8; s > 0; s >>= 1) {
-      norm += __shfl_xor_sync(0xffffffffu, norm, s);
-      dot += __shfl_xor_sync(0xffffffffu, dot, s);
+    for (int k = 0; k < 4; ++k) {
+      float a[8], b[8];
+      widen(wa[k], a);
+      widen(wb[k], b);
+      norm[k] = dot[k] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        norm[k] += a[e] * a[e];
+        dot[k] += a[e] * b[e];
+      }
     }
+  }
+#pragma unroll
+  for (int s = 8; s > 0; s >>= 1)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      norm[k] += __shfl_xor_sync(0xffffffffu, norm[k], s);
+      dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], s);
+    }
+  float most = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
     // a row that is not a number or infinite makes the bound so (the integer order puts both last)
-    most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(norm)));
+    most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(norm[k])));
+    const int i = part * 64 + k * 16 + row16;
     if (queries && sub == 0 && i < p.tq_pad) {
-      const long long row = static_cast<long long>(hb) * p.tq + i;
       float2 s = make_float2(INFINITY, 0.f);
       if (i < len) {
-        const float x = lse[row];
-        if (x > -INFINITY) s = make_float2(x * kLog2e, dot);
+        const float x = lse[static_cast<long long>(hb) * p.tq + i];
+        if (x > -INFINITY) s = make_float2(x * kLog2e, dot[k]);
       }
       stats[static_cast<long long>(hb) * p.tq_pad + i] = s;
     }
@@ -529,7 +564,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
   __shared__ __align__(8) uint64_t rows_full, b_full[BSTAGES], b_empty[BSTAGES], x_full[2], p_full[2], acc_full;
   __shared__ uint32_t tmem_slot;
   __shared__ float window[2][2][256];
-  __shared__ __align__(16) float2 colstats[KEYS ? 2 : 1][2][BN];
+  __shared__ __align__(16) float colx[KEYS ? 2 : 1][2][BN], coly[KEYS ? 2 : 1][2][BN];
   __shared__ float diag[KEYS ? 1 : 8][96];
   __shared__ float dist_s[KEYS ? 1 : 2][KEYS ? 1 : kDistSmem];
   __shared__ float far_s[2][2][4];
@@ -704,23 +739,26 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       const float* bias = p.bias != nullptr ? p.bias + h * (2 * p.reach + 1) : nullptr;
       // distances of the tile's pairs: dlo .. dlo + 190
       const long long dlo = KEYS ? r0 - (at + BN - 1 + off) : at - (r0 + FT - 1 + off);
-      bool flat = bias == nullptr;
+      // one number for the whole tile (a masked score is -inf before it is scaled: c1 > 0), or a window
+      const bool beyond = dlo >= p.reach || dlo + FT + BN - 2 <= -p.reach;
+      const bool flat = c1 > 0.f && (bias == nullptr || beyond);
       float value = 0.f;
       float* win = window[g][turn];
-      if (bias != nullptr) {
-        if (dlo >= p.reach || dlo + FT + BN - 2 <= -p.reach) {
-          flat = true;
-          value = __ldg(bias + (dlo >= p.reach ? 2 * p.reach : 0));
-        } else {
-          for (int w = r; w < FT + BN; w += 128) {
-            long long d = dlo + w;
-            d = d > p.reach ? p.reach : d < -p.reach ? -p.reach : d;
-            win[w] = __ldg(bias + d + p.reach);
-          }
+      if (flat) {
+        if (bias != nullptr) value = __ldg(bias + (dlo >= p.reach ? 2 * p.reach : 0));
+      } else {
+        for (int w = r; w < FT + BN; w += 128) {
+          long long d = dlo + w;
+          d = d > p.reach ? p.reach : d < -p.reach ? -p.reach : d;
+          win[w] = bias != nullptr ? __ldg(bias + d + p.reach) : 0.f;
         }
       }
-      if (KEYS && r < BN)
-        colstats[KEYS ? g : 0][turn][r] = p.stats[(static_cast<long long>(batch) * p.heads + h) * p.tq_pad + at + r];
+      if (KEYS && r < BN) {
+        // per column: what is added to the scaled score, and to Y times f
+        const float2 st = p.stats[(static_cast<long long>(batch) * p.heads + h) * p.tq_pad + at + r];
+        colx[KEYS ? g : 0][turn][r] = (flat ? value : 0.f) + 12.f - st.x;
+        coly[KEYS ? g : 0][turn][r] = -st.y * f;
+      }
       if (KEYS || !flat) group_barrier(1 + g);
       // window[c - r + 127] for query rows, window[r - c + 63] for key rows
       const float* wrow = KEYS ? win + (BN - 1) + r : win + (FT - 1) - r;
@@ -737,55 +775,82 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
         hi = vis - at;
       }
       const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < BN);
-      float run = 0.f, all = 0.f;
+      const bool sweep = !KEYS && !beyond && p.reach > 0;  // sums along the diagonals
+      float run = 0.f;
+      F2 all(0.f, 0.f);
       if (ok) {
         tc_fence_after();
+        const F2 c12(c1, c1), f2(f, f);
+        const float rx = (flat ? value : 0.f) + 12.f - mine.x, ry = -mine.y * f;
 #pragma unroll
         for (int c = 0; c < BN; c += 32) {
           uint32_t x[32], y[32];
           tmem_ld32(x_col + c, x);
           tmem_ld32(y_col + c, y);
           tmem_ld_wait();
+          if (!flat) {  // the window's bias joins the scores here, everything else below
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), c1, KEYS ? wrow[-(c + e)] : wrow[c + e]));
+          }
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c + e < lo || c + e >= hi) {
+                x[e] = 0xff800000u;  // -inf
+                y[e] = 0u;
+              }
+          }
+          const F2 cx = flat ? c12 : F2(1.f, 1.f);
           uint32_t pw[16], dw[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            float pr[2], ds[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int col = c + e + k;
-              const float2 st = KEYS ? colstats[KEYS ? g : 0][turn][col] : mine;
-              const float b = flat ? value : KEYS ? wrow[-col] : wrow[col];
-              const float q = ex2(fmaf(__uint_as_float(x[e + k]), c1, (b + 12.f) - st.x));
-              const float d = q * ((__uint_as_float(y[e + k]) - st.y) * f);
-              const bool in = !masked || (col >= lo && col < hi);
-              pr[k] = in ? q : 0.f;
-              ds[k] = in ? d : 0.f;
-              if (dist_on) {
-                if (flat || p.reach == 0) {
-                  all += ds[k];
-                } else {
-                  // the running sum of a diagonal moves down one lane per column; lane 31 ends it
-                  run = __shfl_up_sync(0xffffffffu, run, 1);
-                  run = (lane == 0 ? 0.f : run) + ds[k];
-                  if (lane == 31) diag[KEYS ? 0 : warp - 4][col] = run;
-                }
-              }
+            F2 sx(rx, rx), sy(ry, ry);
+            if (KEYS) {
+              const float2 ax = *reinterpret_cast<const float2*>(&colx[KEYS ? g : 0][turn][c + e]);
+              const float2 ay = *reinterpret_cast<const float2*>(&coly[KEYS ? g : 0][turn][c + e]);
+              sx = F2(ax.x, ax.y);
+              sy = F2(ay.x, ay.y);
             }
-            pw[e / 2] = pack_half2(pr[0], pr[1]);
-            dw[e / 2] = pack_half2(ds[0], ds[1]);
+            float p0, p1;
+            fma2(F2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), cx, sx).get(p0, p1);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            const F2 ds = mul2(F2(p0, p1), fma2(F2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), f2, sy));
+            float d0, d1;
+            ds.get(d0, d1);
+            if (KEYS) pw[e / 2] = pack_half2(p0, p1);
+            else all = add2(all, ds);
+            dw[e / 2] = pack_half2(d0, d1);
+            if (!KEYS) {
+              y[e] = __float_as_uint(d0);
+              y[e + 1] = __float_as_uint(d1);
+            }
           }
           if (KEYS) tmem_st16(x_col + c / 2, pw);
           tmem_st16(y_col + c / 2, dw);
+          if (c + 32 == BN) {
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&p_full[g]));
+          }
+          if (sweep && dist_on) {
+            // the running sum of a diagonal moves down one lane per column; lane 31 ends it
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              run = __shfl_up_sync(0xffffffffu, run, 1);
+              run = (lane == 0 ? 0.f : run) + __uint_as_float(y[e]);
+              if (lane == 31) diag[KEYS ? 0 : warp - 4][c + e] = run;
+            }
+          }
         }
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(smem_u32(&p_full[g]));
       }
       if (dist_on) {
-        if (flat || p.reach == 0) {
-          // one side of the reach (no bias window without a table: then dist is off)
-          if (dlo >= p.reach) far_hi += all;
-          else far_lo += all;
+        if (!sweep) {  // one side of the reach
+          float a0, a1;
+          all.get(a0, a1);
+          if (dlo >= p.reach) far_hi += a0 + a1;
+          else far_lo += a0 + a1;
         } else {
           // diag[warp][c - 31 + 31]: lane 31 left diagonals -31 .. 32 at 0 .. 63; the others end here
           if (lane < 31) diag[KEYS ? 0 : warp - 4][64 + lane] = run;  // diagonal 63 - lane
@@ -828,7 +893,9 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       group_barrier(1 + g);
       if (p.width <= kDistSmem) {
         float* out = p.dist + (((static_cast<long long>(batch) * p.heads + head) * p.row_tiles + tile) * 2 + g) * p.width;
-        for (int e = r; e < p.width; e += 128) out[e] = dist[e];
+        for (int e = r; e < p.width; e += 128) out[e] = dist[e] * (1.f / up);
+      } else {
+        for (int e = r; e < p.width; e += 128) dist[e] *= 1.f / up;
       }
     }
     // ---- results: group 0 writes dK, group 1 dV; the two share dQ's columns ----
@@ -896,7 +963,7 @@ flash_dist_sum_kernel(const __grid_constant__ FlashBwdParams p, float* __restric
     const long long e = d - dist_low(p.reach, rel_offset(p.q_offset, p.q_offsets, batch), tile * FT);
     if (d > p.reach || e < 0 || e >= p.width) continue;
     const float* q = p.dist + ((static_cast<long long>(batch) * p.heads + head) * p.row_tiles + tile) * 2 * p.width + e;
-    s += (q[0] + q[p.width]) / ds_scale(p, batch, head / p.group);
+    s += q[0] + q[p.width];
   }
   red[warp][lane] = s;
   __syncthreads();
