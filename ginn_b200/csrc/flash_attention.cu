@@ -32,6 +32,7 @@ namespace gb {
 namespace {
 
 constexpr int FT = 128;               // queries or keys per tile
+constexpr int FTHREADS = 128 + 2 * 256;  // two working groups behind the TMA and MMA warps
 constexpr int FCHUNK = FT * 128;      // bytes of 128 rows x 64 halves
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -71,7 +72,7 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, int code, int detail) {
   return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, status, code, detail));
 }
-__device__ __forceinline__ void group_barrier(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void group_barrier(int id) { asm volatile("bar.sync %0, 256;" ::"r"(id) : "memory"); }
 
 struct FlashParams {
   CUtensorMap tmQ, tmK, tmV;
@@ -110,38 +111,27 @@ struct FlashHead {
   }
 };
 
-// Bias of a tile whose smallest distance is `dlo` (window dlo .. dlo + 254): one value for all of
-// it, or window[c - r + 127] for column c of row r.  All 128 threads of a group call it.
+// Bias of the 128 x 128 pairs of a tile whose smallest distance is `dlo`: one value for all of it
+// (`flat`; a masked score is -inf before it is scaled, so that needs a positive scale), or
+// window[c - r + 127] for column c of row r.  All 256 threads of a group call it.
 struct TileBias {
-  float value;         // when !near
-  const float* row;    // when near: row[c] for this thread's row
-  bool near;
-  __device__ __forceinline__ TileBias(const float* bias, long long reach, long long dlo, int r, int slope,
-                                      float* window, bool flat_ok) {
-    value = 0.f;
-    near = false;
-    if (bias == nullptr) {
-      near = !flat_ok;
-      if (near) {
-        window[r] = window[r + 128] = 0.f;
-      }
-    } else if (flat_ok && (dlo >= reach || dlo + 254 <= -reach)) {
-      value = __ldg(bias + (dlo >= reach ? 2 * reach : 0));
+  float value = 0.f;
+  bool near = false;
+  __device__ __forceinline__ TileBias(const float* bias, long long reach, long long dlo, int gt, float* window,
+                                      bool flat_ok) {
+    if (flat_ok && (bias == nullptr || dlo >= reach || dlo + 254 <= -reach)) {
+      if (bias != nullptr) value = __ldg(bias + (dlo >= reach ? 2 * reach : 0));
     } else {
       near = true;
-#pragma unroll
-      for (int w = r; w < 256; w += 128) {
-        long long d = dlo + w;
-        d = d > reach ? reach : d < -reach ? -reach : d;
-        window[w] = __ldg(bias + d + reach);
-      }
+      long long d = dlo + gt;
+      d = d > reach ? reach : d < -reach ? -reach : d;
+      window[gt] = bias != nullptr ? __ldg(bias + d + reach) : 0.f;
     }
-    row = window + 127 + slope * r;
   }
 };
 
 template <int HS, int NST>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(FTHREADS, 1)
 flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ status) {
   constexpr int TILE = FCHUNK * (HS / 64);  // bytes of one operand tile
   extern __shared__ uint8_t smem_raw[];
@@ -149,6 +139,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
   __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2];
   __shared__ uint32_t tmem_slot;
   __shared__ float window[2][2][256];
+  __shared__ float exchange[2][2][2][FT];  // [tile][turn][half]: row maxima, at the end row sums
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -165,7 +156,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
       for (int t = 0; t < 2; ++t) {
         mbar_init(smem_u32(&q_full[t]), 1);
         mbar_init(smem_u32(&s_full[t]), 1);
-        mbar_init(smem_u32(&p_full[t]), 128);
+        mbar_init(smem_u32(&p_full[t]), 256);
         mbar_init(smem_u32(&o_full[t]), 1);
       }
       for (int s = 0; s < NST; ++s) {
@@ -269,7 +260,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
           const uint32_t b = v_s + s * TILE;
 #pragma unroll
           for (int ks = 0; ks < FT / 16; ++ks)
-            mma_f16_ts(tmem + 2 * FT + t * HS, tmem + t * FT + ks * 8, make_smem_desc(b + ks * 2048, FCHUNK, 1024),
+            mma_f16_ts(tmem + 2 * FT + t * HS, tmem + t * FT + (ks / 4) * 64 + (ks % 4) * 8, make_smem_desc(b + ks * 2048, FCHUNK, 1024),
                        IDESC_O, (j > 0 || ks > 0) ? 1u : 0u);
           if (j == nt - 1) tc_commit(smem_u32(&o_full[t]));
         }
@@ -287,53 +278,55 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
     }
   } else if (warp >= 4) {
     // ===================== softmax =====================
-    const int t = (warp - 4) >> 2, r = threadIdx.x & 127;
+    // thread: query row r of tile t, keys 64 half .. 64 half + 63 of every key tile
+    const int t = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;
+    const int r = threadIdx.x & 127, gt = (threadIdx.x - 128) & 255;
     const int nt = t ? n1 : n0;
     const int i = i0 + t * FT + r;
     const int vis = hd.visible(p, i);
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t s_col = lanes + t * FT, o_col = lanes + 2 * FT + t * HS;
+    const uint32_t s_col = lanes + t * FT + half * 64, o_col = lanes + 2 * FT + t * HS + half * (HS / 2);
     const float* bias = p.bias != nullptr ? p.bias + hd.head * (2 * p.reach + 1) : nullptr;
     const float c1 = p.c1;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nt; ++j) {
-      const TileBias tb(bias, p.reach, static_cast<long long>(j) * FT - (i0 + t * FT + FT - 1 + hd.off), r, -1,
-                        window[t][j & 1], c1 > 0.f);
+      float* win = window[t][j & 1];
+      const TileBias tb(bias, p.reach, static_cast<long long>(j) * FT - (i0 + t * FT + FT - 1 + hd.off), gt, win, c1 > 0.f);
       if (tb.near) group_barrier(1 + t);
       // a group that gave up still meets its barriers
       ok = ok && warp_wait(&s_full[t], j & 1, status, DEV_TIMEOUT_ACCUM, 0xc00 + t);
-      if (!ok) continue;
-      tc_fence_after();
-      const int lim = vis - j * FT;  // columns below it are seen
-      const bool masked = __any_sync(0xffffffffu, lim < FT);
-      // 64 scores at a time: raw with a flat bias, finished with a window
+      float mn = -INFINITY;
       uint32_t v[64];
-      auto fetch = [&](int c0) {
-        tmem_ld32(s_col + c0, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-        tmem_ld32(s_col + c0 + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+      if (ok) {
+        tc_fence_after();
+        tmem_ld32(s_col, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+        tmem_ld32(s_col + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
         tmem_ld_wait();
+        // raw scores with a flat bias, finished ones with a window
         if (tb.near) {
+          const float* row = win + (FT - 1) - r + 64 * half;
 #pragma unroll
-          for (int c = 0; c < 64; ++c) v[c] = __float_as_uint(fmaf(__uint_as_float(v[c]), c1, tb.row[c0 + c]));
+          for (int c = 0; c < 64; ++c) v[c] = __float_as_uint(fmaf(__uint_as_float(v[c]), c1, row[c]));
         }
-        if (masked) {
+        const int lim = vis - j * FT - 64 * half;  // columns below it are seen
+        if (__any_sync(0xffffffffu, lim < 64)) {
 #pragma unroll
-          for (int c = 0; c < 64; ++c) v[c] = c0 + c < lim ? v[c] : 0xff800000u;  // -inf
+          for (int c = 0; c < 64; ++c) v[c] = c < lim ? v[c] : 0xff800000u;  // -inf
         }
-      };
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c0 = 0; c0 < FT; c0 += 64) {
-        fetch(c0);
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int c = 0; c < 64; c += 8)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             top[e] = fmaxf(top[e], fmaxf(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])));
+        mn = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        if (!tb.near && mn > -INFINITY) mn = fmaf(mn, c1, tb.value);
       }
-      float mn = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      if (!tb.near && mn > -INFINITY) mn = fmaf(mn, c1, tb.value);
+      exchange[t][j & 1][half][r] = mn;
+      group_barrier(1 + t);
+      if (!ok) continue;
+      mn = fmaxf(mn, exchange[t][j & 1][half ^ 1][r]);
       if (__any_sync(0xffffffffu, mn > m + 8.f)) {  // also a row's first visible key (m = -inf)
         mn = fmaxf(m, mn);
         const float a = mn == -INFINITY ? 1.f : ex2(m - mn);
@@ -341,7 +334,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
         m = mn;
         if (j > 0) {  // O exists from the second tile on
 #pragma unroll
-          for (int c = 0; c < HS; c += 16) {
+          for (int c = 0; c < HS / 2; c += 16) {
             uint32_t w[16];
             tmem_ld16(o_col + c, w);
             tmem_ld_wait();
@@ -356,22 +349,18 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
       const F2 ca2(ca, ca), cb2(cb, cb);
       F2 sum[2] = {F2(0.f, 0.f), F2(0.f, 0.f)};
 #pragma unroll
-      for (int c0 = 0; c0 < FT; c0 += 64) {
-        fetch(c0);
+      for (int c = 0; c < 64; c += 32) {
+        uint32_t w[16];
 #pragma unroll
-        for (int c = 0; c < 64; c += 32) {
-          uint32_t w[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float x, y;
-            fma2(F2(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])), ca2, cb2).get(x, y);
-            x = ex2(x);
-            y = ex2(y);
-            sum[e & 1] = add2(sum[e & 1], F2(x, y));
-            w[e] = pack_half2(x, y);
-          }
-          tmem_st16(s_col + (c0 + c) / 2, w);
+        for (int e = 0; e < 16; ++e) {
+          float x, y;
+          fma2(F2(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])), ca2, cb2).get(x, y);
+          x = ex2(x);
+          y = ex2(y);
+          sum[e & 1] = add2(sum[e & 1], F2(x, y));
+          w[e] = pack_half2(x, y);
         }
+        tmem_st16(s_col + c / 2, w);  // over scores this thread has read
       }
       float sa, sb;
       add2(sum[0], sum[1]).get(sa, sb);
@@ -381,16 +370,20 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
       mbar_arrive(smem_u32(&p_full[t]));
     }
     // ---- result ----
+    // turn nt & 1 of the exchange was last read before the barrier of tile nt - 1
+    exchange[t][nt & 1][half][r] = l;
+    group_barrier(1 + t);
+    l += exchange[t][nt & 1][half ^ 1][r];
     if (nt > 0 && ok) {
       ok = warp_wait(&o_full[t], 0, status, DEV_TIMEOUT_ACCUM, 0xc10 + t);
       tc_fence_after();
     }
     if (ok) {
-      const bool real = i < p.tq;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const bool real = i < p.tq, some = nt > 0 && vis > 0 && l > 0.f;
+      const float inv = some ? 1.f / l : 0.f;
       __half* out = p.O + i * p.ldo + hd.head * p.sho + hd.batch * p.sbo;
 #pragma unroll
-      for (int c = 0; c < HS; c += 16) {
+      for (int c = 0; c < HS / 2; c += 16) {
         uint32_t w[16];
         if (nt > 0) {
           tmem_ld16(o_col + c, w);
@@ -399,13 +392,13 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
         uint32_t h[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          h[e] = vis > 0 && nt > 0 && l > 0.f ? pack_half2(__uint_as_float(w[2 * e]) * inv, __uint_as_float(w[2 * e + 1]) * inv) : 0u;
-        if (real && c < p.hs) *reinterpret_cast<uint4*>(out + c) = make_uint4(h[0], h[1], h[2], h[3]);
-        if (real && c + 8 < p.hs) *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(h[4], h[5], h[6], h[7]);
+          h[e] = some ? pack_half2(__uint_as_float(w[2 * e]) * inv, __uint_as_float(w[2 * e + 1]) * inv) : 0u;
+        const int at = half * (HS / 2) + c;
+        if (real && at < p.hs) *reinterpret_cast<uint4*>(out + at) = make_uint4(h[0], h[1], h[2], h[3]);
+        if (real && at + 8 < p.hs) *reinterpret_cast<uint4*>(out + at + 8) = make_uint4(h[4], h[5], h[6], h[7]);
       }
-      if (real)
-        p.lse[(static_cast<long long>(hd.batch) * p.heads + hd.head) * p.tq + i] =
-            l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+      if (real && half == 0)
+        p.lse[(static_cast<long long>(hd.batch) * p.heads + hd.head) * p.tq + i] = some ? (m + log2f(l)) * kLn2 : -INFINITY;
     }
   }
 
@@ -427,9 +420,10 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
 //                    and the sums of dS by distance for the bias table
 // with P = exp(X - lse), dS = P (Y - delta).  X and Y are formed twice in all (seven products instead of
 // five), which keeps every sum inside one CTA: no atomics on dQ, the same bits every time.
-// Two groups of 128 threads (a thread per row) take the streamed tiles in turn; X and Y of the next
-// tile are formed while they work.  Tensor memory: per group X (64 columns) and Y (64), overwritten
-// by P and dS as fp16 left operands; the results behind them.
+// Two groups of 256 threads (two per row, 32 columns each) take the streamed tiles in turn; X and Y of
+// the next tile are formed while they work.  Tensor memory: per group X (64 columns) and Y (64),
+// overwritten by P and dS as fp16 left operands (each thread over the columns it has read); the results
+// behind them.
 //
 // Range: P enters its product times 2^12 (probabilities down to 2^-26 stay normal numbers).  dS
 // enters times a power of two that brings its bound 2 max|dO| max|v| (Cauchy-Schwarz, per sequence
@@ -556,7 +550,7 @@ flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long lon
 }
 
 template <int HS, bool KEYS>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(FTHREADS, 1)
 flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict__ status) {
   constexpr int ROWS = FCHUNK * (HS / 64);   // bytes of a resident operand
   constexpr int TILE = BCHUNK * (HS / 64);   // bytes of a streamed tile
@@ -565,9 +559,9 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
   __shared__ uint32_t tmem_slot;
   __shared__ float window[2][2][256];
   __shared__ __align__(16) float colx[KEYS ? 2 : 1][2][BN], coly[KEYS ? 2 : 1][2][BN];
-  __shared__ float diag[KEYS ? 1 : 8][96];
+  __shared__ float diag[KEYS ? 1 : 16][64];
   __shared__ float dist_s[KEYS ? 1 : 2][KEYS ? 1 : kDistSmem];
-  __shared__ float far_s[2][2][4];
+  __shared__ float far_s[2][2][8];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -584,7 +578,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       }
       for (int g = 0; g < 2; ++g) {
         mbar_init(smem_u32(&x_full[g]), 1);
-        mbar_init(smem_u32(&p_full[g]), 128);
+        mbar_init(smem_u32(&p_full[g]), 256);
       }
       fence_mbar_init();
     }
@@ -695,12 +689,12 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
 #pragma unroll
         for (int ks = 0; ks < BN / 16; ++ks) {
           if (KEYS)  // dV += P dO
-            mma_f16_ts(tmem + 2 * FT + HS, a + ks * 8, make_smem_desc(b + TILE + ks * 2048, BCHUNK, 1024), IDESC_ACC,
+            mma_f16_ts(tmem + 2 * FT + HS, a + (ks / 2) * 32 + (ks % 2) * 8, make_smem_desc(b + TILE + ks * 2048, BCHUNK, 1024), IDESC_ACC,
                        (it > 0 || ks > 0) ? 1u : 0u);
         }
 #pragma unroll
         for (int ks = 0; ks < BN / 16; ++ks)  // dK += dS Q,  dQ += dS K
-          mma_f16_ts(tmem + 2 * FT, a + BN + ks * 8, make_smem_desc(b + ks * 2048, BCHUNK, 1024), IDESC_ACC,
+          mma_f16_ts(tmem + 2 * FT, a + BN + (ks / 2) * 32 + (ks % 2) * 8, make_smem_desc(b + ks * 2048, BCHUNK, 1024), IDESC_ACC,
                      (it > 0 || ks > 0) ? 1u : 0u);
         tc_commit(smem_u32(&b_empty[s]));
         if (it == n - 1) tc_commit(smem_u32(&acc_full));
@@ -709,10 +703,12 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     }
   } else if (warp >= 4) {
     // ===================== probabilities and their gradient =====================
-    const int g = (warp - 4) >> 2, r = threadIdx.x & 127;
+    // thread: row r, columns 32 half .. 32 half + 31 of every streamed tile of group g
+    const int g = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;
+    const int r = threadIdx.x & 127, gt = (threadIdx.x - 128) & 255;
     const int row = r0 + r;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t x_col = lanes + g * FT, y_col = x_col + BN;
+    const uint32_t x_col = lanes + g * FT + half * 32, y_col = x_col + BN;
     const float c1 = p.c1;
     const float up = ds_scale(p, batch, kv);
     const float f = up * (1.f / 4096.f);  // on P, which is formed times 2^12
@@ -729,7 +725,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     if (dist_on) {
       float* out = p.dist + (((static_cast<long long>(batch) * p.heads + head) * p.row_tiles + tile) * 2 + g) * p.width;
       dist = p.width <= kDistSmem ? dist_s[g] : out;
-      for (int e = r; e < p.width; e += 128) dist[e] = 0.f;
+      for (int e = gt; e < p.width; e += 256) dist[e] = 0.f;
       group_barrier(1 + g);
     }
     bool ok = true;
@@ -747,102 +743,95 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       if (flat) {
         if (bias != nullptr) value = __ldg(bias + (dlo >= p.reach ? 2 * p.reach : 0));
       } else {
-        for (int w = r; w < FT + BN; w += 128) {
-          long long d = dlo + w;
-          d = d > p.reach ? p.reach : d < -p.reach ? -p.reach : d;
-          win[w] = bias != nullptr ? __ldg(bias + d + p.reach) : 0.f;
-        }
+        long long d = dlo + gt;
+        d = d > p.reach ? p.reach : d < -p.reach ? -p.reach : d;
+        win[gt] = bias != nullptr ? __ldg(bias + d + p.reach) : 0.f;
       }
-      if (KEYS && r < BN) {
+      if (KEYS && gt < BN) {
         // per column: what is added to the scaled score, and to Y times f
-        const float2 st = p.stats[(static_cast<long long>(batch) * p.heads + h) * p.tq_pad + at + r];
-        colx[KEYS ? g : 0][turn][r] = (flat ? value : 0.f) + 12.f - st.x;
-        coly[KEYS ? g : 0][turn][r] = -st.y * f;
+        const float2 st = p.stats[(static_cast<long long>(batch) * p.heads + h) * p.tq_pad + at + gt];
+        colx[KEYS ? g : 0][turn][gt] = (flat ? value : 0.f) + 12.f - st.x;
+        coly[KEYS ? g : 0][turn][gt] = -st.y * f;
       }
       if (KEYS || !flat) group_barrier(1 + g);
       // window[c - r + 127] for query rows, window[r - c + 63] for key rows
-      const float* wrow = KEYS ? win + (BN - 1) + r : win + (FT - 1) - r;
+      const float* wrow = KEYS ? win + (BN - 1) + r - 32 * half : win + (FT - 1) - r + 32 * half;
       ok = ok && warp_wait(&x_full[g], turn, status, DEV_TIMEOUT_ACCUM, 0xf00 + g);
-      // columns lo .. hi - 1 of this row take part
-      int lo = 0, hi = BN;
+      // of this thread's columns those from lo to hi - 1 take part
+      int lo = 0, hi = 32;
       if (KEYS) {
-        hi = row < klen ? BN : 0;
+        hi = row < klen ? 32 : 0;
         if (p.causal) {
-          const long long from = row - off - at;
-          lo = from < 0 ? 0 : from > BN ? BN : static_cast<int>(from);
+          const long long from = row - off - at - 32 * half;
+          lo = from < 0 ? 0 : from > 32 ? 32 : static_cast<int>(from);
         }
       } else {
-        hi = vis - at;
+        hi = vis - at - 32 * half;
       }
-      const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < BN);
       const bool sweep = !KEYS && !beyond && p.reach > 0;  // sums along the diagonals
-      float run = 0.f;
       F2 all(0.f, 0.f);
       if (ok) {
         tc_fence_after();
-        const F2 c12(c1, c1), f2(f, f);
         const float rx = (flat ? value : 0.f) + 12.f - mine.x, ry = -mine.y * f;
+        uint32_t x[32], y[32];
+        tmem_ld32(x_col, x);
+        tmem_ld32(y_col, y);
+        tmem_ld_wait();
+        if (!flat) {  // the window's bias joins the scores here, everything else below
 #pragma unroll
-        for (int c = 0; c < BN; c += 32) {
-          uint32_t x[32], y[32];
-          tmem_ld32(x_col + c, x);
-          tmem_ld32(y_col + c, y);
-          tmem_ld_wait();
-          if (!flat) {  // the window's bias joins the scores here, everything else below
+          for (int e = 0; e < 32; ++e)
+            x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), c1, KEYS ? wrow[-e] : wrow[e]));
+        }
+        if (__any_sync(0xffffffffu, lo > 0 || hi < 32)) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), c1, KEYS ? wrow[-(c + e)] : wrow[c + e]));
-          }
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (c + e < lo || c + e >= hi) {
-                x[e] = 0xff800000u;  // -inf
-                y[e] = 0u;
-              }
-          }
-          const F2 cx = flat ? c12 : F2(1.f, 1.f);
-          uint32_t pw[16], dw[16];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            F2 sx(rx, rx), sy(ry, ry);
-            if (KEYS) {
-              const float2 ax = *reinterpret_cast<const float2*>(&colx[KEYS ? g : 0][turn][c + e]);
-              const float2 ay = *reinterpret_cast<const float2*>(&coly[KEYS ? g : 0][turn][c + e]);
-              sx = F2(ax.x, ax.y);
-              sy = F2(ay.x, ay.y);
+          for (int e = 0; e < 32; ++e)
+            if (e < lo || e >= hi) {
+              x[e] = 0xff800000u;  // -inf
+              y[e] = 0u;
             }
-            float p0, p1;
-            fma2(F2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), cx, sx).get(p0, p1);
-            p0 = ex2(p0);
-            p1 = ex2(p1);
-            const F2 ds = mul2(F2(p0, p1), fma2(F2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), f2, sy));
-            float d0, d1;
-            ds.get(d0, d1);
-            if (KEYS) pw[e / 2] = pack_half2(p0, p1);
-            else all = add2(all, ds);
-            dw[e / 2] = pack_half2(d0, d1);
-            if (!KEYS) {
-              y[e] = __float_as_uint(d0);
-              y[e + 1] = __float_as_uint(d1);
-            }
-          }
-          if (KEYS) tmem_st16(x_col + c / 2, pw);
-          tmem_st16(y_col + c / 2, dw);
-          if (c + 32 == BN) {
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(smem_u32(&p_full[g]));
-          }
-          if (sweep && dist_on) {
-            // the running sum of a diagonal moves down one lane per column; lane 31 ends it
+        }
+        const float cx1 = flat ? c1 : 1.f;
+        const F2 cx(cx1, cx1), f2(f, f);
+        uint32_t pw[16], dw[16];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              run = __shfl_up_sync(0xffffffffu, run, 1);
-              run = (lane == 0 ? 0.f : run) + __uint_as_float(y[e]);
-              if (lane == 31) diag[KEYS ? 0 : warp - 4][c + e] = run;
-            }
+        for (int e = 0; e < 32; e += 2) {
+          F2 sx(rx, rx), sy(ry, ry);
+          if (KEYS) {
+            const float2 ax = *reinterpret_cast<const float2*>(&colx[KEYS ? g : 0][turn][32 * half + e]);
+            const float2 ay = *reinterpret_cast<const float2*>(&coly[KEYS ? g : 0][turn][32 * half + e]);
+            sx = F2(ax.x, ax.y);
+            sy = F2(ay.x, ay.y);
           }
+          float p0, p1;
+          fma2(F2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), cx, sx).get(p0, p1);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          const F2 ds = mul2(F2(p0, p1), fma2(F2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), f2, sy));
+          float d0, d1;
+          ds.get(d0, d1);
+          if (KEYS) pw[e / 2] = pack_half2(p0, p1);
+          else all = add2(all, ds);
+          dw[e / 2] = pack_half2(d0, d1);
+          if (!KEYS) {
+            y[e] = __float_as_uint(d0);
+            y[e + 1] = __float_as_uint(d1);
+          }
+        }
+        if (KEYS) tmem_st16(x_col, pw);
+        tmem_st16(y_col, dw);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&p_full[g]));
+        if (sweep && dist_on) {
+          // the running sum of a diagonal moves down one lane per column; lane 31 ends it
+          float run = 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            run = __shfl_up_sync(0xffffffffu, run, 1);
+            run = (lane == 0 ? 0.f : run) + __uint_as_float(y[e]);
+            if (lane == 31) diag[KEYS ? 0 : warp - 4][e] = run;  // diagonal e - 31
+          }
+          if (lane < 31) diag[KEYS ? 0 : warp - 4][32 + lane] = run;  // diagonal 31 - lane
         }
       }
       if (dist_on) {
@@ -852,16 +841,15 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
           if (dlo >= p.reach) far_hi += a0 + a1;
           else far_lo += a0 + a1;
         } else {
-          // diag[warp][c - 31 + 31]: lane 31 left diagonals -31 .. 32 at 0 .. 63; the others end here
-          if (lane < 31) diag[KEYS ? 0 : warp - 4][64 + lane] = run;  // diagonal 63 - lane
           group_barrier(1 + g);
-          for (int w = r; w < FT + BN - 1; w += 128) {
+          if (gt < FT + BN - 1) {
+            const int w = gt;
             float sum = 0.f;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              // column - row = w - 127, row = 32 q + lane: diagonal w - 127 + 32 q of that warp
-              const int dg = w - (FT - 1) + 32 * q;
-              if (dg >= -31 && dg <= 63) sum += diag[KEYS ? 0 : g * 4 + q][dg <= 32 ? dg + 31 : 64 + 63 - dg];
+            for (int q = 0; q < 8; ++q) {
+              // column - row = w - 127; warp q of the group: rows 32 (q % 4) + lane, columns 32 (q / 4) + e
+              const int dg = w - (FT - 1) + 32 * (q & 3) - 32 * (q >> 2);  // e - lane
+              if (dg >= -31 && dg <= 31) sum += diag[KEYS ? 0 : g * 8 + q][dg <= 0 ? dg + 31 : 32 + 31 - dg];
             }
             const long long d = dlo + w;
             if (d >= p.reach) far_hi += sum;
@@ -880,25 +868,25 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
         far_hi += __shfl_xor_sync(0xffffffffu, far_hi, o);
       }
       if (lane == 0) {
-        far_s[g][0][warp & 3] = far_lo;
-        far_s[g][1][warp & 3] = far_hi;
+        far_s[g][0][(warp - 4) & 7] = far_lo;
+        far_s[g][1][(warp - 4) & 7] = far_hi;
       }
       group_barrier(1 + g);
-      if (r == 0) {
-        float s[2];
-        for (int k = 0; k < 2; ++k) s[k] = (far_s[g][k][0] + far_s[g][k][1]) + (far_s[g][k][2] + far_s[g][k][3]);
+      if (gt == 0) {
+        float s[2] = {0.f, 0.f};
+        for (int k = 0; k < 16; ++k) s[k >> 3] += far_s[g][k >> 3][k & 7];
         if (-p.reach - low >= 0 && -p.reach - low < p.width) dist[-p.reach - low] += s[0];
         if (p.reach - low >= 0 && p.reach - low < p.width) dist[p.reach - low] += s[1];
       }
       group_barrier(1 + g);
       if (p.width <= kDistSmem) {
         float* out = p.dist + (((static_cast<long long>(batch) * p.heads + head) * p.row_tiles + tile) * 2 + g) * p.width;
-        for (int e = r; e < p.width; e += 128) out[e] = dist[e] * (1.f / up);
+        for (int e = gt; e < p.width; e += 256) out[e] = dist[e] * (1.f / up);
       } else {
-        for (int e = r; e < p.width; e += 128) dist[e] *= 1.f / up;
+        for (int e = gt; e < p.width; e += 256) dist[e] *= 1.f / up;
       }
     }
-    // ---- results: group 0 writes dK, group 1 dV; the two share dQ's columns ----
+    // ---- results: group 0 writes dK, group 1 dV; both share dQ's columns ----
     if (n > 0 && ok) {
       ok = warp_wait(&acc_full, 0, status, DEV_TIMEOUT_ACCUM, 0xf10 + g);
       tc_fence_after();
@@ -911,7 +899,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       out += row * ld + head * sh + batch * sb;
       const float factor = KEYS && g == 1 ? 1.f / 4096.f : p.scale / up;
       const uint32_t col0 = lanes + 2 * FT + (KEYS && g == 1 ? HS : 0);
-      const int c_from = KEYS ? 0 : g * (HS / 2), c_to = KEYS ? HS : c_from + HS / 2;
+      const int c_from = KEYS ? half * (HS / 2) : (2 * g + half) * (HS / 4), c_to = c_from + (KEYS ? HS / 2 : HS / 4);
       for (int c = c_from; c < c_to; c += 16) {
         uint32_t w[16];
         if (n > 0) {
@@ -1031,7 +1019,7 @@ cudaError_t forward_hs(FlashParams& p, cudaStream_t stream, int* status) {
   p.qblocks = (p.tq + 2 * FT - 1) / (2 * FT);
   const long long grid = static_cast<long long>(p.qblocks) * p.heads * p.batch;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
-  return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(384), smem, stream, pdl_enabled(), p, status);
+  return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(FTHREADS), smem, stream, pdl_enabled(), p, status);
 }
 
 template <int HS, bool KEYS>
@@ -1044,7 +1032,7 @@ cudaError_t backward_hs(const FlashBwdParams& p, cudaStream_t stream, int* statu
   FlashBwdParams q = p;
   q.row_tiles = ((KEYS ? p.tk : p.tq) + FT - 1) / FT;
   const long long grid = static_cast<long long>(q.row_tiles) * (KEYS ? p.kv_heads : p.heads) * p.batch;
-  return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(384), smem, stream, pdl_enabled(), q, status);
+  return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(FTHREADS), smem, stream, pdl_enabled(), q, status);
 }
 
 }  // namespace
