@@ -2117,8 +2117,17 @@ int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, c
   if (dtype == GINN_B200_F16 && t_force_path == PATH_AUTO && gb::flash_supported(f)) {
     Scratch scratch(stream);
     if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
-    CU_TRY(gb::launch_flash_forward(f, stream, ctx->d_status));
-    g_launches.fetch_add(1);
+    long long floats = 0;
+    const int splits = gb::flash_token_splits(f, ctx->num_sms, &floats);
+    int launches = 1;
+    if (splits > 0) {
+      float* parts = nullptr;
+      if (floats > 0) CU_TRY(scratch.take(&parts, floats));
+      CU_TRY(gb::launch_flash_token(f, splits, parts, &launches, stream));
+    } else {
+      CU_TRY(gb::launch_flash_forward(f, stream, ctx->d_status));
+    }
+    g_launches.fetch_add(launches);
     return GINN_B200_OK;
   }
   return relative_composed(device, stream, dtype, *a, nullptr);

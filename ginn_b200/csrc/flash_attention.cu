@@ -410,6 +410,291 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
   }
 }
 
+// ---- a few queries against a long cache ---------------------------------------------------------
+//
+// A token's attention reads every cached key and value once and does little with them: it is bound by
+// HBM, and what counts is many loads in flight and no work per byte beside them.  The queries that
+// share a key head (heads of the group x positions, at most 16 rows) go together, so that the cache is
+// read once.  The keys are split over CTAs, and over the eight warps of a CTA in blocks of 16; a warp
+// keeps its own running maximum, sum and result.  Operands go from global memory to registers in the
+// layout of mma.m16n8k16 without a stop in shared memory: the order in which a contraction runs over
+// the head elements is free, so a lane's 16 contiguous bytes of a key serve as its share of two
+// fragments, and the values of two neighbouring keys, interleaved by byte permutes, as those of the second
+// product.  (A tcgen05 tile would be 128 rows high for these 1 to 16, with the cache passing through
+// shared memory: 370 us where this takes a quarter.)
+constexpr int kTokenRows = 16;
+constexpr int kTokenWarps = 8;
+
+struct TokenParams {
+  const __half *q, *k, *v;
+  long long ldq, shq, sbq, ldk, shk, sbk, ldv, shv, sbv;
+  __half* o;
+  long long ldo, sho, sbo;
+  float* lse;
+  float* part;    // [batch][kv][split][row][HS] results, then their (maximum, sum) pairs
+  float2* stat;   // [batch][kv][split][row]
+  const float* bias;
+  int tq, tk, hs, heads, kv_heads, group, batch, rows, splits, chunk;
+  long long reach, q_offset;
+  const int* q_offsets;
+  const int* q_lengths;
+  const int* k_lengths;
+  float c1;
+  int causal;
+};
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 load_stream(const __half* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+// Final values of one row: o and lse.
+__device__ __forceinline__ void token_store(const TokenParams& p, int batch, int kv, int row, int h, float value, float m, float l) {
+  const int head = kv * p.group + row / p.tq, i = row % p.tq;
+  if (h < p.hs) p.o[h + i * p.ldo + head * p.sho + batch * p.sbo] = __float2half_rn(l > 0.f ? value / l : 0.f);
+  if (h == 0)
+    p.lse[(static_cast<long long>(batch) * p.heads + head) * p.tq + i] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+}
+
+template <int HS>
+__global__ void __launch_bounds__(32 * kTokenWarps, 1)
+flash_token_kernel(const TokenParams p) {
+  __shared__ float res[kTokenRows][HS];
+  __shared__ float mx[kTokenWarps][kTokenRows], sm[kTokenWarps][kTokenRows];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int split = static_cast<int>(blockIdx.x) % p.splits;
+  const long long unit = blockIdx.x / p.splits;
+  const int batch = static_cast<int>(unit / p.kv_heads), kv = static_cast<int>(unit % p.kv_heads);
+  const int klen = rel_length(p.k_lengths, batch, p.tk), qlen = rel_length(p.q_lengths, batch, p.tq);
+  const long long off = rel_offset(p.q_offset, p.q_offsets, batch);
+  // this lane's two rows of the scores: g and g + 8
+  int vis[2];
+  long long pos[2];
+  const float* bias[2] = {nullptr, nullptr};
+  const __half* qrow[2];
+  float far_lo[2] = {0.f, 0.f};
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int row = g + 8 * x, i = row % p.tq, head = kv * p.group + row / p.tq;
+    const bool real = row < p.rows;
+    pos[x] = i + off;
+    vis[x] = real && i < qlen ? rel_visible(p.causal, pos[x], klen) : 0;
+    qrow[x] = real ? p.q + i * p.ldq + head * p.shq + batch * p.sbq : nullptr;
+    if (p.bias != nullptr && real) {
+      bias[x] = p.bias + head * (2 * p.reach + 1) + p.reach;
+      far_lo[x] = bias[x][-p.reach];
+    }
+  }
+  const int last = qlen > 0 ? rel_visible(p.causal, qlen - 1 + off, klen) : 0;  // the most any row sees
+  const long long first_pos = off;
+  const int begin = split * p.chunk, end = begin + p.chunk < last ? begin + p.chunk : last;
+
+  uint32_t q[HS / 32][2][4];
+#pragma unroll
+  for (int s = 0; s < HS / 32; ++s)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (qrow[x] != nullptr && 32 * s + 8 * c < p.hs) w = *reinterpret_cast<const uint4*>(qrow[x] + 32 * s + 8 * c);
+      q[s][x][0] = w.x; q[s][x][1] = w.y; q[s][x][2] = w.z; q[s][x][3] = w.w;
+    }
+  float acc[HS / 8][4];
+#pragma unroll
+  for (int e = 0; e < HS / 8; ++e) acc[e][0] = acc[e][1] = acc[e][2] = acc[e][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+  const __half* kp = p.k + kv * p.shk + batch * p.sbk;
+  const __half* vp = p.v + kv * p.shv + batch * p.sbv;
+  uint4 kr[2][HS / 32], vr[HS / 64][4];
+  auto load_k = [&](int j) {  // keys j + g and j + 8 + g, head elements 32 s + 8 c ..
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int s = 0; s < HS / 32; ++s) {
+        const int key = j + 8 * t + g;
+        kr[t][s] = make_uint4(0, 0, 0, 0);
+        if (key < end && 32 * s + 8 * c < p.hs) kr[t][s] = load_stream(kp + key * p.ldk + 32 * s + 8 * c);
+      }
+  };
+  auto load_v = [&](int j) {  // keys j + 2 c + {0, 1, 8, 9}, head elements 64 s + 8 g ..
+#pragma unroll
+    for (int s = 0; s < HS / 64; ++s)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int key = j + 2 * c + (t & 1) + 8 * (t >> 1);
+        vr[s][t] = make_uint4(0, 0, 0, 0);
+        if (key < end && 64 * s + 8 * g < p.hs) vr[s][t] = load_stream(vp + key * p.ldv + 64 * s + 8 * g);
+      }
+  };
+  int j = begin + 16 * warp;
+  if (j < end) {
+    load_k(j);
+    load_v(j);
+  }
+  for (; j < end; j += 16 * kTokenWarps) {
+    float sc[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+#pragma unroll
+      for (int s = 0; s < HS / 32; ++s) {
+        mma_16816(sc[t], q[s][0][0], q[s][1][0], q[s][0][1], q[s][1][1], kr[t][s].x, kr[t][s].y);
+        mma_16816(sc[t], q[s][0][2], q[s][1][2], q[s][0][3], q[s][1][3], kr[t][s].z, kr[t][s].w);
+      }
+    }
+    const int next = j + 16 * kTokenWarps;
+    if (next < end) load_k(next);
+    // scores of row g + 8 x at keys j + 8 t + 2 c + y: sc[t][2 x + y]
+    const bool flat = p.bias == nullptr || j + 15 - first_pos <= -p.reach;  // for every row: positions only grow
+    const bool full = j + 16 <= vis[0] && j + 16 <= vis[1];
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int key = j + 8 * t + 2 * c + y;
+          float b = far_lo[x];
+          if (!flat && bias[x] != nullptr) {
+            long long d = key - pos[x];
+            d = d > p.reach ? p.reach : d < -p.reach ? -p.reach : d;
+            b = bias[x][d];
+          }
+          float v = fmaf(sc[t][2 * x + y], p.c1, b);
+          if (!full && key >= vis[x]) v = -INFINITY;
+          sc[t][2 * x + y] = v;
+          top[x] = fmaxf(top[x], v);
+        }
+    bool grow = false;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
+      top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
+      grow = grow || top[x] > m[x] + 8.f;
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+      float a[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float mn = fmaxf(m[x], top[x]);
+        a[x] = mn == -INFINITY ? 1.f : ex2(m[x] - mn);
+        m[x] = mn;
+        l[x] *= a[x];
+      }
+#pragma unroll
+      for (int e = 0; e < HS / 8; ++e) {
+        acc[e][0] *= a[0];
+        acc[e][1] *= a[0];
+        acc[e][2] *= a[1];
+        acc[e][3] *= a[1];
+      }
+    }
+    uint32_t pr[2][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float mu = m[x] == -INFINITY ? 0.f : m[x];
+        const float p0 = ex2(sc[t][2 * x] - mu), p1 = ex2(sc[t][2 * x + 1] - mu);
+        l[x] += p0 + p1;
+        pr[t][x] = pack_half2(p0, p1);
+      }
+#pragma unroll
+    for (int s = 0; s < HS / 64; ++s) {
+      const uint32_t v0[4] = {vr[s][0].x, vr[s][0].y, vr[s][0].z, vr[s][0].w}, v1[4] = {vr[s][1].x, vr[s][1].y, vr[s][1].z, vr[s][1].w};
+      const uint32_t v8[4] = {vr[s][2].x, vr[s][2].y, vr[s][2].z, vr[s][2].w}, v9[4] = {vr[s][3].x, vr[s][3].y, vr[s][3].z, vr[s][3].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {  // head element 64 s + 8 n + e for column n of the fragment
+        const uint32_t pick = e & 1 ? 0x7632u : 0x5410u;
+        mma_16816(acc[8 * s + e], pr[0][0], pr[0][1], pr[1][0], pr[1][1], __byte_perm(v0[e / 2], v1[e / 2], pick),
+                  __byte_perm(v8[e / 2], v9[e / 2], pick));
+      }
+    }
+    if (next < end) load_v(next);
+  }
+  // ---- the warps' results together, in order ----
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+    if (c == 0) {
+      mx[warp][g + 8 * x] = m[x];
+      sm[warp][g + 8 * x] = l[x];
+    }
+  }
+  __syncthreads();
+  float scale[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    float all = -INFINITY;
+    for (int w = 0; w < kTokenWarps; ++w) all = fmaxf(all, mx[w][g + 8 * x]);
+    scale[x] = m[x] == -INFINITY ? 0.f : ex2(m[x] - all);
+  }
+  for (int w = 0; w < kTokenWarps; ++w) {
+    if (warp == w) {
+#pragma unroll
+      for (int e = 0; e < HS / 8; ++e)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // element k of the fragment: row g + 8 (k / 2), column n = 2 c + k % 2
+          float& r = res[g + 8 * (k >> 1)][64 * (e >> 3) + 8 * (2 * c + (k & 1)) + (e & 7)];
+          const float v = acc[e][k] * scale[k >> 1];
+          r = w == 0 ? v : r + v;
+        }
+    }
+    __syncthreads();
+  }
+  for (int at = threadIdx.x; at < p.rows * HS; at += 32 * kTokenWarps) {
+    const int row = at / HS, h = at % HS;
+    float all = -INFINITY, sum = 0.f;
+    for (int w = 0; w < kTokenWarps; ++w) all = fmaxf(all, mx[w][row]);
+    for (int w = 0; w < kTokenWarps; ++w) sum += mx[w][row] == -INFINITY ? 0.f : sm[w][row] * ex2(mx[w][row] - all);
+    if (p.splits == 1) {
+      token_store(p, batch, kv, row, h, res[row][h], all, sum);
+    } else {
+      const long long to = (unit * p.splits + split) * p.rows + row;
+      p.part[to * HS + h] = res[row][h];
+      if (h == 0) p.stat[to] = make_float2(all, sum);
+    }
+  }
+}
+
+// The splits' results together, in order: one CTA per row of a (sequence, key head).
+template <int HS>
+__global__ void __launch_bounds__(HS)
+flash_token_join_kernel(const TokenParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const long long unit = blockIdx.x / p.rows;
+  const int row = static_cast<int>(blockIdx.x % p.rows), h = threadIdx.x;
+  const int batch = static_cast<int>(unit / p.kv_heads), kv = static_cast<int>(unit % p.kv_heads);
+  float m = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.stat[(unit * p.splits + s) * p.rows + row].x);
+  float l = 0.f, v = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const long long at = (unit * p.splits + s) * p.rows + row;
+    const float2 st = p.stat[at];
+    if (st.x == -INFINITY) continue;
+    const float a = ex2(st.x - m);
+    l += st.y * a;
+    v += p.part[at * HS + h] * a;
+  }
+  token_store(p, batch, kv, row, h, v, m, l);
+}
+
 // ---- backward -----------------------------------------------------------------------------------
 //
 // Two kernels of one shape: a CTA keeps 128 rows of two operands (A1, A2) in shared memory, streams
@@ -1048,6 +1333,59 @@ cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* s
   FlashParams p;
   if (!fill_params(a, &p)) return cudaErrorInvalidValue;
   return a.hs <= 64 ? forward_hs<64, 3>(p, stream, status) : forward_hs<128, 2>(p, stream, status);
+}
+
+int flash_token_splits(const FlashArgs& a, int num_sms, long long* floats) {
+  const int rows = a.heads / a.kv_heads * a.tq;
+  *floats = 0;
+  if (rows > kTokenRows) return 0;
+  // Eight CTAs' worth of work per SM, so that ragged lengths even out; a CTA takes at least 128 keys (one
+  // block per warp) and in multiples of that.
+  const long long units = static_cast<long long>(a.kv_heads) * a.batch, step = 16 * kTokenWarps;
+  long long chunk = (a.tk * units + 8LL * num_sms - 1) / (8LL * num_sms);
+  chunk = (chunk + step - 1) / step * step;
+  const long long splits = (a.tk + chunk - 1) / chunk;
+  if (splits * units > 0x7fffffffLL || units * rows > 0x7fffffffLL) return 0;
+  if (splits > 1) *floats = units * splits * rows * ((a.hs <= 64 ? 64 : 128) + 2);
+  return static_cast<int>(splits);
+}
+
+cudaError_t launch_flash_token(const FlashArgs& a, int splits, float* scratch, int* launches, cudaStream_t stream) {
+  TokenParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = static_cast<const __half*>(a.q.p);
+  p.k = static_cast<const __half*>(a.k.p);
+  p.v = static_cast<const __half*>(a.v.p);
+  p.o = static_cast<__half*>(const_cast<void*>(a.o.p));
+  p.ldq = a.q.ld; p.shq = a.q.head; p.sbq = a.q.batch;
+  p.ldk = a.k.ld; p.shk = a.k.head; p.sbk = a.k.batch;
+  p.ldv = a.v.ld; p.shv = a.v.head; p.sbv = a.v.batch;
+  p.ldo = a.o.ld; p.sho = a.o.head; p.sbo = a.o.batch;
+  p.lse = a.lse;
+  p.bias = a.bias;
+  p.tq = a.tq; p.tk = a.tk; p.hs = a.hs; p.heads = a.heads; p.kv_heads = a.kv_heads; p.group = a.heads / a.kv_heads;
+  p.batch = a.batch;
+  p.rows = p.group * a.tq;
+  p.splits = splits;
+  const int step = 16 * kTokenWarps;
+  p.chunk = static_cast<int>(((a.tk + splits - 1LL) / splits + step - 1) / step * step);
+  p.reach = a.reach; p.q_offset = a.q_offset;
+  p.q_offsets = a.q_offsets; p.q_lengths = a.q_lengths; p.k_lengths = a.k_lengths;
+  p.c1 = a.scale * kLog2e;
+  p.causal = a.causal;
+  const bool narrow = a.hs <= 64;
+  const long long units = static_cast<long long>(a.kv_heads) * a.batch;
+  if (splits > 1) {  // pairs first: their alignment does not depend on the head size
+    p.stat = reinterpret_cast<float2*>(scratch);
+    p.part = scratch + 2 * units * splits * p.rows;
+  }
+  *launches = 1;
+  cudaError_t e = launch_kernel(narrow ? flash_token_kernel<64> : flash_token_kernel<128>,
+                                dim3(static_cast<unsigned>(units * splits)), dim3(32 * kTokenWarps), 0, stream, pdl_enabled(), p);
+  if (e != cudaSuccess || splits == 1) return e;
+  *launches = 2;
+  return launch_kernel(narrow ? flash_token_join_kernel<64> : flash_token_join_kernel<128>,
+                       dim3(static_cast<unsigned>(units * p.rows)), dim3(narrow ? 64 : 128), 0, stream, pdl_enabled(), p);
 }
 
 bool flash_backward_supported(const FlashArgs& a, const FlashGradArgs& g) {

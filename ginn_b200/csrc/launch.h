@@ -243,6 +243,11 @@ struct FlashArgs {
 // 128, 16-byte aligned bases and strides.
 bool flash_supported(const FlashArgs& a);
 cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* status);
+// Few queries against a long cache (at most 16 rows share a key head): number of parts the keys are
+// split into, 0 when the shape does not qualify, and the scratch the parts need.
+int flash_token_splits(const FlashArgs& a, int num_sms, long long* floats);
+cudaError_t launch_flash_token(const FlashArgs& a, int splits, float* scratch, int* launches,
+                               cudaStream_t stream);
 struct FlashGradArgs {
   FlashOperand d_o, dq, dk, dv;  // results: p null = not wanted
   void* dtable;
