@@ -415,7 +415,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
 // A token's attention reads every cached key and value once and does little with them: it is bound by
 // HBM, and what counts is many loads in flight and no work per byte beside them.  The queries that
 // share a key head (heads of the group x positions, at most 16 rows) go together, so that the cache is
-// read once.  The keys are split over CTAs, and over the eight warps of a CTA in blocks of 16; a warp
+// read once.  The keys are split over CTAs, and over the four warps of a CTA in blocks of 16; a warp
 // keeps its own running maximum, sum and result.  Operands go from global memory to registers in the
 // layout of mma.m16n8k16 without a stop in shared memory: the order in which a contraction runs over
 // the head elements is free, so a lane's 16 contiguous bytes of a key serve as its share of two
@@ -423,7 +423,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
 // product.  (A tcgen05 tile would be 128 rows high for these 1 to 16, with the cache passing through
 // shared memory: 370 us where this takes a quarter.)
 constexpr int kTokenRows = 16;
-constexpr int kTokenWarps = 8;
+constexpr int kTokenWarps = 4;  // two CTAs on an SM: one loads while the other starts or joins its warps
 
 struct TokenParams {
   const __half *q, *k, *v;
@@ -467,9 +467,9 @@ __device__ __forceinline__ void token_store(const TokenParams& p, int batch, int
 }
 
 template <int HS>
-__global__ void __launch_bounds__(32 * kTokenWarps, 1)
+__global__ void __launch_bounds__(32 * kTokenWarps, 2)
 flash_token_kernel(const TokenParams p) {
-  __shared__ float res[kTokenRows][HS];
+  extern __shared__ float res[];  // [warp][row][HS + 4]
   __shared__ float mx[kTokenWarps][kTokenRows], sm[kTokenWarps][kTokenRows];
   pdl_wait();
   pdl_launch_dependents();
@@ -500,6 +500,10 @@ flash_token_kernel(const TokenParams p) {
   const int last = qlen > 0 ? rel_visible(p.causal, qlen - 1 + off, klen) : 0;  // the most any row sees
   const long long first_pos = off;
   const int begin = split * p.chunk, end = begin + p.chunk < last ? begin + p.chunk : last;
+  if (begin >= end && p.splits > 1) {  // nothing here: the join passes it over
+    if (threadIdx.x < p.rows) p.stat[(unit * p.splits + split) * p.rows + threadIdx.x] = make_float2(-INFINITY, 0.f);
+    return;
+  }
 
   uint32_t q[HS / 32][2][4];
 #pragma unroll
@@ -625,48 +629,47 @@ flash_token_kernel(const TokenParams p) {
     }
     if (next < end) load_v(next);
   }
-  // ---- the warps' results together, in order ----
+  // ---- the warps' results together ----
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
     l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+    const int row = g + 8 * x;
     if (c == 0) {
-      mx[warp][g + 8 * x] = m[x];
-      sm[warp][g + 8 * x] = l[x];
+      mx[warp][row] = m[x];
+      sm[warp][row] = l[x];
+    }
+    if (row < p.rows) {
+      // element k of a fragment: row g + 8 (k / 2), column n = 2 c + k % 2, head element 64 s + 8 n + e
+      float* to = res + (warp * p.rows + row) * (HS + 4);
+#pragma unroll
+      for (int s = 0; s < HS / 64; ++s)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; e += 4)
+            *reinterpret_cast<float4*>(to + 64 * s + 8 * (2 * c + k) + e) =
+                make_float4(acc[8 * s + e][2 * x + k], acc[8 * s + e + 1][2 * x + k], acc[8 * s + e + 2][2 * x + k],
+                            acc[8 * s + e + 3][2 * x + k]);
     }
   }
   __syncthreads();
-  float scale[2];
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    float all = -INFINITY;
-    for (int w = 0; w < kTokenWarps; ++w) all = fmaxf(all, mx[w][g + 8 * x]);
-    scale[x] = m[x] == -INFINITY ? 0.f : ex2(m[x] - all);
-  }
-  for (int w = 0; w < kTokenWarps; ++w) {
-    if (warp == w) {
-#pragma unroll
-      for (int e = 0; e < HS / 8; ++e)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          // element k of the fragment: row g + 8 (k / 2), column n = 2 c + k % 2
-          float& r = res[g + 8 * (k >> 1)][64 * (e >> 3) + 8 * (2 * c + (k & 1)) + (e & 7)];
-          const float v = acc[e][k] * scale[k >> 1];
-          r = w == 0 ? v : r + v;
-        }
-    }
-    __syncthreads();
-  }
   for (int at = threadIdx.x; at < p.rows * HS; at += 32 * kTokenWarps) {
     const int row = at / HS, h = at % HS;
-    float all = -INFINITY, sum = 0.f;
+    float all = -INFINITY, sum = 0.f, value = 0.f;
+#pragma unroll
     for (int w = 0; w < kTokenWarps; ++w) all = fmaxf(all, mx[w][row]);
-    for (int w = 0; w < kTokenWarps; ++w) sum += mx[w][row] == -INFINITY ? 0.f : sm[w][row] * ex2(mx[w][row] - all);
+#pragma unroll
+    for (int w = 0; w < kTokenWarps; ++w) {
+      const float a = mx[w][row] == -INFINITY ? 0.f : ex2(mx[w][row] - all);
+      sum += sm[w][row] * a;
+      value += res[(w * p.rows + row) * (HS + 4) + h] * a;
+    }
     if (p.splits == 1) {
-      token_store(p, batch, kv, row, h, res[row][h], all, sum);
+      token_store(p, batch, kv, row, h, value, all, sum);
     } else {
       const long long to = (unit * p.splits + split) * p.rows + row;
-      p.part[to * HS + h] = res[row][h];
+      p.part[to * HS + h] = value;
       if (h == 0) p.stat[to] = make_float2(all, sum);
     }
   }
@@ -1339,7 +1342,7 @@ int flash_token_splits(const FlashArgs& a, int num_sms, long long* floats) {
   const int rows = a.heads / a.kv_heads * a.tq;
   *floats = 0;
   if (rows > kTokenRows) return 0;
-  // Eight CTAs' worth of work per SM, so that ragged lengths even out; a CTA takes at least 128 keys (one
+  // Eight CTAs' worth of work per SM, so that ragged lengths even out; a CTA takes at least 64 keys (one
   // block per warp) and in multiples of that.
   const long long units = static_cast<long long>(a.kv_heads) * a.batch, step = 16 * kTokenWarps;
   long long chunk = (a.tk * units + 8LL * num_sms - 1) / (8LL * num_sms);
@@ -1380,8 +1383,13 @@ cudaError_t launch_flash_token(const FlashArgs& a, int splits, float* scratch, i
     p.part = scratch + 2 * units * splits * p.rows;
   }
   *launches = 1;
-  cudaError_t e = launch_kernel(narrow ? flash_token_kernel<64> : flash_token_kernel<128>,
-                                dim3(static_cast<unsigned>(units * splits)), dim3(32 * kTokenWarps), 0, stream, pdl_enabled(), p);
+  auto kern = narrow ? flash_token_kernel<64> : flash_token_kernel<128>;
+  const int width = (narrow ? 64 : 128) + 4, row_bytes = kTokenWarps * width * static_cast<int>(sizeof(float));
+  static unsigned long long smem_set[2] = {0, 0};  // per kernel
+  cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern), kTokenRows * row_bytes, &smem_set[narrow]);
+  if (e != cudaSuccess) return e;
+  e = launch_kernel(kern, dim3(static_cast<unsigned>(units * splits)), dim3(32 * kTokenWarps), p.rows * row_bytes, stream,
+                    pdl_enabled(), p);
   if (e != cudaSuccess || splits == 1) return e;
   *launches = 2;
   return launch_kernel(narrow ? flash_token_join_kernel<64> : flash_token_join_kernel<128>,
