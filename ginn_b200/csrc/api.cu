@@ -1979,7 +1979,8 @@ int relative_composed(int device, cudaStream_t stream, int dtype, const ginn_b20
   const RelStrides sdq = g ? RelStrides{g->lddq, g->stride_dq_head, g->stride_dq_batch} : RelStrides{0, 0, 0};
   const RelStrides sdk = g ? RelStrides{g->lddk, g->stride_dk_head, g->stride_dk_batch} : RelStrides{0, 0, 0};
   const RelStrides sdv = g ? RelStrides{g->lddv, g->stride_dv_head, g->stride_dv_batch} : RelStrides{0, 0, 0};
-  float* diagonal = nullptr;
+  float *diagonal = nullptr, *sums = nullptr;
+  const int width = gb::rel_dist_width(sc.reach, tk, gb::kRelDiagonal);
   const int64_t qblocks = (tq + gb::kRelDiagonal - 1) / gb::kRelDiagonal;
   if (g) {
     if (int s = rel_dense_in(&scratch, dtype, g->d_o, sdo, hs, tq, a.heads, a.batch, a.q_lengths, &d_o)) return s;
@@ -1990,7 +1991,10 @@ int relative_composed(int device, cudaStream_t stream, int dtype, const ginn_b20
       if (int s = rel_dense_out(&scratch, dtype, g->dk, sdk, hs, tk, kv, a.batch, &dk)) return s;
     if (want_dv)
       if (int s = rel_dense_out(&scratch, dtype, g->dv, sdv, hs, tk, kv, a.batch, &dv)) return s;
-    if (want_dt) CU_TRY(scratch.take(&diagonal, a.heads * a.batch * qblocks * (tq + tk - 1)));
+    if (want_dt) {
+      CU_TRY(scratch.take(&diagonal, a.heads * a.batch * qblocks * width));
+      CU_TRY(scratch.take(&sums, (2 * a.reach + 1) * a.heads));
+    }
   } else {
     if (int s = rel_dense_out(&scratch, dtype, a.o, so, hs, tq, a.heads, a.batch, &o)) return s;
   }
@@ -2011,33 +2015,33 @@ int relative_composed(int device, cudaStream_t stream, int dtype, const ginn_b20
         if (int s = product(1, 0, tk, n, hs, k.p + u0 * k.stride, k.ld, k.stride, q.p + (u0 * group + r) * q.stride + i0 * q.ld,
                             q.ld, group * q.stride, p + r * ms, sc.ld, group * ms, nu, 0))
           return s;
-      CU_TRY(gb::launch_rel_softmax(sc, bias, g ? a.lse : nullptr, a.lse, stream));
-      g_launches.fetch_add(1);
-      for (int64_t r = 0; r < group && !g; ++r)  // O (hs x n) = V P
-        if (int s = product(0, 0, hs, n, tk, v.p + u0 * v.stride, v.ld, v.stride, p + r * ms, sc.ld, group * ms,
-                            o.p + (u0 * group + r) * o.stride + i0 * o.ld, o.ld, group * o.stride, nu, 0))
-          return s;
-      if (!g) continue;
-      const float* dop = d_o.p + u0 * group * d_o.stride + i0 * d_o.ld;
-      for (int64_t r = 0; r < group; ++r) {
-        const int add = dv.packed || !want_dv ? (r > 0 || i0 > 0) : (g->accumulate || r > 0 || i0 > 0);
-        if (want_dv)  // dV (hs x tk) += dO P^T
-          if (int s = product(0, 1, hs, tk, n, dop + r * d_o.stride, d_o.ld, group * d_o.stride, p + r * ms, sc.ld, group * ms,
-                              dv.p + u0 * dv.stride, dv.ld, dv.stride, nu, add))
+      if (!g) {
+        CU_TRY(gb::launch_rel_softmax(sc, bias, a.lse, stream));
+        g_launches.fetch_add(1);
+        for (int64_t r = 0; r < group; ++r)  // O (hs x n) = V P
+          if (int s = product(0, 0, hs, n, tk, v.p + u0 * v.stride, v.ld, v.stride, p + r * ms, sc.ld, group * ms,
+                              o.p + (u0 * group + r) * o.stride + i0 * o.ld, o.ld, group * o.stride, nu, 0))
             return s;
-        if (want_dq || want_dk || want_dt)  // dP (tk x n) = V^T dO
-          if (int s = product(1, 0, tk, n, hs, v.p + u0 * v.stride, v.ld, v.stride, dop + r * d_o.stride, d_o.ld,
-                              group * d_o.stride, dp + r * ms, sc.ld, group * ms, nu, 0))
-            return s;
+        continue;
       }
-      if (!want_dq && !want_dk && !want_dt) continue;
-      // the scale goes with the scores' gradient, but not into the table's: there the pass that
-      // sums the diagonals leaves the scaled values behind
-      CU_TRY(gb::launch_rel_softmax_grad(sc, p, dp, want_dt ? 1.f : a.scale, stream));
+      const float* dop = d_o.p + u0 * group * d_o.stride + i0 * d_o.ld;
+      for (int64_t r = 0; r < group; ++r)  // dP (tk x n) = V^T dO
+        if (int s = product(1, 0, tk, n, hs, v.p + u0 * v.stride, v.ld, v.stride, dop + r * d_o.stride, d_o.ld,
+                            group * d_o.stride, dp + r * ms, sc.ld, group * ms, nu, 0))
+          return s;
+      // The scale goes with the scores' gradient, but not into the table's: there the pass that
+      // sums by distance leaves the scaled values behind.
+      CU_TRY(gb::launch_rel_softmax_grad(sc, bias, a.lse, dp, want_dt ? 1.f : a.scale, stream));
       g_launches.fetch_add(1);
       if (want_dt) {
-        CU_TRY(gb::launch_rel_diagonal(sc, dp, a.scale, diagonal, (int)qblocks, stream));
+        CU_TRY(gb::launch_rel_diagonal(sc, dp, a.scale, diagonal, (int)qblocks, width, stream));
         g_launches.fetch_add(1);
+      }
+      for (int64_t r = 0; r < group && want_dv; ++r) {  // dV (hs x tk) += dO P^T
+        const int add = dv.packed ? (r > 0 || i0 > 0) : (g->accumulate || r > 0 || i0 > 0);
+        if (int s = product(0, 1, hs, tk, n, dop + r * d_o.stride, d_o.ld, group * d_o.stride, p + r * ms, sc.ld, group * ms,
+                            dv.p + u0 * dv.stride, dv.ld, dv.stride, nu, add))
+          return s;
       }
       for (int64_t r = 0; r < group; ++r) {
         if (want_dk) {  // dK (hs x tk) += Q dS^T
@@ -2062,9 +2066,12 @@ int relative_composed(int device, cudaStream_t stream, int dtype, const ginn_b20
   if (want_dv)
     if (int s = rel_finish_out(stream, dtype, dv, g->dv, sdv, hs, tk, kv, a.batch, g->accumulate)) return s;
   if (want_dt) {
-    CU_TRY(gb::launch_rel_table_grad(dtype, sc, diagonal, (int)qblocks, a.heads * a.batch, a.map, (int)a.buckets,
-                                     (int)a.heads, g->accumulate, g->dtable, g->lddt, stream));
-    g_launches.fetch_add(1);
+    gb::RelDist d;
+    d.dist = diagonal;
+    d.batch = (int)a.batch; d.heads = (int)a.heads; d.tiles = (int)qblocks; d.tile_rows = gb::kRelDiagonal; d.width = width;
+    d.reach = a.reach; d.q_offset = a.q_offset; d.q_offsets = a.q_offsets;
+    CU_TRY(gb::launch_rel_table_grad(dtype, d, sums, a.map, (int)a.buckets, g->accumulate ? 1 : 0, g->dtable, g->lddt, stream));
+    g_launches.fetch_add(2);
   }
   return GINN_B200_OK;
 }
@@ -2197,9 +2204,11 @@ int ginn_b200_relative_attention_backward(int device, void* stream_, int dtype, 
   if (g->dv && tk)
     CU_TRY(gb::launch_rel_unpack(dtype, nullptr, (int)hs, 0, (int)tk, (int)a->kv_heads, (int)a->batch, 0, g->dv, g->lddv,
                                  g->stride_dv_head, g->stride_dv_batch, stream));
-  if (g->dtable)
-    CU_TRY(gb::launch_rel_table_grad(dtype, gb::RelScores(), nullptr, 0, 0, a->map, (int)a->buckets, (int)a->heads, 0, g->dtable,
-                                     g->lddt, stream));
+  if (g->dtable) {
+    gb::RelDist d;
+    d.heads = (int)a->heads;
+    CU_TRY(gb::launch_rel_table_grad(dtype, d, nullptr, a->map, (int)a->buckets, 0, g->dtable, g->lddt, stream));
+  }
   g_launches.fetch_add((g->dq && tq) + (g->dk && tk) + (g->dv && tk) + (g->dtable != nullptr));
   return GINN_B200_OK;
 }

@@ -745,12 +745,6 @@ __device__ __forceinline__ float ds_scale(const FlashBwdParams& p, int batch, in
   if (!(b > 1e-30f && b < 1e30f)) return 1.f;
   return exp2f(floorf(14.f - log2f(b)));
 }
-// First distance (clamped to the reach) that query tile i0 .. i0 + 127 keeps a sum of.
-__device__ __forceinline__ long long dist_low(long long reach, long long off, int i0) {
-  const long long d = -(i0 + FT - 1 + off);
-  return d > reach ? reach : d > -reach ? d : -reach;
-}
-
 // delta and lse of every query, and the largest norms of dO and v rows per key head.  Sixteen threads
 // per row; a CTA takes 64 rows of one head, of dO (first `qparts` parts) or of v.
 __global__ void __launch_bounds__(256)
@@ -1007,7 +1001,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       mine = p.stats[(static_cast<long long>(batch) * p.heads + head) * p.tq_pad + row];
       vis = row < qlen ? rel_visible(p.causal, row + off, klen) : 0;
     }
-    const long long low = KEYS ? 0 : dist_low(p.reach, off, r0);
+    const long long low = KEYS ? 0 : rel_dist_low(p.reach, r0 + FT - 1 + off);
     float* dist = nullptr;
     float far_lo = 0.f, far_hi = 0.f;
     if (dist_on) {
@@ -1224,53 +1218,6 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
   }
 }
 
-// sums[head][reach + d] = the query tiles' sums of dS at distance d over all sequences, in order; a CTA
-// serves 32 distances, its eight warps every eighth (sequence, tile).
-__global__ void __launch_bounds__(256)
-flash_dist_sum_kernel(const __grid_constant__ FlashBwdParams p, float* __restrict__ sums) {
-  __shared__ float red[8][32];
-  pdl_wait();
-  pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y;
-  const long long at = static_cast<long long>(blockIdx.x) * 32 + lane, d = at - p.reach;
-  float s = 0.f;
-  for (int k = warp; k < p.batch * p.row_tiles; k += 8) {
-    const int batch = k / p.row_tiles, tile = k - batch * p.row_tiles;
-    const long long e = d - dist_low(p.reach, rel_offset(p.q_offset, p.q_offsets, batch), tile * FT);
-    if (d > p.reach || e < 0 || e >= p.width) continue;
-    const float* q = p.dist + ((static_cast<long long>(batch) * p.heads + head) * p.row_tiles + tile) * 2 * p.width + e;
-    s += q[0] + q[p.width];
-  }
-  red[warp][lane] = s;
-  __syncthreads();
-  if (warp != 0 || d > p.reach) return;
-  float a = 0.f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) a += red[w][lane];
-  sums[head * (2 * p.reach + 1) + at] = a;
-}
-
-// dtable[bucket, head] (+)= the sums of the distances that map to it; one warp per (bucket, head).
-__global__ void __launch_bounds__(256)
-flash_table_kernel(const float* __restrict__ sums, const int* __restrict__ map, long long reach, int buckets, int heads,
-                   int accumulate, __half* __restrict__ dtable, long long lddt) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const long long at = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (at >= static_cast<long long>(buckets) * heads) return;
-  const int head = static_cast<int>(at / buckets), bucket = static_cast<int>(at % buckets);
-  const float* s = sums + head * (2 * reach + 1);
-  float sum = 0.f;
-  for (long long d = lane; d < 2 * reach + 1; d += 32)
-    if (map[d] == bucket) sum += s[d];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane != 0) return;
-  __half* out = dtable + head * lddt + bucket;
-  *out = __float2half_rn(accumulate ? __half2float(*out) + sum : sum);
-}
-
 bool heads_aligned(const FlashOperand& x, long long t, long long heads, long long batch) {
   if ((reinterpret_cast<uintptr_t>(x.p) & 15u) != 0) return false;
   const long long n[3] = {t, heads, batch}, s[3] = {x.ld, x.head, x.batch};
@@ -1410,8 +1357,7 @@ FlashScratch flash_backward_scratch(const FlashArgs& a, bool table) {
   const long long rows = static_cast<long long>(a.heads) * a.batch, tiles = (a.tq + FT - 1) / FT;
   s.stats = rows * tiles * FT * 2;
   s.norms = 2LL * a.batch * a.kv_heads;
-  const long long width = 2 * a.reach + 1 < a.tk + FT - 1 ? 2 * a.reach + 1 : a.tk + FT - 1;
-  s.dist = table ? rows * tiles * 2 * width : 0;
+  s.dist = table ? rows * tiles * 2 * rel_dist_width(a.reach, a.tk, FT) : 0;
   s.sums = table ? (2 * a.reach + 1) * a.heads : 0;
   return s;
 }
@@ -1451,7 +1397,7 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
   p.c1 = a.scale * kLog2e;
   p.causal = a.causal;
   p.accumulate = g.accumulate;
-  p.width = static_cast<int>(2 * a.reach + 1 < a.tk + FT - 1 ? 2 * a.reach + 1 : a.tk + FT - 1);
+  p.width = rel_dist_width(a.reach, a.tk, FT);
   cudaError_t e = cudaMemsetAsync(norms, 0, sizeof(unsigned) * 2 * a.batch * a.kv_heads, stream);
   if (e != cudaSuccess) return e;
   const int qparts = qtiles * 2;
@@ -1475,15 +1421,12 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
     if (e != cudaSuccess) return e;
   }
   if (dist == nullptr) return cudaSuccess;
-  p.row_tiles = qtiles;
-  const long long n = 2 * a.reach + 1;
-  e = launch_kernel(flash_dist_sum_kernel, dim3(static_cast<unsigned>((n + 31) / 32), static_cast<unsigned>(a.heads)), dim3(256), 0,
-                    stream, pdl_enabled(), p, sums);
-  if (e != cudaSuccess) return e;
+  RelDist d;
+  d.dist = dist;
+  d.batch = a.batch; d.heads = a.heads; d.tiles = qtiles; d.tile_rows = FT; d.slots = 2; d.width = p.width;
+  d.reach = a.reach; d.q_offset = a.q_offset; d.q_offsets = a.q_offsets;
   *launches += 2;
-  return launch_kernel(flash_table_kernel, dim3(static_cast<unsigned>((static_cast<long long>(g.buckets) * a.heads + 7) / 8)), dim3(256), 0,
-                       stream, pdl_enabled(), static_cast<const float*>(sums), g.map, a.reach, g.buckets, a.heads, g.accumulate,
-                       static_cast<__half*>(g.dtable), g.lddt);
+  return launch_rel_table_grad(1, d, sums, g.map, g.buckets, g.accumulate, g.dtable, g.lddt, stream);
 }
 
 }  // namespace gb

@@ -208,19 +208,20 @@ cudaError_t launch_rel_pack(int dtype, const void* src, long long ld, long long 
 cudaError_t launch_rel_unpack(int dtype, const float* src, int hs, int hsp, int t_len, int heads,
                               int batch, int accumulate, void* dst, long long ld, long long sh,
                               long long sb, cudaStream_t stream);
-// Scores to probabilities in place; lse_in null: the statistics are formed and written to lse_out.
-cudaError_t launch_rel_softmax(const RelScores& s, const float* bias, const float* lse_in,
-                               float* lse_out, cudaStream_t stream);
-// dp = factor * p (.) (dp - colsum(p (.) dp)).
-cudaError_t launch_rel_softmax_grad(const RelScores& s, const float* p, float* dp, float factor,
-                                    cudaStream_t stream);
-// Diagonal sums of ds per block of kRelDiagonal queries: out[matrix][block][tq + tk - 1]; ds is left
+// Scores to probabilities in place; statistics to lse.
+cudaError_t launch_rel_softmax(const RelScores& s, const float* bias, float* lse, cudaStream_t stream);
+// Scores to probabilities from the kept statistics, dp = factor * p (.) (dp - colsum(p (.) dp)).
+cudaError_t launch_rel_softmax_grad(const RelScores& s, const float* bias, const float* lse, float* dp,
+                                    float factor, cudaStream_t stream);
+// Sums of ds by distance per block of kRelDiagonal queries: dist[matrix][block][width]; ds is left
 // multiplied by `factor`.
-cudaError_t launch_rel_diagonal(const RelScores& s, float* ds, float factor, float* out, int blocks,
-                                cudaStream_t stream);
-cudaError_t launch_rel_table_grad(int dtype, const RelScores& s, const float* diagonal, int blocks,
-                                  long long matrices, const int* map, int buckets, int heads,
-                                  int accumulate, void* dtable, long long lddt, cudaStream_t stream);
+cudaError_t launch_rel_diagonal(const RelScores& s, float* ds, float factor, float* dist, int blocks,
+                                int width, cudaStream_t stream);
+// dtable (+)= the sums of every bucket's distances; two kernels, one when d.dist is null (zeros).
+// sums: (2 * reach + 1) * heads floats of scratch.
+cudaError_t launch_rel_table_grad(int dtype, const RelDist& d, float* sums, const int* map,
+                                  int buckets, int accumulate, void* dtable, long long lddt,
+                                  cudaStream_t stream);
 
 // --- the same attention without the scores in memory, fp16 (flash_attention.cu) ---
 struct FlashOperand {

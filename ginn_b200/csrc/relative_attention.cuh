@@ -6,7 +6,7 @@
 
 namespace gb {
 
-constexpr int kRelDiagonal = 256;  // queries whose diagonal sums are formed together
+constexpr int kRelDiagonal = 32;  // queries whose sums by distance are formed together
 
 // Scores of `matrices` (sequence, head) pairs from pair number `matrix0` on, queries q0 .. q0 + nq - 1
 // of tq: s[matrix][query][ld], keys contiguous.
@@ -35,6 +35,24 @@ __device__ __forceinline__ long long rel_offset(long long offset, const int* off
 __device__ __forceinline__ int rel_visible(int causal, long long pos, int klen) {
   if (!causal || pos >= klen - 1) return klen;
   return pos < 0 ? 0 : static_cast<int>(pos) + 1;
+}
+
+// Sums of dS by distance as the backward kernels leave them: dist[sequence][head][tile][slot][width].
+struct RelDist {
+  const float* dist = nullptr;
+  int batch = 0, heads = 0, tiles = 0, tile_rows = 1, slots = 1, width = 0;
+  long long reach = 0, q_offset = 0;
+  const int* q_offsets = nullptr;
+};
+// First distance (clamped to the reach) that a tile of queries keeps a sum of; `last`: position of
+// its last query.
+__device__ __forceinline__ long long rel_dist_low(long long reach, long long last) {
+  return -last > reach ? reach : -last > -reach ? -last : -reach;
+}
+// Distances a tile of `rows` queries can need a sum for.
+inline int rel_dist_width(long long reach, long long tk, int rows) {
+  const long long w = tk + rows - 1;
+  return static_cast<int>(2 * reach + 1 < w ? 2 * reach + 1 : w);
 }
 
 // The query of score column `col` of a RelScores.
