@@ -2094,6 +2094,22 @@ gb::FlashArgs flash_args(const ginn_b200_relative_attention& a) {
   f.causal = a.causal ? 1 : 0;
   return f;
 }
+// Planes of fp32 operands for the flash kernels.
+int flash_split(Scratch* scratch, gb::FlashArgs* f, gb::FlashOperand* d_o) {
+  float *work, *q, *k, *v, *d = nullptr;
+  CU_TRY(scratch->take(&work, 8LL * f->batch * f->kv_heads));
+  CU_TRY(scratch->take(&q, gb::flash_planes(f->tq, f->heads, f->batch)));
+  CU_TRY(scratch->take(&k, gb::flash_planes(f->tk, f->kv_heads, f->batch)));
+  CU_TRY(scratch->take(&v, gb::flash_planes(f->tk, f->kv_heads, f->batch)));
+  if (d_o) CU_TRY(scratch->take(&d, gb::flash_planes(f->tq, f->heads, f->batch)));
+  f->q.planes = q; f->k.planes = k; f->v.planes = v;
+  if (d_o) d_o->planes = d;
+  CU_TRY(gb::launch_flash_split(f, d_o, work, scratch->stream));
+  g_launches.fetch_add(2);
+  return GINN_B200_OK;
+}
+// Few queries go through other kernels.
+bool token_rows(const ginn_b200_relative_attention& a) { return a.heads / a.kv_heads * a.tq <= 16; }
 // Bias of every distance and head, times log2(e), for the flash kernels.
 int flash_bias(Scratch* scratch, int dtype, const ginn_b200_relative_attention& a, gb::FlashArgs* f) {
   if (!a.table) return GINN_B200_OK;
@@ -2137,6 +2153,14 @@ int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, c
     g_launches.fetch_add(launches);
     return GINN_B200_OK;
   }
+  if (dtype == GINN_B200_F32 && t_force_path == PATH_AUTO && !token_rows(*a) && gb::flash_split_supported(f, false)) {
+    Scratch scratch(stream);
+    if (int s = flash_split(&scratch, &f, nullptr)) return s;
+    if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
+    CU_TRY(gb::launch_flash_forward(f, stream, ctx->d_status));
+    g_launches.fetch_add(1);
+    return GINN_B200_OK;
+  }
   return relative_composed(device, stream, dtype, *a, nullptr);
 }
 
@@ -2175,9 +2199,12 @@ int ginn_b200_relative_attention_backward(int device, void* stream_, int dtype, 
     fg.map = a->map;
     fg.buckets = (int)a->buckets;
     fg.accumulate = g->accumulate ? 1 : 0;
-    if (dtype != GINN_B200_F16 || t_force_path != PATH_AUTO || !gb::flash_backward_supported(f, fg))
+    const bool half = dtype == GINN_B200_F16;
+    if (t_force_path != PATH_AUTO || !(half ? gb::flash_backward_supported(f, fg) : gb::flash_split_supported(f, true)))
       return relative_composed(device, stream, dtype, *a, g);
     Scratch scratch(stream);
+    if (!half)
+      if (int s = flash_split(&scratch, &f, &fg.d_o)) return s;
     if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
     const gb::FlashScratch need = gb::flash_backward_scratch(f, g->dtable != nullptr);
     float *stats, *norms, *dist = nullptr, *sums = nullptr;

@@ -22,6 +22,7 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cstring>
+#include <type_traits>
 #include "ptx.cuh"
 #include "math.cuh"
 #include "launch.h"
@@ -37,6 +38,13 @@ constexpr int FCHUNK = FT * 128;      // bytes of 128 rows x 64 halves
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+__device__ __forceinline__ uint32_t pack_half2(float a, float b);
+// A pair of fp32 values as two Half pairs: what the first leaves, the second holds.
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack_half2(a, b);
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  lo = pack_half2(a - h.x, b - h.y);
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -64,6 +72,39 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
   return d;
 }
+// Eight results of a row in the storage type: 16-byte stores where they are allowed (`vec`; always for
+// Half), element by element behind them and at the row's end.
+__device__ __forceinline__ void store_row8(__half* to, int n, int vec, const float (&x)[8], bool add) {
+  if (n <= 0) return;  // n is a multiple of eight: head sizes are
+  uint32_t w[4];
+  uint4 old = make_uint4(0, 0, 0, 0);
+  if (add) old = *reinterpret_cast<const uint4*>(to);
+  const uint32_t o[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float2 q = make_float2(0.f, 0.f);
+    if (add) q = __half22float2(*reinterpret_cast<const __half2*>(&o[e]));
+    const __half2 h = __floats2half2_rn(x[2 * e] + q.x, x[2 * e + 1] + q.y);
+    w[e] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store_row8(float* to, int n, int vec, const float (&x)[8], bool add) {
+  if (vec && n >= 8) {
+    float4 a = make_float4(x[0], x[1], x[2], x[3]), b = make_float4(x[4], x[5], x[6], x[7]);
+    if (add) {
+      const float4 c = *reinterpret_cast<const float4*>(to), d = *reinterpret_cast<const float4*>(to + 4);
+      a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
+      b.x += d.x; b.y += d.y; b.z += d.z; b.w += d.w;
+    }
+    *reinterpret_cast<float4*>(to) = a;
+    *reinterpret_cast<float4*>(to + 4) = b;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) to[e] = add ? to[e] + x[e] : x[e];
+  }
+}
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -76,11 +117,13 @@ __device__ __forceinline__ void group_barrier(int id) { asm volatile("bar.sync %
 
 struct FlashParams {
   CUtensorMap tmQ, tmK, tmV;
-  __half* O;
+  void* O;
   long long ldo, sho, sbo;
   float* lse;
   const float* bias;
-  int tq, tk, hs, heads, group, batch, qblocks;
+  const float *iq, *ik, *iv;  // split operands: inverse scales, [batch][kv heads]
+  int tq, tk, hs, heads, kv_heads, group, batch, qblocks;
+  int vec;                    // fp32 results: rows allow 16-byte accesses
   long long reach, q_offset;
   const int* q_offsets;
   const int* q_lengths;
@@ -130,10 +173,14 @@ struct TileBias {
   }
 };
 
-template <int HS, int NST>
+// SPLIT: fp32 operands as two Half planes each (see split_planes_kernel), HS = 64.
+template <int HS, int NST, bool SPLIT>
 __global__ void __launch_bounds__(FTHREADS, 1)
 flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ status) {
-  constexpr int TILE = FCHUNK * (HS / 64);  // bytes of one operand tile
+  static_assert(!SPLIT || HS == 64, "a split operand's two planes take the place of two 64-wide chunks");
+  constexpr int CHUNKS = SPLIT ? 2 : HS / 64;
+  constexpr int TILE = FCHUNK * CHUNKS;  // bytes of one operand tile
+  constexpr float PSHIFT = SPLIT ? 7.f : 0.f;  // probabilities are formed times 2^PSHIFT: their low parts stay normal
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t q_full[2], k_full[NST], k_empty[NST], v_full[NST], v_empty[NST];
   __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2];
@@ -188,25 +235,22 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
 
   if (warp == 0) {
     // ===================== TMA producer =====================
+    auto load = [&](uint32_t dst, const CUtensorMap* map, uint64_t* bar, int at, int head) {
+      mbar_arrive_expect_tx(smem_u32(bar), TILE);
+      for (int c = 0; c < CHUNKS; ++c)
+        tma_load_4d(dst + c * FCHUNK, map, smem_u32(bar), SPLIT ? 0 : 64 * c, at, head, hd.batch + (SPLIT ? c * p.batch : 0));
+    };
     if (elect_one()) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if ((t ? n1 : n0) == 0) continue;
-        mbar_arrive_expect_tx(smem_u32(&q_full[t]), TILE);
-        for (int c = 0; c < HS / 64; ++c)
-          tma_load_4d(q_s + t * TILE + c * FCHUNK, &p.tmQ, smem_u32(&q_full[t]), 64 * c, i0 + t * FT, hd.head, hd.batch);
-      }
+      for (int t = 0; t < 2; ++t)
+        if ((t ? n1 : n0) > 0) load(q_s + t * TILE, &p.tmQ, &q_full[t], i0 + t * FT, hd.head);
       for (int j = 0; j < n; ++j) {
         const int s = j % NST;
         const uint32_t ph = (j / NST) & 1;
         if (!mbar_wait(smem_u32(&k_empty[s]), ph ^ 1u, status, DEV_TIMEOUT_EMPTY, 0xa00)) break;
-        mbar_arrive_expect_tx(smem_u32(&k_full[s]), TILE);
-        for (int c = 0; c < HS / 64; ++c)
-          tma_load_4d(k_s + s * TILE + c * FCHUNK, &p.tmK, smem_u32(&k_full[s]), 64 * c, j * FT, hd.kv, hd.batch);
+        load(k_s + s * TILE, &p.tmK, &k_full[s], j * FT, hd.kv);
         if (!mbar_wait(smem_u32(&v_empty[s]), ph ^ 1u, status, DEV_TIMEOUT_EMPTY, 0xa01)) break;
-        mbar_arrive_expect_tx(smem_u32(&v_full[s]), TILE);
-        for (int c = 0; c < HS / 64; ++c)
-          tma_load_4d(v_s + s * TILE + c * FCHUNK, &p.tmV, smem_u32(&v_full[s]), 64 * c, j * FT, hd.kv, hd.batch);
+        load(v_s + s * TILE, &p.tmV, &v_full[s], j * FT, hd.kv);
       }
     }
     __syncwarp();
@@ -218,11 +262,15 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
     auto scores = [&](int t, int j) {
       if (leader) {
         const uint32_t a = q_s + t * TILE, b = k_s + (j % NST) * TILE;
+        // split operands: low x high and high x low first, while the accumulator is small
 #pragma unroll
-        for (int ks = 0; ks < HS / 16; ++ks) {
-          const uint32_t at = (ks / 4) * FCHUNK + (ks % 4) * 32;
-          mma_f16(tmem + t * FT, make_smem_desc(a + at, 16, 1024), make_smem_desc(b + at, 16, 1024), IDESC_S, ks > 0);
-        }
+        for (int term = 0; term < (SPLIT ? 3 : 1); ++term)
+#pragma unroll
+          for (int ks = 0; ks < HS / 16; ++ks) {
+            const uint32_t at = (ks / 4) * FCHUNK + (ks % 4) * 32;
+            mma_f16(tmem + t * FT, make_smem_desc(a + at + (SPLIT && term == 0 ? FCHUNK : 0), 16, 1024),
+                    make_smem_desc(b + at + (SPLIT && term == 1 ? FCHUNK : 0), 16, 1024), IDESC_S, term > 0 || ks > 0);
+          }
         tc_commit(smem_u32(&s_full[t]));
       }
     };
@@ -239,11 +287,11 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
     for (int j = 0; j < n && ok; ++j) {
       const int s = j % NST, s2 = (j + 1) % NST;
       ok = warp_wait(&v_full[s], (j / NST) & 1, status, DEV_TIMEOUT_FULL, 0xb02);
-      if (ok && hd.klen < p.tk && (j + 1) * FT > hd.klen) {
+      if (!SPLIT && ok && hd.klen < p.tk && (j + 1) * FT > hd.klen) {
         // rows behind the sequence's end may hold anything: their probabilities are zero, and so
         // must they be
         for (int at = lane * 16; at < ((j + 1) * FT - hd.klen) * 128; at += 512)
-          for (int c = 0; c < HS / 64; ++c)
+          for (int c = 0; c < CHUNKS; ++c)
             *reinterpret_cast<uint4*>(base_ptr + (v_s - base) + s * TILE + c * FCHUNK + (hd.klen - j * FT) * 128 + at) =
                 make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
@@ -259,9 +307,17 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
         if (leader) {
           const uint32_t b = v_s + s * TILE;
 #pragma unroll
-          for (int ks = 0; ks < FT / 16; ++ks)
-            mma_f16_ts(tmem + 2 * FT + t * HS, tmem + t * FT + (ks / 4) * 64 + (ks % 4) * 8, make_smem_desc(b + ks * 2048, FCHUNK, 1024),
-                       IDESC_O, (j > 0 || ks > 0) ? 1u : 0u);
+          for (int ks = 0; ks < FT / 16; ++ks) {
+            const uint32_t o = tmem + 2 * FT + t * HS, a = tmem + t * FT + (ks / 4) * 64 + (ks % 4) * 8;
+            const uint32_t add = (j > 0 || ks > 0) ? 1u : 0u;
+            mma_f16_ts(o, a, make_smem_desc(b + ks * 2048, FCHUNK, 1024), IDESC_O, add);
+            if (SPLIT) {
+              // The cross terms have an accumulator of their own: the tensor core truncates when it adds, so
+              // the long chain of the main one should be as short as it can be.
+              mma_f16_ts(o + 2 * HS, a, make_smem_desc(b + FCHUNK + ks * 2048, FCHUNK, 1024), IDESC_O, add);
+              mma_f16_ts(o + 2 * HS, a + 32, make_smem_desc(b + ks * 2048, FCHUNK, 1024), IDESC_O, 1u);
+            }
+          }
           if (j == nt - 1) tc_commit(smem_u32(&o_full[t]));
         }
         if (j + 1 < nt) {
@@ -287,7 +343,8 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_col = lanes + t * FT + half * 64, o_col = lanes + 2 * FT + t * HS + half * (HS / 2);
     const float* bias = p.bias != nullptr ? p.bias + hd.head * (2 * p.reach + 1) : nullptr;
-    const float c1 = p.c1;
+    const int unit = hd.batch * p.kv_heads + hd.kv;
+    const float c1 = SPLIT ? p.c1 * p.iq[unit] * p.ik[unit] : p.c1;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nt; ++j) {
@@ -334,23 +391,24 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
         m = mn;
         if (j > 0) {  // O exists from the second tile on
 #pragma unroll
-          for (int c = 0; c < HS / 2; c += 16) {
+          for (int c = 0; c < (SPLIT ? HS : HS / 2); c += 16) {
+            const uint32_t col = o_col + c + (c >= HS / 2 ? 2 * HS - HS / 2 : 0);  // behind the main result: the cross terms
             uint32_t w[16];
-            tmem_ld16(o_col + c, w);
+            tmem_ld16(col, w);
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * a);
-            tmem_st16(o_col + c, w);
+            tmem_st16(col, w);
           }
         }
       }
       const float mu = m == -INFINITY ? 0.f : m;
-      const float ca = tb.near ? 1.f : c1, cb = tb.value - mu;
+      const float ca = tb.near ? 1.f : c1, cb = tb.value - mu + PSHIFT;
       const F2 ca2(ca, ca), cb2(cb, cb);
       F2 sum[2] = {F2(0.f, 0.f), F2(0.f, 0.f)};
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
-        uint32_t w[16];
+        uint32_t w[16], low[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           float x, y;
@@ -358,9 +416,11 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
           x = ex2(x);
           y = ex2(y);
           sum[e & 1] = add2(sum[e & 1], F2(x, y));
-          w[e] = pack_half2(x, y);
+          if (SPLIT) split_pair(x, y, w[e], low[e]);
+          else w[e] = pack_half2(x, y);
         }
         tmem_st16(s_col + c / 2, w);  // over scores this thread has read
+        if (SPLIT) tmem_st16(s_col + 32 + c / 2, low);
       }
       float sa, sb;
       add2(sum[0], sum[1]).get(sa, sb);
@@ -380,25 +440,26 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
     }
     if (ok) {
       const bool real = i < p.tq, some = nt > 0 && vis > 0 && l > 0.f;
-      const float inv = some ? 1.f / l : 0.f;
-      __half* out = p.O + i * p.ldo + hd.head * p.sho + hd.batch * p.sbo;
+      const float inv = some ? (SPLIT ? p.iv[unit] : 1.f) / l : 0.f;
+      using Out = typename std::conditional<SPLIT, float, __half>::type;
+      Out* out = static_cast<Out*>(p.O) + i * p.ldo + hd.head * p.sho + hd.batch * p.sbo;
 #pragma unroll
-      for (int c = 0; c < HS / 2; c += 16) {
-        uint32_t w[16];
+      for (int c = 0; c < HS / 2; c += 8) {
+        uint32_t w[8], x[8];
         if (nt > 0) {
-          tmem_ld16(o_col + c, w);
+          tmem_ld8(o_col + c, w);
+          if (SPLIT) tmem_ld8(o_col + 2 * HS + c, x);
           tmem_ld_wait();
         }
-        uint32_t h[8];
+        float res[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          h[e] = some ? pack_half2(__uint_as_float(w[2 * e]) * inv, __uint_as_float(w[2 * e + 1]) * inv) : 0u;
+          res[e] = some ? (SPLIT ? __uint_as_float(w[e]) + __uint_as_float(x[e]) : __uint_as_float(w[e])) * inv : 0.f;
         const int at = half * (HS / 2) + c;
-        if (real && at < p.hs) *reinterpret_cast<uint4*>(out + at) = make_uint4(h[0], h[1], h[2], h[3]);
-        if (real && at + 8 < p.hs) *reinterpret_cast<uint4*>(out + at + 8) = make_uint4(h[4], h[5], h[6], h[7]);
+        if (real) store_row8(out + at, p.hs - at, p.vec, res, false);
       }
       if (real && half == 0)
-        p.lse[(static_cast<long long>(hd.batch) * p.heads + hd.head) * p.tq + i] = some ? (m + log2f(l)) * kLn2 : -INFINITY;
+        p.lse[(static_cast<long long>(hd.batch) * p.heads + hd.head) * p.tq + i] = some ? (m + log2f(l) - PSHIFT) * kLn2 : -INFINITY;
     }
   }
 
@@ -407,6 +468,115 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---- fp32 operands as Half planes -----------------------------------------------------------------
+//
+// An fp32 matrix times a power of two that brings its largest magnitude (per sequence and key head) to
+// [2^14, 2^15) is written as the sum of two Half matrices, high = rn(x), low = rn(x - high): 22 bits of
+// every element down to 2^-18 of the largest, and an absolute error of 2^-40 of the largest below
+// that.  A product is then three Half products, high x high + high x low + low x high, at twice the
+// rate of three TF32 products and with the same 2^-22 left out.  The planes are dense,
+// [plane][sequence][head][t][64], zero behind the head size and behind the sequences' lengths.
+struct SplitOperand {
+  const float* x;
+  long long ld, head, batch;
+  __half* planes;
+  const int* lengths;
+  int t, heads, per;      // heads per scale
+  long long block0;       // first CTA of this operand
+};
+struct SplitParams {
+  SplitOperand op[4];
+  int count, hs, batch, kv_heads;
+  unsigned* most;         // [operand][batch][kv heads]: bits of the largest magnitude
+  float* inverse;         // [operand][batch][kv heads]: what a scaled value is multiplied by to get it back
+};
+// Rows 64 part .. 64 part + 63 of one head, by CTA; the operand's fields selected one by one (indexing
+// the parameters would copy them to local memory).
+struct SplitPart {
+  const float* x = nullptr;
+  __half* planes = nullptr;
+  long long ld = 0, plane = 0;
+  int which = 0, unit = 0, row0 = 0, rows = 0, real = 0;
+  bool first = false;
+  __device__ __forceinline__ explicit SplitPart(const SplitParams& p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i >= p.count || blockIdx.x < p.op[i].block0) continue;
+      const long long at = blockIdx.x - p.op[i].block0;
+      const int parts = (p.op[i].t + 63) / 64, hb = static_cast<int>(at / parts), b = hb / p.op[i].heads, h = hb % p.op[i].heads;
+      which = i;
+      unit = b * p.kv_heads + h / p.op[i].per;
+      row0 = static_cast<int>(at % parts) * 64;
+      rows = p.op[i].t;
+      real = rel_length(p.op[i].lengths, b, rows);
+      ld = p.op[i].ld;
+      x = p.op[i].x + h * p.op[i].head + b * p.op[i].batch;
+      planes = p.op[i].planes + static_cast<long long>(hb) * rows * 64;
+      plane = static_cast<long long>(p.batch) * p.op[i].heads * rows * 64;
+      first = row0 == 0;
+    }
+  }
+};
+
+__global__ void __launch_bounds__(256)
+split_most_kernel(const __grid_constant__ SplitParams p) {
+  __shared__ unsigned red[8];
+  pdl_wait();
+  pdl_launch_dependents();
+  const SplitPart part(p);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned m = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int row = part.row0 + warp * 8 + k;
+    if (row >= part.real) continue;
+    const float* x = part.x + row * part.ld;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (lane + 32 * e < p.hs) m = max(m, __float_as_uint(fabsf(x[lane + 32 * e])));
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (lane == 0) red[warp] = m;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < 8; ++w) m = max(m, red[w]);
+  atomicMax(p.most + part.which * p.batch * p.kv_heads + part.unit, m);  // a maximum: the order does not matter
+}
+
+__global__ void __launch_bounds__(256)
+split_planes_kernel(const __grid_constant__ SplitParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const SplitPart part(p);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int at = part.which * p.batch * p.kv_heads + part.unit;
+  const unsigned most = p.most[at];
+  // 2^(14 - exponent of the largest); not numbers and infinities go through as they are
+  int e = 14 - (static_cast<int>(most >> 23) - 127);
+  e = e > 126 ? 126 : e;
+  if (most == 0 || most >= 0x7f800000u) e = 0;
+  const float scale = __uint_as_float(static_cast<unsigned>(e + 127) << 23);
+  if (part.first && threadIdx.x == 0) p.inverse[at] = 1.f / scale;
+  float x[8][2];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int row = part.row0 + warp * 8 + k;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      x[k][c] = row < part.real && 2 * lane + c < p.hs ? part.x[row * part.ld + 2 * lane + c] * scale : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int row = part.row0 + warp * 8 + k;
+    if (row >= part.rows) continue;
+    uint32_t hi, lo;
+    split_pair(x[k][0], x[k][1], hi, lo);
+    __half* to = part.planes + static_cast<long long>(row) * 64 + 2 * lane;
+    *reinterpret_cast<uint32_t*>(to) = hi;
+    *reinterpret_cast<uint32_t*>(to + part.plane) = lo;
   }
 }
 
@@ -724,13 +894,15 @@ constexpr int kDistSmem = 1024;    // distances whose sums fit in shared memory 
 struct FlashBwdParams {
   CUtensorMap tmQ, tmK, tmV, tmDO;      // boxes of 128 rows
   CUtensorMap tmQ64, tmK64, tmV64, tmDO64;
-  __half *dq, *dk, *dv;
+  void *dq, *dk, *dv;
   long long lddq, shdq, sbdq, lddk, shdk, sbdk, lddv, shdv, sbdv;
   const float2* stats;        // [batch][heads][tq_pad]: lse * log2(e) (+inf = empty), delta
   const unsigned* norms;      // [2][batch][kv heads]: bits of max |dO|^2, max |v|^2
   float* dist;                // [batch][heads][query tile][2][width] sums of dS by distance; null = not wanted
   const float* bias;
+  const float *iq, *ik, *iv, *ido;  // split operands: inverse scales, [batch][kv heads]
   int tq, tk, hs, heads, kv_heads, group, batch, tq_pad, row_tiles, width;
+  int vec_dq, vec_dk, vec_dv;       // fp32 results: rows allow 16-byte accesses
   long long reach, q_offset;
   const int* q_offsets;
   const int* q_lengths;
@@ -739,17 +911,47 @@ struct FlashBwdParams {
   int causal, accumulate;
 };
 
-__device__ __forceinline__ float ds_scale(const FlashBwdParams& p, int batch, int kv) {
-  const int at = batch * p.kv_heads + kv;
-  const float b = 2.f * sqrtf(__uint_as_float(p.norms[at])) * sqrtf(__uint_as_float(p.norms[p.batch * p.kv_heads + at]));
-  if (!(b > 1e-30f && b < 1e30f)) return 1.f;
-  return exp2f(floorf(14.f - log2f(b)));
+// Power of two dS is multiplied with.  Split operands' norms are those of the scaled values.
+template <bool SPLIT>
+__device__ __forceinline__ float ds_scale(const FlashBwdParams& p, int unit) {
+  const float a = __uint_as_float(p.norms[unit]), b = __uint_as_float(p.norms[p.batch * p.kv_heads + unit]);
+  float e = 13.f - 0.5f * (log2f(a) + log2f(b));
+  if (SPLIT) e -= log2f(p.ido[unit]) + log2f(p.iv[unit]);
+  if (!(a > 0.f && b > 0.f && a < INFINITY && b < INFINITY)) return 1.f;
+  return exp2f(floorf(fminf(fmaxf(e, -120.f), 120.f)));
 }
+// Eight consecutive elements as they are stored, zero behind the first n.
+template <typename T>
+struct Eight;
+template <>
+struct Eight<__half> {
+  uint4 w;
+  __device__ __forceinline__ void load(const __half* p, int n) {  // n: 0 or at least 8 (head sizes are multiples of it)
+    w = make_uint4(0, 0, 0, 0);
+    if (n > 0) w = *reinterpret_cast<const uint4*>(p);
+  }
+  __device__ __forceinline__ float get(int e) const {
+    const uint32_t u = e < 2 ? w.x : e < 4 ? w.y : e < 6 ? w.z : w.w;
+    const __half2 h = *reinterpret_cast<const __half2*>(&u);
+    return e & 1 ? __high2float(h) : __low2float(h);
+  }
+};
+template <>
+struct Eight<float> {
+  float x[8];
+  __device__ __forceinline__ void load(const float* p, int n) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = e < n ? p[e] : 0.f;
+  }
+  __device__ __forceinline__ float get(int e) const { return x[e]; }
+};
+
 // delta and lse of every query, and the largest norms of dO and v rows per key head.  Sixteen threads
 // per row; a CTA takes 64 rows of one head, of dO (first `qparts` parts) or of v.
+template <typename T>
 __global__ void __launch_bounds__(256)
-flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long long sbdo, const __half* o, long long ldo,
-                     long long sho, long long sbo, const __half* v, long long ldv, long long shv, long long sbv,
+flash_prepare_kernel(const T* d_o, long long lddo, long long shdo, long long sbdo, const T* o, long long ldo,
+                     long long sho, long long sbo, const T* v, long long ldv, long long shv, long long sbv,
                      const float* __restrict__ lse, const FlashBwdParams p, float2* __restrict__ stats,
                      unsigned* __restrict__ norms, int qparts, long long qblocks) {
   __shared__ float red[16];
@@ -764,38 +966,26 @@ flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long lon
   const int batch = hb / heads, head = hb - batch * heads;
   const int kv = queries ? head / p.group : head;
   const int len = queries ? rel_length(p.q_lengths, batch, p.tq) : rel_length(p.k_lengths, batch, p.tk);
-  auto widen = [&](uint4 w, float (&f)[8]) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
-      f[2 * e] = q.x;
-      f[2 * e + 1] = q.y;
-    }
-  };
+  const int unit = batch * p.kv_heads + kv;
+  const float to = sizeof(T) == 4 ? 1.f / (queries ? p.ido : p.iv)[unit] : 1.f;  // as the planes hold it
   float norm[4], dot[4];
   {
-    uint4 wa[4], wb[4];
+    Eight<T> wa[4], wb[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {  // all loads before the first sum
       const int i = part * 64 + k * 16 + row16;
-      wa[k] = wb[k] = make_uint4(0, 0, 0, 0);
-      if (i < len && sub * 8 < p.hs) {
-        wa[k] = *reinterpret_cast<const uint4*>(queries ? d_o + i * lddo + head * shdo + batch * sbdo + sub * 8
-                                                        : v + i * ldv + head * shv + batch * sbv + sub * 8);
-        if (queries) wb[k] = *reinterpret_cast<const uint4*>(o + i * ldo + head * sho + batch * sbo + sub * 8);
-      }
+      const int n = i < len ? p.hs - sub * 8 : 0;  // elements of this thread
+      wa[k].load(queries ? d_o + i * lddo + head * shdo + batch * sbdo + sub * 8 : v + i * ldv + head * shv + batch * sbv + sub * 8, n);
+      wb[k].load(o + i * ldo + head * sho + batch * sbo + sub * 8, queries ? n : 0);
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      float a[8], b[8];
-      widen(wa[k], a);
-      widen(wb[k], b);
       norm[k] = dot[k] = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        norm[k] += a[e] * a[e];
-        dot[k] += a[e] * b[e];
+        const float a = wa[k].get(e);
+        norm[k] += (a * to) * (a * to);
+        dot[k] += a * wb[k].get(e);
       }
     }
   }
@@ -827,15 +1017,19 @@ flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long lon
     unsigned m = 0;
     for (int k = 0; k < 16; ++k) m = max(m, __float_as_uint(red[k]));
     // a maximum of non-negative floats: the order of the updates does not matter
-    atomicMax(norms + (queries ? 0 : p.batch * p.kv_heads) + batch * p.kv_heads + kv, m);
+    atomicMax(norms + (queries ? 0 : p.batch * p.kv_heads) + unit, m);
   }
 }
 
-template <int HS, bool KEYS>
+template <int HS, bool KEYS, bool SPLIT>
 __global__ void __launch_bounds__(FTHREADS, 1)
 flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict__ status) {
-  constexpr int ROWS = FCHUNK * (HS / 64);   // bytes of a resident operand
-  constexpr int TILE = BCHUNK * (HS / 64);   // bytes of a streamed tile
+  static_assert(!SPLIT || HS == 64, "a split operand's two planes take the place of two 64-wide chunks");
+  constexpr int CHUNKS = SPLIT ? 2 : HS / 64;
+  constexpr int ROWS = FCHUNK * CHUNKS;   // bytes of a resident operand
+  constexpr int TILE = BCHUNK * CHUNKS;   // bytes of a streamed tile
+  constexpr float PSHIFT = SPLIT ? 14.f : 12.f;  // P is formed times 2^PSHIFT
+  constexpr float PINV = SPLIT ? 1.f / 16384.f : 1.f / 4096.f;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t rows_full, b_full[BSTAGES], b_empty[BSTAGES], x_full[2], p_full[2], acc_full;
   __shared__ uint32_t tmem_slot;
@@ -904,9 +1098,10 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     // ===================== TMA producer =====================
     if (n > 0 && elect_one()) {
       mbar_arrive_expect_tx(smem_u32(&rows_full), 2 * ROWS);
-      for (int c = 0; c < HS / 64; ++c) {
-        tma_load_4d(a1_s + c * FCHUNK, KEYS ? &p.tmK : &p.tmQ, smem_u32(&rows_full), 64 * c, r0, head, batch);
-        tma_load_4d(a2_s + c * FCHUNK, KEYS ? &p.tmV : &p.tmDO, smem_u32(&rows_full), 64 * c, r0, head, batch);
+      for (int c = 0; c < CHUNKS; ++c) {
+        const int x = SPLIT ? 0 : 64 * c, w = batch + (SPLIT ? c * p.batch : 0);
+        tma_load_4d(a1_s + c * FCHUNK, KEYS ? &p.tmK : &p.tmQ, smem_u32(&rows_full), x, r0, head, w);
+        tma_load_4d(a2_s + c * FCHUNK, KEYS ? &p.tmV : &p.tmDO, smem_u32(&rows_full), x, r0, head, w);
       }
       for (int it = 0; it < n; ++it) {
         const int s = it % BSTAGES;
@@ -914,9 +1109,10 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
         const uint32_t bar = smem_u32(&b_full[s]), dst = b_s + s * 2 * TILE;
         const int at = (first + it % per) * BN, h = KEYS ? head * p.group + it / per : kv;
         mbar_arrive_expect_tx(bar, 2 * TILE);
-        for (int c = 0; c < HS / 64; ++c) {
-          tma_load_4d(dst + c * BCHUNK, KEYS ? &p.tmQ64 : &p.tmK64, bar, 64 * c, at, h, batch);
-          tma_load_4d(dst + TILE + c * BCHUNK, KEYS ? &p.tmDO64 : &p.tmV64, bar, 64 * c, at, h, batch);
+        for (int c = 0; c < CHUNKS; ++c) {
+          const int x = SPLIT ? 0 : 64 * c, w = batch + (SPLIT ? c * p.batch : 0);
+          tma_load_4d(dst + c * BCHUNK, KEYS ? &p.tmQ64 : &p.tmK64, bar, x, at, h, w);
+          tma_load_4d(dst + TILE + c * BCHUNK, KEYS ? &p.tmDO64 : &p.tmV64, bar, x, at, h, w);
         }
       }
     }
@@ -933,13 +1129,13 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       ok = warp_wait(&b_full[s], (it / BSTAGES) & 1, status, DEV_TIMEOUT_FULL, 0xe01);
       if (!ok) return;
       tc_fence_after();
-      if (blen < bt && at + BN > blen) {
+      if (!SPLIT && blen < bt && at + BN > blen) {
         // rows behind the sequence's end may hold anything: the second products meet them with
         // zeros, and so they have to be zero
         uint8_t* stage = base_ptr + (b_s - base) + s * 2 * TILE;
         const int from = blen - at;  // > 0: tiles behind the end are not streamed
         for (int x = lane * 16; x < (BN - from) * 128; x += 512)
-          for (int c = 0; c < 2 * (HS / 64); ++c)
+          for (int c = 0; c < 2 * CHUNKS; ++c)
             *reinterpret_cast<uint4*>(stage + c * BCHUNK + from * 128 + x) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
         __syncwarp();
@@ -947,15 +1143,16 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       if (leader) {
         const uint32_t b = b_s + s * 2 * TILE, d = tmem + (it & 1) * FT;
 #pragma unroll
-        for (int ks = 0; ks < HS / 16; ++ks) {
-          const uint32_t aa = (ks / 4) * FCHUNK + (ks % 4) * 32, bb = (ks / 4) * BCHUNK + (ks % 4) * 32;
-          mma_f16(d, make_smem_desc(a1_s + aa, 16, 1024), make_smem_desc(b + bb, 16, 1024), IDESC_X, ks > 0);
-        }
+        for (int y = 0; y < 2; ++y)  // X = A1 B1^T, Y = A2 B2^T
 #pragma unroll
-        for (int ks = 0; ks < HS / 16; ++ks) {
-          const uint32_t aa = (ks / 4) * FCHUNK + (ks % 4) * 32, bb = (ks / 4) * BCHUNK + (ks % 4) * 32;
-          mma_f16(d + BN, make_smem_desc(a2_s + aa, 16, 1024), make_smem_desc(b + TILE + bb, 16, 1024), IDESC_X, ks > 0);
-        }
+          for (int term = 0; term < (SPLIT ? 3 : 1); ++term)
+#pragma unroll
+            for (int ks = 0; ks < HS / 16; ++ks) {
+              const uint32_t aa = (ks / 4) * FCHUNK + (ks % 4) * 32 + (SPLIT && term == 0 ? FCHUNK : 0);
+              const uint32_t bb = (ks / 4) * BCHUNK + (ks % 4) * 32 + (SPLIT && term == 1 ? BCHUNK : 0);
+              mma_f16(d + y * BN, make_smem_desc((y ? a2_s : a1_s) + aa, 16, 1024), make_smem_desc(b + y * TILE + bb, 16, 1024),
+                      IDESC_X, term > 0 || ks > 0);
+            }
         tc_commit(smem_u32(&x_full[it & 1]));
       }
     };
@@ -968,16 +1165,20 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       tc_fence_after();
       if (leader) {
         const uint32_t b = b_s + s * 2 * TILE, a = tmem + g * FT;
+        // the result behind a left operand at `a`, split operands' cross terms beside it
+        auto product = [&](uint32_t d, uint32_t left, uint32_t right) {
 #pragma unroll
-        for (int ks = 0; ks < BN / 16; ++ks) {
-          if (KEYS)  // dV += P dO
-            mma_f16_ts(tmem + 2 * FT + HS, a + (ks / 2) * 32 + (ks % 2) * 8, make_smem_desc(b + TILE + ks * 2048, BCHUNK, 1024), IDESC_ACC,
-                       (it > 0 || ks > 0) ? 1u : 0u);
-        }
-#pragma unroll
-        for (int ks = 0; ks < BN / 16; ++ks)  // dK += dS Q,  dQ += dS K
-          mma_f16_ts(tmem + 2 * FT, a + BN + (ks / 2) * 32 + (ks % 2) * 8, make_smem_desc(b + ks * 2048, BCHUNK, 1024), IDESC_ACC,
-                     (it > 0 || ks > 0) ? 1u : 0u);
+          for (int ks = 0; ks < BN / 16; ++ks) {
+            const uint32_t l = left + (ks / 2) * 32 + (ks % 2) * 8, add = (it > 0 || ks > 0) ? 1u : 0u;
+            mma_f16_ts(d, l, make_smem_desc(right + ks * 2048, BCHUNK, 1024), IDESC_ACC, add);
+            if (SPLIT) {
+              mma_f16_ts(d + HS, l, make_smem_desc(right + BCHUNK + ks * 2048, BCHUNK, 1024), IDESC_ACC, add);
+              mma_f16_ts(d + HS, l + 16, make_smem_desc(right + ks * 2048, BCHUNK, 1024), IDESC_ACC, 1u);
+            }
+          }
+        };
+        if (KEYS) product(tmem + 2 * FT + (SPLIT ? 2 * HS : HS), a, b + TILE);  // dV += P dO
+        product(tmem + 2 * FT, a + BN, b);                                      // dK += dS Q,  dQ += dS K
         tc_commit(smem_u32(&b_empty[s]));
         if (it == n - 1) tc_commit(smem_u32(&acc_full));
       }
@@ -991,9 +1192,11 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     const int row = r0 + r;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t x_col = lanes + g * FT + half * 32, y_col = x_col + BN;
-    const float c1 = p.c1;
-    const float up = ds_scale(p, batch, kv);
-    const float f = up * (1.f / 4096.f);  // on P, which is formed times 2^12
+    const int unit = batch * p.kv_heads + kv;
+    const float c1 = SPLIT ? p.c1 * p.iq[unit] * p.ik[unit] : p.c1;
+    const float up = ds_scale<SPLIT>(p, unit);
+    const float f = up * PINV;  // on P, which is formed times 2^PSHIFT
+    const float fy = SPLIT ? f * p.iv[unit] * p.ido[unit] : f;
     const bool dist_on = !KEYS && p.dist != nullptr;
     float2 mine = make_float2(INFINITY, 0.f);
     int vis = 0;
@@ -1032,7 +1235,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       if (KEYS && gt < BN) {
         // per column: what is added to the scaled score, and to Y times f
         const float2 st = p.stats[(static_cast<long long>(batch) * p.heads + h) * p.tq_pad + at + gt];
-        colx[KEYS ? g : 0][turn][gt] = (flat ? value : 0.f) + 12.f - st.x;
+        colx[KEYS ? g : 0][turn][gt] = (flat ? value : 0.f) + PSHIFT - st.x;
         coly[KEYS ? g : 0][turn][gt] = -st.y * f;
       }
       if (KEYS || !flat) group_barrier(1 + g);
@@ -1054,7 +1257,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       F2 all(0.f, 0.f);
       if (ok) {
         tc_fence_after();
-        const float rx = (flat ? value : 0.f) + 12.f - mine.x, ry = -mine.y * f;
+        const float rx = (flat ? value : 0.f) + PSHIFT - mine.x, ry = -mine.y * f;
         uint32_t x[32], y[32];
         tmem_ld32(x_col, x);
         tmem_ld32(y_col, y);
@@ -1073,8 +1276,8 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
             }
         }
         const float cx1 = flat ? c1 : 1.f;
-        const F2 cx(cx1, cx1), f2(f, f);
-        uint32_t pw[16], dw[16];
+        const F2 cx(cx1, cx1), f2(fy, fy);
+        uint32_t pw[16], dw[16], plow[16], dlow[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           F2 sx(rx, rx), sy(ry, ry);
@@ -1091,9 +1294,14 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
           const F2 ds = mul2(F2(p0, p1), fma2(F2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), f2, sy));
           float d0, d1;
           ds.get(d0, d1);
-          if (KEYS) pw[e / 2] = pack_half2(p0, p1);
-          else all = add2(all, ds);
-          dw[e / 2] = pack_half2(d0, d1);
+          if (!KEYS) all = add2(all, ds);
+          if (SPLIT) {
+            if (KEYS) split_pair(p0, p1, pw[e / 2], plow[e / 2]);
+            split_pair(d0, d1, dw[e / 2], dlow[e / 2]);
+          } else {
+            if (KEYS) pw[e / 2] = pack_half2(p0, p1);
+            dw[e / 2] = pack_half2(d0, d1);
+          }
           if (!KEYS) {
             y[e] = __float_as_uint(d0);
             y[e + 1] = __float_as_uint(d1);
@@ -1101,6 +1309,10 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
         }
         if (KEYS) tmem_st16(x_col, pw);
         tmem_st16(y_col, dw);
+        if (SPLIT) {
+          if (KEYS) tmem_st16(x_col + 16, plow);
+          tmem_st16(y_col + 16, dlow);
+        }
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(smem_u32(&p_full[g]));
@@ -1173,39 +1385,30 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       ok = warp_wait(&acc_full, 0, status, DEV_TIMEOUT_ACCUM, 0xf10 + g);
       tc_fence_after();
     }
-    __half* out = KEYS ? (g == 0 ? p.dk : p.dv) : p.dq;
+    using Out = typename std::conditional<SPLIT, float, __half>::type;
+    Out* out = static_cast<Out*>(KEYS ? (g == 0 ? p.dk : p.dv) : p.dq);
     const bool real = row < (KEYS ? p.tk : p.tq);
     if (ok && out != nullptr && (n > 0 || !p.accumulate)) {
       const long long ld = KEYS ? (g == 0 ? p.lddk : p.lddv) : p.lddq, sh = KEYS ? (g == 0 ? p.shdk : p.shdv) : p.shdq,
                       sb = KEYS ? (g == 0 ? p.sbdk : p.sbdv) : p.sbdq;
+      const int vec = KEYS ? (g == 0 ? p.vec_dk : p.vec_dv) : p.vec_dq;
       out += row * ld + head * sh + batch * sb;
-      const float factor = KEYS && g == 1 ? 1.f / 4096.f : p.scale / up;
-      const uint32_t col0 = lanes + 2 * FT + (KEYS && g == 1 ? HS : 0);
+      float factor = KEYS && g == 1 ? PINV : p.scale / up;
+      if (SPLIT) factor *= KEYS ? (g == 1 ? p.ido[unit] : p.iq[unit]) : p.ik[unit];
+      const uint32_t col0 = lanes + 2 * FT + (KEYS && g == 1 ? (SPLIT ? 2 * HS : HS) : 0);
       const int c_from = KEYS ? half * (HS / 2) : (2 * g + half) * (HS / 4), c_to = c_from + (KEYS ? HS / 2 : HS / 4);
-      for (int c = c_from; c < c_to; c += 16) {
-        uint32_t w[16];
+      for (int c = c_from; c < c_to; c += 8) {
+        uint32_t w[8], x[8];
         if (n > 0) {
-          tmem_ld16(col0 + c, w);
+          tmem_ld8(col0 + c, w);
+          if (SPLIT) tmem_ld8(col0 + HS + c, x);
           tmem_ld_wait();
         }
+        float res[8];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (!real || c + 8 * half >= p.hs) continue;
-          uint4* dst = reinterpret_cast<uint4*>(out + c + 8 * half);
-          uint32_t old[4] = {0, 0, 0, 0}, res[4];
-          if (p.accumulate) {
-            const uint4 q = *dst;
-            old[0] = q.x; old[1] = q.y; old[2] = q.z; old[3] = q.w;
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&old[e]));
-            const float a = n > 0 ? __uint_as_float(w[8 * half + 2 * e]) * factor : 0.f;
-            const float b = n > 0 ? __uint_as_float(w[8 * half + 2 * e + 1]) * factor : 0.f;
-            res[e] = p.accumulate ? pack_half2(a + q.x, b + q.y) : pack_half2(a, b);
-          }
-          *dst = make_uint4(res[0], res[1], res[2], res[3]);
-        }
+        for (int e = 0; e < 8; ++e)
+          res[e] = n > 0 ? (SPLIT ? __uint_as_float(w[e]) + __uint_as_float(x[e]) : __uint_as_float(w[e])) * factor : 0.f;
+        if (real) store_row8(out + c, p.hs - c, vec, res, p.accumulate != 0);
       }
     }
   }
@@ -1226,17 +1429,32 @@ bool heads_aligned(const FlashOperand& x, long long t, long long heads, long lon
   return true;
 }
 
+// Tensor map of an operand: Half as it lies, or the planes of a split one (twice the sequences).
+bool encode_operand(CUtensorMap* map, const FlashOperand& x, int hs, int t, int heads, int batch, int rows, bool split) {
+  if (split) return encode_heads_tmap(map, x.planes, 64, t, heads, 2LL * batch, 64, 64LL * t, 64LL * t * heads, rows);
+  return encode_heads_tmap(map, x.p, hs, t, heads, batch, x.ld, x.head, x.batch, rows);
+}
+// Rows of an fp32 result allow 16-byte accesses.
+int rows16(const FlashOperand& x) {
+  return (reinterpret_cast<uintptr_t>(x.p) & 15u) == 0 && x.ld % 4 == 0 && x.head % 4 == 0 && x.batch % 4 == 0;
+}
+
 bool fill_params(const FlashArgs& a, FlashParams* p) {
   std::memset(p, 0, sizeof(*p));
-  if (!encode_heads_tmap(&p->tmQ, a.q.p, a.hs, a.tq, a.heads, a.batch, a.q.ld, a.q.head, a.q.batch, FT) ||
-      !encode_heads_tmap(&p->tmK, a.k.p, a.hs, a.tk, a.kv_heads, a.batch, a.k.ld, a.k.head, a.k.batch, FT) ||
-      !encode_heads_tmap(&p->tmV, a.v.p, a.hs, a.tk, a.kv_heads, a.batch, a.v.ld, a.v.head, a.v.batch, FT))
+  const bool split = a.inverse != nullptr;
+  if (!encode_operand(&p->tmQ, a.q, a.hs, a.tq, a.heads, a.batch, FT, split) ||
+      !encode_operand(&p->tmK, a.k, a.hs, a.tk, a.kv_heads, a.batch, FT, split) ||
+      !encode_operand(&p->tmV, a.v, a.hs, a.tk, a.kv_heads, a.batch, FT, split))
     return false;
-  p->O = static_cast<__half*>(const_cast<void*>(a.o.p));
+  p->O = const_cast<void*>(a.o.p);
+  p->vec = rows16(a.o);
   p->ldo = a.o.ld; p->sho = a.o.head; p->sbo = a.o.batch;
   p->lse = a.lse;
   p->bias = a.bias;
-  p->tq = a.tq; p->tk = a.tk; p->hs = a.hs; p->heads = a.heads; p->group = a.heads / a.kv_heads; p->batch = a.batch;
+  const long long units = static_cast<long long>(a.batch) * a.kv_heads;
+  p->iq = a.inverse; p->ik = a.inverse + units; p->iv = a.inverse + 2 * units;
+  p->tq = a.tq; p->tk = a.tk; p->hs = a.hs; p->heads = a.heads; p->kv_heads = a.kv_heads; p->group = a.heads / a.kv_heads;
+  p->batch = a.batch;
   p->reach = a.reach; p->q_offset = a.q_offset;
   p->q_offsets = a.q_offsets; p->q_lengths = a.q_lengths; p->k_lengths = a.k_lengths;
   p->c1 = a.scale * kLog2e;
@@ -1244,11 +1462,11 @@ bool fill_params(const FlashArgs& a, FlashParams* p) {
   return true;
 }
 
-template <int HS, int NST>
+template <int HS, int NST, bool SPLIT>
 cudaError_t forward_hs(FlashParams& p, cudaStream_t stream, int* status) {
-  const int smem = (2 + 2 * NST) * FCHUNK * (HS / 64) + 1024;
+  const int smem = (2 + 2 * NST) * FCHUNK * (SPLIT ? 2 : HS / 64) + 1024;
   static unsigned long long smem_set = 0;  // per template instantiation
-  auto kern = flash_forward_kernel<HS, NST>;
+  auto kern = flash_forward_kernel<HS, NST, SPLIT>;
   cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern), smem, &smem_set);
   if (e != cudaSuccess) return e;
   p.qblocks = (p.tq + 2 * FT - 1) / (2 * FT);
@@ -1257,17 +1475,34 @@ cudaError_t forward_hs(FlashParams& p, cudaStream_t stream, int* status) {
   return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(FTHREADS), smem, stream, pdl_enabled(), p, status);
 }
 
-template <int HS, bool KEYS>
+template <int HS, bool KEYS, bool SPLIT>
 cudaError_t backward_hs(const FlashBwdParams& p, cudaStream_t stream, int* status) {
-  const int smem = 2 * FCHUNK * (HS / 64) + BSTAGES * 2 * BCHUNK * (HS / 64) + 1024;
+  const int smem = (2 * FCHUNK + BSTAGES * 2 * BCHUNK) * (SPLIT ? 2 : HS / 64) + 1024;
   static unsigned long long smem_set = 0;  // per template instantiation
-  auto kern = flash_backward_kernel<HS, KEYS>;
+  auto kern = flash_backward_kernel<HS, KEYS, SPLIT>;
   cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern), smem, &smem_set);
   if (e != cudaSuccess) return e;
   FlashBwdParams q = p;
   q.row_tiles = ((KEYS ? p.tk : p.tq) + FT - 1) / FT;
   const long long grid = static_cast<long long>(q.row_tiles) * (KEYS ? p.kv_heads : p.heads) * p.batch;
   return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(FTHREADS), smem, stream, pdl_enabled(), q, status);
+}
+template <bool KEYS>
+cudaError_t backward_any(const FlashBwdParams& p, bool split, cudaStream_t stream, int* status) {
+  if (split) return backward_hs<64, KEYS, true>(p, stream, status);
+  return p.hs <= 64 ? backward_hs<64, KEYS, false>(p, stream, status) : backward_hs<128, KEYS, false>(p, stream, status);
+}
+
+template <typename T>
+cudaError_t prepare_t(const FlashArgs& a, const FlashGradArgs& g, const FlashBwdParams& p, float* stats, float* norms, int qparts,
+                      cudaStream_t stream) {
+  const long long qblocks = static_cast<long long>(qparts) * a.heads * a.batch,
+                  blocks = qblocks + static_cast<long long>((a.tk + 63) / 64) * a.kv_heads * a.batch;
+  return launch_kernel(flash_prepare_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, pdl_enabled(),
+                       static_cast<const T*>(g.d_o.p), g.d_o.ld, g.d_o.head, g.d_o.batch, static_cast<const T*>(a.o.p), a.o.ld,
+                       a.o.head, a.o.batch, static_cast<const T*>(a.v.p), a.v.ld, a.v.head, a.v.batch,
+                       static_cast<const float*>(a.lse), p, reinterpret_cast<float2*>(stats), reinterpret_cast<unsigned*>(norms),
+                       qparts, qblocks);
 }
 
 }  // namespace
@@ -1282,7 +1517,49 @@ bool flash_supported(const FlashArgs& a) {
 cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* status) {
   FlashParams p;
   if (!fill_params(a, &p)) return cudaErrorInvalidValue;
-  return a.hs <= 64 ? forward_hs<64, 3>(p, stream, status) : forward_hs<128, 2>(p, stream, status);
+  if (a.inverse != nullptr) return forward_hs<64, 2, true>(p, stream, status);
+  return a.hs <= 64 ? forward_hs<64, 3, false>(p, stream, status) : forward_hs<128, 2, false>(p, stream, status);
+}
+
+// fp32 through Half planes: head size up to 64 (two planes take the shared memory of a 128-wide Half
+// operand) and contractions of at most 2048: an accumulator is added to once per 16 of them, and the
+// tensor core truncates each time, about 2^-25 of the running sum.
+bool flash_split_supported(const FlashArgs& a, bool backward) {
+  const long long group = a.heads / a.kv_heads, parts = (a.tq + 63) / 64 + (a.tk + 63) / 64;
+  return tmap_encoder_available() && a.hs <= 64 && a.tk <= 2048 && (!backward || group * a.tq <= 2048) &&
+         parts * a.heads * a.batch <= 0x1fffffffLL;
+}
+long long flash_planes(long long t, long long heads, long long batch) { return 64 * t * heads * batch; }
+
+cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, cudaStream_t stream) {
+  SplitParams p;
+  std::memset(&p, 0, sizeof(p));
+  const long long units = static_cast<long long>(a->batch) * a->kv_heads;
+  p.count = d_o != nullptr ? 4 : 3;
+  p.hs = a->hs; p.batch = a->batch; p.kv_heads = a->kv_heads;
+  p.most = reinterpret_cast<unsigned*>(work);
+  p.inverse = work + 4 * units;
+  a->inverse = p.inverse;
+  FlashOperand* ops[4] = {&a->q, &a->k, &a->v, d_o};
+  long long blocks = 0;
+  for (int i = 0; i < p.count; ++i) {
+    const bool query = i == 0 || i == 3;
+    SplitOperand& o = p.op[i];
+    o.x = static_cast<const float*>(ops[i]->p);
+    o.ld = ops[i]->ld; o.head = ops[i]->head; o.batch = ops[i]->batch;
+    o.planes = static_cast<__half*>(ops[i]->planes);
+    o.lengths = query ? a->q_lengths : a->k_lengths;
+    o.t = query ? a->tq : a->tk;
+    o.heads = query ? a->heads : a->kv_heads;
+    o.per = query ? a->heads / a->kv_heads : 1;
+    o.block0 = blocks;
+    blocks += static_cast<long long>((o.t + 63) / 64) * o.heads * a->batch;
+  }
+  cudaError_t e = cudaMemsetAsync(p.most, 0, sizeof(unsigned) * 4 * units, stream);
+  if (e != cudaSuccess) return e;
+  e = launch_kernel(split_most_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, pdl_enabled(), p);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(split_planes_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, pdl_enabled(), p);
 }
 
 int flash_token_splits(const FlashArgs& a, int num_sms, long long* floats) {
@@ -1366,6 +1643,7 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
                                   float* sums, int* launches, cudaStream_t stream, int* status) {
   FlashBwdParams p;
   std::memset(&p, 0, sizeof(p));
+  const bool split = a.inverse != nullptr;
   const struct {
     CUtensorMap* map;
     const FlashOperand* x;
@@ -1375,11 +1653,13 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
               {&p.tmQ64, &a.q, a.tq, a.heads, BN},   {&p.tmDO64, &g.d_o, a.tq, a.heads, BN},
               {&p.tmK64, &a.k, a.tk, a.kv_heads, BN}, {&p.tmV64, &a.v, a.tk, a.kv_heads, BN}};
   for (const auto& m : maps)
-    if (!encode_heads_tmap(m.map, m.x->p, a.hs, m.t, m.heads, a.batch, m.x->ld, m.x->head, m.x->batch, m.rows))
-      return cudaErrorInvalidValue;
-  p.dq = static_cast<__half*>(const_cast<void*>(g.dq.p));
-  p.dk = static_cast<__half*>(const_cast<void*>(g.dk.p));
-  p.dv = static_cast<__half*>(const_cast<void*>(g.dv.p));
+    if (!encode_operand(m.map, *m.x, a.hs, m.t, m.heads, a.batch, m.rows, split)) return cudaErrorInvalidValue;
+  const long long units = static_cast<long long>(a.batch) * a.kv_heads;
+  p.iq = a.inverse; p.ik = a.inverse + units; p.iv = a.inverse + 2 * units; p.ido = a.inverse + 3 * units;
+  p.vec_dq = rows16(g.dq); p.vec_dk = rows16(g.dk); p.vec_dv = rows16(g.dv);
+  p.dq = const_cast<void*>(g.dq.p);
+  p.dk = const_cast<void*>(g.dk.p);
+  p.dv = const_cast<void*>(g.dv.p);
   p.lddq = g.dq.ld; p.shdq = g.dq.head; p.sbdq = g.dq.batch;
   p.lddk = g.dk.ld; p.shdk = g.dk.head; p.sbdk = g.dk.batch;
   p.lddv = g.dv.ld; p.shdv = g.dv.head; p.sbdv = g.dv.batch;
@@ -1401,22 +1681,16 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
   cudaError_t e = cudaMemsetAsync(norms, 0, sizeof(unsigned) * 2 * a.batch * a.kv_heads, stream);
   if (e != cudaSuccess) return e;
   const int qparts = qtiles * 2;
-  const long long qblocks = static_cast<long long>(qparts) * a.heads * a.batch,
-                  blocks = qblocks + static_cast<long long>((a.tk + 63) / 64) * a.kv_heads * a.batch;
-  e = launch_kernel(flash_prepare_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, pdl_enabled(),
-                    static_cast<const __half*>(g.d_o.p), g.d_o.ld, g.d_o.head, g.d_o.batch, static_cast<const __half*>(a.o.p),
-                    a.o.ld, a.o.head, a.o.batch, static_cast<const __half*>(a.v.p), a.v.ld, a.v.head, a.v.batch,
-                    static_cast<const float*>(a.lse), p, reinterpret_cast<float2*>(stats), reinterpret_cast<unsigned*>(norms),
-                    qparts, qblocks);
+  e = split ? prepare_t<float>(a, g, p, stats, norms, qparts, stream) : prepare_t<__half>(a, g, p, stats, norms, qparts, stream);
   *launches = 1;
   if (e != cudaSuccess) return e;
   if (p.dk != nullptr || p.dv != nullptr) {
-    e = a.hs <= 64 ? backward_hs<64, true>(p, stream, status) : backward_hs<128, true>(p, stream, status);
+    e = backward_any<true>(p, split, stream, status);
     ++*launches;
     if (e != cudaSuccess) return e;
   }
   if (p.dq != nullptr || dist != nullptr) {
-    e = a.hs <= 64 ? backward_hs<64, false>(p, stream, status) : backward_hs<128, false>(p, stream, status);
+    e = backward_any<false>(p, split, stream, status);
     ++*launches;
     if (e != cudaSuccess) return e;
   }
@@ -1426,7 +1700,7 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
   d.batch = a.batch; d.heads = a.heads; d.tiles = qtiles; d.tile_rows = FT; d.slots = 2; d.width = p.width;
   d.reach = a.reach; d.q_offset = a.q_offset; d.q_offsets = a.q_offsets;
   *launches += 2;
-  return launch_rel_table_grad(1, d, sums, g.map, g.buckets, g.accumulate, g.dtable, g.lddt, stream);
+  return launch_rel_table_grad(split ? 0 : 1, d, sums, g.map, g.buckets, g.accumulate, g.dtable, g.lddt, stream);
 }
 
 }  // namespace gb

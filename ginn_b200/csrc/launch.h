@@ -227,11 +227,13 @@ cudaError_t launch_rel_table_grad(int dtype, const RelDist& d, float* sums, cons
 struct FlashOperand {
   const void* p;
   long long ld, head, batch;
+  void* planes;  // fp32 operands: room for their two Half planes, flash_planes(...) floats
 };
 struct FlashArgs {
   FlashOperand q, k, v, o;
   float* lse;
   const float* bias;  // [head][2 * reach + 1], times log2(e); null = none
+  const float* inverse;  // fp32 operands, split: their inverse scales (set by launch_flash_split)
   int tq, tk, hs, heads, kv_heads, batch;
   long long reach, q_offset;
   const int* q_offsets;
@@ -244,6 +246,11 @@ struct FlashArgs {
 // 128, 16-byte aligned bases and strides.
 bool flash_supported(const FlashArgs& a);
 cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* status);
+// fp32 operands of the same kernels: split into two Half planes each, two kernels.  `work`:
+// 8 * batch * kv heads floats; d_o null: forward only.
+bool flash_split_supported(const FlashArgs& a, bool backward);
+long long flash_planes(long long t, long long heads, long long batch);
+cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, cudaStream_t stream);
 // Few queries against a long cache (at most 16 rows share a key head): number of parts the keys are
 // split into, 0 when the shape does not qualify, and the scratch the parts need.
 int flash_token_splits(const FlashArgs& a, int num_sms, long long* floats);
