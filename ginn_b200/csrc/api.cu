@@ -2095,7 +2095,7 @@ gb::FlashArgs flash_args(const ginn_b200_relative_attention& a) {
   return f;
 }
 // Planes of fp32 operands for the flash kernels.
-int flash_split(Scratch* scratch, gb::FlashArgs* f, gb::FlashOperand* d_o) {
+int flash_split(Scratch* scratch, gb::FlashArgs* f, gb::FlashOperand* d_o, float* stats, float* norms) {
   float *work, *q, *k, *v, *d = nullptr;
   CU_TRY(scratch->take(&work, 8LL * f->batch * f->kv_heads));
   CU_TRY(scratch->take(&q, gb::flash_planes(f->tq, f->heads, f->batch)));
@@ -2104,7 +2104,7 @@ int flash_split(Scratch* scratch, gb::FlashArgs* f, gb::FlashOperand* d_o) {
   if (d_o) CU_TRY(scratch->take(&d, gb::flash_planes(f->tq, f->heads, f->batch)));
   f->q.planes = q; f->k.planes = k; f->v.planes = v;
   if (d_o) d_o->planes = d;
-  CU_TRY(gb::launch_flash_split(f, d_o, work, scratch->stream));
+  CU_TRY(gb::launch_flash_split(f, d_o, work, stats, norms, scratch->stream));
   g_launches.fetch_add(2);
   return GINN_B200_OK;
 }
@@ -2155,7 +2155,7 @@ int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, c
   }
   if (dtype == GINN_B200_F32 && t_force_path == PATH_AUTO && !token_rows(*a) && gb::flash_split_supported(f, false)) {
     Scratch scratch(stream);
-    if (int s = flash_split(&scratch, &f, nullptr)) return s;
+    if (int s = flash_split(&scratch, &f, nullptr, nullptr, nullptr)) return s;
     if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
     CU_TRY(gb::launch_flash_forward(f, stream, ctx->d_status));
     g_launches.fetch_add(1);
@@ -2203,13 +2203,13 @@ int ginn_b200_relative_attention_backward(int device, void* stream_, int dtype, 
     if (t_force_path != PATH_AUTO || !(half ? gb::flash_backward_supported(f, fg) : gb::flash_split_supported(f, true)))
       return relative_composed(device, stream, dtype, *a, g);
     Scratch scratch(stream);
-    if (!half)
-      if (int s = flash_split(&scratch, &f, &fg.d_o)) return s;
     if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
     const gb::FlashScratch need = gb::flash_backward_scratch(f, g->dtable != nullptr);
     float *stats, *norms, *dist = nullptr, *sums = nullptr;
     CU_TRY(scratch.take(&stats, need.stats));
     CU_TRY(scratch.take(&norms, need.norms));
+    if (!half)
+      if (int s = flash_split(&scratch, &f, &fg.d_o, stats, norms)) return s;
     if (g->dtable) {
       CU_TRY(scratch.take(&dist, need.dist));
       CU_TRY(scratch.take(&sums, need.sums));

@@ -485,65 +485,107 @@ struct SplitOperand {
   __half* planes;
   const int* lengths;
   int t, heads, per;      // heads per scale
+  int vec;                // rows allow 16-byte accesses
   long long block0;       // first CTA of this operand
 };
 struct SplitParams {
-  SplitOperand op[4];
+  SplitOperand op[4];     // q, k, v and, for the backward pass, d_o
   int count, hs, batch, kv_heads;
   unsigned* most;         // [operand][batch][kv heads]: bits of the largest magnitude
+  unsigned* norms;        // backward: [d_o, v][batch][kv heads]: bits of the largest row's squared norm
   float* inverse;         // [operand][batch][kv heads]: what a scaled value is multiplied by to get it back
+  // backward: delta = sum d_o o and lse of every query
+  const float* o;
+  long long ldo, sho, sbo;
+  int vec_o, tq_pad;
+  const float* lse;
+  float2* stats;
 };
-// Rows 64 part .. 64 part + 63 of one head, by CTA; the operand's fields selected one by one (indexing
-// the parameters would copy them to local memory).
+constexpr int kSplitRows = 128;  // per CTA: sixteen threads to a row, four elements each, eight sweeps
+// Rows row0 .. row0 + 127 of one head, by CTA; the operand's fields selected one by one (indexing the
+// parameters would copy them to local memory).
 struct SplitPart {
   const float* x = nullptr;
   __half* planes = nullptr;
   long long ld = 0, plane = 0;
-  int which = 0, unit = 0, row0 = 0, rows = 0, real = 0;
-  bool first = false;
+  int which = 0, unit = 0, row0 = 0, rows = 0, real = 0, vec = 0, batch = 0, head = 0, heads = 1;
   __device__ __forceinline__ explicit SplitPart(const SplitParams& p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (i >= p.count || blockIdx.x < p.op[i].block0) continue;
       const long long at = blockIdx.x - p.op[i].block0;
-      const int parts = (p.op[i].t + 63) / 64, hb = static_cast<int>(at / parts), b = hb / p.op[i].heads, h = hb % p.op[i].heads;
+      const int parts = (p.op[i].t + kSplitRows - 1) / kSplitRows, hb = static_cast<int>(at / parts);
+      heads = p.op[i].heads;
+      batch = hb / heads;
+      head = hb - batch * heads;
       which = i;
-      unit = b * p.kv_heads + h / p.op[i].per;
-      row0 = static_cast<int>(at % parts) * 64;
+      unit = batch * p.kv_heads + head / p.op[i].per;
+      row0 = static_cast<int>(at % parts) * kSplitRows;
       rows = p.op[i].t;
-      real = rel_length(p.op[i].lengths, b, rows);
+      real = rel_length(p.op[i].lengths, batch, rows);
+      vec = p.op[i].vec;
       ld = p.op[i].ld;
-      x = p.op[i].x + h * p.op[i].head + b * p.op[i].batch;
+      x = p.op[i].x + head * p.op[i].head + batch * p.op[i].batch;
       planes = p.op[i].planes + static_cast<long long>(hb) * rows * 64;
-      plane = static_cast<long long>(p.batch) * p.op[i].heads * rows * 64;
-      first = row0 == 0;
+      plane = static_cast<long long>(p.batch) * heads * rows * 64;
     }
   }
 };
+// Elements col .. col + 3 of a row, zero from n on.
+__device__ __forceinline__ float4 load_four(const float* x, int n, int vec) {
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (vec && n >= 4) return *reinterpret_cast<const float4*>(x);
+  if (n > 0) v.x = x[0];
+  if (n > 1) v.y = x[1];
+  if (n > 2) v.z = x[2];
+  if (n > 3) v.w = x[3];
+  return v;
+}
 
+// Largest magnitude of every unit and, for the backward pass, the largest row norms of d_o and v.
 __global__ void __launch_bounds__(256)
 split_most_kernel(const __grid_constant__ SplitParams p) {
-  __shared__ unsigned red[8];
+  __shared__ unsigned red[2][8];
   pdl_wait();
   pdl_launch_dependents();
   const SplitPart part(p);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  unsigned m = 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = 4 * (lane & 15);
+  const bool norm = p.norms != nullptr && part.which >= 2;
+  float4 x[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const int row = part.row0 + warp * 8 + k;
-    if (row >= part.real) continue;
-    const float* x = part.x + row * part.ld;
+    const int row = part.row0 + 16 * k + 2 * warp + (lane >> 4);
+    x[k] = load_four(part.x + row * part.ld + col, row < part.real ? p.hs - col : 0, part.vec);
+  }
+  unsigned m = 0, q = 0;
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (lane + 32 * e < p.hs) m = max(m, __float_as_uint(fabsf(x[lane + 32 * e])));
+  for (int k = 0; k < 8; ++k) {
+    const float4 v = x[k];
+    m = max(max(m, max(__float_as_uint(fabsf(v.x)), __float_as_uint(fabsf(v.y)))),
+            max(__float_as_uint(fabsf(v.z)), __float_as_uint(fabsf(v.w))));
+    if (norm) {
+      float s = (v.x * v.x + v.y * v.y) + (v.z * v.z + v.w * v.w);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      q = max(q, __float_as_uint(s));
+    }
   }
   m = __reduce_max_sync(0xffffffffu, m);
-  if (lane == 0) red[warp] = m;
+  q = __reduce_max_sync(0xffffffffu, q);
+  if (lane == 0) {
+    red[0][warp] = m;
+    red[1][warp] = q;
+  }
   __syncthreads();
   if (threadIdx.x != 0) return;
-  for (int w = 1; w < 8; ++w) m = max(m, red[w]);
-  atomicMax(p.most + part.which * p.batch * p.kv_heads + part.unit, m);  // a maximum: the order does not matter
+  for (int w = 1; w < 8; ++w) {
+    m = max(m, red[0][w]);
+    q = max(q, red[1][w]);
+  }
+  // maxima of non-negative values: the order of the updates does not matter
+  const int units = p.batch * p.kv_heads;
+  atomicMax(p.most + part.which * units + part.unit, m);
+  if (norm) atomicMax(p.norms + (part.which == 3 ? 0 : units) + part.unit, q);
 }
 
 __global__ void __launch_bounds__(256)
@@ -551,7 +593,7 @@ split_planes_kernel(const __grid_constant__ SplitParams p) {
   pdl_wait();
   pdl_launch_dependents();
   const SplitPart part(p);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = 4 * (lane & 15);
   const int at = part.which * p.batch * p.kv_heads + part.unit;
   const unsigned most = p.most[at];
   // 2^(14 - exponent of the largest); not numbers and infinities go through as they are
@@ -559,24 +601,40 @@ split_planes_kernel(const __grid_constant__ SplitParams p) {
   e = e > 126 ? 126 : e;
   if (most == 0 || most >= 0x7f800000u) e = 0;
   const float scale = __uint_as_float(static_cast<unsigned>(e + 127) << 23);
-  if (part.first && threadIdx.x == 0) p.inverse[at] = 1.f / scale;
-  float x[8][2];
+  if (part.row0 == 0 && threadIdx.x == 0) p.inverse[at] = 1.f / scale;
+  const bool dot = p.stats != nullptr && part.which == 3;
+  float4 x[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const int row = part.row0 + warp * 8 + k;
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-      x[k][c] = row < part.real && 2 * lane + c < p.hs ? part.x[row * part.ld + 2 * lane + c] * scale : 0.f;
+    const int row = part.row0 + 16 * k + 2 * warp + (lane >> 4);
+    x[k] = load_four(part.x + row * part.ld + col, row < part.real ? p.hs - col : 0, part.vec);
   }
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const int row = part.row0 + warp * 8 + k;
-    if (row >= part.rows) continue;
-    uint32_t hi, lo;
-    split_pair(x[k][0], x[k][1], hi, lo);
-    __half* to = part.planes + static_cast<long long>(row) * 64 + 2 * lane;
-    *reinterpret_cast<uint32_t*>(to) = hi;
-    *reinterpret_cast<uint32_t*>(to + part.plane) = lo;
+    const int row = part.row0 + 16 * k + 2 * warp + (lane >> 4);
+    if (row < part.rows) {
+      uint2 hi, lo;
+      split_pair(x[k].x * scale, x[k].y * scale, hi.x, lo.x);
+      split_pair(x[k].z * scale, x[k].w * scale, hi.y, lo.y);
+      __half* to = part.planes + static_cast<long long>(row) * 64 + col;
+      *reinterpret_cast<uint2*>(to) = hi;
+      *reinterpret_cast<uint2*>(to + part.plane) = lo;
+    }
+    if (!dot) continue;  // uniform over the CTA
+    const float4 o = load_four(p.o + row * p.ldo + part.head * p.sho + part.batch * p.sbo + col, row < part.real ? p.hs - col : 0,
+                               p.vec_o);
+    float s = (x[k].x * o.x + x[k].y * o.y) + (x[k].z * o.z + x[k].w * o.w);
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+    if ((lane & 15) == 0 && row < p.tq_pad) {
+      const long long hb = static_cast<long long>(part.batch) * part.heads + part.head;
+      float2 st = make_float2(INFINITY, 0.f);
+      if (row < part.real) {
+        const float l = p.lse[hb * part.rows + row];
+        if (l > -INFINITY) st = make_float2(l * kLog2e, s);
+      }
+      p.stats[hb * p.tq_pad + row] = st;
+    }
   }
 }
 
@@ -911,47 +969,25 @@ struct FlashBwdParams {
   int causal, accumulate;
 };
 
-// Power of two dS is multiplied with.  Split operands' norms are those of the scaled values.
+// Power of two dS is multiplied with: the bound from the rows' norms or, where their squares leave fp32
+// (split operands only), from the largest elements.
 template <bool SPLIT>
 __device__ __forceinline__ float ds_scale(const FlashBwdParams& p, int unit) {
-  const float a = __uint_as_float(p.norms[unit]), b = __uint_as_float(p.norms[p.batch * p.kv_heads + unit]);
-  float e = 13.f - 0.5f * (log2f(a) + log2f(b));
-  if (SPLIT) e -= log2f(p.ido[unit]) + log2f(p.iv[unit]);
-  if (!(a > 0.f && b > 0.f && a < INFINITY && b < INFINITY)) return 1.f;
+  float e = 13.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float q = __uint_as_float(p.norms[i * p.batch * p.kv_heads + unit]);
+    if (q > 1e-36f && q < 1e36f) e -= 0.5f * log2f(q);
+    else if (SPLIT) e -= 15.f + 3.f + log2f((i == 0 ? p.ido : p.iv)[unit]);  // 64 elements below 2^15 as scaled
+    else return 1.f;
+  }
   return exp2f(floorf(fminf(fmaxf(e, -120.f), 120.f)));
 }
-// Eight consecutive elements as they are stored, zero behind the first n.
-template <typename T>
-struct Eight;
-template <>
-struct Eight<__half> {
-  uint4 w;
-  __device__ __forceinline__ void load(const __half* p, int n) {  // n: 0 or at least 8 (head sizes are multiples of it)
-    w = make_uint4(0, 0, 0, 0);
-    if (n > 0) w = *reinterpret_cast<const uint4*>(p);
-  }
-  __device__ __forceinline__ float get(int e) const {
-    const uint32_t u = e < 2 ? w.x : e < 4 ? w.y : e < 6 ? w.z : w.w;
-    const __half2 h = *reinterpret_cast<const __half2*>(&u);
-    return e & 1 ? __high2float(h) : __low2float(h);
-  }
-};
-template <>
-struct Eight<float> {
-  float x[8];
-  __device__ __forceinline__ void load(const float* p, int n) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = e < n ? p[e] : 0.f;
-  }
-  __device__ __forceinline__ float get(int e) const { return x[e]; }
-};
-
 // delta and lse of every query, and the largest norms of dO and v rows per key head.  Sixteen threads
 // per row; a CTA takes 64 rows of one head, of dO (first `qparts` parts) or of v.
-template <typename T>
 __global__ void __launch_bounds__(256)
-flash_prepare_kernel(const T* d_o, long long lddo, long long shdo, long long sbdo, const T* o, long long ldo,
-                     long long sho, long long sbo, const T* v, long long ldv, long long shv, long long sbv,
+flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long long sbdo, const __half* o, long long ldo,
+                     long long sho, long long sbo, const __half* v, long long ldv, long long shv, long long sbv,
                      const float* __restrict__ lse, const FlashBwdParams p, float2* __restrict__ stats,
                      unsigned* __restrict__ norms, int qparts, long long qblocks) {
   __shared__ float red[16];
@@ -967,25 +1003,38 @@ flash_prepare_kernel(const T* d_o, long long lddo, long long shdo, long long sbd
   const int kv = queries ? head / p.group : head;
   const int len = queries ? rel_length(p.q_lengths, batch, p.tq) : rel_length(p.k_lengths, batch, p.tk);
   const int unit = batch * p.kv_heads + kv;
-  const float to = sizeof(T) == 4 ? 1.f / (queries ? p.ido : p.iv)[unit] : 1.f;  // as the planes hold it
+  auto widen = [&](uint4 w, float (&f)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
+      f[2 * e] = q.x;
+      f[2 * e + 1] = q.y;
+    }
+  };
   float norm[4], dot[4];
   {
-    Eight<T> wa[4], wb[4];
+    uint4 wa[4], wb[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {  // all loads before the first sum
       const int i = part * 64 + k * 16 + row16;
-      const int n = i < len ? p.hs - sub * 8 : 0;  // elements of this thread
-      wa[k].load(queries ? d_o + i * lddo + head * shdo + batch * sbdo + sub * 8 : v + i * ldv + head * shv + batch * sbv + sub * 8, n);
-      wb[k].load(o + i * ldo + head * sho + batch * sbo + sub * 8, queries ? n : 0);
+      wa[k] = wb[k] = make_uint4(0, 0, 0, 0);
+      if (i < len && sub * 8 < p.hs) {
+        wa[k] = *reinterpret_cast<const uint4*>(queries ? d_o + i * lddo + head * shdo + batch * sbdo + sub * 8
+                                                        : v + i * ldv + head * shv + batch * sbv + sub * 8);
+        if (queries) wb[k] = *reinterpret_cast<const uint4*>(o + i * ldo + head * sho + batch * sbo + sub * 8);
+      }
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+      float a[8], b[8];
+      widen(wa[k], a);
+      widen(wb[k], b);
       norm[k] = dot[k] = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float a = wa[k].get(e);
-        norm[k] += (a * to) * (a * to);
-        dot[k] += a * wb[k].get(e);
+        norm[k] += a[e] * a[e];
+        dot[k] += a[e] * b[e];
       }
     }
   }
@@ -1493,14 +1542,13 @@ cudaError_t backward_any(const FlashBwdParams& p, bool split, cudaStream_t strea
   return p.hs <= 64 ? backward_hs<64, KEYS, false>(p, stream, status) : backward_hs<128, KEYS, false>(p, stream, status);
 }
 
-template <typename T>
-cudaError_t prepare_t(const FlashArgs& a, const FlashGradArgs& g, const FlashBwdParams& p, float* stats, float* norms, int qparts,
-                      cudaStream_t stream) {
+cudaError_t prepare(const FlashArgs& a, const FlashGradArgs& g, const FlashBwdParams& p, float* stats, float* norms, int qparts,
+                    cudaStream_t stream) {
   const long long qblocks = static_cast<long long>(qparts) * a.heads * a.batch,
                   blocks = qblocks + static_cast<long long>((a.tk + 63) / 64) * a.kv_heads * a.batch;
-  return launch_kernel(flash_prepare_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, pdl_enabled(),
-                       static_cast<const T*>(g.d_o.p), g.d_o.ld, g.d_o.head, g.d_o.batch, static_cast<const T*>(a.o.p), a.o.ld,
-                       a.o.head, a.o.batch, static_cast<const T*>(a.v.p), a.v.ld, a.v.head, a.v.batch,
+  return launch_kernel(flash_prepare_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, pdl_enabled(),
+                       static_cast<const __half*>(g.d_o.p), g.d_o.ld, g.d_o.head, g.d_o.batch, static_cast<const __half*>(a.o.p),
+                       a.o.ld, a.o.head, a.o.batch, static_cast<const __half*>(a.v.p), a.v.ld, a.v.head, a.v.batch,
                        static_cast<const float*>(a.lse), p, reinterpret_cast<float2*>(stats), reinterpret_cast<unsigned*>(norms),
                        qparts, qblocks);
 }
@@ -1531,7 +1579,7 @@ bool flash_split_supported(const FlashArgs& a, bool backward) {
 }
 long long flash_planes(long long t, long long heads, long long batch) { return 64 * t * heads * batch; }
 
-cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, cudaStream_t stream) {
+cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, float* stats, float* norms, cudaStream_t stream) {
   SplitParams p;
   std::memset(&p, 0, sizeof(p));
   const long long units = static_cast<long long>(a->batch) * a->kv_heads;
@@ -1540,6 +1588,16 @@ cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, cud
   p.most = reinterpret_cast<unsigned*>(work);
   p.inverse = work + 4 * units;
   a->inverse = p.inverse;
+  if (d_o != nullptr) {
+    p.norms = reinterpret_cast<unsigned*>(norms);
+    p.o = static_cast<const float*>(a->o.p);
+    p.ldo = a->o.ld; p.sho = a->o.head; p.sbo = a->o.batch;
+    p.vec_o = rows16(a->o);
+    p.lse = a->lse;
+    p.stats = reinterpret_cast<float2*>(stats);
+    p.tq_pad = (a->tq + FT - 1) / FT * FT;
+    static_assert(kSplitRows == FT, "the CTAs of d_o cover the padded queries");
+  }
   FlashOperand* ops[4] = {&a->q, &a->k, &a->v, d_o};
   long long blocks = 0;
   for (int i = 0; i < p.count; ++i) {
@@ -1552,16 +1610,17 @@ cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, cud
     o.t = query ? a->tq : a->tk;
     o.heads = query ? a->heads : a->kv_heads;
     o.per = query ? a->heads / a->kv_heads : 1;
+    o.vec = rows16(*ops[i]);
     o.block0 = blocks;
-    blocks += static_cast<long long>((o.t + 63) / 64) * o.heads * a->batch;
+    blocks += static_cast<long long>((o.t + kSplitRows - 1) / kSplitRows) * o.heads * a->batch;
   }
   cudaError_t e = cudaMemsetAsync(p.most, 0, sizeof(unsigned) * 4 * units, stream);
+  if (e == cudaSuccess && d_o != nullptr) e = cudaMemsetAsync(norms, 0, sizeof(unsigned) * 2 * units, stream);
   if (e != cudaSuccess) return e;
   e = launch_kernel(split_most_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, pdl_enabled(), p);
   if (e != cudaSuccess) return e;
   return launch_kernel(split_planes_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, pdl_enabled(), p);
 }
-
 int flash_token_splits(const FlashArgs& a, int num_sms, long long* floats) {
   const int rows = a.heads / a.kv_heads * a.tq;
   *floats = 0;
@@ -1678,12 +1737,14 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
   p.causal = a.causal;
   p.accumulate = g.accumulate;
   p.width = rel_dist_width(a.reach, a.tk, FT);
-  cudaError_t e = cudaMemsetAsync(norms, 0, sizeof(unsigned) * 2 * a.batch * a.kv_heads, stream);
-  if (e != cudaSuccess) return e;
-  const int qparts = qtiles * 2;
-  e = split ? prepare_t<float>(a, g, p, stats, norms, qparts, stream) : prepare_t<__half>(a, g, p, stats, norms, qparts, stream);
-  *launches = 1;
-  if (e != cudaSuccess) return e;
+  cudaError_t e = cudaSuccess;
+  *launches = 0;
+  if (!split) {  // split operands came with their statistics
+    e = cudaMemsetAsync(norms, 0, sizeof(unsigned) * 2 * a.batch * a.kv_heads, stream);
+    if (e == cudaSuccess) e = prepare(a, g, p, stats, norms, qtiles * 2, stream);
+    *launches = 1;
+    if (e != cudaSuccess) return e;
+  }
   if (p.dk != nullptr || p.dv != nullptr) {
     e = backward_any<true>(p, split, stream, status);
     ++*launches;

@@ -247,10 +247,11 @@ struct FlashArgs {
 bool flash_supported(const FlashArgs& a);
 cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* status);
 // fp32 operands of the same kernels: split into two Half planes each, two kernels.  `work`:
-// 8 * batch * kv heads floats; d_o null: forward only.
+// 8 * batch * kv heads floats; d_o null: forward only, else also the backward pass's stats and norms.
 bool flash_split_supported(const FlashArgs& a, bool backward);
 long long flash_planes(long long t, long long heads, long long batch);
-cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, cudaStream_t stream);
+cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, float* stats,
+                               float* norms, cudaStream_t stream);
 // Few queries against a long cache (at most 16 rows share a key head): number of parts the keys are
 // split into, 0 when the shape does not qualify, and the scratch the parts need.
 int flash_token_splits(const FlashArgs& a, int num_sms, long long* floats);
@@ -264,7 +265,8 @@ struct FlashGradArgs {
   int buckets, accumulate;
 };
 bool flash_backward_supported(const FlashArgs& a, const FlashGradArgs& g);
-// Scratch of the backward pass, in floats; dist and sums only when the table's gradient is wanted.
+// Scratch of the backward pass, in floats: stats and norms filled by launch_flash_split for fp32
+// operands and by launch_flash_backward for Half ones; dist and sums only when the table's gradient is wanted.
 struct FlashScratch {
   long long stats, norms, dist, sums;
 };

@@ -247,13 +247,18 @@ rel_diagonal_kernel(const RelScores s, float* __restrict__ ds, float factor, flo
   for (int at = threadIdx.x; at < s.tk + n - 1; at += 256) {
     // keys at - (n - 1) + i of query i: one distance
     float sum = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      const int j = at - (n - 1) + i;
-      if (j >= 0 && j < s.tk) {
-        const float v = m[i * s.ld + j];
-        sum += v;
-        m[i * s.ld + j] = v * factor;
+    for (int i0 = 0; i0 < n; i0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // all loads before the first store
+        const int j = at - (n - 1) + i0 + i;
+        v[i] = i0 + i < n && j >= 0 && j < s.tk ? m[(i0 + i) * s.ld + j] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = at - (n - 1) + i0 + i;
+        sum += v[i];
+        if (i0 + i < n && j >= 0 && j < s.tk) m[(i0 + i) * s.ld + j] = v[i] * factor;
       }
     }
     const long long d = at - (n - 1) - first;
@@ -281,18 +286,18 @@ rel_diagonal_kernel(const RelScores s, float* __restrict__ ds, float factor, flo
 
 // sums[head][reach + d] = the query tiles' sums of dS at distance d over all sequences, in order.
 // dist[sequence][head][tile][slot][width]: entry e of a tile belongs to distance low + e, low the
-// clamped smallest distance of its last query.  A CTA serves 32 distances, its eight warps every
-// eighth (sequence, tile).
-__global__ void __launch_bounds__(256)
+// clamped smallest distance of its last query.  A CTA serves 32 distances, its 32 warps every
+// 32nd (sequence, tile).
+__global__ void __launch_bounds__(1024)
 rel_dist_sum_kernel(const RelDist p, float* __restrict__ sums) {
-  __shared__ float red[8][32];
+  __shared__ float red[32][32];
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y;
   const long long at = static_cast<long long>(blockIdx.x) * 32 + lane, d = at - p.reach;
   float s = 0.f;
 #pragma unroll 4
-  for (int k = warp; k < p.batch * p.tiles; k += 8) {
+  for (int k = warp; k < p.batch * p.tiles; k += 32) {
     const int batch = k / p.tiles, tile = k - batch * p.tiles;
     const long long last = static_cast<long long>(tile + 1) * p.tile_rows - 1 + rel_offset(p.q_offset, p.q_offsets, batch);
     const long long e = d - rel_dist_low(p.reach, last);
@@ -305,7 +310,7 @@ rel_dist_sum_kernel(const RelDist p, float* __restrict__ sums) {
   if (warp != 0 || d > p.reach) return;
   float a = 0.f;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) a += red[w][lane];
+  for (int w = 0; w < 32; ++w) a += red[w][lane];
   sums[head * (2 * p.reach + 1) + at] = a;
 }
 
@@ -404,7 +409,7 @@ cudaError_t launch_rel_table_grad(int dtype, const RelDist& d, float* sums, cons
   if (d.dist != nullptr) {
     const long long n = 2 * d.reach + 1;
     const cudaError_t e = launch_kernel(rel_dist_sum_kernel,
-                                        dim3(static_cast<unsigned>((n + 31) / 32), static_cast<unsigned>(d.heads)), dim3(256), 0,
+                                        dim3(static_cast<unsigned>((n + 31) / 32), static_cast<unsigned>(d.heads)), dim3(1024), 0,
                                         stream, pdl_enabled(), d, sums);
     if (e != cudaSuccess) return e;
   }
