@@ -1638,7 +1638,7 @@ int norm_backward(int device, void* stream_, int dtype, const gb::NormGradArgs& 
   DevCtx* ctx;
   if (int s = get_ctx(device, &ctx)) return s;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  const int parts = gb::norm_backward_parts(a.rows, a.cols, ctx->num_sms);
+  const int parts = gb::norm_backward_parts(dtype, a.rows, a.cols, ctx->num_sms);
   void* partial = nullptr;
   if (weights && parts > 0)
     CU_TRY(cudaMallocAsync(&partial, static_cast<size_t>(parts) * 2 * a.rows * sizeof(float), stream));

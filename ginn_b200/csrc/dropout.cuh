@@ -32,8 +32,8 @@ struct Philox {
     c2 = static_cast<uint32_t>(off);
     c3 = static_cast<uint32_t>(off >> 32);
   }
-  // Bit i of the result: element 8 * block + i is kept.
-  __device__ __forceinline__ uint32_t keep8(unsigned long long block) const {
+  // The four output words of a block.
+  __device__ __forceinline__ uint4 words(unsigned long long block) const {
     uint32_t x0 = static_cast<uint32_t>(block), x1 = static_cast<uint32_t>(block >> 32), x2 = c2, x3 = c3;
     uint32_t a = k0, b = k1;
 #pragma unroll
@@ -47,12 +47,28 @@ struct Philox {
       a += 0x9E3779B9u;
       b += 0xBB67AE85u;
     }
-    const uint32_t w[4] = {x0, x1, x2, x3};
+    return make_uint4(x0, x1, x2, x3);
+  }
+  // x[i] of element 8 * block + i: times `factor` when it is kept, 0 otherwise.  Both halves of a word
+  // are compared in its upper sixteen bits.
+  __device__ __forceinline__ void drop8(unsigned long long block, float factor, float (&x)[8]) const {
+    const uint4 r = words(block);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w}, limit = threshold << 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = (w[i] << 16) >= limit ? x[2 * i] * factor : 0.f;
+      x[2 * i + 1] = w[i] >= limit ? x[2 * i + 1] * factor : 0.f;
+    }
+  }
+  // Bit i of the result: element 8 * block + i is kept.
+  __device__ __forceinline__ uint32_t keep8(unsigned long long block) const {
+    const uint4 r = words(block);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w}, limit = threshold << 16;
     uint32_t bits = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      bits |= ((w[i] & 0xffffu) >= threshold ? 1u : 0u) << (2 * i);
-      bits |= ((w[i] >> 16) >= threshold ? 1u : 0u) << (2 * i + 1);
+      bits |= ((w[i] << 16) >= limit ? 1u : 0u) << (2 * i);
+      bits |= (w[i] >= limit ? 1u : 0u) << (2 * i + 1);
     }
     return bits;
   }

@@ -91,31 +91,64 @@ __device__ __forceinline__ void store_piece(T* col, long long r0, long long rows
     }
   }
 }
-// Keep bits of those eight elements (the whole warp calls it).
+// Dropout of those eight elements (the whole warp calls it).
 template <bool VEC>
-__device__ __forceinline__ uint32_t keep_piece(const Philox& gen, long long col, long long rows,
-                                               long long r0, int lane) {
+__device__ __forceinline__ void drop_piece(const Philox& gen, float factor, long long col, long long rows, long long r0,
+                                           int lane, float (&x)[8]) {
   const unsigned long long e0 = static_cast<unsigned long long>(col) * rows;
-  if (VEC) return gen.keep8((e0 + r0) >> 3);  // rows % 8 == 0: r0 starts a block
-  return gen.keep_strided(e0 + (r0 - lane), lane);
-}
-__device__ __forceinline__ void drop8(float (&x)[8], uint32_t keep, float factor) {
+  if (VEC) {  // rows % 8 == 0: r0 starts a block
+    gen.drop8((e0 + r0) >> 3, factor, x);
+    return;
+  }
+  const uint32_t keep = gen.keep_strided(e0 + (r0 - lane), lane);
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = (keep >> e) & 1u ? x[e] * factor : 0.f;
 }
 
-// Sum over the G threads (a multiple of 32) that share a column; `slot` holds one value per warp
+// Eight elements as they lie in memory: what a prefetch keeps of a column.
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<__half> {
+  uint4 w;
+  __device__ __forceinline__ void load(const __half* p) { w = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+};
+template <>
+struct Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = *reinterpret_cast<const float4*>(p);
+    b = *reinterpret_cast<const float4*>(p + 4);
+  }
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+};
+
+// Sum over the G threads (a power of two, at least 32) that share a column; `slot` holds one value per warp
 // of the CTA and alternates between two buffers, so one barrier per reduction is enough.
 __device__ __forceinline__ float group_sum(float v, int G, int t, float* slot) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if (G == 32) return v;
-  const int warp = threadIdx.x >> 5, first = warp - (t >> 5);
-  if ((t & 31) == 0) slot[warp] = v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = G >> 5;
+  if (lane == 0) slot[warp] = v;
   asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / G), "r"(G) : "memory");
-  float s = 0.f;
-  for (int w = 0; w < G / 32; ++w) s += slot[first + w];
-  return s;
+  v = lane < n ? slot[warp - (t >> 5) + lane] : 0.f;
+  for (int o = n >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return __shfl_sync(0xffffffffu, v, 0);
 }
 // Two sums at once.
 __device__ __forceinline__ float2 group_sum2(float2 v, int G, int t, float2* slot) {
@@ -125,15 +158,15 @@ __device__ __forceinline__ float2 group_sum2(float2 v, int G, int t, float2* slo
     v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
   }
   if (G == 32) return v;
-  const int warp = threadIdx.x >> 5, first = warp - (t >> 5);
-  if ((t & 31) == 0) slot[warp] = v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = G >> 5;
+  if (lane == 0) slot[warp] = v;
   asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / G), "r"(G) : "memory");
-  float2 s = make_float2(0.f, 0.f);
-  for (int w = 0; w < G / 32; ++w) {
-    s.x += slot[first + w].x;
-    s.y += slot[first + w].y;
+  v = lane < n ? slot[warp - (t >> 5) + lane] : make_float2(0.f, 0.f);
+  for (int o = n >> 1; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
   }
-  return s;
+  return make_float2(__shfl_sync(0xffffffffu, v.x, 0), __shfl_sync(0xffffffffu, v.y, 0));
 }
 
 template <typename T>
@@ -157,7 +190,7 @@ __device__ __forceinline__ void form_h(const NormFwd<T>& p, const Philox& gen, l
                                        long long r0, int lane, float (&v)[8]) {
   load_piece<VEC>(p.x + col * p.ldx, r0, p.rows, v);
   if (p.h == nullptr) return;
-  if (p.drop.threshold != 0) drop8(v, keep_piece<VEC>(gen, col, p.rows, r0, lane), p.drop.factor);
+  if (p.drop.threshold != 0) drop_piece<VEC>(gen, p.drop.factor, col, p.rows, r0, lane, v);
   if (p.res != nullptr) {
     float q[8];
     load_piece<VEC>(p.res + col * p.ldres, r0, p.rows, q);
@@ -202,18 +235,28 @@ norm_forward_kernel(const NormFwd<T> p, int G) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     form_h<VEC>(p, gen, col, first_row<VEC>(i, G, t), lane, v[i]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s += v[i][e];
+    s += ((v[i][0] + v[i][1]) + (v[i][2] + v[i][3])) + ((v[i][4] + v[i][5]) + (v[i][6] + v[i][7]));
   }
   const float mean = group_sum(s, G, t, slot[0]) / static_cast<float>(p.rows);
   float q = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const long long r0 = first_row<VEC>(i, G, t);
+    if (VEC) {
+      F2 a(0.f);
+      const F2 m2(-mean);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float d = v[i][e] - mean;
-      if (VEC ? r0 < p.rows : r0 + 32 * e < p.rows) q += d * d;
+      for (int e = 0; e < 8; e += 2) {
+        const F2 d = add2(F2(v[i][e], v[i][e + 1]), m2);
+        a = fma2(d, d, a);
+      }
+      if (r0 < p.rows) q += a.sum();
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = v[i][e] - mean;
+        if (r0 + 32 * e < p.rows) q += d * d;
+      }
     }
   }
   const float rstd = 1.f / sqrtf(group_sum(q, G, t, slot[1]) / static_cast<float>(p.rows) + p.eps);
@@ -286,45 +329,70 @@ struct NormBwd {
   Dropout drop;
 };
 
-// Gradient of the normalisation's input from the column sums, and its two destinations.
+// The gradient of h to its two destinations.
 template <bool VEC, typename T>
-__device__ __forceinline__ void write_dh(const NormBwd<T>& p, const Philox& gen, long long col,
-                                         long long r0, int lane, float rstd, float2 m,
-                                         const float (&xh)[8], const float (&g)[8]) {
-  float d[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) d[e] = rstd * (g[e] - m.x - xh[e] * m.y);
-  if (p.dh != nullptr) {
-    float q[8];
-    load_piece<VEC>(p.dh + col * p.lddh, r0, p.rows, q);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) d[e] += q[e];
-  }
+__device__ __forceinline__ void write_out(const NormBwd<T>& p, const Philox& gen, long long col, long long r0, int lane,
+                                          float (&d)[8]) {
   float o[8];
   if (p.dres != nullptr) {
     T* c = p.dres + col * p.lddres;
+    if (p.accumulate) {
+      load_piece<VEC>(c, r0, p.rows, o);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = 0.f;
-    if (p.accumulate) load_piece<VEC>(c, r0, p.rows, o);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] += d[e];
-    store_piece<VEC>(c, r0, p.rows, o);
+      for (int e = 0; e < 8; ++e) o[e] += d[e];
+      store_piece<VEC>(c, r0, p.rows, o);
+    } else {
+      store_piece<VEC>(c, r0, p.rows, d);
+    }
   }
   if (p.dx != nullptr) {
     T* c = p.dx + col * p.lddx;
+    if (p.drop.threshold != 0) drop_piece<VEC>(gen, p.drop.factor, col, p.rows, r0, lane, d);
+    if (p.accumulate) {
+      load_piece<VEC>(c, r0, p.rows, o);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = 0.f;
-    if (p.accumulate) load_piece<VEC>(c, r0, p.rows, o);
-    if (p.drop.threshold != 0) drop8(d, keep_piece<VEC>(gen, col, p.rows, r0, lane), p.drop.factor);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] += d[e];
-    store_piece<VEC>(c, r0, p.rows, o);
+      for (int e = 0; e < 8; ++e) d[e] += o[e];
+    }
+    store_piece<VEC>(c, r0, p.rows, d);
   }
+}
+// Gradient of the normalisation's input from the column sums, added to d.
+__device__ __forceinline__ void add_input_grad(float rstd, float2 m, const float (&xh)[8], const float (&g)[8], float (&d)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) d[e] += rstd * (g[e] - m.x - xh[e] * m.y);
+}
+
+// A CTA's weight gradients: the groups add theirs through shared memory, in order, and the sums go to
+// this CTA's partial vector.
+template <bool VEC, int NV, typename T>
+__device__ __forceinline__ void leave_partial(const NormBwd<T>& p, int G, int t, int group, int groups, float* sums,
+                                              const float (&dg)[NV][8], const float (&db)[NV][8]) {
+  if (p.partial == nullptr) return;
+  for (int k = 0; k < groups; ++k) {
+    __syncthreads();
+    if (group != k) continue;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const long long r0 = first_row<VEC>(i, G, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const long long r = r0 + row_step<VEC>() * e;
+        if (r < p.rows) {
+          sums[r] = (k ? sums[r] : 0.f) + dg[i][e];
+          sums[p.rows + r] = (k ? sums[p.rows + r] : 0.f) + db[i][e];
+        }
+      }
+    }
+  }
+  __syncthreads();
+  float* out = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.rows;
+  for (long long r = threadIdx.x; r < 2 * p.rows; r += blockDim.x) out[r] = sums[r];
 }
 
 // Groups of G threads walk the columns; a thread meets the same rows in every column, so the
 // weight gradients stay in its registers until the end, where the groups of the CTA add theirs
 // through shared memory (2 x rows floats).
+// Columns off the 16-byte grid, and fp32 columns too long to hold twice, are loaded when their turn comes.
 template <typename T, bool VEC, int NV>
 __global__ void __launch_bounds__(512, 1)
 norm_backward_kernel(const NormBwd<T> p, int G) {
@@ -374,30 +442,122 @@ norm_backward_kernel(const NormBwd<T> p, int G) {
     s.x *= inv;
     s.y *= inv;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      write_dh<VEC>(p, gen, col, first_row<VEC>(i, G, t), lane, rstd, s, xh[i], g[i]);
-  }
-  if (p.partial == nullptr) return;
-  // the groups take turns, in order
-  for (int k = 0; k < groups; ++k) {
-    __syncthreads();
-    if (group != k) continue;
-#pragma unroll
     for (int i = 0; i < NV; ++i) {
       const long long r0 = first_row<VEC>(i, G, t);
+      float d[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const long long r = r0 + row_step<VEC>() * e;
-        if (r < p.rows) {
-          sums[r] = (k ? sums[r] : 0.f) + dg[i][e];
-          sums[p.rows + r] = (k ? sums[p.rows + r] : 0.f) + db[i][e];
-        }
-      }
+      for (int e = 0; e < 8; ++e) d[e] = 0.f;
+      if (p.dh != nullptr) load_piece<VEC>(p.dh + col * p.lddh, r0, p.rows, d);
+      add_input_grad(rstd, s, xh[i], g[i], d);
+      write_out<VEC>(p, gen, col, r0, lane, d);
     }
   }
+  leave_partial<VEC, NV>(p, G, t, group, groups, sums, dg, db);
+}
+
+// The same with the next column's operands on their way while this one is worked on: a column's reduction
+// (a barrier behind two shuffles trees) waits for all of its loads, so without them the memory idles
+// between columns.  What is kept of a column is packed as it lies in memory.
+// The gain lies in shared memory as fp32 (behind the place of the weight sums).  DH: there is a gradient
+// from elsewhere.
+template <typename T, int NV, bool DH>
+__global__ void __launch_bounds__(512, 1)
+norm_backward_ahead_kernel(const NormBwd<T> p, int G) {
+  __shared__ float2 slot[2][16];
+  extern __shared__ __align__(16) float sums[];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int groups = blockDim.x / G, group = threadIdx.x / G;
+  const int t = threadIdx.x % G, lane = threadIdx.x & 31, rows = static_cast<int>(p.rows);
+  const Philox gen(p.drop);
+  float* gain = sums + (p.partial != nullptr ? 2 * rows : 0);
+  for (int r = threadIdx.x; r < rows; r += blockDim.x) gain[r] = p.gain != nullptr ? to_f(p.gain[r]) : 1.f;
   __syncthreads();
-  float* out = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.rows;
-  for (long long r = threadIdx.x; r < 2 * p.rows; r += blockDim.x) out[r] = sums[r];
+  F2 dg[NV][4], db[NV][4];
+  Raw8<T> x[NV], y[NV], z[DH ? NV : 1];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dg[i][e] = db[i][e] = F2(0.f);
+  const float inv = 1.f / static_cast<float>(p.rows);
+  const long long step = static_cast<long long>(gridDim.x) * groups;
+  float mean = 0.f, rstd = 0.f;
+  auto fetch = [&](long long col) {
+    if (col >= p.cols) return;
+    mean = p.mean[col];
+    rstd = p.rstd[col];
+    const T* h = p.h + col * p.ldh;
+    const T* dy = p.dy + col * p.lddy;
+    const T* dh = p.dh + col * p.lddh;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int r0 = (i * G + t) * kEl;
+      if (r0 < rows) {
+        x[i].load(h + r0);
+        y[i].load(dy + r0);
+        if (DH) z[i].load(dh + r0);
+      } else {
+        x[i].zero();
+        y[i].zero();
+        if (DH) z[i].zero();
+      }
+    }
+  };
+  long long col = static_cast<long long>(blockIdx.x) * groups + group;
+  fetch(col);
+  for (int turn = 0; col < p.cols; col += step, turn ^= 1) {
+    const F2 rs(rstd), shift(-mean * rstd);
+    const float rstd1 = rstd;
+    F2 xh[NV][4], g[NV][4], sx(0.f), sy(0.f);
+    Raw8<T> cz[DH ? NV : 1];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float a[8], b[8];
+      x[i].get(a);
+      y[i].get(b);
+      if (DH) cz[i] = z[i];
+      const int r0 = (i * G + t) * kEl;
+      const float4* w = reinterpret_cast<const float4*>(gain + (r0 < rows ? r0 : 0));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // (x - mean) rstd as one multiply-add: off by 2^-24 of |mean| rstd, as the subtraction's
+        // operands are
+        xh[i][e] = fma2(F2(a[2 * e], a[2 * e + 1]), rs, shift);
+        const F2 d(b[2 * e], b[2 * e + 1]);  // zero behind the last row
+        dg[i][e] = fma2(d, xh[i][e], dg[i][e]);
+        db[i][e] = add2(db[i][e], d);
+        const float4 k = w[e >> 1];
+        g[i][e] = mul2(d, e & 1 ? F2(k.z, k.w) : F2(k.x, k.y));
+        sx = add2(sx, g[i][e]);
+        sy = fma2(g[i][e], xh[i][e], sy);
+      }
+    }
+    fetch(col + step);
+    const float2 s = group_sum2(make_float2(sx.sum(), sy.sum()), G, t, slot[turn]);
+    // rstd (g - s.x / rows - xh s.y / rows)
+    const F2 c0(-rstd1 * s.x * inv), c1(-rstd1 * s.y * inv);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float d[8], q[8];
+      if (DH) cz[i].get(q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        F2 v = fma2(g[i][e], rs, fma2(xh[i][e], c1, c0));
+        if (DH) v = add2(v, F2(q[2 * e], q[2 * e + 1]));
+        v.get(d[2 * e], d[2 * e + 1]);
+      }
+      write_out<true>(p, gen, col, (i * G + t) * kEl, lane, d);
+    }
+  }
+  float sum_g[NV][8], sum_b[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      dg[i][e].get(sum_g[i][2 * e], sum_g[i][2 * e + 1]);
+      db[i][e].get(sum_b[i][2 * e], sum_b[i][2 * e + 1]);
+    }
+  leave_partial<true, NV>(p, G, t, group, groups, sums, sum_g, sum_b);
 }
 
 // Long columns: the column sums and the input's gradient in two sweeps, one CTA per column.
@@ -439,9 +599,13 @@ norm_backward_long_kernel(const NormBwd<T> p) {
   s.y /= static_cast<float>(p.rows);
   for (long long i = 0; i < pieces; ++i) {
     const long long r0 = first_row<VEC>(i, G, t);
-    float xh[8], g[8];
+    float xh[8], g[8], d[8];
     fetch(r0, xh, g);
-    write_dh<VEC>(p, gen, col, r0, lane, rstd, s, xh, g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d[e] = 0.f;
+    if (p.dh != nullptr) load_piece<VEC>(p.dh + col * p.lddh, r0, p.rows, d);
+    add_input_grad(rstd, s, xh, g, d);
+    write_out<VEC>(p, gen, col, r0, lane, d);
   }
 }
 
@@ -467,12 +631,12 @@ norm_weight_grad_kernel(const NormBwd<T> p, long long cols_per_part) {
 }
 
 // dgain / dbias (+)= the sum over `parts` partial vectors, always in the same order.  A CTA serves
-// 32 rows; its eight warps take every eighth vector.
+// 32 rows; its 32 warps take every 32nd vector.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 norm_weight_sum_kernel(const float* __restrict__ partial, int parts, long long rows,
                        T* __restrict__ dgain, T* __restrict__ dbias, int accumulate) {
-  __shared__ float red[8][32];
+  __shared__ float red[32][32];
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -481,13 +645,13 @@ norm_weight_sum_kernel(const float* __restrict__ partial, int parts, long long r
   if (out == nullptr) return;
   float s = 0.f;
   if (r < rows)
-    for (int k = warp; k < parts; k += 8) s += partial[(2LL * k + blockIdx.y) * rows + r];
+    for (int k = warp; k < parts; k += 32) s += partial[(2LL * k + blockIdx.y) * rows + r];
   red[warp][lane] = s;
   __syncthreads();
   if (warp != 0 || r >= rows) return;
   float a = accumulate ? to_f(out[r]) : 0.f;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) a += red[w][lane];
+  for (int w = 0; w < 32; ++w) a += red[w][lane];
   out[r] = from_f<T>(a);
 }
 
@@ -495,54 +659,68 @@ norm_weight_sum_kernel(const float* __restrict__ partial, int parts, long long r
 // gradient itself when it accumulates; VEC as above, with col_len the length of one contiguous run
 // (the whole matrix when nothing lies between its columns).
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 5)
 dropout_kernel(const T* x, long long ldx, const T* add, long long lda, T* y, long long ldy,
                long long rows, long long cols, Dropout drop) {
   pdl_wait();
   pdl_launch_dependents();
   const Philox gen(drop);
-  const long long per_col = (rows + 7) / 8, n = VEC ? per_col * cols : rows * cols;
   const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
-  for (long long q = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; q < n; q += stride) {
-    if (VEC) {
-      const long long col = cols == 1 ? 0 : q / per_col, r0 = (q - col * per_col) * 8;
-      const T* xp = x + col * ldx + r0;
-      const T* ap = add + col * lda + r0;
-      T* yp = y + col * ldy + r0;
-      float v[8], a[8];
-      const bool full = r0 + 8 <= rows;  // only the last run of a flat matrix may be short
-      if (full) {
-        load8(xp, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = r0 + e < rows ? to_f(xp[e]) : 0.f;
-      }
-      if (drop.threshold != 0)
-        drop8(v, gen.keep8((static_cast<unsigned long long>(col) * rows + r0) >> 3), drop.factor);
-      if (add != nullptr) {
-        if (full) {
-          load8(ap, a);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) a[e] = r0 + e < rows ? to_f(ap[e]) : 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += a[e];
-      }
-      if (full) {
-        store8(yp, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (r0 + e < rows) yp[e] = from_f<T>(v[e]);
-      }
-    } else {
+  const long long tid = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (!VEC) {
+    for (long long q = tid; q < rows * cols; q += stride) {
       const long long col = q / rows, r = q - col * rows;
       float v = to_f(x[col * ldx + r]);
       if (drop.threshold != 0)
         v = (gen.keep8(static_cast<unsigned long long>(q) >> 3) >> (q & 7)) & 1u ? v * drop.factor : 0.f;
       if (add != nullptr) v += to_f(add[col * lda + r]);
       y[col * ldy + r] = from_f<T>(v);
+    }
+    return;
+  }
+  // the next block's loads are on their way while a block is worked on
+  const long long per_col = (rows + 7) / 8, n = per_col * cols;
+  Raw8<T> xr, ar;
+  auto place = [&](long long q, long long& col, long long& r0) {
+    col = cols == 1 ? 0 : q / per_col;
+    r0 = (q - col * per_col) * 8;
+  };
+  auto fetch = [&](long long q) {
+    xr.zero();
+    ar.zero();
+    if (q >= n) return;
+    long long col, r0;
+    place(q, col, r0);
+    if (r0 + 8 > rows) return;  // the last run of a flat matrix may be shorter: element by element below
+    xr.load(x + col * ldx + r0);
+    if (add != nullptr) ar.load(add + col * lda + r0);
+  };
+  fetch(tid);
+  for (long long q = tid; q < n; q += stride) {
+    float v[8], a[8];
+    xr.get(v);
+    ar.get(a);
+    fetch(q + stride);
+    long long col, r0;
+    place(q, col, r0);
+    const bool full = r0 + 8 <= rows;
+    if (!full)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (r0 + e < rows) {
+          v[e] = to_f(x[col * ldx + r0 + e]);
+          if (add != nullptr) a[e] = to_f(add[col * lda + r0 + e]);
+        }
+    if (drop.threshold != 0) gen.drop8((static_cast<unsigned long long>(col) * rows + r0) >> 3, drop.factor, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += a[e];
+    T* yp = y + col * ldy + r0;
+    if (full) {
+      store8(yp, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (r0 + e < rows) yp[e] = from_f<T>(v[e]);
     }
   }
 }
@@ -558,6 +736,10 @@ int group_size(long long rows, int nv) {
     if (rows <= 8LL * nv * g) return g;
   return 0;
 }
+
+// Sweeps of eight rows per thread in the backward pass.  Half: two from 257 rows on; fp32: one as long as
+// 512 threads cover the column, since only then a second column fits in the registers beside the first.
+int backward_pieces(long long rows, int es) { return rows <= (es == 2 ? 256 : 4096) ? 1 : 2; }
 
 template <typename T, bool VEC>
 cudaError_t forward_tv(const NormFwd<T>& p, cudaStream_t stream) {
@@ -613,13 +795,17 @@ cudaError_t backward_tv(const NormBwd<T>& p, const NormGradArgs& a, int parts, c
                          dim3(static_cast<unsigned>((p.rows + 255) / 256), static_cast<unsigned>(parts)), dim3(256), 0,
                          stream, pdl_enabled(), p, per);
   }
-  const int nv = p.rows <= 256 ? 1 : 2;
+  const int nv = backward_pieces(p.rows, sizeof(T));
   const int G = group_size(p.rows, nv);
   auto kern = nv == 1 ? norm_backward_kernel<T, VEC, 1> : norm_backward_kernel<T, VEC, 2>;
-  const int smem = p.partial != nullptr ? static_cast<int>(2 * p.rows * sizeof(float)) : 0;
-  static unsigned long long smem_set[2] = {0, 0};  // per template instantiation
-  cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern),
-                                      2 * kNormRegisterRows * static_cast<int>(sizeof(float)), &smem_set[nv - 1]);
+  constexpr int kTwo = sizeof(T) == 2 ? 2 : 1;  // fp32 columns of two sweeps do not fit twice
+  const bool ahead = VEC && nv <= kTwo, dh = p.dh != nullptr;
+  if (ahead && nv == 1) kern = dh ? norm_backward_ahead_kernel<T, 1, true> : norm_backward_ahead_kernel<T, 1, false>;
+  if (ahead && nv == 2) kern = dh ? norm_backward_ahead_kernel<T, kTwo, true> : norm_backward_ahead_kernel<T, kTwo, false>;
+  const int smem = static_cast<int>(((p.partial != nullptr ? 2 : 0) + (ahead ? 1 : 0)) * p.rows * sizeof(float));
+  static unsigned long long smem_set[8] = {};  // one per kernel of this template instantiation
+  cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern), 3 * kNormRegisterRows * static_cast<int>(sizeof(float)),
+                                      &smem_set[(nv - 1) * 4 + ahead * 2 + dh]);
   if (e != cudaSuccess) return e;
   return launch_kernel(kern, dim3(static_cast<unsigned>(parts)), dim3(512), smem, stream, pdl_enabled(), p, G);
 }
@@ -649,7 +835,7 @@ cudaError_t backward_t(const NormGradArgs& a, int parts, float* partial, cudaStr
     if (e != cudaSuccess) return e;
   }
   if (a.dgain == nullptr && a.dbias == nullptr) return cudaSuccess;
-  return launch_kernel(norm_weight_sum_kernel<T>, dim3(static_cast<unsigned>((a.rows + 31) / 32), 2), dim3(256), 0, stream,
+  return launch_kernel(norm_weight_sum_kernel<T>, dim3(static_cast<unsigned>((a.rows + 31) / 32), 2), dim3(1024), 0, stream,
                        pdl_enabled(), static_cast<const float*>(partial), a.cols > 0 ? parts : 0, a.rows,
                        static_cast<T*>(a.dgain), static_cast<T*>(a.dbias), a.accumulate);
 }
@@ -665,7 +851,7 @@ cudaError_t dropout_t(const void* x, long long ldx, const void* add, long long l
   const bool vec = (cols == 1 || rows % 8 == 0) && cols16(x, ldx, es, cols) && cols16(y, ldy, es, cols) &&
                    cols16(add, lda, es, cols);
   const long long work = vec ? (rows + 7) / 8 * cols : rows * cols;
-  const long long want = (work + 255) / 256, most = static_cast<long long>(num_sms) * 8;
+  const long long want = (work + 255) / 256, most = static_cast<long long>(num_sms) * 5;
   const unsigned grid = static_cast<unsigned>(want < most ? want : most);
   auto kern = vec ? dropout_kernel<T, true> : dropout_kernel<T, false>;
   return launch_kernel(kern, dim3(grid), dim3(256), 0, stream, pdl_enabled(), static_cast<const T*>(x), ldx,
@@ -674,7 +860,7 @@ cudaError_t dropout_t(const void* x, long long ldx, const void* add, long long l
 
 }  // namespace
 
-int norm_backward_parts(long long rows, long long cols, int num_sms) {
+int norm_backward_parts(int dtype, long long rows, long long cols, int num_sms) {
   if (cols <= 0) return 0;
   if (rows > kNormRegisterRows) {
     // enough CTAs to fill the device with 256 rows each, at most 64 partial vectors
@@ -685,7 +871,7 @@ int norm_backward_parts(long long rows, long long cols, int num_sms) {
     const long long per = (cols + parts - 1) / parts;
     return static_cast<int>((cols + per - 1) / per);
   }
-  const int groups = 512 / group_size(rows, rows <= 256 ? 1 : 2);
+  const int groups = 512 / group_size(rows, backward_pieces(rows, dtype == 0 ? 4 : 2));
   const long long want = (cols + groups - 1) / groups;
   return static_cast<int>(want < num_sms ? want : num_sms);
 }
