@@ -189,7 +189,13 @@ def _dtype_of(t: torch.Tensor) -> int:
     raise GinnB200Error(2, f"unsupported tensor dtype {t.dtype}")
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(t: torch.Tensor) -> int:
+    # the handle without a Stream object around it: a tenth of the time, on every call
+    if _raw_stream is not None and t.device.index is not None:
+        return _raw_stream(t.device.index)
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
@@ -462,11 +468,16 @@ def softmax_backward(y: torch.Tensor, dy: torch.Tensor, dx: torch.Tensor, accumu
 def _matrix(t: torch.Tensor, name: str, like: torch.Tensor) -> tuple:
     """(pointer, leading dimension) of a column-major matrix with the shape, type and device of
     `like`."""
-    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+    shape = t.shape
+    if t is not like and (shape != like.shape or t.dtype != like.dtype or t.device != like.device):
         raise GinnB200Error(1, f"{name}: shape, type or device differs from the other operands'")
-    if t.dim() != 2 or (t.shape[0] > 1 and t.stride(0) != 1) or (t.shape[1] > 1 and t.stride(1) < max(t.shape[0], 1)):
+    if len(shape) != 2:
         raise GinnB200Error(1, f"{name}: matrix must be column-major")
-    return t.data_ptr(), _ld(t)
+    rows, cols = shape
+    step, ld = t.stride()
+    if (rows > 1 and step != 1) or (cols > 1 and ld < max(rows, 1)):
+        raise GinnB200Error(1, f"{name}: matrix must be column-major")
+    return t.data_ptr(), ld if cols > 1 else max(rows, 1)
 
 
 def _opt_matrix(t: Optional[torch.Tensor], name: str, like: torch.Tensor) -> tuple:
@@ -574,40 +585,44 @@ def relative_buckets(buckets: int, max_distance: int, bidirectional: bool,
     return out
 
 
-def _heads(t: torch.Tensor, name: str, shape, like: torch.Tensor) -> tuple:
+def _heads(t: torch.Tensor, name: str, shape, dtype, device) -> tuple:
     """(pointer, ld, head stride, batch stride) of a (head size, time, heads, batch) tensor."""
-    if tuple(t.shape) != tuple(shape) or t.dtype != like.dtype or t.device != like.device:
-        raise GinnB200Error(1, f"{name}: expected {tuple(shape)} of {like.dtype} on {like.device}")
-    if t.shape[0] > 1 and t.stride(0) != 1:
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise GinnB200Error(1, f"{name}: expected {tuple(shape)} of {dtype} on {device}")
+    step, ld, head, batch = t.stride()
+    if step != 1 and shape[0] > 1:
         raise GinnB200Error(1, f"{name}: the elements of a head must be contiguous")
-    return t.data_ptr(), t.stride(1), t.stride(2), t.stride(3)
+    return t.data_ptr(), ld, head, batch
 
 
 def _relative_attention(q, k, v, table, bucket_map, o, lse, scale, causal, q_offset, q_offsets,
                         q_lengths, k_lengths):
-    for name, t in (("q", q), ("k", k)):
-        if t.dim() != 4:
+    qs, ks = q.shape, k.shape
+    for name, x in (("q", qs), ("k", ks)):
+        if len(x) != 4:
             raise GinnB200Error(1, f"{name}: expected (head size, time, heads, batch)")
-    hs, tq, heads, batch = q.shape
-    tk, kv = k.shape[1], k.shape[2]
+    hs, tq, heads, batch = qs
+    if ks[0] != hs or ks[3] != batch:
+        raise GinnB200Error(1, "k: head size or batch differs from q's")
+    dtype, device = q.dtype, q.device
     tab, ldt, buckets, reach, bmap = None, 0, 0, 0, None
     if table is not None:
-        if table.dim() != 2 or table.shape[1] != heads or table.dtype != q.dtype or table.device != q.device:
-            raise GinnB200Error(1, f"table: expected buckets x {heads} of {q.dtype} on {q.device}")
+        if table.dim() != 2 or table.shape[1] != heads or table.dtype != dtype or table.device != device:
+            raise GinnB200Error(1, f"table: expected buckets x {heads} of {dtype} on {device}")
         if bucket_map is None or bucket_map.dim() != 1 or bucket_map.numel() % 2 == 0:
             raise GinnB200Error(1, "bucket_map: expected 2 * reach + 1 ints")
         buckets, reach = table.shape[0], bucket_map.numel() // 2
         tab, ldt = _matrix(table, "table", table)
-        bmap = _vector(bucket_map, "bucket_map", 2 * reach + 1, torch.int32, q.device)
+        bmap = _vector(bucket_map, "bucket_map", 2 * reach + 1, torch.int32, device)
     return _RelativeAttention(
-        tq, tk, hs, heads, kv, batch, *_heads(q, "q", (hs, tq, heads, batch), q),
-        *_heads(k, "k", (hs, tk, kv, batch), q), *_heads(v, "v", (hs, tk, kv, batch), q), tab, ldt,
-        buckets, bmap, reach, scale, int(causal), q_offset,
-        _vector(q_offsets, "q_offsets", batch, torch.int32, q.device),
-        _vector(q_lengths, "q_lengths", batch, torch.int32, q.device),
-        _vector(k_lengths, "k_lengths", batch, torch.int32, q.device),
-        *_heads(o, "o", (hs, tq, heads, batch), q),
-        _vector(lse, "lse", tq * heads * batch, torch.float32, q.device))
+        tq, ks[1], hs, heads, ks[2], batch, *_heads(q, "q", qs, dtype, device),
+        *_heads(k, "k", ks, dtype, device), *_heads(v, "v", ks, dtype, device), tab, ldt,
+        buckets, bmap, reach, scale, causal, q_offset,
+        _vector(q_offsets, "q_offsets", batch, torch.int32, device),
+        _vector(q_lengths, "q_lengths", batch, torch.int32, device),
+        _vector(k_lengths, "k_lengths", batch, torch.int32, device),
+        *_heads(o, "o", qs, dtype, device),
+        _vector(lse, "lse", tq * heads * batch, torch.float32, device))
 
 
 def relative_attention_forward(q, k, v, table, bucket_map, o, lse, scale: float,
@@ -630,10 +645,10 @@ def relative_attention_backward(q, k, v, table, bucket_map, o, lse, d_o, dq=None
     (accumulate=False) assigned (ginn_b200_relative_attention_backward)."""
     a = _relative_attention(q, k, v, table, bucket_map, o, lse, scale, causal, q_offset, q_offsets,
                             q_lengths, k_lengths)
-    out = [(None, 0, 0, 0) if t is None else _heads(t, n, x.shape, q)
+    out = [(None, 0, 0, 0) if t is None else _heads(t, n, x.shape, q.dtype, q.device)
            for n, t, x in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v))]
     dt = (None, 0) if dtable is None else _matrix(dtable, "dtable", dtable if table is None else table)
-    g = _RelativeAttentionGrad(*_heads(d_o, "d_o", q.shape, q), *out[0], *out[1], *out[2], *dt,
+    g = _RelativeAttentionGrad(*_heads(d_o, "d_o", q.shape, q.dtype, q.device), *out[0], *out[1], *out[2], *dt,
                                int(accumulate))
     _check(lib().ginn_b200_relative_attention_backward(_dev(q), _stream(q), _dtype_of(q),
                                                        C.byref(a), C.byref(g)))

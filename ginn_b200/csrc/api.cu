@@ -5,6 +5,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <string>
@@ -1626,7 +1627,7 @@ int norm_forward(int device, void* stream, int dtype, const gb::NormArgs& a) {
   if (!(a.eps > 0.f)) return fail(GINN_B200_BAD_ARGUMENT, "eps must be positive (got %g)", (double)a.eps);
   DevCtx* ctx;
   if (int s = get_ctx(device, &ctx)) return s;
-  CU_TRY(gb::launch_norm_forward(dtype, a, static_cast<cudaStream_t>(stream)));
+  CU_TRY(gb::launch_norm_forward(dtype, a, ctx->num_sms, static_cast<cudaStream_t>(stream)));
   g_launches.fetch_add(1);
   return GINN_B200_OK;
 }
@@ -1788,7 +1789,30 @@ struct Scratch {
   ~Scratch() {
     for (int i = 0; i < count; ++i) cudaFreeAsync(held[i], stream);
   }
+  // One allocation for parts that are known together: take() hands them out of it, 256 bytes apart,
+  // until it is used up (an allocation from the pool costs about a microsecond of host time).
+  char* block = nullptr;
+  size_t left = 0;
+  static size_t padded(long long n) { return (static_cast<size_t>(n > 0 ? n : 1) * sizeof(float) + 255) & ~size_t(255); }
+  cudaError_t reserve(std::initializer_list<long long> parts) {
+    size_t bytes = 0;
+    for (long long n : parts) bytes += padded(n);
+    if (count == 16) return cudaErrorMemoryAllocation;
+    void* p = nullptr;
+    const cudaError_t e = cudaMallocAsync(&p, bytes, stream);
+    if (e != cudaSuccess) return e;
+    held[count++] = p;
+    block = static_cast<char*>(p);
+    left = bytes;
+    return cudaSuccess;
+  }
   cudaError_t take(float** out, long long n) {
+    if (padded(n) <= left) {
+      *out = reinterpret_cast<float*>(block);
+      block += padded(n);
+      left -= padded(n);
+      return cudaSuccess;
+    }
     void* p = nullptr;
     if (count == 16) return cudaErrorMemoryAllocation;
     const cudaError_t e = cudaMallocAsync(&p, static_cast<size_t>(n > 0 ? n : 1) * sizeof(float), stream);
@@ -2094,10 +2118,12 @@ gb::FlashArgs flash_args(const ginn_b200_relative_attention& a) {
   f.causal = a.causal ? 1 : 0;
   return f;
 }
+long long split_work(const gb::FlashArgs& f) { return 8LL * f.batch * f.kv_heads; }
+long long bias_floats(const ginn_b200_relative_attention& a) { return a.table ? (2 * a.reach + 1) * a.heads : 0; }
 // Planes of fp32 operands for the flash kernels.
 int flash_split(Scratch* scratch, gb::FlashArgs* f, gb::FlashOperand* d_o, float* stats, float* norms) {
   float *work, *q, *k, *v, *d = nullptr;
-  CU_TRY(scratch->take(&work, 8LL * f->batch * f->kv_heads));
+  CU_TRY(scratch->take(&work, split_work(*f)));
   CU_TRY(scratch->take(&q, gb::flash_planes(f->tq, f->heads, f->batch)));
   CU_TRY(scratch->take(&k, gb::flash_planes(f->tk, f->kv_heads, f->batch)));
   CU_TRY(scratch->take(&v, gb::flash_planes(f->tk, f->kv_heads, f->batch)));
@@ -2139,9 +2165,10 @@ int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, c
   gb::FlashArgs f = flash_args(*a);
   if (dtype == GINN_B200_F16 && t_force_path == PATH_AUTO && gb::flash_supported(f)) {
     Scratch scratch(stream);
-    if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
     long long floats = 0;
     const int splits = gb::flash_token_splits(f, ctx->num_sms, &floats);
+    if (a->table || floats > 0) CU_TRY(scratch.reserve({bias_floats(*a), floats}));
+    if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
     int launches = 1;
     if (splits > 0) {
       float* parts = nullptr;
@@ -2155,6 +2182,8 @@ int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, c
   }
   if (dtype == GINN_B200_F32 && t_force_path == PATH_AUTO && !token_rows(*a) && gb::flash_split_supported(f, false)) {
     Scratch scratch(stream);
+    const long long keys = gb::flash_planes(f.tk, f.kv_heads, f.batch);
+    CU_TRY(scratch.reserve({split_work(f), gb::flash_planes(f.tq, f.heads, f.batch), keys, keys, bias_floats(*a)}));
     if (int s = flash_split(&scratch, &f, nullptr, nullptr, nullptr)) return s;
     if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
     CU_TRY(gb::launch_flash_forward(f, stream, ctx->d_status));
@@ -2203,8 +2232,10 @@ int ginn_b200_relative_attention_backward(int device, void* stream_, int dtype, 
     if (t_force_path != PATH_AUTO || !(half ? gb::flash_backward_supported(f, fg) : gb::flash_split_supported(f, true)))
       return relative_composed(device, stream, dtype, *a, g);
     Scratch scratch(stream);
-    if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
     const gb::FlashScratch need = gb::flash_backward_scratch(f, g->dtable != nullptr);
+    const long long queries = half ? 0 : gb::flash_planes(f.tq, f.heads, f.batch), keys = half ? 0 : gb::flash_planes(f.tk, f.kv_heads, f.batch);
+    CU_TRY(scratch.reserve({bias_floats(*a), need.stats, need.norms, need.dist, need.sums, split_work(f), queries, queries, keys, keys}));
+    if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
     float *stats, *norms, *dist = nullptr, *sums = nullptr;
     CU_TRY(scratch.take(&stats, need.stats));
     CU_TRY(scratch.take(&norms, need.norms));

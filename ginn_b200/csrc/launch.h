@@ -187,7 +187,7 @@ struct NormGradArgs {
 constexpr long long kNormRegisterRows = 8192;
 // Partial vectors (2 x rows floats each) the weight gradients of a backward pass need.
 int norm_backward_parts(int dtype, long long rows, long long cols, int num_sms);
-cudaError_t launch_norm_forward(int dtype, const NormArgs& a, cudaStream_t stream);
+cudaError_t launch_norm_forward(int dtype, const NormArgs& a, int num_sms, cudaStream_t stream);
 // `partial`: norm_backward_parts(...) x 2 x rows floats, null when neither dgain nor dbias is set.
 cudaError_t launch_norm_backward(int dtype, const NormGradArgs& a, int parts, float* partial,
                                  cudaStream_t stream);

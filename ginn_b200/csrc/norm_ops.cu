@@ -202,19 +202,28 @@ __device__ __forceinline__ void form_h(const NormFwd<T>& p, const Philox& gen, l
   store_piece<VEC>(p.h + col * p.ldh, r0, p.rows, v);
 }
 
+// y = ((h - mean) rstd) gain + bias, two values at a time.  The mean is subtracted first: a constant
+// column gives exactly the bias.
 template <bool VEC, typename T>
 __device__ __forceinline__ void write_y(const NormFwd<T>& p, long long col, long long r0, float mean,
                                         float rstd, float (&v)[8]) {
-  float g[8], b[8];
+  const F2 rs(rstd), shift(-mean);
+  F2 x[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    g[e] = 1.f;
-    b[e] = 0.f;
+  for (int e = 0; e < 4; ++e) x[e] = mul2(add2(F2(v[2 * e], v[2 * e + 1]), shift), rs);
+  float g[8];
+  if (p.gain != nullptr) {
+    load_piece<VEC>(p.gain, r0, p.rows, g);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = mul2(x[e], F2(g[2 * e], g[2 * e + 1]));
   }
-  if (p.gain != nullptr) load_piece<VEC>(p.gain, r0, p.rows, g);
-  if (p.bias != nullptr) load_piece<VEC>(p.bias, r0, p.rows, b);
+  if (p.bias != nullptr) {
+    load_piece<VEC>(p.bias, r0, p.rows, g);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (v[e] - mean) * rstd * g[e] + b[e];
+    for (int e = 0; e < 4; ++e) x[e] = add2(x[e], F2(g[2 * e], g[2 * e + 1]));
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e].get(v[2 * e], v[2 * e + 1]);
   store_piece<VEC>(p.y + col * p.ldy, r0, p.rows, v);
 }
 
@@ -655,73 +664,79 @@ norm_weight_sum_kernel(const float* __restrict__ partial, int parts, long long r
   out[r] = from_f<T>(a);
 }
 
-// y = (add) + drop(x): eight elements per thread and pass.  `add` is the residual forward and the
-// gradient itself when it accumulates; VEC as above, with col_len the length of one contiguous run
-// (the whole matrix when nothing lies between its columns).
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256, 5)
-dropout_kernel(const T* x, long long ldx, const T* add, long long lda, T* y, long long ldy,
-               long long rows, long long cols, Dropout drop) {
+// y = (add) + drop(x) on runs of `len` elements, eight per thread and pass, the next eight on their way
+// meanwhile.  `add` is the residual forward and the gradient itself when it accumulates.  COLS: one warp
+// per column of a matrix with gaps between its columns (rows % 8 == 0); otherwise the whole matrix is
+// one run.  Runs start on 16-byte boundaries.
+template <typename T, bool COLS>
+__global__ void __launch_bounds__(256)
+dropout_kernel(const T* x, long long ldx, const T* add, long long lda, T* y, long long ldy, long long len,
+               long long cols, Dropout drop) {
   pdl_wait();
   pdl_launch_dependents();
   const Philox gen(drop);
-  const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
-  const long long tid = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (!VEC) {
-    for (long long q = tid; q < rows * cols; q += stride) {
-      const long long col = q / rows, r = q - col * rows;
-      float v = to_f(x[col * ldx + r]);
-      if (drop.threshold != 0)
-        v = (gen.keep8(static_cast<unsigned long long>(q) >> 3) >> (q & 7)) & 1u ? v * drop.factor : 0.f;
-      if (add != nullptr) v += to_f(add[col * lda + r]);
-      y[col * ldy + r] = from_f<T>(v);
-    }
-    return;
-  }
-  // the next block's loads are on their way while a block is worked on
-  const long long per_col = (rows + 7) / 8, n = per_col * cols;
-  Raw8<T> xr, ar;
-  auto place = [&](long long q, long long& col, long long& r0) {
-    col = cols == 1 ? 0 : q / per_col;
-    r0 = (q - col * per_col) * 8;
-  };
-  auto fetch = [&](long long q) {
-    xr.zero();
+  const int lane = threadIdx.x & 31;
+  long long col = COLS ? static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5) : 0;
+  const long long col_step = COLS ? static_cast<long long>(gridDim.x) * 8 : 1;
+  const long long first = COLS ? lane : static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const long long step = COLS ? 32 : static_cast<long long>(gridDim.x) * 256;
+  const long long blocks = len >> 3;  // whole ones
+  for (; col < cols; col += col_step) {
+    const T* xp = x + col * ldx + first * 8;
+    const T* ap = add + col * lda + first * 8;
+    T* yp = y + col * ldy + first * 8;
+    const unsigned long long b0 = static_cast<unsigned long long>(col) * blocks;
+    Raw8<T> xr, ar;
     ar.zero();
-    if (q >= n) return;
-    long long col, r0;
-    place(q, col, r0);
-    if (r0 + 8 > rows) return;  // the last run of a flat matrix may be shorter: element by element below
-    xr.load(x + col * ldx + r0);
-    if (add != nullptr) ar.load(add + col * lda + r0);
-  };
-  fetch(tid);
-  for (long long q = tid; q < n; q += stride) {
-    float v[8], a[8];
-    xr.get(v);
-    ar.get(a);
-    fetch(q + stride);
-    long long col, r0;
-    place(q, col, r0);
-    const bool full = r0 + 8 <= rows;
-    if (!full)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (r0 + e < rows) {
-          v[e] = to_f(x[col * ldx + r0 + e]);
-          if (add != nullptr) a[e] = to_f(add[col * lda + r0 + e]);
-        }
-    if (drop.threshold != 0) gen.drop8((static_cast<unsigned long long>(col) * rows + r0) >> 3, drop.factor, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += a[e];
-    T* yp = y + col * ldy + r0;
-    if (full) {
-      store8(yp, v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (r0 + e < rows) yp[e] = from_f<T>(v[e]);
+    if (first < blocks) {
+      xr.load(xp);
+      if (add != nullptr) ar.load(ap);
     }
+    for (long long q = first; q < blocks; q += step) {
+      float v[8], a[8];
+      xr.get(v);
+      ar.get(a);
+      xp += step * 8;
+      ap += step * 8;
+      if (q + step < blocks) {
+        xr.load(xp);
+        if (add != nullptr) ar.load(ap);
+      }
+      if (drop.threshold != 0) gen.drop8(b0 + q, drop.factor, v);
+      if (add != nullptr)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += a[e];
+      store8(yp, v);
+      yp += step * 8;
+    }
+    // the elements behind the last whole block of a flat matrix
+    if (!COLS && first == 0 && (len & 7) != 0) {
+      const uint32_t keep = drop.threshold != 0 ? gen.keep8(blocks) : 0xffu;
+      for (int e = 0; e < (len & 7); ++e) {
+        float v = (keep >> e) & 1u ? to_f(x[blocks * 8 + e]) * drop.factor : 0.f;
+        if (add != nullptr) v += to_f(add[blocks * 8 + e]);
+        y[blocks * 8 + e] = from_f<T>(v);
+      }
+    }
+  }
+}
+
+// The same for any alignment, element by element.
+template <typename T>
+__global__ void __launch_bounds__(256)
+dropout_any_kernel(const T* x, long long ldx, const T* add, long long lda, T* y, long long ldy, long long rows,
+                   long long cols, Dropout drop) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const Philox gen(drop);
+  for (long long q = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; q < rows * cols;
+       q += static_cast<long long>(gridDim.x) * 256) {
+    const long long col = q / rows, r = q - col * rows;
+    float v = to_f(x[col * ldx + r]);
+    if (drop.threshold != 0)
+      v = (gen.keep8(static_cast<unsigned long long>(q) >> 3) >> (q & 7)) & 1u ? v * drop.factor : 0.f;
+    if (add != nullptr) v += to_f(add[col * lda + r]);
+    y[col * ldy + r] = from_f<T>(v);
   }
 }
 
@@ -742,10 +757,13 @@ int group_size(long long rows, int nv) {
 int backward_pieces(long long rows, int es) { return rows <= (es == 2 ? 256 : 4096) ? 1 : 2; }
 
 template <typename T, bool VEC>
-cudaError_t forward_tv(const NormFwd<T>& p, cudaStream_t stream) {
-  int nv = 1, G = 32;
-  if (p.rows > 256) nv = p.rows <= 512 ? 2 : 4;
-  G = group_size(p.rows, nv);
+cudaError_t forward_tv(const NormFwd<T>& p, int num_sms, cudaStream_t stream) {
+  // Rows per thread: 32 as long as one CTA covers the column that way; 16 off the 16-byte grid, where 32
+  // hold twice the registers (1001 x 5003 fp32: 28 us with 32).  Fewer where the columns alone would
+  // leave SMs idle: then a column's latency counts.
+  int nv = p.rows <= 256 ? 1 : p.rows <= 512 || (!VEC && p.rows <= 8192) ? 2 : 4;
+  while (nv > 1 && p.rows <= 2048 * nv && p.cols * group_size(p.rows, nv) < 256LL * num_sms) nv /= 2;
+  const int G = group_size(p.rows, nv);
   if (G == 0) {
     if (p.cols > 0x7fffffffLL) return cudaErrorInvalidValue;
     return launch_kernel(norm_forward_long_kernel<T, VEC>, dim3(static_cast<unsigned>(p.cols)), dim3(512), 0,
@@ -759,7 +777,7 @@ cudaError_t forward_tv(const NormFwd<T>& p, cudaStream_t stream) {
 }
 
 template <typename T>
-cudaError_t forward_t(const NormArgs& a, cudaStream_t stream) {
+cudaError_t forward_t(const NormArgs& a, int num_sms, cudaStream_t stream) {
   NormFwd<T> p;
   p.x = static_cast<const T*>(a.x);
   p.res = static_cast<const T*>(a.res);
@@ -777,7 +795,7 @@ cudaError_t forward_t(const NormArgs& a, cudaStream_t stream) {
   const bool vec = a.rows % 8 == 0 && cols16(a.x, a.ldx, es, a.cols) && cols16(a.y, a.ldy, es, a.cols) &&
                    cols16(a.res, a.ldres, es, a.cols) && cols16(a.h, a.ldh, es, a.cols) &&
                    cols16(a.gain, 0, es, 1) && cols16(a.bias, 0, es, 1);
-  return vec ? forward_tv<T, true>(p, stream) : forward_tv<T, false>(p, stream);
+  return vec ? forward_tv<T, true>(p, num_sms, stream) : forward_tv<T, false>(p, num_sms, stream);
 }
 
 template <typename T, bool VEC>
@@ -850,12 +868,19 @@ cudaError_t dropout_t(const void* x, long long ldx, const void* add, long long l
   const int es = sizeof(T);
   const bool vec = (cols == 1 || rows % 8 == 0) && cols16(x, ldx, es, cols) && cols16(y, ldy, es, cols) &&
                    cols16(add, lda, es, cols);
-  const long long work = vec ? (rows + 7) / 8 * cols : rows * cols;
-  const long long want = (work + 255) / 256, most = static_cast<long long>(num_sms) * 5;
-  const unsigned grid = static_cast<unsigned>(want < most ? want : most);
-  auto kern = vec ? dropout_kernel<T, true> : dropout_kernel<T, false>;
-  return launch_kernel(kern, dim3(grid), dim3(256), 0, stream, pdl_enabled(), static_cast<const T*>(x), ldx,
-                       static_cast<const T*>(add), lda, static_cast<T*>(y), ldy, rows, cols, drop);
+  const T* xp = static_cast<const T*>(x);
+  const T* ap = static_cast<const T*>(add);
+  T* yp = static_cast<T*>(y);
+  const long long most = static_cast<long long>(num_sms) * 8;
+  auto grid = [&](long long want) { return dim3(static_cast<unsigned>(want < 1 ? 1 : want < most ? want : most)); };
+  if (!vec)
+    return launch_kernel(dropout_any_kernel<T>, grid((rows * cols + 255) / 256), dim3(256), 0, stream, pdl_enabled(), xp, ldx, ap,
+                         lda, yp, ldy, rows, cols, drop);
+  if (cols > 1)
+    return launch_kernel(dropout_kernel<T, true>, grid((cols + 7) / 8), dim3(256), 0, stream, pdl_enabled(), xp, ldx, ap, lda, yp,
+                         ldy, rows, cols, drop);
+  return launch_kernel(dropout_kernel<T, false>, grid((rows / 8 + 255) / 256), dim3(256), 0, stream, pdl_enabled(), xp, ldx, ap,
+                       lda, yp, ldy, rows, cols, drop);
 }
 
 }  // namespace
@@ -876,8 +901,8 @@ int norm_backward_parts(int dtype, long long rows, long long cols, int num_sms) 
   return static_cast<int>(want < num_sms ? want : num_sms);
 }
 
-cudaError_t launch_norm_forward(int dtype, const NormArgs& a, cudaStream_t stream) {
-  return dtype == 0 ? forward_t<float>(a, stream) : forward_t<__half>(a, stream);
+cudaError_t launch_norm_forward(int dtype, const NormArgs& a, int num_sms, cudaStream_t stream) {
+  return dtype == 0 ? forward_t<float>(a, num_sms, stream) : forward_t<__half>(a, num_sms, stream);
 }
 
 cudaError_t launch_norm_backward(int dtype, const NormGradArgs& a, int parts, float* partial,
