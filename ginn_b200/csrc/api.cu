@@ -2124,14 +2124,35 @@ long long bias_floats(const ginn_b200_relative_attention& a) { return a.table ? 
 int flash_split(Scratch* scratch, gb::FlashArgs* f, gb::FlashOperand* d_o, float* stats, float* norms) {
   float *work, *q, *k, *v, *d = nullptr;
   CU_TRY(scratch->take(&work, split_work(*f)));
-  CU_TRY(scratch->take(&q, gb::flash_planes(f->tq, f->heads, f->batch)));
-  CU_TRY(scratch->take(&k, gb::flash_planes(f->tk, f->kv_heads, f->batch)));
-  CU_TRY(scratch->take(&v, gb::flash_planes(f->tk, f->kv_heads, f->batch)));
-  if (d_o) CU_TRY(scratch->take(&d, gb::flash_planes(f->tq, f->heads, f->batch)));
+  CU_TRY(scratch->take(&q, gb::flash_planes(f->hs, f->tq, f->heads, f->batch)));
+  CU_TRY(scratch->take(&k, gb::flash_planes(f->hs, f->tk, f->kv_heads, f->batch)));
+  CU_TRY(scratch->take(&v, gb::flash_planes(f->hs, f->tk, f->kv_heads, f->batch)));
+  if (d_o) CU_TRY(scratch->take(&d, gb::flash_planes(f->hs, f->tq, f->heads, f->batch)));
   f->q.planes = q; f->k.planes = k; f->v.planes = v;
   if (d_o) d_o->planes = d;
   CU_TRY(gb::launch_flash_split(f, d_o, work, stats, norms, scratch->stream));
   g_launches.fetch_add(2);
+  return GINN_B200_OK;
+}
+// Dense copies of Half operands the kernels cannot take where they are: q, k, v and, for the backward
+// pass, d_o and o.
+int flash_pack(Scratch* scratch, DevCtx* ctx, gb::FlashArgs* f, gb::FlashOperand* d_o) {
+  const long long queries = gb::flash_packed(f->hs, f->tq, f->heads, f->batch), keys = gb::flash_packed(f->hs, f->tk, f->kv_heads, f->batch);
+  CU_TRY(scratch->reserve({queries, keys, keys, d_o ? queries : 0, d_o ? queries : 0}));
+  auto pack = [&](gb::FlashOperand* x, bool query) {
+    float* to;
+    const cudaError_t e = scratch->take(&to, query ? queries : keys);
+    if (e != cudaSuccess) return e;
+    return gb::launch_flash_pack(x, f->hs, query ? f->tq : f->tk, query ? f->heads : f->kv_heads, f->batch, to, ctx->num_sms, scratch->stream);
+  };
+  CU_TRY(pack(&f->q, true));
+  CU_TRY(pack(&f->k, false));
+  CU_TRY(pack(&f->v, false));
+  if (d_o) {
+    CU_TRY(pack(d_o, true));
+    CU_TRY(pack(&f->o, true));
+  }
+  g_launches.fetch_add(d_o ? 5 : 3);
   return GINN_B200_OK;
 }
 // Few queries go through other kernels.
@@ -2163,8 +2184,10 @@ int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, c
     return GINN_B200_OK;
   }
   gb::FlashArgs f = flash_args(*a);
-  if (dtype == GINN_B200_F16 && t_force_path == PATH_AUTO && gb::flash_supported(f)) {
+  if (dtype == GINN_B200_F16 && t_force_path == PATH_AUTO && gb::flash_fits(f)) {
     Scratch scratch(stream);
+    if (!gb::flash_supported(f))
+      if (int s = flash_pack(&scratch, ctx, &f, nullptr)) return s;
     long long floats = 0;
     const int splits = gb::flash_token_splits(f, ctx->num_sms, &floats);
     if (a->table || floats > 0) CU_TRY(scratch.reserve({bias_floats(*a), floats}));
@@ -2182,8 +2205,8 @@ int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, c
   }
   if (dtype == GINN_B200_F32 && t_force_path == PATH_AUTO && !token_rows(*a) && gb::flash_split_supported(f, false)) {
     Scratch scratch(stream);
-    const long long keys = gb::flash_planes(f.tk, f.kv_heads, f.batch);
-    CU_TRY(scratch.reserve({split_work(f), gb::flash_planes(f.tq, f.heads, f.batch), keys, keys, bias_floats(*a)}));
+    const long long keys = gb::flash_planes(f.hs, f.tk, f.kv_heads, f.batch);
+    CU_TRY(scratch.reserve({split_work(f), gb::flash_planes(f.hs, f.tq, f.heads, f.batch), keys, keys, bias_floats(*a)}));
     if (int s = flash_split(&scratch, &f, nullptr, nullptr, nullptr)) return s;
     if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
     CU_TRY(gb::launch_flash_forward(f, stream, ctx->d_status));
@@ -2229,11 +2252,13 @@ int ginn_b200_relative_attention_backward(int device, void* stream_, int dtype, 
     fg.buckets = (int)a->buckets;
     fg.accumulate = g->accumulate ? 1 : 0;
     const bool half = dtype == GINN_B200_F16;
-    if (t_force_path != PATH_AUTO || !(half ? gb::flash_backward_supported(f, fg) : gb::flash_split_supported(f, true)))
+    if (t_force_path != PATH_AUTO || !(half ? gb::flash_fits(f) : gb::flash_split_supported(f, true)))
       return relative_composed(device, stream, dtype, *a, g);
     Scratch scratch(stream);
+    if (half && !gb::flash_backward_supported(f, fg))
+      if (int s = flash_pack(&scratch, ctx, &f, &fg.d_o)) return s;
     const gb::FlashScratch need = gb::flash_backward_scratch(f, g->dtable != nullptr);
-    const long long queries = half ? 0 : gb::flash_planes(f.tq, f.heads, f.batch), keys = half ? 0 : gb::flash_planes(f.tk, f.kv_heads, f.batch);
+    const long long queries = half ? 0 : gb::flash_planes(f.hs, f.tq, f.heads, f.batch), keys = half ? 0 : gb::flash_planes(f.hs, f.tk, f.kv_heads, f.batch);
     CU_TRY(scratch.reserve({bias_floats(*a), need.stats, need.norms, need.dist, need.sums, split_work(f), queries, queries, keys, keys}));
     if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
     float *stats, *norms, *dist = nullptr, *sums = nullptr;

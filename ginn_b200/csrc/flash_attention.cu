@@ -33,7 +33,7 @@ namespace gb {
 namespace {
 
 constexpr int FT = 128;               // queries or keys per tile
-constexpr int FTHREADS = 128 + 2 * 256;  // two working groups behind the TMA and MMA warps
+constexpr int FTHREADS = 128 + 2 * 256;  // two working groups behind the warpgroup of TMA and MMA
 constexpr int FCHUNK = FT * 128;      // bytes of 128 rows x 64 halves
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -50,22 +50,27 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Eight results of a row in the storage type: 16-byte stores where they are allowed (`vec`; always for
-// Half), element by element behind them and at the row's end.
+// Eight results of a row in the storage type, of which the first n exist: 16-byte stores where they are
+// allowed (`vec`), element by element elsewhere and at the row's end.
 __device__ __forceinline__ void store_row8(__half* to, int n, int vec, const float (&x)[8], bool add) {
-  if (n <= 0) return;  // n is a multiple of eight: head sizes are
-  uint32_t w[4];
-  uint4 old = make_uint4(0, 0, 0, 0);
-  if (add) old = *reinterpret_cast<const uint4*>(to);
-  const uint32_t o[4] = {old.x, old.y, old.z, old.w};
+  if (vec && n >= 8) {
+    uint32_t w[4];
+    uint4 old = make_uint4(0, 0, 0, 0);
+    if (add) old = *reinterpret_cast<const uint4*>(to);
+    const uint32_t o[4] = {old.x, old.y, old.z, old.w};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float2 q = make_float2(0.f, 0.f);
-    if (add) q = __half22float2(*reinterpret_cast<const __half2*>(&o[e]));
-    const __half2 h = __floats2half2_rn(x[2 * e] + q.x, x[2 * e + 1] + q.y);
-    w[e] = *reinterpret_cast<const uint32_t*>(&h);
+    for (int e = 0; e < 4; ++e) {
+      float2 q = make_float2(0.f, 0.f);
+      if (add) q = __half22float2(*reinterpret_cast<const __half2*>(&o[e]));
+      const __half2 h = __floats2half2_rn(x[2 * e] + q.x, x[2 * e + 1] + q.y);
+      w[e] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) to[e] = __float2half_rn(add ? __half2float(to[e]) + x[e] : x[e]);
   }
-  *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 __device__ __forceinline__ void store_row8(float* to, int n, int vec, const float (&x)[8], bool add) {
   if (vec && n >= 8) {
@@ -101,7 +106,7 @@ struct FlashParams {
   const float* bias;
   const float *iq, *ik, *iv;  // split operands: inverse scales, [batch][kv heads]
   int tq, tk, hs, heads, kv_heads, group, batch, qblocks;
-  int vec;                    // fp32 results: rows allow 16-byte accesses
+  int vec;                    // the result's rows allow 16-byte accesses
   long long reach, q_offset;
   const int* q_offsets;
   const int* q_lengths;
@@ -151,12 +156,15 @@ struct TileBias {
   }
 };
 
-// SPLIT: fp32 operands as two Half planes each (see split_planes_kernel), HS = 64.
-template <int HS, int NST, bool SPLIT>
-__global__ void __launch_bounds__(FTHREADS, 1)
+// SPLIT: fp32 operands as two Half planes each (see split_planes_kernel).  NQ: query tiles per CTA, one
+// where two would not fit (128-wide split operands: 64 KB a tile); then K and V have one stage each,
+// which is loaded again while the other's product and the softmax run.
+template <int HS, int NST, int NQ, bool SPLIT>
+__global__ void __launch_bounds__(128 + 256 * NQ, 1)
 flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ status) {
-  static_assert(!SPLIT || HS == 64, "a split operand's two planes take the place of two 64-wide chunks");
-  constexpr int CHUNKS = SPLIT ? 2 : HS / 64;
+  constexpr int WIDE = HS / 64;                  // 64-wide chunks of a plane
+  constexpr int CHUNKS = (SPLIT ? 2 : 1) * WIDE;
+  constexpr int CROSS = NQ * HS;                 // tensor memory: from a tile's result to its cross terms
   constexpr int TILE = FCHUNK * CHUNKS;  // bytes of one operand tile
   constexpr float PSHIFT = SPLIT ? 7.f : 0.f;  // probabilities are formed times 2^PSHIFT: their low parts stay normal
   extern __shared__ uint8_t smem_raw[];
@@ -169,7 +177,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t q_s = base, k_s = base + 2 * TILE, v_s = k_s + NST * TILE;
+  const uint32_t q_s = base, k_s = base + NQ * TILE, v_s = k_s + NST * TILE;
 
   if (warp == 0 && lane == 0) {
     prefetch_tmap(&p.tmQ);
@@ -207,8 +215,8 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
   const int hbs = p.heads * p.batch;
   const int qb = p.qblocks - 1 - static_cast<int>(blockIdx.x) / hbs;
   const FlashHead hd(p, static_cast<int>(blockIdx.x) % hbs);
-  const int i0 = qb * 2 * FT;
-  const int n0 = hd.tiles(p, i0), n1 = hd.tiles(p, i0 + FT);
+  const int i0 = qb * NQ * FT;
+  const int n0 = hd.tiles(p, i0), n1 = NQ > 1 ? hd.tiles(p, i0 + FT) : 0;
   const int n = n0 > n1 ? n0 : n1;
 
   if (warp == 0) {
@@ -216,7 +224,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
     auto load = [&](uint32_t dst, const CUtensorMap* map, uint64_t* bar, int at, int head) {
       mbar_arrive_expect_tx(smem_u32(bar), TILE);
       for (int c = 0; c < CHUNKS; ++c)
-        tma_load_4d(dst + c * FCHUNK, map, smem_u32(bar), SPLIT ? 0 : 64 * c, at, head, hd.batch + (SPLIT ? c * p.batch : 0));
+        tma_load_4d(dst + c * FCHUNK, map, smem_u32(bar), 64 * (c % WIDE), at, head, hd.batch + c / WIDE * p.batch);
     };
     if (elect_one()) {
 #pragma unroll
@@ -246,8 +254,8 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
 #pragma unroll
           for (int ks = 0; ks < HS / 16; ++ks) {
             const uint32_t at = (ks / 4) * FCHUNK + (ks % 4) * 32;
-            mma_f16(tmem + t * FT, make_smem_desc(a + at + (SPLIT && term == 0 ? FCHUNK : 0), 16, 1024),
-                    make_smem_desc(b + at + (SPLIT && term == 1 ? FCHUNK : 0), 16, 1024), IDESC_S, term > 0 || ks > 0);
+            mma_f16(tmem + t * FT, make_smem_desc(a + at + (SPLIT && term == 0 ? WIDE * FCHUNK : 0), 16, 1024),
+                    make_smem_desc(b + at + (SPLIT && term == 1 ? WIDE * FCHUNK : 0), 16, 1024), IDESC_S, term > 0 || ks > 0);
           }
         tc_commit(smem_u32(&s_full[t]));
       }
@@ -292,8 +300,8 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
             if (SPLIT) {
               // The cross terms have an accumulator of their own: the tensor core truncates when it adds, so
               // the long chain of the main one should be as short as it can be.
-              mma_f16_ts(o + 2 * HS, a, make_smem_desc(b + FCHUNK + ks * 2048, FCHUNK, 1024), IDESC_O, add);
-              mma_f16_ts(o + 2 * HS, a + 32, make_smem_desc(b + ks * 2048, FCHUNK, 1024), IDESC_O, 1u);
+              mma_f16_ts(o + CROSS, a, make_smem_desc(b + WIDE * FCHUNK + ks * 2048, FCHUNK, 1024), IDESC_O, add);
+              mma_f16_ts(o + CROSS, a + 32, make_smem_desc(b + ks * 2048, FCHUNK, 1024), IDESC_O, 1u);
             }
           }
           if (j == nt - 1) tc_commit(smem_u32(&o_full[t]));
@@ -370,7 +378,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
         if (j > 0) {  // O exists from the second tile on
 #pragma unroll
           for (int c = 0; c < (SPLIT ? HS : HS / 2); c += 16) {
-            const uint32_t col = o_col + c + (c >= HS / 2 ? 2 * HS - HS / 2 : 0);  // behind the main result: the cross terms
+            const uint32_t col = o_col + c + (c >= HS / 2 ? CROSS - HS / 2 : 0);  // behind the main result: the cross terms
             uint32_t w[16];
             tmem_ld16(col, w);
             tmem_ld_wait();
@@ -426,7 +434,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
         uint32_t w[8], x[8];
         if (nt > 0) {
           tmem_ld8(o_col + c, w);
-          if (SPLIT) tmem_ld8(o_col + 2 * HS + c, x);
+          if (SPLIT) tmem_ld8(o_col + CROSS + c, x);
           tmem_ld_wait();
         }
         float res[8];
@@ -456,7 +464,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
 // every element down to 2^-18 of the largest, and an absolute error of 2^-40 of the largest below
 // that.  A product is then three Half products, high x high + high x low + low x high, at twice the
 // rate of three TF32 products and with the same 2^-22 left out.  The planes are dense,
-// [plane][sequence][head][t][64], zero behind the head size and behind the sequences' lengths.
+// [plane][sequence][head][t][64 or 128], zero behind the head size and behind the sequences' lengths.
 struct SplitOperand {
   const float* x;
   long long ld, head, batch;
@@ -479,7 +487,7 @@ struct SplitParams {
   const float* lse;
   float2* stats;
 };
-constexpr int kSplitRows = 128;  // per CTA: sixteen threads to a row, four elements each, eight sweeps
+constexpr int kSplitRows = 128;  // per CTA: four elements of a row to a thread
 // Rows row0 .. row0 + 127 of one head, by CTA; the operand's fields selected one by one (indexing the
 // parameters would copy them to local memory).
 struct SplitPart {
@@ -487,7 +495,7 @@ struct SplitPart {
   __half* planes = nullptr;
   long long ld = 0, plane = 0;
   int which = 0, unit = 0, row0 = 0, rows = 0, real = 0, vec = 0, batch = 0, head = 0, heads = 1;
-  __device__ __forceinline__ explicit SplitPart(const SplitParams& p) {
+  __device__ __forceinline__ SplitPart(const SplitParams& p, int width) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (i >= p.count || blockIdx.x < p.op[i].block0) continue;
@@ -504,8 +512,8 @@ struct SplitPart {
       vec = p.op[i].vec;
       ld = p.op[i].ld;
       x = p.op[i].x + head * p.op[i].head + batch * p.op[i].batch;
-      planes = p.op[i].planes + static_cast<long long>(hb) * rows * 64;
-      plane = static_cast<long long>(p.batch) * heads * rows * 64;
+      planes = p.op[i].planes + static_cast<long long>(hb) * rows * width;
+      plane = static_cast<long long>(p.batch) * heads * rows * width;
     }
   }
 };
@@ -521,30 +529,32 @@ __device__ __forceinline__ float4 load_four(const float* x, int n, int vec) {
 }
 
 // Largest magnitude of every unit and, for the backward pass, the largest row norms of d_o and v.
+template <int W>
 __global__ void __launch_bounds__(256)
 split_most_kernel(const __grid_constant__ SplitParams p) {
   __shared__ unsigned red[2][8];
   pdl_wait();
   pdl_launch_dependents();
-  const SplitPart part(p);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = 4 * (lane & 15);
+  constexpr int LANES = W / 4, PER = 32 / LANES, SWEEPS = kSplitRows / (8 * PER);  // lanes to a row, rows to a warp
+  const SplitPart part(p, W);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = 4 * (lane % LANES);
   const bool norm = p.norms != nullptr && part.which >= 2;
-  float4 x[8];
+  float4 x[SWEEPS];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int row = part.row0 + 16 * k + 2 * warp + (lane >> 4);
+  for (int k = 0; k < SWEEPS; ++k) {
+    const int row = part.row0 + (8 * k + warp) * PER + lane / LANES;
     x[k] = load_four(part.x + row * part.ld + col, row < part.real ? p.hs - col : 0, part.vec);
   }
   unsigned m = 0, q = 0;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
+  for (int k = 0; k < SWEEPS; ++k) {
     const float4 v = x[k];
     m = max(max(m, max(__float_as_uint(fabsf(v.x)), __float_as_uint(fabsf(v.y)))),
             max(__float_as_uint(fabsf(v.z)), __float_as_uint(fabsf(v.w))));
     if (norm) {
       float s = (v.x * v.x + v.y * v.y) + (v.z * v.z + v.w * v.w);
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       q = max(q, __float_as_uint(s));
     }
   }
@@ -566,12 +576,14 @@ split_most_kernel(const __grid_constant__ SplitParams p) {
   if (norm) atomicMax(p.norms + (part.which == 3 ? 0 : units) + part.unit, q);
 }
 
+template <int W>
 __global__ void __launch_bounds__(256)
 split_planes_kernel(const __grid_constant__ SplitParams p) {
   pdl_wait();
   pdl_launch_dependents();
-  const SplitPart part(p);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = 4 * (lane & 15);
+  constexpr int LANES = W / 4, PER = 32 / LANES, SWEEPS = kSplitRows / (8 * PER);  // lanes to a row, rows to a warp
+  const SplitPart part(p, W);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = 4 * (lane % LANES);
   const int at = part.which * p.batch * p.kv_heads + part.unit;
   const unsigned most = p.most[at];
   // 2^(14 - exponent of the largest); not numbers and infinities go through as they are
@@ -581,20 +593,20 @@ split_planes_kernel(const __grid_constant__ SplitParams p) {
   const float scale = __uint_as_float(static_cast<unsigned>(e + 127) << 23);
   if (part.row0 == 0 && threadIdx.x == 0) p.inverse[at] = 1.f / scale;
   const bool dot = p.stats != nullptr && part.which == 3;
-  float4 x[8];
+  float4 x[SWEEPS];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int row = part.row0 + 16 * k + 2 * warp + (lane >> 4);
+  for (int k = 0; k < SWEEPS; ++k) {
+    const int row = part.row0 + (8 * k + warp) * PER + lane / LANES;
     x[k] = load_four(part.x + row * part.ld + col, row < part.real ? p.hs - col : 0, part.vec);
   }
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int row = part.row0 + 16 * k + 2 * warp + (lane >> 4);
+  for (int k = 0; k < SWEEPS; ++k) {
+    const int row = part.row0 + (8 * k + warp) * PER + lane / LANES;
     if (row < part.rows) {
       uint2 hi, lo;
       split_pair(x[k].x * scale, x[k].y * scale, hi.x, lo.x);
       split_pair(x[k].z * scale, x[k].w * scale, hi.y, lo.y);
-      __half* to = part.planes + static_cast<long long>(row) * 64 + col;
+      __half* to = part.planes + static_cast<long long>(row) * W + col;
       *reinterpret_cast<uint2*>(to) = hi;
       *reinterpret_cast<uint2*>(to + part.plane) = lo;
     }
@@ -603,8 +615,8 @@ split_planes_kernel(const __grid_constant__ SplitParams p) {
                                p.vec_o);
     float s = (x[k].x * o.x + x[k].y * o.y) + (x[k].z * o.z + x[k].w * o.w);
 #pragma unroll
-    for (int w = 8; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    if ((lane & 15) == 0 && row < p.tq_pad) {
+    for (int w = LANES / 2; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+    if (lane % LANES == 0 && row < p.tq_pad) {
       const long long hb = static_cast<long long>(part.batch) * part.heads + part.head;
       float2 st = make_float2(INFINITY, 0.f);
       if (row < part.real) {
@@ -613,6 +625,23 @@ split_planes_kernel(const __grid_constant__ SplitParams p) {
       }
       p.stats[hb * p.tq_pad + row] = st;
     }
+  }
+}
+
+// Half operands off the 16-byte grid (head sizes that are no multiple of 8, odd strides): a dense copy,
+// dst[sequence][head][t][W], zero behind the head size.  One warp per row and sweep.
+template <int W>
+__global__ void __launch_bounds__(256)
+flash_pack_kernel(const __half* __restrict__ src, long long ld, long long sh, long long sb, int hs, int t, int heads,
+                  long long rows, __half* __restrict__ dst) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  for (long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); row < rows; row += static_cast<long long>(gridDim.x) * 8) {
+    const long long hb = row / t, b = hb / heads;
+    const __half* x = src + (row - hb * t) * ld + (hb - b * heads) * sh + b * sb;
+#pragma unroll
+    for (int c = 0; c < W; c += 32) dst[row * W + c + lane] = c + lane < hs ? x[c + lane] : __float2half(0.f);
   }
 }
 
@@ -924,7 +953,6 @@ flash_token_join_kernel(const TokenParams p) {
 // and key head) to 2^14, so neither large nor small upstream gradients leave a Half's range.
 constexpr int BN = 64;             // rows of a streamed tile
 constexpr int BCHUNK = BN * 128;   // bytes of 64 rows x 64 halves
-constexpr int BSTAGES = 4;
 constexpr int kDistSmem = 1024;    // distances whose sums fit in shared memory (per group)
 
 struct FlashBwdParams {
@@ -938,7 +966,7 @@ struct FlashBwdParams {
   const float* bias;
   const float *iq, *ik, *iv, *ido;  // split operands: inverse scales, [batch][kv heads]
   int tq, tk, hs, heads, kv_heads, group, batch, tq_pad, row_tiles, width;
-  int vec_dq, vec_dk, vec_dv;       // fp32 results: rows allow 16-byte accesses
+  int vec_dq, vec_dk, vec_dv;       // the results' rows allow 16-byte accesses
   long long reach, q_offset;
   const int* q_offsets;
   const int* q_lengths;
@@ -956,7 +984,7 @@ __device__ __forceinline__ float ds_scale(const FlashBwdParams& p, int unit) {
   for (int i = 0; i < 2; ++i) {
     const float q = __uint_as_float(p.norms[i * p.batch * p.kv_heads + unit]);
     if (q > 1e-36f && q < 1e36f) e -= 0.5f * log2f(q);
-    else if (SPLIT) e -= 15.f + 3.f + log2f((i == 0 ? p.ido : p.iv)[unit]);  // 64 elements below 2^15 as scaled
+    else if (SPLIT) e -= 15.f + 3.5f + log2f((i == 0 ? p.ido : p.iv)[unit]);  // 128 elements below 2^15 as scaled
     else return 1.f;
   }
   return exp2f(floorf(fminf(fmaxf(e, -120.f), 120.f)));
@@ -1048,11 +1076,18 @@ flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long lon
   }
 }
 
-template <int HS, bool KEYS, bool SPLIT>
+// MODE: what a launch forms.  128-wide split operands leave room in tensor memory for one result (with its
+// cross terms) beside X and Y, and in shared memory for one stage: dK and dV are then two launches.
+enum FlashMode { KEYS_BOTH = 0, QUERIES = 1, KEYS_DK = 2, KEYS_DV = 3 };
+
+template <int HS, int MODE, int BSTAGES, bool SPLIT>
 __global__ void __launch_bounds__(FTHREADS, 1)
 flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict__ status) {
-  static_assert(!SPLIT || HS == 64, "a split operand's two planes take the place of two 64-wide chunks");
-  constexpr int CHUNKS = SPLIT ? 2 : HS / 64;
+  constexpr bool KEYS = MODE != QUERIES;
+  constexpr bool WANT_P = MODE == KEYS_BOTH || MODE == KEYS_DV, WANT_D = MODE != KEYS_DV;
+  constexpr int WIDE = HS / 64;           // 64-wide chunks of a plane
+  constexpr int CHUNKS = (SPLIT ? 2 : 1) * WIDE;
+  constexpr int PV_COL = MODE == KEYS_BOTH ? (SPLIT ? 2 * HS : HS) : 0;  // tensor memory: dV behind dK
   constexpr int ROWS = FCHUNK * CHUNKS;   // bytes of a resident operand
   constexpr int TILE = BCHUNK * CHUNKS;   // bytes of a streamed tile
   constexpr float PSHIFT = SPLIT ? 14.f : 12.f;  // P is formed times 2^PSHIFT
@@ -1126,7 +1161,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     if (n > 0 && elect_one()) {
       mbar_arrive_expect_tx(smem_u32(&rows_full), 2 * ROWS);
       for (int c = 0; c < CHUNKS; ++c) {
-        const int x = SPLIT ? 0 : 64 * c, w = batch + (SPLIT ? c * p.batch : 0);
+        const int x = 64 * (c % WIDE), w = batch + c / WIDE * p.batch;
         tma_load_4d(a1_s + c * FCHUNK, KEYS ? &p.tmK : &p.tmQ, smem_u32(&rows_full), x, r0, head, w);
         tma_load_4d(a2_s + c * FCHUNK, KEYS ? &p.tmV : &p.tmDO, smem_u32(&rows_full), x, r0, head, w);
       }
@@ -1137,7 +1172,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
         const int at = (first + it % per) * BN, h = KEYS ? head * p.group + it / per : kv;
         mbar_arrive_expect_tx(bar, 2 * TILE);
         for (int c = 0; c < CHUNKS; ++c) {
-          const int x = SPLIT ? 0 : 64 * c, w = batch + (SPLIT ? c * p.batch : 0);
+          const int x = 64 * (c % WIDE), w = batch + c / WIDE * p.batch;
           tma_load_4d(dst + c * BCHUNK, KEYS ? &p.tmQ64 : &p.tmK64, bar, x, at, h, w);
           tma_load_4d(dst + TILE + c * BCHUNK, KEYS ? &p.tmDO64 : &p.tmV64, bar, x, at, h, w);
         }
@@ -1170,13 +1205,13 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       if (leader) {
         const uint32_t b = b_s + s * 2 * TILE, d = tmem + (it & 1) * FT;
 #pragma unroll
-        for (int y = 0; y < 2; ++y)  // X = A1 B1^T, Y = A2 B2^T
+        for (int y = 0; y < (WANT_D ? 2 : 1); ++y)  // X = A1 B1^T, Y = A2 B2^T
 #pragma unroll
           for (int term = 0; term < (SPLIT ? 3 : 1); ++term)
 #pragma unroll
             for (int ks = 0; ks < HS / 16; ++ks) {
-              const uint32_t aa = (ks / 4) * FCHUNK + (ks % 4) * 32 + (SPLIT && term == 0 ? FCHUNK : 0);
-              const uint32_t bb = (ks / 4) * BCHUNK + (ks % 4) * 32 + (SPLIT && term == 1 ? BCHUNK : 0);
+              const uint32_t aa = (ks / 4) * FCHUNK + (ks % 4) * 32 + (SPLIT && term == 0 ? WIDE * FCHUNK : 0);
+              const uint32_t bb = (ks / 4) * BCHUNK + (ks % 4) * 32 + (SPLIT && term == 1 ? WIDE * BCHUNK : 0);
               mma_f16(d + y * BN, make_smem_desc((y ? a2_s : a1_s) + aa, 16, 1024), make_smem_desc(b + y * TILE + bb, 16, 1024),
                       IDESC_X, term > 0 || ks > 0);
             }
@@ -1186,7 +1221,8 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     if (n > 0 && ok) scores(0);
     for (int it = 0; it < n && ok; ++it) {
       const int s = it % BSTAGES, g = it & 1;
-      if (it + 1 < n) scores(it + 1);  // overwrites P and dS of tile it - 1, whose products are issued
+      // overwrites P and dS of tile it - 1, whose products are issued; a single stage is still in use
+      if (BSTAGES > 1 && it + 1 < n) scores(it + 1);
       ok = ok && warp_wait(&p_full[g], (it >> 1) & 1, status, DEV_TIMEOUT_FULL, 0xe02);
       if (!ok) break;
       tc_fence_after();
@@ -1199,17 +1235,18 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
             const uint32_t l = left + (ks / 2) * 32 + (ks % 2) * 8, add = (it > 0 || ks > 0) ? 1u : 0u;
             mma_f16_ts(d, l, make_smem_desc(right + ks * 2048, BCHUNK, 1024), IDESC_ACC, add);
             if (SPLIT) {
-              mma_f16_ts(d + HS, l, make_smem_desc(right + BCHUNK + ks * 2048, BCHUNK, 1024), IDESC_ACC, add);
+              mma_f16_ts(d + HS, l, make_smem_desc(right + WIDE * BCHUNK + ks * 2048, BCHUNK, 1024), IDESC_ACC, add);
               mma_f16_ts(d + HS, l + 16, make_smem_desc(right + ks * 2048, BCHUNK, 1024), IDESC_ACC, 1u);
             }
           }
         };
-        if (KEYS) product(tmem + 2 * FT + (SPLIT ? 2 * HS : HS), a, b + TILE);  // dV += P dO
-        product(tmem + 2 * FT, a + BN, b);                                      // dK += dS Q,  dQ += dS K
+        if (WANT_P) product(tmem + 2 * FT + PV_COL, a, b + TILE);  // dV += P dO
+        if (WANT_D) product(tmem + 2 * FT, a + BN, b);             // dK += dS Q,  dQ += dS K
         tc_commit(smem_u32(&b_empty[s]));
         if (it == n - 1) tc_commit(smem_u32(&acc_full));
       }
       __syncwarp();
+      if (BSTAGES == 1 && it + 1 < n) scores(it + 1);
     }
   } else if (warp >= 4) {
     // ===================== probabilities and their gradient =====================
@@ -1287,7 +1324,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
         const float rx = (flat ? value : 0.f) + PSHIFT - mine.x, ry = -mine.y * f;
         uint32_t x[32], y[32];
         tmem_ld32(x_col, x);
-        tmem_ld32(y_col, y);
+        if (WANT_D) tmem_ld32(y_col, y);
         tmem_ld_wait();
         if (!flat) {  // the window's bias joins the scores here, everything else below
 #pragma unroll
@@ -1299,7 +1336,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
           for (int e = 0; e < 32; ++e)
             if (e < lo || e >= hi) {
               x[e] = 0xff800000u;  // -inf
-              y[e] = 0u;
+              if (WANT_D) y[e] = 0u;
             }
         }
         const float cx1 = flat ? c1 : 1.f;
@@ -1318,28 +1355,27 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
           fma2(F2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), cx, sx).get(p0, p1);
           p0 = ex2(p0);
           p1 = ex2(p1);
-          const F2 ds = mul2(F2(p0, p1), fma2(F2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), f2, sy));
-          float d0, d1;
-          ds.get(d0, d1);
-          if (!KEYS) all = add2(all, ds);
-          if (SPLIT) {
-            if (KEYS) split_pair(p0, p1, pw[e / 2], plow[e / 2]);
-            split_pair(d0, d1, dw[e / 2], dlow[e / 2]);
-          } else {
-            if (KEYS) pw[e / 2] = pack_half2(p0, p1);
-            dw[e / 2] = pack_half2(d0, d1);
+          if (WANT_P) {
+            if (SPLIT) split_pair(p0, p1, pw[e / 2], plow[e / 2]);
+            else pw[e / 2] = pack_half2(p0, p1);
           }
-          if (!KEYS) {
-            y[e] = __float_as_uint(d0);
-            y[e + 1] = __float_as_uint(d1);
+          if (WANT_D) {
+            const F2 ds = mul2(F2(p0, p1), fma2(F2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), f2, sy));
+            float d0, d1;
+            ds.get(d0, d1);
+            if (SPLIT) split_pair(d0, d1, dw[e / 2], dlow[e / 2]);
+            else dw[e / 2] = pack_half2(d0, d1);
+            if (!KEYS) {
+              all = add2(all, ds);
+              y[e] = __float_as_uint(d0);
+              y[e + 1] = __float_as_uint(d1);
+            }
           }
         }
-        if (KEYS) tmem_st16(x_col, pw);
-        tmem_st16(y_col, dw);
-        if (SPLIT) {
-          if (KEYS) tmem_st16(x_col + 16, plow);
-          tmem_st16(y_col + 16, dlow);
-        }
+        if (WANT_P) tmem_st16(x_col, pw);
+        if (WANT_P && SPLIT) tmem_st16(x_col + 16, plow);
+        if (WANT_D) tmem_st16(y_col, dw);
+        if (WANT_D && SPLIT) tmem_st16(y_col + 16, dlow);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(smem_u32(&p_full[g]));
@@ -1407,23 +1443,25 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
         for (int e = gt; e < p.width; e += 256) dist[e] *= 1.f / up;
       }
     }
-    // ---- results: group 0 writes dK, group 1 dV; both share dQ's columns ----
+    // ---- results: of two, group 0 writes dK and group 1 dV; a single one's columns are shared ----
     if (n > 0 && ok) {
       ok = warp_wait(&acc_full, 0, status, DEV_TIMEOUT_ACCUM, 0xf10 + g);
       tc_fence_after();
     }
     using Out = typename std::conditional<SPLIT, float, __half>::type;
-    Out* out = static_cast<Out*>(KEYS ? (g == 0 ? p.dk : p.dv) : p.dq);
+    const bool values = MODE == KEYS_DV || (MODE == KEYS_BOTH && g == 1);  // this thread writes dV
+    Out* out = static_cast<Out*>(KEYS ? (values ? p.dv : p.dk) : p.dq);
     const bool real = row < (KEYS ? p.tk : p.tq);
     if (ok && out != nullptr && (n > 0 || !p.accumulate)) {
-      const long long ld = KEYS ? (g == 0 ? p.lddk : p.lddv) : p.lddq, sh = KEYS ? (g == 0 ? p.shdk : p.shdv) : p.shdq,
-                      sb = KEYS ? (g == 0 ? p.sbdk : p.sbdv) : p.sbdq;
-      const int vec = KEYS ? (g == 0 ? p.vec_dk : p.vec_dv) : p.vec_dq;
+      const long long ld = KEYS ? (values ? p.lddv : p.lddk) : p.lddq, sh = KEYS ? (values ? p.shdv : p.shdk) : p.shdq,
+                      sb = KEYS ? (values ? p.sbdv : p.sbdk) : p.sbdq;
+      const int vec = KEYS ? (values ? p.vec_dv : p.vec_dk) : p.vec_dq;
       out += row * ld + head * sh + batch * sb;
-      float factor = KEYS && g == 1 ? PINV : p.scale / up;
-      if (SPLIT) factor *= KEYS ? (g == 1 ? p.ido[unit] : p.iq[unit]) : p.ik[unit];
-      const uint32_t col0 = lanes + 2 * FT + (KEYS && g == 1 ? (SPLIT ? 2 * HS : HS) : 0);
-      const int c_from = KEYS ? half * (HS / 2) : (2 * g + half) * (HS / 4), c_to = c_from + (KEYS ? HS / 2 : HS / 4);
+      float factor = values ? PINV : p.scale / up;
+      if (SPLIT) factor *= KEYS ? (values ? p.ido[unit] : p.iq[unit]) : p.ik[unit];
+      const uint32_t col0 = lanes + 2 * FT + (values ? PV_COL : 0);
+      constexpr bool SHARED = MODE != KEYS_BOTH;
+      const int c_from = SHARED ? (2 * g + half) * (HS / 4) : half * (HS / 2), c_to = c_from + (SHARED ? HS / 4 : HS / 2);
       for (int c = c_from; c < c_to; c += 8) {
         uint32_t w[8], x[8];
         if (n > 0) {
@@ -1456,14 +1494,17 @@ bool heads_aligned(const FlashOperand& x, long long t, long long heads, long lon
   return true;
 }
 
+// Width of the kernels' operand tiles.
+int flash_width(int hs) { return hs <= 64 ? 64 : 128; }
 // Tensor map of an operand: Half as it lies, or the planes of a split one (twice the sequences).
 bool encode_operand(CUtensorMap* map, const FlashOperand& x, int hs, int t, int heads, int batch, int rows, bool split) {
-  if (split) return encode_heads_tmap(map, x.planes, 64, t, heads, 2LL * batch, 64, 64LL * t, 64LL * t * heads, rows);
+  const long long w = flash_width(hs);
+  if (split) return encode_heads_tmap(map, x.planes, static_cast<int>(w), t, heads, 2LL * batch, w, w * t, w * t * heads, rows);
   return encode_heads_tmap(map, x.p, hs, t, heads, batch, x.ld, x.head, x.batch, rows);
 }
-// Rows of an fp32 result allow 16-byte accesses.
-int rows16(const FlashOperand& x) {
-  return (reinterpret_cast<uintptr_t>(x.p) & 15u) == 0 && x.ld % 4 == 0 && x.head % 4 == 0 && x.batch % 4 == 0;
+// Rows allow 16-byte accesses (`n` elements).
+int rows16(const FlashOperand& x, int n) {
+  return (reinterpret_cast<uintptr_t>(x.p) & 15u) == 0 && x.ld % n == 0 && x.head % n == 0 && x.batch % n == 0;
 }
 
 bool fill_params(const FlashArgs& a, FlashParams* p) {
@@ -1474,7 +1515,7 @@ bool fill_params(const FlashArgs& a, FlashParams* p) {
       !encode_operand(&p->tmV, a.v, a.hs, a.tk, a.kv_heads, a.batch, FT, split))
     return false;
   p->O = const_cast<void*>(a.o.p);
-  p->vec = rows16(a.o);
+  p->vec = rows16(a.o, split ? 4 : 8);
   p->ldo = a.o.ld; p->sho = a.o.head; p->sbo = a.o.batch;
   p->lse = a.lse;
   p->bias = a.bias;
@@ -1489,35 +1530,36 @@ bool fill_params(const FlashArgs& a, FlashParams* p) {
   return true;
 }
 
-template <int HS, int NST, bool SPLIT>
+template <int HS, int NST, int NQ, bool SPLIT>
 cudaError_t forward_hs(FlashParams& p, cudaStream_t stream, int* status) {
-  const int smem = (2 + 2 * NST) * FCHUNK * (SPLIT ? 2 : HS / 64) + 1024;
+  const int smem = (NQ + 2 * NST) * FCHUNK * (SPLIT ? 2 : 1) * (HS / 64) + 1024;
   static unsigned long long smem_set = 0;  // per template instantiation
-  auto kern = flash_forward_kernel<HS, NST, SPLIT>;
+  auto kern = flash_forward_kernel<HS, NST, NQ, SPLIT>;
   cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern), smem, &smem_set);
   if (e != cudaSuccess) return e;
-  p.qblocks = (p.tq + 2 * FT - 1) / (2 * FT);
+  p.qblocks = (p.tq + NQ * FT - 1) / (NQ * FT);
   const long long grid = static_cast<long long>(p.qblocks) * p.heads * p.batch;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
-  return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(FTHREADS), smem, stream, pdl_enabled(), p, status);
+  return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(128 + 256 * NQ), smem, stream, pdl_enabled(), p, status);
 }
 
-template <int HS, bool KEYS, bool SPLIT>
+template <int HS, int MODE, int BSTAGES, bool SPLIT>
 cudaError_t backward_hs(const FlashBwdParams& p, cudaStream_t stream, int* status) {
-  const int smem = (2 * FCHUNK + BSTAGES * 2 * BCHUNK) * (SPLIT ? 2 : HS / 64) + 1024;
+  const int smem = (2 * FCHUNK + BSTAGES * 2 * BCHUNK) * (SPLIT ? 2 : 1) * (HS / 64) + 1024;
   static unsigned long long smem_set = 0;  // per template instantiation
-  auto kern = flash_backward_kernel<HS, KEYS, SPLIT>;
+  auto kern = flash_backward_kernel<HS, MODE, BSTAGES, SPLIT>;
   cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern), smem, &smem_set);
   if (e != cudaSuccess) return e;
   FlashBwdParams q = p;
-  q.row_tiles = ((KEYS ? p.tk : p.tq) + FT - 1) / FT;
-  const long long grid = static_cast<long long>(q.row_tiles) * (KEYS ? p.kv_heads : p.heads) * p.batch;
+  constexpr bool keys = MODE != QUERIES;
+  q.row_tiles = ((keys ? p.tk : p.tq) + FT - 1) / FT;
+  const long long grid = static_cast<long long>(q.row_tiles) * (keys ? p.kv_heads : p.heads) * p.batch;
   return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(FTHREADS), smem, stream, pdl_enabled(), q, status);
 }
-template <bool KEYS>
+template <int MODE>
 cudaError_t backward_any(const FlashBwdParams& p, bool split, cudaStream_t stream, int* status) {
-  if (split) return backward_hs<64, KEYS, true>(p, stream, status);
-  return p.hs <= 64 ? backward_hs<64, KEYS, false>(p, stream, status) : backward_hs<128, KEYS, false>(p, stream, status);
+  if (split) return backward_hs<64, MODE, 4, true>(p, stream, status);
+  return p.hs <= 64 ? backward_hs<64, MODE, 4, false>(p, stream, status) : backward_hs<128, MODE, 4, false>(p, stream, status);
 }
 
 cudaError_t prepare(const FlashArgs& a, const FlashGradArgs& g, const FlashBwdParams& p, float* stats, float* norms, int qparts,
@@ -1533,29 +1575,52 @@ cudaError_t prepare(const FlashArgs& a, const FlashGradArgs& g, const FlashBwdPa
 
 }  // namespace
 
+// Sizes the Half kernels take, wherever the operands lie.
+bool flash_fits(const FlashArgs& a) {
+  const auto fits = [](long long parts, long long heads, long long batch) { return parts * heads * batch <= 0x3fffffffLL; };
+  return tmap_encoder_available() && a.hs <= 128 && fits((a.tq + 127) / 128 * 2, a.heads, a.batch) &&
+         fits((a.tk + 63) / 64, a.kv_heads, a.batch);
+}
+
 bool flash_supported(const FlashArgs& a) {
-  return tmap_encoder_available() && a.hs % 8 == 0 && a.hs >= 8 && a.hs <= 128 && heads_aligned(a.q, a.tq, a.heads, a.batch) &&
+  return flash_fits(a) && a.hs % 8 == 0 && heads_aligned(a.q, a.tq, a.heads, a.batch) &&
          heads_aligned(a.k, a.tk, a.kv_heads, a.batch) && heads_aligned(a.v, a.tk, a.kv_heads, a.batch) &&
-         heads_aligned(a.o, a.tq, a.heads, a.batch) &&
-         static_cast<long long>((a.tq + 2 * FT - 1) / (2 * FT)) * a.heads * a.batch <= 0x7fffffffLL;
+         heads_aligned(a.o, a.tq, a.heads, a.batch);
 }
 
 cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* status) {
   FlashParams p;
   if (!fill_params(a, &p)) return cudaErrorInvalidValue;
-  if (a.inverse != nullptr) return forward_hs<64, 2, true>(p, stream, status);
-  return a.hs <= 64 ? forward_hs<64, 3, false>(p, stream, status) : forward_hs<128, 2, false>(p, stream, status);
+  if (a.inverse != nullptr)
+    return a.hs <= 64 ? forward_hs<64, 2, 2, true>(p, stream, status) : forward_hs<128, 1, 1, true>(p, stream, status);
+  return a.hs <= 64 ? forward_hs<64, 3, 2, false>(p, stream, status) : forward_hs<128, 2, 2, false>(p, stream, status);
 }
 
-// fp32 through Half planes: head size up to 64 (two planes take the shared memory of a 128-wide Half
-// operand) and contractions of at most 2048: an accumulator is added to once per 16 of them, and the
-// tensor core truncates each time, about 2^-25 of the running sum.
+long long flash_packed(int hs, long long t, long long heads, long long batch) {
+  return (flash_width(hs) * t * heads * batch + 1) / 2;
+}
+
+cudaError_t launch_flash_pack(FlashOperand* x, int hs, int t, int heads, int batch, float* to, int num_sms, cudaStream_t stream) {
+  const long long rows = static_cast<long long>(t) * heads * batch, want = (rows + 7) / 8, most = 16LL * num_sms;
+  const long long w = flash_width(hs);
+  const cudaError_t e = launch_kernel(w == 64 ? flash_pack_kernel<64> : flash_pack_kernel<128>,
+                                      dim3(static_cast<unsigned>(want < most ? want : most)), dim3(256), 0, stream, pdl_enabled(),
+                                      static_cast<const __half*>(x->p), x->ld, x->head, x->batch, hs, t, heads, rows,
+                                      reinterpret_cast<__half*>(to));
+  x->p = to;
+  x->ld = w; x->head = w * t; x->batch = w * t * heads;
+  return e;
+}
+
+// fp32 through Half planes: contractions of at most 2048, since an accumulator is added to once per 16
+// of them and the tensor core truncates each time, about 2^-25 of the running sum (measured: 3e-7 of the
+// result at 256, 2e-6 at 2048; longer ones run on the composed path, whose products cut the chain).
 bool flash_split_supported(const FlashArgs& a, bool backward) {
   const long long group = a.heads / a.kv_heads, parts = (a.tq + 63) / 64 + (a.tk + 63) / 64;
-  return tmap_encoder_available() && a.hs <= 64 && a.tk <= 2048 && (!backward || group * a.tq <= 2048) &&
+  return tmap_encoder_available() && a.hs <= 128 && a.tk <= 2048 && (!backward || group * a.tq <= 2048) &&
          parts * a.heads * a.batch <= 0x1fffffffLL;
 }
-long long flash_planes(long long t, long long heads, long long batch) { return 64 * t * heads * batch; }
+long long flash_planes(int hs, long long t, long long heads, long long batch) { return flash_width(hs) * t * heads * batch; }
 
 cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, float* stats, float* norms, cudaStream_t stream) {
   SplitParams p;
@@ -1570,7 +1635,7 @@ cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, flo
     p.norms = reinterpret_cast<unsigned*>(norms);
     p.o = static_cast<const float*>(a->o.p);
     p.ldo = a->o.ld; p.sho = a->o.head; p.sbo = a->o.batch;
-    p.vec_o = rows16(a->o);
+    p.vec_o = rows16(a->o, 4);
     p.lse = a->lse;
     p.stats = reinterpret_cast<float2*>(stats);
     p.tq_pad = (a->tq + FT - 1) / FT * FT;
@@ -1588,16 +1653,18 @@ cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, flo
     o.t = query ? a->tq : a->tk;
     o.heads = query ? a->heads : a->kv_heads;
     o.per = query ? a->heads / a->kv_heads : 1;
-    o.vec = rows16(*ops[i]);
+    o.vec = rows16(*ops[i], 4);
     o.block0 = blocks;
     blocks += static_cast<long long>((o.t + kSplitRows - 1) / kSplitRows) * o.heads * a->batch;
   }
   cudaError_t e = cudaMemsetAsync(p.most, 0, sizeof(unsigned) * 4 * units, stream);
   if (e == cudaSuccess && d_o != nullptr) e = cudaMemsetAsync(norms, 0, sizeof(unsigned) * 2 * units, stream);
   if (e != cudaSuccess) return e;
-  e = launch_kernel(split_most_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, pdl_enabled(), p);
+  const bool narrow = a->hs <= 64;
+  e = launch_kernel(narrow ? split_most_kernel<64> : split_most_kernel<128>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
+                    pdl_enabled(), p);
   if (e != cudaSuccess) return e;
-  return launch_kernel(split_planes_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, pdl_enabled(), p);
+  return launch_kernel(narrow ? split_planes_kernel<64> : split_planes_kernel<128>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, pdl_enabled(), p);
 }
 int flash_token_splits(const FlashArgs& a, int num_sms, long long* floats) {
   const int rows = a.heads / a.kv_heads * a.tq;
@@ -1658,12 +1725,7 @@ cudaError_t launch_flash_token(const FlashArgs& a, int splits, float* scratch, i
 }
 
 bool flash_backward_supported(const FlashArgs& a, const FlashGradArgs& g) {
-  const auto fits = [](long long parts, long long heads, long long batch) { return parts * heads * batch <= 0x3fffffffLL; };
-  return flash_supported(a) && heads_aligned(g.d_o, a.tq, a.heads, a.batch) &&
-         (g.dq.p == nullptr || heads_aligned(g.dq, a.tq, a.heads, a.batch)) &&
-         (g.dk.p == nullptr || heads_aligned(g.dk, a.tk, a.kv_heads, a.batch)) &&
-         (g.dv.p == nullptr || heads_aligned(g.dv, a.tk, a.kv_heads, a.batch)) &&
-         fits((a.tq + 127) / 128 * 2, a.heads, a.batch) && fits((a.tk + 63) / 64, a.kv_heads, a.batch);
+  return flash_supported(a) && heads_aligned(g.d_o, a.tq, a.heads, a.batch);
 }
 
 FlashScratch flash_backward_scratch(const FlashArgs& a, bool table) {
@@ -1693,7 +1755,8 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
     if (!encode_operand(m.map, *m.x, a.hs, m.t, m.heads, a.batch, m.rows, split)) return cudaErrorInvalidValue;
   const long long units = static_cast<long long>(a.batch) * a.kv_heads;
   p.iq = a.inverse; p.ik = a.inverse + units; p.iv = a.inverse + 2 * units; p.ido = a.inverse + 3 * units;
-  p.vec_dq = rows16(g.dq); p.vec_dk = rows16(g.dk); p.vec_dv = rows16(g.dv);
+  const int per16 = split ? 4 : 8;
+  p.vec_dq = rows16(g.dq, per16); p.vec_dk = rows16(g.dk, per16); p.vec_dv = rows16(g.dv, per16);
   p.dq = const_cast<void*>(g.dq.p);
   p.dk = const_cast<void*>(g.dk.p);
   p.dv = const_cast<void*>(g.dv.p);
@@ -1723,13 +1786,24 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
     *launches = 1;
     if (e != cudaSuccess) return e;
   }
-  if (p.dk != nullptr || p.dv != nullptr) {
-    e = backward_any<true>(p, split, stream, status);
+  const bool wide = split && a.hs > 64;
+  if (!wide && (p.dk != nullptr || p.dv != nullptr)) {
+    e = backward_any<KEYS_BOTH>(p, split, stream, status);
+    ++*launches;
+    if (e != cudaSuccess) return e;
+  }
+  if (wide && p.dk != nullptr) {
+    e = backward_hs<128, KEYS_DK, 1, true>(p, stream, status);
+    ++*launches;
+    if (e != cudaSuccess) return e;
+  }
+  if (wide && p.dv != nullptr) {
+    e = backward_hs<128, KEYS_DV, 1, true>(p, stream, status);
     ++*launches;
     if (e != cudaSuccess) return e;
   }
   if (p.dq != nullptr || dist != nullptr) {
-    e = backward_any<false>(p, split, stream, status);
+    e = wide ? backward_hs<128, QUERIES, 1, true>(p, stream, status) : backward_any<QUERIES>(p, split, stream, status);
     ++*launches;
     if (e != cudaSuccess) return e;
   }

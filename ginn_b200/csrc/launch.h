@@ -242,14 +242,19 @@ struct FlashArgs {
   float scale;
   int causal;
 };
-// True when the operands can be described by tensor maps: fp16, head size a multiple of 8 up to
-// 128, 16-byte aligned bases and strides.
+// Head size up to 128 (and no more CTAs than a grid holds).
+bool flash_fits(const FlashArgs& a);
+// True when the Half operands can be described by tensor maps where they are: head size a multiple of
+// 8, 16-byte aligned bases and strides.  Others go through dense copies (flash_packed floats each).
 bool flash_supported(const FlashArgs& a);
+long long flash_packed(int hs, long long t, long long heads, long long batch);
+cudaError_t launch_flash_pack(FlashOperand* x, int hs, int t, int heads, int batch, float* to,
+                              int num_sms, cudaStream_t stream);
 cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* status);
 // fp32 operands of the same kernels: split into two Half planes each, two kernels.  `work`:
 // 8 * batch * kv heads floats; d_o null: forward only, else also the backward pass's stats and norms.
 bool flash_split_supported(const FlashArgs& a, bool backward);
-long long flash_planes(long long t, long long heads, long long batch);
+long long flash_planes(int hs, long long t, long long heads, long long batch);
 cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, float* stats,
                                float* norms, cudaStream_t stream);
 // Few queries against a long cache (at most 16 rows share a key head): number of parts the keys are
