@@ -2155,8 +2155,6 @@ int flash_pack(Scratch* scratch, DevCtx* ctx, gb::FlashArgs* f, gb::FlashOperand
   g_launches.fetch_add(d_o ? 5 : 3);
   return GINN_B200_OK;
 }
-// Few queries go through other kernels.
-bool token_rows(const ginn_b200_relative_attention& a) { return a.heads / a.kv_heads * a.tq <= 16; }
 // Bias of every distance and head, times log2(e), for the flash kernels.
 int flash_bias(Scratch* scratch, int dtype, const ginn_b200_relative_attention& a, gb::FlashArgs* f) {
   if (!a.table) return GINN_B200_OK;
@@ -2184,36 +2182,31 @@ int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, c
     return GINN_B200_OK;
   }
   gb::FlashArgs f = flash_args(*a);
-  if (dtype == GINN_B200_F16 && t_force_path == PATH_AUTO && gb::flash_fits(f)) {
-    Scratch scratch(stream);
-    if (!gb::flash_supported(f))
-      if (int s = flash_pack(&scratch, ctx, &f, nullptr)) return s;
-    long long floats = 0;
-    const int splits = gb::flash_token_splits(f, ctx->num_sms, &floats);
-    if (a->table || floats > 0) CU_TRY(scratch.reserve({bias_floats(*a), floats}));
-    if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
-    int launches = 1;
-    if (splits > 0) {
-      float* parts = nullptr;
-      if (floats > 0) CU_TRY(scratch.take(&parts, floats));
-      CU_TRY(gb::launch_flash_token(f, splits, parts, &launches, stream));
-    } else {
-      CU_TRY(gb::launch_flash_forward(f, stream, ctx->d_status));
-    }
-    g_launches.fetch_add(launches);
-    return GINN_B200_OK;
-  }
-  if (dtype == GINN_B200_F32 && t_force_path == PATH_AUTO && !token_rows(*a) && gb::flash_split_supported(f, false)) {
-    Scratch scratch(stream);
-    const long long keys = gb::flash_planes(f.hs, f.tk, f.kv_heads, f.batch);
-    CU_TRY(scratch.reserve({split_work(f), gb::flash_planes(f.hs, f.tq, f.heads, f.batch), keys, keys, bias_floats(*a)}));
-    if (int s = flash_split(&scratch, &f, nullptr, nullptr, nullptr)) return s;
-    if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
+  const bool half = dtype == GINN_B200_F16;
+  long long floats = 0;
+  const int splits = t_force_path == PATH_AUTO ? gb::flash_token_splits(f, ctx->num_sms, &floats) : 0;
+  if (t_force_path != PATH_AUTO || !(splits > 0 || (half ? gb::flash_fits(f) : gb::flash_split_supported(f, false))))
+    return relative_composed(device, stream, dtype, *a, nullptr);
+  Scratch scratch(stream);
+  if (half && !gb::flash_supported(f))
+    if (int s = flash_pack(&scratch, ctx, &f, nullptr)) return s;
+  const bool split = !half && splits == 0;
+  const long long queries = split ? gb::flash_planes(f.hs, f.tq, f.heads, f.batch) : 0, keys = split ? gb::flash_planes(f.hs, f.tk, f.kv_heads, f.batch) : 0;
+  if (a->table || floats > 0 || split)
+    CU_TRY(scratch.reserve({bias_floats(*a), floats, split ? split_work(f) : 0, queries, keys, keys}));
+  if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
+  int launches = 1;
+  if (splits > 0) {
+    float* parts = nullptr;
+    if (floats > 0) CU_TRY(scratch.take(&parts, floats));
+    CU_TRY(gb::launch_flash_token(dtype, f, splits, parts, &launches, stream));
+  } else {
+    if (split)
+      if (int s = flash_split(&scratch, &f, nullptr, nullptr, nullptr)) return s;
     CU_TRY(gb::launch_flash_forward(f, stream, ctx->d_status));
-    g_launches.fetch_add(1);
-    return GINN_B200_OK;
   }
-  return relative_composed(device, stream, dtype, *a, nullptr);
+  g_launches.fetch_add(launches);
+  return GINN_B200_OK;
 }
 
 int ginn_b200_relative_attention_backward(int device, void* stream_, int dtype, const ginn_b200_relative_attention* a,

@@ -661,15 +661,16 @@ constexpr int kTokenRows = 16;
 constexpr int kTokenWarps = 4;  // two CTAs on an SM: one loads while the other starts or joins its warps
 
 struct TokenParams {
-  const __half *q, *k, *v;
+  const void *q, *k, *v;
   long long ldq, shq, sbq, ldk, shk, sbk, ldv, shv, sbv;
-  __half* o;
+  void* o;
   long long ldo, sho, sbo;
   float* lse;
   float* part;    // [batch][kv][split][row][HS] results, then their (maximum, sum) pairs
   float2* stat;   // [batch][kv][split][row]
   const float* bias;
   int tq, tk, hs, heads, kv_heads, group, batch, rows, splits, chunk;
+  int vec_q, vec_k, vec_v;  // fp32: rows allow 16-byte accesses
   long long reach, q_offset;
   const int* q_offsets;
   const int* q_lengths;
@@ -694,113 +695,68 @@ __device__ __forceinline__ uint4 load_stream(const __half* p) {
 }
 
 // Final values of one row: o and lse.
+template <typename T>
 __device__ __forceinline__ void token_store(const TokenParams& p, int batch, int kv, int row, int h, float value, float m, float l) {
   const int head = kv * p.group + row / p.tq, i = row % p.tq;
-  if (h < p.hs) p.o[h + i * p.ldo + head * p.sho + batch * p.sbo] = __float2half_rn(l > 0.f ? value / l : 0.f);
+  if (h < p.hs) static_cast<T*>(p.o)[h + i * p.ldo + head * p.sho + batch * p.sbo] = from_f<T>(l > 0.f ? value / l : 0.f);
   if (h == 0)
     p.lse[(static_cast<long long>(batch) * p.heads + head) * p.tq + i] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
 }
 
-template <int HS>
-__global__ void __launch_bounds__(32 * kTokenWarps, 2)
-flash_token_kernel(const TokenParams p) {
-  extern __shared__ float res[];  // [warp][row][HS + 4]
-  __shared__ float mx[kTokenWarps][kTokenRows], sm[kTokenWarps][kTokenRows];
-  pdl_wait();
-  pdl_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int split = static_cast<int>(blockIdx.x) % p.splits;
-  const long long unit = blockIdx.x / p.splits;
-  const int batch = static_cast<int>(unit / p.kv_heads), kv = static_cast<int>(unit % p.kv_heads);
-  const int klen = rel_length(p.k_lengths, batch, p.tk), qlen = rel_length(p.q_lengths, batch, p.tq);
-  const long long off = rel_offset(p.q_offset, p.q_offsets, batch);
-  // this lane's two rows of the scores: g and g + 8
+// What a lane knows of its two rows of the scores, g and g + 8, and of its CTA's keys.
+struct TokenLane {
+  int warp, lane, g, c, split, batch, kv, begin, end;
+  long long unit, first_pos;
   int vis[2];
   long long pos[2];
-  const float* bias[2] = {nullptr, nullptr};
-  const __half* qrow[2];
-  float far_lo[2] = {0.f, 0.f};
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int row = g + 8 * x, i = row % p.tq, head = kv * p.group + row / p.tq;
-    const bool real = row < p.rows;
-    pos[x] = i + off;
-    vis[x] = real && i < qlen ? rel_visible(p.causal, pos[x], klen) : 0;
-    qrow[x] = real ? p.q + i * p.ldq + head * p.shq + batch * p.sbq : nullptr;
-    if (p.bias != nullptr && real) {
-      bias[x] = p.bias + head * (2 * p.reach + 1) + p.reach;
-      far_lo[x] = bias[x][-p.reach];
-    }
-  }
-  const int last = qlen > 0 ? rel_visible(p.causal, qlen - 1 + off, klen) : 0;  // the most any row sees
-  const long long first_pos = off;
-  const int begin = split * p.chunk, end = begin + p.chunk < last ? begin + p.chunk : last;
-  if (begin >= end && p.splits > 1) {  // nothing here: the join passes it over
-    if (threadIdx.x < p.rows) p.stat[(unit * p.splits + split) * p.rows + threadIdx.x] = make_float2(-INFINITY, 0.f);
-    return;
-  }
-
-  uint32_t q[HS / 32][2][4];
-#pragma unroll
-  for (int s = 0; s < HS / 32; ++s)
+  const float* bias[2];
+  float far_lo[2];
+  float m[2], l[2];
+  __device__ __forceinline__ explicit TokenLane(const TokenParams& p) {
+    warp = threadIdx.x >> 5;
+    lane = threadIdx.x & 31;
+    g = lane >> 2;
+    c = lane & 3;
+    split = static_cast<int>(blockIdx.x) % p.splits;
+    unit = blockIdx.x / p.splits;
+    batch = static_cast<int>(unit / p.kv_heads);
+    kv = static_cast<int>(unit % p.kv_heads);
+    const int klen = rel_length(p.k_lengths, batch, p.tk), qlen = rel_length(p.q_lengths, batch, p.tq);
+    first_pos = rel_offset(p.q_offset, p.q_offsets, batch);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (qrow[x] != nullptr && 32 * s + 8 * c < p.hs) w = *reinterpret_cast<const uint4*>(qrow[x] + 32 * s + 8 * c);
-      q[s][x][0] = w.x; q[s][x][1] = w.y; q[s][x][2] = w.z; q[s][x][3] = w.w;
+      const int row = g + 8 * x, i = row % p.tq, head = kv * p.group + row / p.tq;
+      const bool real = row < p.rows;
+      pos[x] = i + first_pos;
+      vis[x] = real && i < qlen ? rel_visible(p.causal, pos[x], klen) : 0;
+      bias[x] = nullptr;
+      far_lo[x] = 0.f;
+      if (p.bias != nullptr && real) {
+        bias[x] = p.bias + head * (2 * p.reach + 1) + p.reach;
+        far_lo[x] = bias[x][-p.reach];
+      }
+      m[x] = -INFINITY;
+      l[x] = 0.f;
     }
-  float acc[HS / 8][4];
-#pragma unroll
-  for (int e = 0; e < HS / 8; ++e) acc[e][0] = acc[e][1] = acc[e][2] = acc[e][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
-  const __half* kp = p.k + kv * p.shk + batch * p.sbk;
-  const __half* vp = p.v + kv * p.shv + batch * p.sbv;
-  uint4 kr[2][HS / 32], vr[HS / 64][4];
-  auto load_k = [&](int j) {  // keys j + g and j + 8 + g, head elements 32 s + 8 c ..
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int s = 0; s < HS / 32; ++s) {
-        const int key = j + 8 * t + g;
-        kr[t][s] = make_uint4(0, 0, 0, 0);
-        if (key < end && 32 * s + 8 * c < p.hs) kr[t][s] = load_stream(kp + key * p.ldk + 32 * s + 8 * c);
-      }
-  };
-  auto load_v = [&](int j) {  // keys j + 2 c + {0, 1, 8, 9}, head elements 64 s + 8 g ..
-#pragma unroll
-    for (int s = 0; s < HS / 64; ++s)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int key = j + 2 * c + (t & 1) + 8 * (t >> 1);
-        vr[s][t] = make_uint4(0, 0, 0, 0);
-        if (key < end && 64 * s + 8 * g < p.hs) vr[s][t] = load_stream(vp + key * p.ldv + 64 * s + 8 * g);
-      }
-  };
-  int j = begin + 16 * warp;
-  if (j < end) {
-    load_k(j);
-    load_v(j);
+    const int last = qlen > 0 ? rel_visible(p.causal, qlen - 1 + first_pos, klen) : 0;  // the most any row sees
+    begin = split * p.chunk;
+    end = begin + p.chunk < last ? begin + p.chunk : last;
   }
-  for (; j < end; j += 16 * kTokenWarps) {
-    float sc[2][4];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
-#pragma unroll
-      for (int s = 0; s < HS / 32; ++s) {
-        mma_16816(sc[t], q[s][0][0], q[s][1][0], q[s][0][1], q[s][1][1], kr[t][s].x, kr[t][s].y);
-        mma_16816(sc[t], q[s][0][2], q[s][1][2], q[s][0][3], q[s][1][3], kr[t][s].z, kr[t][s].w);
-      }
-    }
-    const int next = j + 16 * kTokenWarps;
-    if (next < end) load_k(next);
-    // scores of row g + 8 x at keys j + 8 t + 2 c + y: sc[t][2 x + y]
-    const bool flat = p.bias == nullptr || j + 15 - first_pos <= -p.reach;  // for every row: positions only grow
-    const bool full = j + 16 <= vis[0] && j + 16 <= vis[1];
+  // A CTA without keys leaves what the join passes over.
+  __device__ __forceinline__ bool nothing(const TokenParams& p) const {
+    if (begin < end || p.splits == 1) return false;
+    if (threadIdx.x < p.rows) p.stat[(unit * p.splits + split) * p.rows + threadIdx.x] = make_float2(-INFINITY, 0.f);
+    return true;
+  }
+  // Raw scores of keys j .. j + 8 M - 1 (row g + 8 x at key j + 8 t + 2 c + y: sc[t][2 x + y]) become
+  // probabilities; when a row's maximum grew, the result so far is rescaled.
+  template <int N, int M>
+  __device__ __forceinline__ void softmax(const TokenParams& p, int j, float (&sc)[M][4], float (&acc)[N][4]) {
+    const bool flat = p.bias == nullptr || j + 8 * M - 1 - first_pos <= -p.reach;  // for every row: positions only grow
+    const bool full = j + 8 * M <= vis[0] && j + 8 * M <= vis[1];
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < M; ++t)
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -834,23 +790,130 @@ flash_token_kernel(const TokenParams p) {
         l[x] *= a[x];
       }
 #pragma unroll
-      for (int e = 0; e < HS / 8; ++e) {
+      for (int e = 0; e < N; ++e) {
         acc[e][0] *= a[0];
         acc[e][1] *= a[0];
         acc[e][2] *= a[1];
         acc[e][3] *= a[1];
       }
     }
+#pragma unroll
+    for (int t = 0; t < M; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float mu = m[x] == -INFINITY ? 0.f : m[x];
+        sc[t][2 * x] = ex2(sc[t][2 * x] - mu);
+        sc[t][2 * x + 1] = ex2(sc[t][2 * x + 1] - mu);
+        l[x] += sc[t][2 * x] + sc[t][2 * x + 1];
+      }
+  }
+  // The warps' results together: res holds [warp][row][HS + 4] once every warp has written its own.
+  template <int HS, typename T>
+  __device__ __forceinline__ void join(const TokenParams& p, const float* res, float (*mx)[kTokenRows], float (*sm)[kTokenRows]) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+      if (c == 0) {
+        mx[warp][g + 8 * x] = m[x];
+        sm[warp][g + 8 * x] = l[x];
+      }
+    }
+    __syncthreads();
+    for (int at = threadIdx.x; at < p.rows * HS; at += 32 * kTokenWarps) {
+      const int row = at / HS, h = at % HS;
+      float all = -INFINITY, sum = 0.f, value = 0.f;
+#pragma unroll
+      for (int w = 0; w < kTokenWarps; ++w) all = fmaxf(all, mx[w][row]);
+#pragma unroll
+      for (int w = 0; w < kTokenWarps; ++w) {
+        const float a = mx[w][row] == -INFINITY ? 0.f : ex2(mx[w][row] - all);
+        sum += sm[w][row] * a;
+        value += res[(w * p.rows + row) * (HS + 4) + h] * a;
+      }
+      if (p.splits == 1) {
+        token_store<T>(p, batch, kv, row, h, value, all, sum);
+      } else {
+        const long long to = (unit * p.splits + split) * p.rows + row;
+        p.part[to * HS + h] = value;
+        if (h == 0) p.stat[to] = make_float2(all, sum);
+      }
+    }
+  }
+};
+
+template <int HS>
+__global__ void __launch_bounds__(32 * kTokenWarps, 2)
+flash_token_kernel(const TokenParams p) {
+  extern __shared__ float res[];  // [warp][row][HS + 4]
+  __shared__ float mx[kTokenWarps][kTokenRows], sm[kTokenWarps][kTokenRows];
+  pdl_wait();
+  pdl_launch_dependents();
+  TokenLane w(p);
+  if (w.nothing(p)) return;
+  const int g = w.g, c = w.c, end = w.end;
+  uint32_t q[HS / 32][2][4];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int row = g + 8 * x;
+    const __half* from = static_cast<const __half*>(p.q) + row % p.tq * p.ldq + (w.kv * p.group + row / p.tq) * p.shq + w.batch * p.sbq;
+#pragma unroll
+    for (int s = 0; s < HS / 32; ++s) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (row < p.rows && 32 * s + 8 * c < p.hs) v = *reinterpret_cast<const uint4*>(from + 32 * s + 8 * c);
+      q[s][x][0] = v.x; q[s][x][1] = v.y; q[s][x][2] = v.z; q[s][x][3] = v.w;
+    }
+  }
+  float acc[HS / 8][4];
+#pragma unroll
+  for (int e = 0; e < HS / 8; ++e) acc[e][0] = acc[e][1] = acc[e][2] = acc[e][3] = 0.f;
+  const __half* kp = static_cast<const __half*>(p.k) + w.kv * p.shk + w.batch * p.sbk;
+  const __half* vp = static_cast<const __half*>(p.v) + w.kv * p.shv + w.batch * p.sbv;
+  uint4 kr[2][HS / 32], vr[HS / 64][4];
+  auto load_k = [&](int j) {  // keys j + g and j + 8 + g, head elements 32 s + 8 c ..
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int s = 0; s < HS / 32; ++s) {
+        const int key = j + 8 * t + g;
+        kr[t][s] = make_uint4(0, 0, 0, 0);
+        if (key < end && 32 * s + 8 * c < p.hs) kr[t][s] = load_stream(kp + key * p.ldk + 32 * s + 8 * c);
+      }
+  };
+  auto load_v = [&](int j) {  // keys j + 2 c + {0, 1, 8, 9}, head elements 64 s + 8 g ..
+#pragma unroll
+    for (int s = 0; s < HS / 64; ++s)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int key = j + 2 * c + (t & 1) + 8 * (t >> 1);
+        vr[s][t] = make_uint4(0, 0, 0, 0);
+        if (key < end && 64 * s + 8 * g < p.hs) vr[s][t] = load_stream(vp + key * p.ldv + 64 * s + 8 * g);
+      }
+  };
+  int j = w.begin + 16 * w.warp;
+  if (j < end) {
+    load_k(j);
+    load_v(j);
+  }
+  for (; j < end; j += 16 * kTokenWarps) {
+    float sc[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+#pragma unroll
+      for (int s = 0; s < HS / 32; ++s) {
+        mma_16816(sc[t], q[s][0][0], q[s][1][0], q[s][0][1], q[s][1][1], kr[t][s].x, kr[t][s].y);
+        mma_16816(sc[t], q[s][0][2], q[s][1][2], q[s][0][3], q[s][1][3], kr[t][s].z, kr[t][s].w);
+      }
+    }
+    const int next = j + 16 * kTokenWarps;
+    if (next < end) load_k(next);
+    w.softmax(p, j, sc, acc);
     uint32_t pr[2][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float mu = m[x] == -INFINITY ? 0.f : m[x];
-        const float p0 = ex2(sc[t][2 * x] - mu), p1 = ex2(sc[t][2 * x + 1] - mu);
-        l[x] += p0 + p1;
-        pr[t][x] = pack_half2(p0, p1);
-      }
+      for (int x = 0; x < 2; ++x) pr[t][x] = pack_half2(sc[t][2 * x], sc[t][2 * x + 1]);
 #pragma unroll
     for (int s = 0; s < HS / 64; ++s) {
       const uint32_t v0[4] = {vr[s][0].x, vr[s][0].y, vr[s][0].z, vr[s][0].w}, v1[4] = {vr[s][1].x, vr[s][1].y, vr[s][1].z, vr[s][1].w};
@@ -864,54 +927,167 @@ flash_token_kernel(const TokenParams p) {
     }
     if (next < end) load_v(next);
   }
-  // ---- the warps' results together ----
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
     const int row = g + 8 * x;
-    if (c == 0) {
-      mx[warp][row] = m[x];
-      sm[warp][row] = l[x];
-    }
-    if (row < p.rows) {
-      // element k of a fragment: row g + 8 (k / 2), column n = 2 c + k % 2, head element 64 s + 8 n + e
-      float* to = res + (warp * p.rows + row) * (HS + 4);
+    if (row >= p.rows) continue;
+    // element k of a fragment: row g + 8 (k / 2), column n = 2 c + k % 2, head element 64 s + 8 n + e
+    float* to = res + (w.warp * p.rows + row) * (HS + 4);
 #pragma unroll
-      for (int s = 0; s < HS / 64; ++s)
+    for (int s = 0; s < HS / 64; ++s)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int e = 0; e < 8; e += 4)
-            *reinterpret_cast<float4*>(to + 64 * s + 8 * (2 * c + k) + e) =
-                make_float4(acc[8 * s + e][2 * x + k], acc[8 * s + e + 1][2 * x + k], acc[8 * s + e + 2][2 * x + k],
-                            acc[8 * s + e + 3][2 * x + k]);
-    }
+        for (int e = 0; e < 8; e += 4)
+          *reinterpret_cast<float4*>(to + 64 * s + 8 * (2 * c + k) + e) =
+              make_float4(acc[8 * s + e][2 * x + k], acc[8 * s + e + 1][2 * x + k], acc[8 * s + e + 2][2 * x + k],
+                          acc[8 * s + e + 3][2 * x + k]);
+  }
+  w.join<HS, __half>(p, res, mx, sm);
+}
+
+// fp32: three TF32 products per term on mma.m16n8k8, values split as they arrive (high: rounded to the
+// upper 11 bits of the mantissa, low: the exact rest; what is not a number stays so through the rest).  A lane's four consecutive head elements of a key are its shares
+// of two fragments, its four of a value those of four; the queries' two parts lie in shared memory.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void mma_1688(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int HS>
+__global__ void __launch_bounds__(32 * kTokenWarps, 2)
+flash_token32_kernel(const TokenParams p) {
+  constexpr int M = HS > 64 ? 1 : 2, KEYS = 8 * M;  // keys per block: as many as the registers hold twice
+  extern __shared__ float res[];  // [warp][row][HS + 4], then the queries: [part][row 16][HS + 4]
+  __shared__ float mx[kTokenWarps][kTokenRows], sm[kTokenWarps][kTokenRows];
+  constexpr int PITCH = HS + 4;
+  float* qs = res + kTokenWarps * p.rows * PITCH;
+  pdl_wait();
+  pdl_launch_dependents();
+  TokenLane w(p);
+  if (w.nothing(p)) return;
+  const int g = w.g, c = w.c, end = w.end;
+  for (int at = threadIdx.x; at < kTokenRows * HS; at += 32 * kTokenWarps) {
+    const int row = at / HS, h = at % HS;
+    float v = 0.f;
+    if (row < p.rows && h < p.hs)
+      v = static_cast<const float*>(p.q)[h + row % p.tq * p.ldq + (w.kv * p.group + row / p.tq) * p.shq + w.batch * p.sbq];
+    uint32_t hi, lo;
+    split_tf32(v, hi, lo);
+    qs[row * PITCH + h] = __uint_as_float(hi);
+    qs[(kTokenRows + row) * PITCH + h] = __uint_as_float(lo);
   }
   __syncthreads();
-  for (int at = threadIdx.x; at < p.rows * HS; at += 32 * kTokenWarps) {
-    const int row = at / HS, h = at % HS;
-    float all = -INFINITY, sum = 0.f, value = 0.f;
+  float acc[HS / 8][4];
 #pragma unroll
-    for (int w = 0; w < kTokenWarps; ++w) all = fmaxf(all, mx[w][row]);
+  for (int e = 0; e < HS / 8; ++e) acc[e][0] = acc[e][1] = acc[e][2] = acc[e][3] = 0.f;
+  const float* kp = static_cast<const float*>(p.k) + w.kv * p.shk + w.batch * p.sbk;
+  const float* vp = static_cast<const float*>(p.v) + w.kv * p.shv + w.batch * p.sbv;
+  float4 kr[M][HS / 16], vr[HS / 32][2 * M];
+  auto load_k = [&](int j) {  // keys j + 8 t + g, head elements 16 s + 4 c ..
 #pragma unroll
-    for (int w = 0; w < kTokenWarps; ++w) {
-      const float a = mx[w][row] == -INFINITY ? 0.f : ex2(mx[w][row] - all);
-      sum += sm[w][row] * a;
-      value += res[(w * p.rows + row) * (HS + 4) + h] * a;
-    }
-    if (p.splits == 1) {
-      token_store(p, batch, kv, row, h, value, all, sum);
-    } else {
-      const long long to = (unit * p.splits + split) * p.rows + row;
-      p.part[to * HS + h] = value;
-      if (h == 0) p.stat[to] = make_float2(all, sum);
-    }
+    for (int t = 0; t < M; ++t)
+#pragma unroll
+      for (int s = 0; s < HS / 16; ++s) {
+        const int key = j + 8 * t + g, h = 16 * s + 4 * c;
+        kr[t][s] = load_four(kp + key * p.ldk + h, key < end ? p.hs - h : 0, p.vec_k);
+      }
+  };
+  auto load_v = [&](int j) {  // keys j + 8 t + 2 c and the next, head elements 32 s + 4 g ..
+#pragma unroll
+    for (int s = 0; s < HS / 32; ++s)
+#pragma unroll
+      for (int t = 0; t < 2 * M; ++t) {
+        const int key = j + 2 * c + (t & 1) + 8 * (t >> 1), h = 32 * s + 4 * g;
+        vr[s][t] = load_four(vp + key * p.ldv + h, key < end ? p.hs - h : 0, p.vec_v);
+      }
+  };
+  int j = w.begin + KEYS * w.warp;
+  if (j < end) {
+    load_k(j);
+    load_v(j);
   }
+  for (; j < end; j += KEYS * kTokenWarps) {
+    float sc[M][4];
+#pragma unroll
+    for (int t = 0; t < M; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+#pragma unroll
+    for (int s = 0; s < HS / 16; ++s) {
+      float4 q[2][2];  // [part][row g, g + 8]: elements 16 s + 4 c ..
+#pragma unroll
+      for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          q[part][x] = *reinterpret_cast<const float4*>(qs + (part * kTokenRows + g + 8 * x) * PITCH + 16 * s + 4 * c);
+#pragma unroll
+      for (int t = 0; t < M; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {  // contraction indices c and c + 4: head elements 4 c + 2 u and the next
+          uint32_t bh[2], bl[2], a[2][4];
+          split_tf32(u ? kr[t][s].z : kr[t][s].x, bh[0], bl[0]);
+          split_tf32(u ? kr[t][s].w : kr[t][s].y, bh[1], bl[1]);
+#pragma unroll
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              a[part][x] = __float_as_uint(u ? q[part][x].z : q[part][x].x);
+              a[part][2 + x] = __float_as_uint(u ? q[part][x].w : q[part][x].y);
+            }
+          mma_1688(sc[t], a[1][0], a[1][1], a[1][2], a[1][3], bh[0], bh[1]);
+          mma_1688(sc[t], a[0][0], a[0][1], a[0][2], a[0][3], bl[0], bl[1]);
+          mma_1688(sc[t], a[0][0], a[0][1], a[0][2], a[0][3], bh[0], bh[1]);
+        }
+    }
+    const int next = j + KEYS * kTokenWarps;
+    if (next < end) load_k(next);
+    w.softmax(p, j, sc, acc);
+#pragma unroll
+    for (int t = 0; t < M; ++t) {  // keys j + 8 t ..: contraction index c is key 2 c, c + 4 is key 2 c + 1
+      uint32_t ph[4], pl[4];       // rows g, g + 8 at key 2 c, then at 2 c + 1
+      split_tf32(sc[t][0], ph[0], pl[0]);
+      split_tf32(sc[t][2], ph[1], pl[1]);
+      split_tf32(sc[t][1], ph[2], pl[2]);
+      split_tf32(sc[t][3], ph[3], pl[3]);
+#pragma unroll
+      for (int s = 0; s < HS / 32; ++s) {
+        const float4 v0 = vr[s][2 * t], v1 = vr[s][2 * t + 1];
+        const float f0[4] = {v0.x, v0.y, v0.z, v0.w}, f1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // head element 32 s + 4 n + e for column n of the fragment
+          uint32_t bh[2], bl[2];
+          split_tf32(f0[e], bh[0], bl[0]);
+          split_tf32(f1[e], bh[1], bl[1]);
+          mma_1688(acc[4 * s + e], pl[0], pl[1], pl[2], pl[3], bh[0], bh[1]);
+          mma_1688(acc[4 * s + e], ph[0], ph[1], ph[2], ph[3], bl[0], bl[1]);
+          mma_1688(acc[4 * s + e], ph[0], ph[1], ph[2], ph[3], bh[0], bh[1]);
+        }
+      }
+    }
+    if (next < end) load_v(next);
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int row = g + 8 * x;
+    if (row >= p.rows) continue;
+    float* to = res + (w.warp * p.rows + row) * PITCH;
+#pragma unroll
+    for (int s = 0; s < HS / 32; ++s)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)  // column n = 2 c + k
+        *reinterpret_cast<float4*>(to + 32 * s + 4 * (2 * c + k)) =
+            make_float4(acc[4 * s][2 * x + k], acc[4 * s + 1][2 * x + k], acc[4 * s + 2][2 * x + k], acc[4 * s + 3][2 * x + k]);
+  }
+  w.join<HS, float>(p, res, mx, sm);
 }
 
 // The splits' results together, in order: one CTA per row of a (sequence, key head).
-template <int HS>
+template <int HS, typename T>
 __global__ void __launch_bounds__(HS)
 flash_token_join_kernel(const TokenParams p) {
   pdl_wait();
@@ -930,7 +1106,7 @@ flash_token_join_kernel(const TokenParams p) {
     l += st.y * a;
     v += p.part[at * HS + h] * a;
   }
-  token_store(p, batch, kv, row, h, v, m, l);
+  token_store<T>(p, batch, kv, row, h, v, m, l);
 }
 
 // ---- backward -----------------------------------------------------------------------------------
@@ -1612,12 +1788,12 @@ cudaError_t launch_flash_pack(FlashOperand* x, int hs, int t, int heads, int bat
   return e;
 }
 
-// fp32 through Half planes: contractions of at most 2048, since an accumulator is added to once per 16
-// of them and the tensor core truncates each time, about 2^-25 of the running sum (measured: 3e-7 of the
-// result at 256, 2e-6 at 2048; longer ones run on the composed path, whose products cut the chain).
+// fp32 through Half planes: contractions of at most 4096, since an accumulator is added to once per 16
+// of them and the tensor core truncates each time, about 2^-25 of the running sum (measured: 4e-7 of the
+// result at 256, 2.5e-6 at 2048; longer ones run on the composed path, whose products cut the chain).
 bool flash_split_supported(const FlashArgs& a, bool backward) {
   const long long group = a.heads / a.kv_heads, parts = (a.tq + 63) / 64 + (a.tk + 63) / 64;
-  return tmap_encoder_available() && a.hs <= 128 && a.tk <= 2048 && (!backward || group * a.tq <= 2048) &&
+  return tmap_encoder_available() && a.hs <= 128 && a.tk <= 4096 && (!backward || group * a.tq <= 4096) &&
          parts * a.heads * a.batch <= 0x1fffffffLL;
 }
 long long flash_planes(int hs, long long t, long long heads, long long batch) { return flash_width(hs) * t * heads * batch; }
@@ -1667,9 +1843,9 @@ cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, flo
   return launch_kernel(narrow ? split_planes_kernel<64> : split_planes_kernel<128>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, pdl_enabled(), p);
 }
 int flash_token_splits(const FlashArgs& a, int num_sms, long long* floats) {
-  const int rows = a.heads / a.kv_heads * a.tq;
+  const long long rows = static_cast<long long>(a.heads / a.kv_heads) * a.tq;
   *floats = 0;
-  if (rows > kTokenRows) return 0;
+  if (rows > kTokenRows || a.hs > 128) return 0;
   // Eight CTAs' worth of work per SM, so that ragged lengths even out; a CTA takes at least 64 keys (one
   // block per warp) and in multiples of that.
   const long long units = static_cast<long long>(a.kv_heads) * a.batch, step = 16 * kTokenWarps;
@@ -1681,13 +1857,14 @@ int flash_token_splits(const FlashArgs& a, int num_sms, long long* floats) {
   return static_cast<int>(splits);
 }
 
-cudaError_t launch_flash_token(const FlashArgs& a, int splits, float* scratch, int* launches, cudaStream_t stream) {
+cudaError_t launch_flash_token(int dtype, const FlashArgs& a, int splits, float* scratch, int* launches, cudaStream_t stream) {
   TokenParams p;
   std::memset(&p, 0, sizeof(p));
-  p.q = static_cast<const __half*>(a.q.p);
-  p.k = static_cast<const __half*>(a.k.p);
-  p.v = static_cast<const __half*>(a.v.p);
-  p.o = static_cast<__half*>(const_cast<void*>(a.o.p));
+  p.q = a.q.p;
+  p.k = a.k.p;
+  p.v = a.v.p;
+  p.o = const_cast<void*>(a.o.p);
+  p.vec_q = rows16(a.q, 4); p.vec_k = rows16(a.k, 4); p.vec_v = rows16(a.v, 4);
   p.ldq = a.q.ld; p.shq = a.q.head; p.sbq = a.q.batch;
   p.ldk = a.k.ld; p.shk = a.k.head; p.sbk = a.k.batch;
   p.ldv = a.v.ld; p.shv = a.v.head; p.sbv = a.v.batch;
@@ -1711,17 +1888,22 @@ cudaError_t launch_flash_token(const FlashArgs& a, int splits, float* scratch, i
     p.part = scratch + 2 * units * splits * p.rows;
   }
   *launches = 1;
-  auto kern = narrow ? flash_token_kernel<64> : flash_token_kernel<128>;
-  const int width = (narrow ? 64 : 128) + 4, row_bytes = kTokenWarps * width * static_cast<int>(sizeof(float));
-  static unsigned long long smem_set[2] = {0, 0};  // per kernel
-  cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern), kTokenRows * row_bytes, &smem_set[narrow]);
+  const bool half = dtype != 0;
+  auto kern = half ? (narrow ? flash_token_kernel<64> : flash_token_kernel<128>)
+                   : (narrow ? flash_token32_kernel<64> : flash_token32_kernel<128>);
+  const int row_bytes = ((narrow ? 64 : 128) + 4) * static_cast<int>(sizeof(float));
+  const int queries = half ? 0 : 2 * kTokenRows * row_bytes;
+  static unsigned long long smem_set[4] = {};  // per kernel
+  cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern), kTokenRows * kTokenWarps * row_bytes + queries,
+                                      &smem_set[half * 2 + narrow]);
   if (e != cudaSuccess) return e;
-  e = launch_kernel(kern, dim3(static_cast<unsigned>(units * splits)), dim3(32 * kTokenWarps), p.rows * row_bytes, stream,
-                    pdl_enabled(), p);
+  e = launch_kernel(kern, dim3(static_cast<unsigned>(units * splits)), dim3(32 * kTokenWarps), p.rows * kTokenWarps * row_bytes + queries,
+                    stream, pdl_enabled(), p);
   if (e != cudaSuccess || splits == 1) return e;
   *launches = 2;
-  return launch_kernel(narrow ? flash_token_join_kernel<64> : flash_token_join_kernel<128>,
-                       dim3(static_cast<unsigned>(units * p.rows)), dim3(narrow ? 64 : 128), 0, stream, pdl_enabled(), p);
+  auto join = half ? (narrow ? flash_token_join_kernel<64, __half> : flash_token_join_kernel<128, __half>)
+                   : (narrow ? flash_token_join_kernel<64, float> : flash_token_join_kernel<128, float>);
+  return launch_kernel(join, dim3(static_cast<unsigned>(units * p.rows)), dim3(narrow ? 64 : 128), 0, stream, pdl_enabled(), p);
 }
 
 bool flash_backward_supported(const FlashArgs& a, const FlashGradArgs& g) {
