@@ -1137,6 +1137,7 @@ struct FlashBwdParams {
   void *dq, *dk, *dv;
   long long lddq, shdq, sbdq, lddk, shdk, sbdk, lddv, shdv, sbdv;
   const float2* stats;        // [batch][heads][tq_pad]: lse * log2(e) (+inf = empty), delta
+  float2* delta;              // the same, for the launch that corrects delta
   const unsigned* norms;      // [2][batch][kv heads]: bits of max |dO|^2, max |v|^2
   float* dist;                // [batch][heads][query tile][2][width] sums of dS by distance; null = not wanted
   const float* bias;
@@ -1254,12 +1255,20 @@ flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long lon
 
 // MODE: what a launch forms.  128-wide split operands leave room in tensor memory for one result (with its
 // cross terms) beside X and Y, and in shared memory for one stage: dK and dV are then two launches.
-enum FlashMode { KEYS_BOTH = 0, QUERIES = 1, KEYS_DK = 2, KEYS_DV = 3 };
+//
+// DELTA runs before the others and adds sum_j P (Y - delta) to delta, which is what delta is off by.  delta
+// from the stored o carries o's rounding: for Half that is the largest error of a gradient where o is
+// as large as v, in queries that see few keys (two keys: 5.1e-4 of dq instead of 2.9e-4; 500 keys: 3.0e-4);
+// for fp32 it is the truncation of o's long accumulation, which the table's gradient, whose terms all
+// but cancel, shows several times enlarged (1313 keys: 6.6e-6).  So Half tiles that see at most
+// kDeltaHalf keys and fp32 tiles that see more than kDeltaSplit take the two extra products.
+enum FlashMode { KEYS_BOTH = 0, QUERIES = 1, KEYS_DK = 2, KEYS_DV = 3, DELTA = 4 };
+constexpr int kDeltaHalf = 256, kDeltaSplit = 512;
 
 template <int HS, int MODE, int BSTAGES, bool SPLIT>
 __global__ void __launch_bounds__(FTHREADS, 1)
 flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict__ status) {
-  constexpr bool KEYS = MODE != QUERIES;
+  constexpr bool KEYS = MODE != QUERIES && MODE != DELTA;
   constexpr bool WANT_P = MODE == KEYS_BOTH || MODE == KEYS_DV, WANT_D = MODE != KEYS_DV;
   constexpr int WIDE = HS / 64;           // 64-wide chunks of a plane
   constexpr int CHUNKS = (SPLIT ? 2 : 1) * WIDE;
@@ -1276,6 +1285,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
   __shared__ float diag[KEYS ? 1 : 16][64];
   __shared__ float dist_s[KEYS ? 1 : 2][KEYS ? 1 : kDistSmem];
   __shared__ float far_s[2][2][8];
+  __shared__ float delta_s[MODE == DELTA ? 4 : 1][FT];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -1329,6 +1339,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
   } else if (r0 < qlen) {
     const int last = r0 + FT - 1 < qlen - 1 ? r0 + FT - 1 : qlen - 1;
     per = (rel_visible(p.causal, last + off, klen) + BN - 1) / BN;
+    if (MODE == DELTA && (SPLIT ? per <= kDeltaSplit / BN : per > kDeltaHalf / BN)) per = 0;
   }
   const int n = per * (KEYS ? p.group : 1);
 
@@ -1417,7 +1428,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
           }
         };
         if (WANT_P) product(tmem + 2 * FT + PV_COL, a, b + TILE);  // dV += P dO
-        if (WANT_D) product(tmem + 2 * FT, a + BN, b);             // dK += dS Q,  dQ += dS K
+        if (WANT_D && MODE != DELTA) product(tmem + 2 * FT, a + BN, b);  // dK += dS Q,  dQ += dS K
         tc_commit(smem_u32(&b_empty[s]));
         if (it == n - 1) tc_commit(smem_u32(&acc_full));
       }
@@ -1437,7 +1448,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     const float up = ds_scale<SPLIT>(p, unit);
     const float f = up * PINV;  // on P, which is formed times 2^PSHIFT
     const float fy = SPLIT ? f * p.iv[unit] * p.ido[unit] : f;
-    const bool dist_on = !KEYS && p.dist != nullptr;
+    const bool dist_on = MODE == QUERIES && p.dist != nullptr;
     float2 mine = make_float2(INFINITY, 0.f);
     int vis = 0;
     if (!KEYS && row < p.tq) {
@@ -1475,8 +1486,9 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       if (KEYS && gt < BN) {
         // per column: what is added to the scaled score, and to Y times f
         const float2 st = p.stats[(static_cast<long long>(batch) * p.heads + h) * p.tq_pad + at + gt];
+        const bool alone = rel_visible(p.causal, at + gt + off, klen) <= 1;
         colx[KEYS ? g : 0][turn][gt] = (flat ? value : 0.f) + PSHIFT - st.x;
-        coly[KEYS ? g : 0][turn][gt] = -st.y * f;
+        coly[KEYS ? g : 0][turn][gt] = alone ? 0.f : -st.y * f;
       }
       if (KEYS || !flat) group_barrier(1 + g);
       // window[c - r + 127] for query rows, window[r - c + 63] for key rows
@@ -1497,7 +1509,8 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       F2 all(0.f, 0.f);
       if (ok) {
         tc_fence_after();
-        const float rx = (flat ? value : 0.f) + PSHIFT - mine.x, ry = -mine.y * f;
+        const bool alone = !KEYS && vis <= 1;
+        const float rx = (flat ? value : 0.f) + PSHIFT - mine.x, ry = alone ? 0.f : -mine.y * f;
         uint32_t x[32], y[32];
         tmem_ld32(x_col, x);
         if (WANT_D) tmem_ld32(y_col, y);
@@ -1514,6 +1527,13 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
               x[e] = 0xff800000u;  // -inf
               if (WANT_D) y[e] = 0u;
             }
+        }
+        // A query that sees one key gives it all its weight whatever the score: dS is zero, not what is
+        // left of two roundings.  The first query of a causal sequence, or every one over a single key.
+        if (WANT_D && (KEYS ? klen <= 1 || (p.causal && at + off <= 0) : __any_sync(0xffffffffu, alone))) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (KEYS ? klen <= 1 || at + 32 * half + e + off <= 0 : alone) y[e] = 0u;
         }
         const float cx1 = flat ? c1 : 1.f;
         const F2 cx(cx1, cx1), f2(fy, fy);
@@ -1550,8 +1570,8 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
         }
         if (WANT_P) tmem_st16(x_col, pw);
         if (WANT_P && SPLIT) tmem_st16(x_col + 16, plow);
-        if (WANT_D) tmem_st16(y_col, dw);
-        if (WANT_D && SPLIT) tmem_st16(y_col + 16, dlow);
+        if (WANT_D && MODE != DELTA) tmem_st16(y_col, dw);
+        if (WANT_D && MODE != DELTA && SPLIT) tmem_st16(y_col + 16, dlow);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(smem_u32(&p_full[g]));
@@ -1567,6 +1587,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
           if (lane < 31) diag[KEYS ? 0 : warp - 4][32 + lane] = run;  // diagonal 31 - lane
         }
       }
+      if (MODE == DELTA) far_lo += all.sum();
       if (dist_on) {
         if (!sweep) {  // one side of the reach
           float a0, a1;
@@ -1619,8 +1640,9 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
         for (int e = gt; e < p.width; e += 256) dist[e] *= 1.f / up;
       }
     }
+    if (MODE == DELTA) delta_s[2 * g + half][r] = ok ? far_lo / up : 0.f;
     // ---- results: of two, group 0 writes dK and group 1 dV; a single one's columns are shared ----
-    if (n > 0 && ok) {
+    if (MODE != DELTA && n > 0 && ok) {
       ok = warp_wait(&acc_full, 0, status, DEV_TIMEOUT_ACCUM, 0xf10 + g);
       tc_fence_after();
     }
@@ -1628,7 +1650,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     const bool values = MODE == KEYS_DV || (MODE == KEYS_BOTH && g == 1);  // this thread writes dV
     Out* out = static_cast<Out*>(KEYS ? (values ? p.dv : p.dk) : p.dq);
     const bool real = row < (KEYS ? p.tk : p.tq);
-    if (ok && out != nullptr && (n > 0 || !p.accumulate)) {
+    if (MODE != DELTA && ok && out != nullptr && (n > 0 || !p.accumulate)) {
       const long long ld = KEYS ? (values ? p.lddv : p.lddk) : p.lddq, sh = KEYS ? (values ? p.shdv : p.shdk) : p.shdq,
                       sb = KEYS ? (values ? p.sbdv : p.sbdk) : p.sbdq;
       const int vec = KEYS ? (values ? p.vec_dv : p.vec_dk) : p.vec_dq;
@@ -1656,6 +1678,10 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
 
   tc_fence_before();
   __syncthreads();
+  if (MODE == DELTA && n > 0 && threadIdx.x < FT && r0 + threadIdx.x < qlen) {
+    float2* st = p.delta + (static_cast<long long>(batch) * p.heads + head) * p.tq_pad + r0 + threadIdx.x;
+    st->y += (delta_s[0][threadIdx.x] + delta_s[1][threadIdx.x]) + (delta_s[2][threadIdx.x] + delta_s[3][threadIdx.x]);
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -1727,13 +1753,14 @@ cudaError_t backward_hs(const FlashBwdParams& p, cudaStream_t stream, int* statu
   cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern), smem, &smem_set);
   if (e != cudaSuccess) return e;
   FlashBwdParams q = p;
-  constexpr bool keys = MODE != QUERIES;
-  q.row_tiles = ((keys ? p.tk : p.tq) + FT - 1) / FT;
+  constexpr bool keys = MODE != QUERIES && MODE != DELTA;
+  q.row_tiles = MODE == DELTA ? p.row_tiles : ((keys ? p.tk : p.tq) + FT - 1) / FT;
   const long long grid = static_cast<long long>(q.row_tiles) * (keys ? p.kv_heads : p.heads) * p.batch;
   return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(FTHREADS), smem, stream, pdl_enabled(), q, status);
 }
 template <int MODE>
 cudaError_t backward_any(const FlashBwdParams& p, bool split, cudaStream_t stream, int* status) {
+  if (split && p.hs > 64) return backward_hs<128, MODE == KEYS_BOTH ? DELTA : MODE, 1, true>(p, stream, status);
   if (split) return backward_hs<64, MODE, 4, true>(p, stream, status);
   return p.hs <= 64 ? backward_hs<64, MODE, 4, false>(p, stream, status) : backward_hs<128, MODE, 4, false>(p, stream, status);
 }
@@ -1968,6 +1995,23 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
     *launches = 1;
     if (e != cudaSuccess) return e;
   }
+  // query tiles, from the first on, that may qualify for the correction of delta
+  p.delta = reinterpret_cast<float2*>(stats);
+  p.row_tiles = qtiles;
+  if (split) {
+    if (a.tk <= kDeltaSplit) p.row_tiles = 0;
+  } else if (a.k_lengths == nullptr && a.tk > kDeltaHalf) {
+    if (!a.causal) p.row_tiles = 0;
+    if (a.causal && a.q_offsets == nullptr) {
+      const long long tiles = (kDeltaHalf - a.q_offset + FT - 1) / FT;
+      p.row_tiles = tiles < 0 ? 0 : tiles < qtiles ? static_cast<int>(tiles) : qtiles;
+    }
+  }
+  if (p.row_tiles > 0) {
+    e = backward_any<DELTA>(p, split, stream, status);
+    ++*launches;
+    if (e != cudaSuccess) return e;
+  }
   const bool wide = split && a.hs > 64;
   if (!wide && (p.dk != nullptr || p.dv != nullptr)) {
     e = backward_any<KEYS_BOTH>(p, split, stream, status);
@@ -1985,7 +2029,7 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
     if (e != cudaSuccess) return e;
   }
   if (p.dq != nullptr || dist != nullptr) {
-    e = wide ? backward_hs<128, QUERIES, 1, true>(p, stream, status) : backward_any<QUERIES>(p, split, stream, status);
+    e = backward_any<QUERIES>(p, split, stream, status);
     ++*launches;
     if (e != cudaSuccess) return e;
   }

@@ -172,7 +172,8 @@ rel_softmax_kernel(const RelScores s, const float* __restrict__ bias, float* __r
 }
 
 // Backward: scores -> probabilities in place from the kept statistics, and over dp
-// dS = factor * P (.) (dP - sum_j P dP).  One sweep with both in registers, NV = 0 two.
+// dS = factor * P (.) (dP - sum_j P dP).  One sweep with both in registers, NV = 0 two.  A query that sees
+// one key gives it all its weight whatever the score: its dS is zero, not what is left of two roundings.
 template <int NV, bool BLOCK>
 __global__ void __launch_bounds__(256)
 rel_softmax_grad_kernel(const RelScores s, const float* __restrict__ bias, const float* __restrict__ lse,
@@ -215,12 +216,12 @@ rel_softmax_grad_kernel(const RelScores s, const float* __restrict__ bias, const
     const int j = g + G * k;
     if (j < s.ld) {
       sc[j] = v[k];
-      dc[j] = j < last ? factor * (v[k] * (d[k] - sum)) : 0.f;
+      dc[j] = j < last && last > 1 ? factor * (v[k] * (d[k] - sum)) : 0.f;
     }
   }
   if (NV == 0)
     for (int j = g; j < s.ld; j += G) {
-      dc[j] = j < last ? factor * (sc[j] * (dc[j] - sum)) : 0.f;
+      dc[j] = j < last && last > 1 ? factor * (sc[j] * (dc[j] - sum)) : 0.f;
       if (j >= last) sc[j] = 0.f;
     }
 }

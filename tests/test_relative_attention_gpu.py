@@ -166,7 +166,8 @@ DT = [np.float32, np.float16]
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("hs,tq,tk", [(64, 1, 1), (64, 1, 200), (64, 5, 300), (64, 64, 64), (64, 128, 128), (64, 129, 127), (64, 300, 300), (64, 513, 130),
                                       (128, 128, 256), (128, 257, 257), (32, 100, 100), (16, 40, 70), (80, 150, 150), (96, 130, 140), (40, 200, 99),
-                                      (57, 65, 66), (1, 9, 9), (192, 33, 140), (256, 20, 20), (64, 1, 2500), (128, 1100, 1100)])
+                                      (57, 65, 66), (1, 9, 9), (192, 33, 140), (256, 20, 20), (64, 1, 2500), (128, 1100, 1100),
+                                      (64, 300, 1500), (128, 700, 600), (120, 3, 3000), (72, 16, 900), (17, 2, 777), (64, 1300, 2100)])
 def test_shapes(gpu, dt, causal, hs, tq, tk):
     check(gpu, Case(dt, hs, tq, tk, causal=causal, offsets=max(tk - tq, 0) if causal else 0))
 
