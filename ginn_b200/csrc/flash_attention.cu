@@ -425,7 +425,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
       tc_fence_after();
     }
     if (ok) {
-      const bool real = i < p.tq, some = nt > 0 && vis > 0 && l > 0.f;
+      const bool real = i < p.tq, some = nt > 0 && vis > 0 && l != 0.f;  // (not a number stays one)
       const float inv = some ? (SPLIT ? p.iv[unit] : 1.f) / l : 0.f;
       using Out = typename std::conditional<SPLIT, float, __half>::type;
       Out* out = static_cast<Out*>(p.O) + i * p.ldo + hd.head * p.sho + hd.batch * p.sbo;
@@ -621,7 +621,7 @@ split_planes_kernel(const __grid_constant__ SplitParams p) {
       float2 st = make_float2(INFINITY, 0.f);
       if (row < part.real) {
         const float l = p.lse[hb * part.rows + row];
-        if (l > -INFINITY) st = make_float2(l * kLog2e, s);
+        if (l != -INFINITY) st = make_float2(l * kLog2e, s);
       }
       p.stats[hb * p.tq_pad + row] = st;
     }
@@ -698,9 +698,9 @@ __device__ __forceinline__ uint4 load_stream(const __half* p) {
 template <typename T>
 __device__ __forceinline__ void token_store(const TokenParams& p, int batch, int kv, int row, int h, float value, float m, float l) {
   const int head = kv * p.group + row / p.tq, i = row % p.tq;
-  if (h < p.hs) static_cast<T*>(p.o)[h + i * p.ldo + head * p.sho + batch * p.sbo] = from_f<T>(l > 0.f ? value / l : 0.f);
+  if (h < p.hs) static_cast<T*>(p.o)[h + i * p.ldo + head * p.sho + batch * p.sbo] = from_f<T>(l != 0.f ? value / l : 0.f);
   if (h == 0)
-    p.lse[(static_cast<long long>(batch) * p.heads + head) * p.tq + i] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+    p.lse[(static_cast<long long>(batch) * p.heads + head) * p.tq + i] = l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
 }
 
 // What a lane knows of its two rows of the scores, g and g + 8, and of its CTA's keys.
@@ -1101,8 +1101,8 @@ flash_token_join_kernel(const TokenParams p) {
   for (int s = 0; s < p.splits; ++s) {
     const long long at = (unit * p.splits + s) * p.rows + row;
     const float2 st = p.stat[at];
-    if (st.x == -INFINITY) continue;
-    const float a = ex2(st.x - m);
+    if (st.x == -INFINITY && st.y == 0.f) continue;  // no keys; its result was not written
+    const float a = st.x == -INFINITY ? 0.f : ex2(st.x - m);
     l += st.y * a;
     v += p.part[at * HS + h] * a;
   }
@@ -1238,7 +1238,7 @@ flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long lon
       float2 s = make_float2(INFINITY, 0.f);
       if (i < len) {
         const float x = lse[static_cast<long long>(hb) * p.tq + i];
-        if (x > -INFINITY) s = make_float2(x * kLog2e, dot[k]);
+        if (x != -INFINITY) s = make_float2(x * kLog2e, dot[k]);
       }
       stats[static_cast<long long>(hb) * p.tq_pad + i] = s;
     }

@@ -162,7 +162,7 @@ rel_softmax_kernel(const RelScores s, const float* __restrict__ bias, float* __r
   if (NV == 0)
     for (int j = g; j < last; j += G) sum += exp_fast(score(sc[j], j) - m);
   sum = column_reduce<BLOCK, false>(sum, red);
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
   if (g == 0) lse[(static_cast<long long>(w.batch) * s.heads + w.head) * s.tq + w.query] = logf(sum) + m;
 #pragma unroll
   for (int k = 0; k < NV; ++k)

@@ -270,6 +270,26 @@ def test_what_lies_behind_the_lengths_is_not_looked_at(gpu, dt):
 
 
 @pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("hs,tq,tk", [(64, 40, 300), (128, 1, 700), (192, 20, 50)])
+def test_what_is_not_a_number_stays_one(gpu, dt, hs, tq, tk):
+    """A key that is not a number reaches every query that sees it, in o, lse and dq; a query that is not one
+    only its own.  Nothing is turned into zeros on the way."""
+    c = Case(dt, hs, tq, tk, heads=2, kv=2, batch=2)
+    c.k[:, tk // 3, 1, 0] = np.nan
+    c.q[:, 0, 0, 1] = np.nan
+    c.upload()
+    c.forward(gpu)
+    c.backward(gpu)
+    ref, tol = c.reference()
+    o, lse, dq = host(c.O), host(c.L), host(c.DQ)
+    assert np.isnan(o[:, :, 1, 0]).all() and np.isnan(lse[0, 1]).all() and np.isnan(dq[:, :, 1, 0]).all()
+    assert np.isnan(o[:, 0, 0, 1]).all() and np.isnan(lse[1, 0, 0]) and np.isnan(dq[:, 0, 0, 1]).all()
+    compare("o", c.O[:, :, 0, 0], ref["o"][:, :, 0, 0], tol["o"][:, :, 0, 0])
+    compare("o", c.O[:, 1:, 0, 1], ref["o"][:, 1:, 0, 1], tol["o"][:, 1:, 0, 1])
+    compare("dq", c.DQ[:, :, 0, 0], ref["dq"][:, :, 0, 0], tol["dq"][:, :, 0, 0])
+
+
+@pytest.mark.parametrize("dt", DT)
 def test_no_keys_and_no_queries(gpu, dt):
     c = Case(dt, 64, 30, 30).upload()
     none_k, none_q = c.K[:, :0], c.Q[:, :0]
