@@ -1605,6 +1605,13 @@ int check_matrix(const char* name, const void* p, int64_t ld, int64_t rows) {
   return GINN_B200_OK;
 }
 
+// A result may be an operand itself, element on element.
+int check_in_place(const char* name, const void* out, int64_t ldo, const char* other, const void* in, int64_t ldi, int64_t cols) {
+  if (out && out == in && cols > 1 && ldo != ldi)
+    return fail(GINN_B200_BAD_ARGUMENT, "%s is %s with another leading dimension", name, other);
+  return GINN_B200_OK;
+}
+
 int check_dropout(const ginn_b200_dropout* d, gb::Dropout* out) {
   *out = gb::Dropout();
   if (!d) return fail(GINN_B200_BAD_ARGUMENT, "null dropout description");
@@ -1660,6 +1667,7 @@ int ginn_b200_layer_norm_forward(int device, void* stream, int dtype, int64_t ro
   if (rows == 0 || cols == 0) return GINN_B200_OK;
   if (int s = check_matrix("x", x, ldx, rows)) return s;
   if (int s = check_matrix("y", y, ldy, rows)) return s;
+  if (int s = check_in_place("y", y, ldy, "x", x, ldx, cols)) return s;
   gb::NormArgs a = {};
   a.x = x; a.gain = gain; a.bias = bias; a.y = y; a.mean = mean; a.rstd = rstd;
   a.ldx = ldx; a.ldy = ldy; a.rows = rows; a.cols = cols;
@@ -1677,6 +1685,7 @@ int ginn_b200_layer_norm_backward(int device, void* stream, int dtype, int64_t r
     if (int s = check_matrix("dy", dy, lddy, rows)) return s;
     if (dx)
       if (int s = check_matrix("dx", dx, lddx, rows)) return s;
+    if (int s = check_in_place("dx", dx, lddx, "dy", dy, lddy, cols)) return s;
     if (!mean || !rstd) return fail(GINN_B200_BAD_ARGUMENT, "mean and rstd of the forward pass are needed");
   }
   gb::NormGradArgs a = {};
@@ -1697,6 +1706,8 @@ int ginn_b200_dropout_forward(int device, void* stream, int dtype, int64_t rows,
   if (int s = check_matrix("y", y, ldy, rows)) return s;
   if (residual)
     if (int s = check_matrix("residual", residual, ldr, rows)) return s;
+  if (int s = check_in_place("y", y, ldy, "x", x, ldx, cols)) return s;
+  if (int s = check_in_place("y", y, ldy, "residual", residual, ldr, cols)) return s;
   DevCtx* ctx;
   if (int s = get_ctx(device, &ctx)) return s;
   CU_TRY(gb::launch_dropout(dtype, x, ldx, residual, ldr, y, ldy, rows, cols, d, ctx->num_sms,
@@ -1714,6 +1725,7 @@ int ginn_b200_dropout_backward(int device, void* stream, int dtype, int64_t rows
   if (rows == 0 || cols == 0) return GINN_B200_OK;
   if (int s = check_matrix("dy", dy, lddy, rows)) return s;
   if (int s = check_matrix("dx", dx, lddx, rows)) return s;
+  if (int s = check_in_place("dx", dx, lddx, "dy", dy, lddy, cols)) return s;
   DevCtx* ctx;
   if (int s = get_ctx(device, &ctx)) return s;
   CU_TRY(gb::launch_dropout(dtype, dy, lddy, accumulate ? dx : nullptr, lddx, dx, lddx, rows, cols, d,
@@ -1738,6 +1750,8 @@ int ginn_b200_residual_norm_forward(int device, void* stream, int dtype, int64_t
     if (int s = check_matrix("residual", residual, ldr, rows)) return s;
   if (y == h || y == x || y == residual)
     return fail(GINN_B200_BAD_ARGUMENT, "y must be storage of its own");
+  if (int s = check_in_place("h", h, ldh, "x", x, ldx, cols)) return s;
+  if (int s = check_in_place("h", h, ldh, "residual", residual, ldr, cols)) return s;
   a.x = x; a.res = residual; a.gain = gain; a.bias = bias; a.h = h; a.y = y; a.mean = mean; a.rstd = rstd;
   a.ldx = ldx; a.ldres = ldr; a.ldh = ldh; a.ldy = ldy; a.rows = rows; a.cols = cols;
   a.eps = eps;
@@ -1764,6 +1778,10 @@ int ginn_b200_residual_norm_backward(int device, void* stream, int dtype, int64_
     if (dres)
       if (int s = check_matrix("dres", dres, lddres, rows)) return s;
     if (dx && dx == dres) return fail(GINN_B200_BAD_ARGUMENT, "dx and dres are the same tensor");
+    if (int s = check_in_place("dx", dx, lddx, "dy", dy, lddy, cols)) return s;
+    if (int s = check_in_place("dx", dx, lddx, "dh", dh, lddh, cols)) return s;
+    if (int s = check_in_place("dres", dres, lddres, "dy", dy, lddy, cols)) return s;
+    if (int s = check_in_place("dres", dres, lddres, "dh", dh, lddh, cols)) return s;
     if (!mean || !rstd) return fail(GINN_B200_BAD_ARGUMENT, "mean and rstd of the forward pass are needed");
   }
   a.h = h; a.gain = gain; a.mean = mean; a.rstd = rstd; a.dy = dy; a.dh = dh; a.dx = dx; a.dres = dres;
@@ -1886,6 +1904,7 @@ int check_relative(int dtype, const ginn_b200_relative_attention* a) {
     if (int s = check_heads("v", a->v, v)) return s;
   }
   if (int s = check_heads_out("o", a->o, o, a->head_size, a->tq, a->heads, a->batch)) return s;
+  if (a->o == a->q || a->o == a->k || a->o == a->v) return fail(GINN_B200_BAD_ARGUMENT, "o must be storage of its own");
   if (!a->lse) return fail(GINN_B200_BAD_ARGUMENT, "lse is a null pointer");
   return GINN_B200_OK;
 }
@@ -1896,11 +1915,14 @@ struct RelDense {
   long long ld = 0, stride = 0;
 };
 
-// `src` as it is when it already has that form and no length cuts it, else a packed copy.
+// `src` as it is when it already has that form and is looked at from end to end, else a packed copy.
 int rel_dense_in(Scratch* scratch, int dtype, const void* src, const RelStrides& s, int64_t hs, int64_t t, int64_t heads,
-                 int64_t batch, const int* lengths, RelDense* out) {
+                 int64_t batch, const gb::RelExtent& extent, bool query, RelDense* out) {
   const bool even = batch == 1 || s.batch == heads * s.head;
-  if (dtype == GINN_B200_F32 && even && lengths == nullptr && s.ld >= hs) {
+  const bool whole = query ? extent.q_lengths == nullptr
+                           : extent.k_lengths == nullptr &&
+                                 (!extent.causal || (!extent.q_offsets && !extent.q_lengths && extent.q_offset + extent.tq >= extent.tk));
+  if (dtype == GINN_B200_F32 && even && whole && s.ld >= hs) {
     out->p = static_cast<const float*>(src);
     out->ld = s.ld;
     out->stride = s.head;
@@ -1909,7 +1931,7 @@ int rel_dense_in(Scratch* scratch, int dtype, const void* src, const RelStrides&
   const int hsp = static_cast<int>((hs + 3) & ~int64_t(3));
   float* p;
   CU_TRY(scratch->take(&p, hsp * t * heads * batch));
-  CU_TRY(gb::launch_rel_pack(dtype, src, s.ld, s.head, s.batch, (int)hs, hsp, (int)t, (int)heads, (int)batch, lengths, p,
+  CU_TRY(gb::launch_rel_pack(dtype, src, s.ld, s.head, s.batch, (int)hs, hsp, (int)t, (int)heads, (int)batch, extent, query, p,
                              scratch->stream));
   g_launches.fetch_add(1);
   out->p = p;
@@ -1965,10 +1987,11 @@ int relative_composed(int device, cudaStream_t stream, int dtype, const ginn_b20
   const int64_t hs = a.head_size, tq = a.tq, tk = a.tk, kv = a.kv_heads, group = a.heads / kv, units = kv * a.batch;
   const RelStrides sq = {a.ldq, a.stride_q_head, a.stride_q_batch}, sk = {a.ldk, a.stride_k_head, a.stride_k_batch},
                    sv = {a.ldv, a.stride_v_head, a.stride_v_batch}, so = {a.ldo, a.stride_o_head, a.stride_o_batch};
+  const gb::RelExtent extent = {(int)tq, (int)tk, a.causal ? 1 : 0, a.q_offset, a.q_offsets, a.q_lengths, a.k_lengths};
   RelDense q, k, v, d_o;
-  if (int s = rel_dense_in(&scratch, dtype, a.q, sq, hs, tq, a.heads, a.batch, a.q_lengths, &q)) return s;
-  if (int s = rel_dense_in(&scratch, dtype, a.k, sk, hs, tk, kv, a.batch, a.k_lengths, &k)) return s;
-  if (int s = rel_dense_in(&scratch, dtype, a.v, sv, hs, tk, kv, a.batch, a.k_lengths, &v)) return s;
+  if (int s = rel_dense_in(&scratch, dtype, a.q, sq, hs, tq, a.heads, a.batch, extent, true, &q)) return s;
+  if (int s = rel_dense_in(&scratch, dtype, a.k, sk, hs, tk, kv, a.batch, extent, false, &k)) return s;
+  if (int s = rel_dense_in(&scratch, dtype, a.v, sv, hs, tk, kv, a.batch, extent, false, &v)) return s;
   float* bias = nullptr;
   if (a.table) {
     CU_TRY(scratch.take(&bias, (2 * a.reach + 1) * a.heads));
@@ -2007,7 +2030,7 @@ int relative_composed(int device, cudaStream_t stream, int dtype, const ginn_b20
   const int width = gb::rel_dist_width(sc.reach, tk, gb::kRelDiagonal);
   const int64_t qblocks = (tq + gb::kRelDiagonal - 1) / gb::kRelDiagonal;
   if (g) {
-    if (int s = rel_dense_in(&scratch, dtype, g->d_o, sdo, hs, tq, a.heads, a.batch, a.q_lengths, &d_o)) return s;
+    if (int s = rel_dense_in(&scratch, dtype, g->d_o, sdo, hs, tq, a.heads, a.batch, extent, true, &d_o)) return s;
     CU_TRY(scratch.take(&dp, per * group * nq * sc.ld));
     if (want_dq)
       if (int s = rel_dense_out(&scratch, dtype, g->dq, sdq, hs, tq, a.heads, a.batch, &dq)) return s;
@@ -2228,6 +2251,14 @@ int ginn_b200_relative_attention_backward(int device, void* stream_, int dtype, 
     if (int s = check_heads_out("dk", g->dk, {g->lddk, g->stride_dk_head, g->stride_dk_batch}, hs, tk, a->kv_heads, a->batch)) return s;
   if (g->dv && tk)
     if (int s = check_heads_out("dv", g->dv, {g->lddv, g->stride_dv_head, g->stride_dv_batch}, hs, tk, a->kv_heads, a->batch)) return s;
+  const void* const out[3] = {g->dq, g->dk, g->dv};
+  const void* const in[5] = {a->q, a->k, a->v, a->o, g->d_o};
+  for (int i = 0; i < 3 && !none; ++i) {  // read by one kernel while another writes
+    bool own = true;
+    for (int j = 0; j < 3; ++j) own = own && (j == i || out[i] == nullptr || out[i] != out[j]);
+    for (const void* x : in) own = own && (out[i] == nullptr || out[i] != x);
+    if (!own) return fail(GINN_B200_BAD_ARGUMENT, "d%c must be storage of its own", "qkv"[i]);
+  }
   if (none && g->accumulate) return GINN_B200_OK;
   DevCtx* ctx;
   if (int s = get_ctx(device, &ctx)) return s;

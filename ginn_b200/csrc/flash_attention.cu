@@ -124,7 +124,7 @@ struct FlashHead {
     head = hb - batch * p.heads;
     kv = head / p.group;
     qlen = rel_length(p.q_lengths, batch, p.tq);
-    klen = rel_length(p.k_lengths, batch, p.tk);
+    klen = rel_keys(p, batch);
     off = rel_offset(p.q_offset, p.q_offsets, batch);
   }
   __device__ __forceinline__ int visible(const FlashParams& p, int i) const {
@@ -464,18 +464,20 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
 // every element down to 2^-18 of the largest, and an absolute error of 2^-40 of the largest below
 // that.  A product is then three Half products, high x high + high x low + low x high, at twice the
 // rate of three TF32 products and with the same 2^-22 left out.  The planes are dense,
-// [plane][sequence][head][t][64 or 128], zero behind the head size and behind the sequences' lengths.
+// [plane][sequence][head][t][64 or 128], zero behind the head size, in queries behind the
+// lengths and in keys that no query sees.
 struct SplitOperand {
   const float* x;
   long long ld, head, batch;
   __half* planes;
-  const int* lengths;
   int t, heads, per;      // heads per scale
+  bool query;
   int vec;                // rows allow 16-byte accesses
   long long block0;       // first CTA of this operand
 };
 struct SplitParams {
   SplitOperand op[4];     // q, k, v and, for the backward pass, d_o
+  RelExtent extent;
   int count, hs, batch, kv_heads;
   unsigned* most;         // [operand][batch][kv heads]: bits of the largest magnitude
   unsigned* norms;        // backward: [d_o, v][batch][kv heads]: bits of the largest row's squared norm
@@ -508,7 +510,7 @@ struct SplitPart {
       unit = batch * p.kv_heads + head / p.op[i].per;
       row0 = static_cast<int>(at % parts) * kSplitRows;
       rows = p.op[i].t;
-      real = rel_length(p.op[i].lengths, batch, rows);
+      real = rel_rows(p.extent, p.op[i].query, batch);
       vec = p.op[i].vec;
       ld = p.op[i].ld;
       x = p.op[i].x + head * p.op[i].head + batch * p.op[i].batch;
@@ -1184,7 +1186,7 @@ flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long lon
   const int heads = queries ? p.heads : p.kv_heads;
   const int batch = hb / heads, head = hb - batch * heads;
   const int kv = queries ? head / p.group : head;
-  const int len = queries ? rel_length(p.q_lengths, batch, p.tq) : rel_length(p.k_lengths, batch, p.tk);
+  const int len = queries ? rel_length(p.q_lengths, batch, p.tq) : rel_keys(p, batch);
   const int unit = batch * p.kv_heads + kv;
   auto widen = [&](uint4 w, float (&f)[8]) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -1265,6 +1267,42 @@ flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long lon
 enum FlashMode { KEYS_BOTH = 0, QUERIES = 1, KEYS_DK = 2, KEYS_DV = 3, DELTA = 4 };
 constexpr int kDeltaHalf = 256, kDeltaSplit = 512;
 
+// What a CTA works on: 128 rows of one head of one sequence, and the streamed tiles first .. first + per - 1
+// of every query head of the group.
+template <int MODE, bool SPLIT>
+struct FlashBwdTile {
+  int tile, batch, head, kv, r0, qlen, klen, first = 0, per = 0;
+  long long off;
+  __device__ __forceinline__ explicit FlashBwdTile(const FlashBwdParams& p) {
+    constexpr bool KEYS = MODE != QUERIES && MODE != DELTA;
+    // the CTAs with the most work first: under a causal mask the first keys and the last queries
+    const int heads = KEYS ? p.kv_heads : p.heads;
+    const int hbs = heads * p.batch, hb = static_cast<int>(blockIdx.x) % hbs;
+    tile = KEYS ? static_cast<int>(blockIdx.x) / hbs : p.row_tiles - 1 - static_cast<int>(blockIdx.x) / hbs;
+    batch = hb / heads;
+    head = hb - batch * heads;
+    kv = KEYS ? head : head / p.group;
+    r0 = tile * FT;
+    qlen = rel_length(p.q_lengths, batch, p.tq);
+    klen = rel_keys(p, batch);
+    off = rel_offset(p.q_offset, p.q_offsets, batch);
+    if (KEYS) {
+      if (r0 < klen && qlen > 0) {
+        long long i = p.causal ? r0 - off : 0;  // the first query that sees key r0
+        i = i < 0 ? 0 : i;
+        if (i < qlen) {
+          first = static_cast<int>(i / BN);
+          per = (qlen + BN - 1) / BN - first;
+        }
+      }
+    } else if (r0 < qlen) {
+      const int last = r0 + FT - 1 < qlen - 1 ? r0 + FT - 1 : qlen - 1;
+      per = (rel_visible(p.causal, last + off, klen) + BN - 1) / BN;
+      if (MODE == DELTA && (SPLIT ? per <= kDeltaSplit / BN : per > kDeltaHalf / BN)) per = 0;
+    }
+  }
+};
+
 template <int HS, int MODE, int BSTAGES, bool SPLIT>
 __global__ void __launch_bounds__(FTHREADS, 1)
 flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict__ status) {
@@ -1292,6 +1330,10 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
   uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t a1_s = base, a2_s = base + ROWS, b_s = base + 2 * ROWS;  // stage: B1, B2
 
+  if (MODE == DELTA) {  // most of its CTAs have nothing to do
+    pdl_wait();
+    if (FlashBwdTile<MODE, SPLIT>(p).per == 0) return;
+  }
   if (warp == 1) {
     if (lane == 0) {
       mbar_init(smem_u32(&rows_full), 1);
@@ -1317,30 +1359,10 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
   pdl_wait();
   pdl_launch_dependents();
 
-  // the CTAs with the most work first: under a causal mask the first keys and the last queries
-  const int heads = KEYS ? p.kv_heads : p.heads;
-  const int hbs = heads * p.batch, hb = static_cast<int>(blockIdx.x) % hbs;
-  const int tile = KEYS ? static_cast<int>(blockIdx.x) / hbs : p.row_tiles - 1 - static_cast<int>(blockIdx.x) / hbs;
-  const int batch = hb / heads, head = hb - batch * heads, kv = KEYS ? head : head / p.group;
-  const int r0 = tile * FT;  // first row
-  const int qlen = rel_length(p.q_lengths, batch, p.tq), klen = rel_length(p.k_lengths, batch, p.tk);
-  const long long off = rel_offset(p.q_offset, p.q_offsets, batch);
-  // streamed tiles: first .. first + per - 1, for every query head of the group
-  int first = 0, per = 0;
-  if (KEYS) {
-    if (r0 < klen && qlen > 0) {
-      long long i = p.causal ? r0 - off : 0;  // the first query that sees key r0
-      i = i < 0 ? 0 : i;
-      if (i < qlen) {
-        first = static_cast<int>(i / BN);
-        per = (qlen + BN - 1) / BN - first;
-      }
-    }
-  } else if (r0 < qlen) {
-    const int last = r0 + FT - 1 < qlen - 1 ? r0 + FT - 1 : qlen - 1;
-    per = (rel_visible(p.causal, last + off, klen) + BN - 1) / BN;
-    if (MODE == DELTA && (SPLIT ? per <= kDeltaSplit / BN : per > kDeltaHalf / BN)) per = 0;
-  }
+  const FlashBwdTile<MODE, SPLIT> w(p);
+  const int tile = w.tile, batch = w.batch, head = w.head, kv = w.kv, r0 = w.r0, qlen = w.qlen, klen = w.klen;
+  const int first = w.first, per = w.per;
+  const long long off = w.off;
   const int n = per * (KEYS ? p.group : 1);
 
   if (warp == 0) {
@@ -1348,9 +1370,9 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     if (n > 0 && elect_one()) {
       mbar_arrive_expect_tx(smem_u32(&rows_full), 2 * ROWS);
       for (int c = 0; c < CHUNKS; ++c) {
-        const int x = 64 * (c % WIDE), w = batch + c / WIDE * p.batch;
-        tma_load_4d(a1_s + c * FCHUNK, KEYS ? &p.tmK : &p.tmQ, smem_u32(&rows_full), x, r0, head, w);
-        tma_load_4d(a2_s + c * FCHUNK, KEYS ? &p.tmV : &p.tmDO, smem_u32(&rows_full), x, r0, head, w);
+        const int x = 64 * (c % WIDE), plane = batch + c / WIDE * p.batch;
+        tma_load_4d(a1_s + c * FCHUNK, KEYS ? &p.tmK : &p.tmQ, smem_u32(&rows_full), x, r0, head, plane);
+        tma_load_4d(a2_s + c * FCHUNK, KEYS ? &p.tmV : &p.tmDO, smem_u32(&rows_full), x, r0, head, plane);
       }
       for (int it = 0; it < n; ++it) {
         const int s = it % BSTAGES;
@@ -1359,9 +1381,9 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
         const int at = (first + it % per) * BN, h = KEYS ? head * p.group + it / per : kv;
         mbar_arrive_expect_tx(bar, 2 * TILE);
         for (int c = 0; c < CHUNKS; ++c) {
-          const int x = 64 * (c % WIDE), w = batch + c / WIDE * p.batch;
-          tma_load_4d(dst + c * BCHUNK, KEYS ? &p.tmQ64 : &p.tmK64, bar, x, at, h, w);
-          tma_load_4d(dst + TILE + c * BCHUNK, KEYS ? &p.tmDO64 : &p.tmV64, bar, x, at, h, w);
+          const int x = 64 * (c % WIDE), plane = batch + c / WIDE * p.batch;
+          tma_load_4d(dst + c * BCHUNK, KEYS ? &p.tmQ64 : &p.tmK64, bar, x, at, h, plane);
+          tma_load_4d(dst + TILE + c * BCHUNK, KEYS ? &p.tmDO64 : &p.tmV64, bar, x, at, h, plane);
         }
       }
     }
@@ -1829,6 +1851,7 @@ cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, flo
   SplitParams p;
   std::memset(&p, 0, sizeof(p));
   const long long units = static_cast<long long>(a->batch) * a->kv_heads;
+  p.extent = {a->tq, a->tk, a->causal, a->q_offset, a->q_offsets, a->q_lengths, a->k_lengths};
   p.count = d_o != nullptr ? 4 : 3;
   p.hs = a->hs; p.batch = a->batch; p.kv_heads = a->kv_heads;
   p.most = reinterpret_cast<unsigned*>(work);
@@ -1852,7 +1875,7 @@ cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, flo
     o.x = static_cast<const float*>(ops[i]->p);
     o.ld = ops[i]->ld; o.head = ops[i]->head; o.batch = ops[i]->batch;
     o.planes = static_cast<__half*>(ops[i]->planes);
-    o.lengths = query ? a->q_lengths : a->k_lengths;
+    o.query = query;
     o.t = query ? a->tq : a->tk;
     o.heads = query ? a->heads : a->kv_heads;
     o.per = query ? a->heads / a->kv_heads : 1;
@@ -2007,7 +2030,7 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
       p.row_tiles = tiles < 0 ? 0 : tiles < qtiles ? static_cast<int>(tiles) : qtiles;
     }
   }
-  if (p.row_tiles > 0) {
+  if (p.row_tiles > 0 && (p.dk != nullptr || p.dq != nullptr || dist != nullptr)) {
     e = backward_any<DELTA>(p, split, stream, status);
     ++*launches;
     if (e != cudaSuccess) return e;

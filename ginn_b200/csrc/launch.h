@@ -201,10 +201,11 @@ cudaError_t launch_dropout(int dtype, const void* x, long long ldx, const void* 
 cudaError_t launch_rel_bias_expand(int dtype, const void* table, long long ldt, const int* map,
                                    int buckets, long long reach, int heads, float factor, float* out,
                                    cudaStream_t stream);
-// dst[b][head][t][hsp] = src(h, t, head, b) in fp32, zero behind hs and behind the lengths.
+// dst[b][head][t][hsp] = src(h, t, head, b) in fp32, zero behind hs, in queries behind the lengths and
+// in keys that no query sees.
 cudaError_t launch_rel_pack(int dtype, const void* src, long long ld, long long sh, long long sb,
-                            int hs, int hsp, int t_len, int heads, int batch, const int* lengths,
-                            float* dst, cudaStream_t stream);
+                            int hs, int hsp, int t_len, int heads, int batch, const RelExtent& extent,
+                            bool query, float* dst, cudaStream_t stream);
 cudaError_t launch_rel_unpack(int dtype, const float* src, int hs, int hsp, int t_len, int heads,
                               int batch, int accumulate, void* dst, long long ld, long long sh,
                               long long sb, cudaStream_t stream);

@@ -42,12 +42,12 @@ rel_bias_expand_kernel(const T* __restrict__ table, long long ldt, const int* __
   out[at] = b >= 0 && b < buckets ? to_f(table[head * ldt + b]) * factor : 0.f;
 }
 
-// dst[b][head][t][hsp] (fp32, dense, rows hs..hsp zero) = src(h, t, head, b); positions behind the
-// sequence's length become zero whatever they hold.
+// dst[b][head][t][hsp] (fp32, dense, rows hs..hsp zero) = src(h, t, head, b); queries behind the
+// sequence's length and keys that no query sees become zero whatever they hold.
 template <typename T>
 __global__ void __launch_bounds__(256)
 rel_pack_kernel(const T* __restrict__ src, long long ld, long long sh, long long sb, int hs, int hsp, int t_len,
-                int heads, const int* __restrict__ lengths, long long total, float* __restrict__ dst) {
+                int heads, const RelExtent extent, bool query, long long total, float* __restrict__ dst) {
   pdl_wait();
   pdl_launch_dependents();
   for (long long at = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; at < total;
@@ -57,7 +57,7 @@ rel_pack_kernel(const T* __restrict__ src, long long ld, long long sh, long long
     const int t = static_cast<int>(r % t_len);
     r /= t_len;
     const int head = static_cast<int>(r % heads), b = static_cast<int>(r / heads);
-    const bool real = h < hs && t < rel_length(lengths, b, t_len);
+    const bool real = h < hs && t < rel_rows(extent, query, b);
     dst[at] = real ? to_f(src[h + t * ld + head * sh + b * sb]) : 0.f;
   }
 }
@@ -364,13 +364,13 @@ cudaError_t launch_rel_bias_expand(int dtype, const void* table, long long ldt, 
 }
 
 cudaError_t launch_rel_pack(int dtype, const void* src, long long ld, long long sh, long long sb, int hs, int hsp,
-                            int t_len, int heads, int batch, const int* lengths, float* dst, cudaStream_t stream) {
+                            int t_len, int heads, int batch, const RelExtent& extent, bool query, float* dst, cudaStream_t stream) {
   const long long total = static_cast<long long>(hsp) * t_len * heads * batch;
   if (dtype == 0)
     return launch_kernel(rel_pack_kernel<float>, dim3(blocks_for(total)), dim3(256), 0, stream, pdl_enabled(),
-                         static_cast<const float*>(src), ld, sh, sb, hs, hsp, t_len, heads, lengths, total, dst);
+                         static_cast<const float*>(src), ld, sh, sb, hs, hsp, t_len, heads, extent, query, total, dst);
   return launch_kernel(rel_pack_kernel<__half>, dim3(blocks_for(total)), dim3(256), 0, stream, pdl_enabled(),
-                       static_cast<const __half*>(src), ld, sh, sb, hs, hsp, t_len, heads, lengths, total, dst);
+                       static_cast<const __half*>(src), ld, sh, sb, hs, hsp, t_len, heads, extent, query, total, dst);
 }
 
 cudaError_t launch_rel_unpack(int dtype, const float* src, int hs, int hsp, int t_len, int heads, int batch,

@@ -37,6 +37,27 @@ __device__ __forceinline__ int rel_visible(int causal, long long pos, int klen) 
   return pos < 0 ? 0 : static_cast<int>(pos) + 1;
 }
 
+// Keys 0 .. n - 1 of a sequence that some query sees: under a causal mask those behind the last query's
+// position are no more looked at than those behind the length (a cache that is filled so far, say).
+template <typename P>
+__device__ __forceinline__ int rel_keys(const P& p, int batch) {
+  const int klen = rel_length(p.k_lengths, batch, p.tk);
+  if (!p.causal) return klen;
+  const long long last = rel_length(p.q_lengths, batch, p.tq) + rel_offset(p.q_offset, p.q_offsets, batch);
+  return last >= klen ? klen : last < 0 ? 0 : static_cast<int>(last);
+}
+// What rel_keys reads, for the passes that need nothing else of the attention.
+struct RelExtent {
+  int tq = 0, tk = 0, causal = 0;
+  long long q_offset = 0;
+  const int* q_offsets = nullptr;
+  const int* q_lengths = nullptr;
+  const int* k_lengths = nullptr;
+};
+__device__ __forceinline__ int rel_rows(const RelExtent& x, bool query, int batch) {
+  return query ? rel_length(x.q_lengths, batch, x.tq) : rel_keys(x, batch);
+}
+
 // Sums of dS by distance as the backward kernels leave them: dist[sequence][head][tile][slot][width].
 struct RelDist {
   const float* dist = nullptr;

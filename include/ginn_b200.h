@@ -354,8 +354,11 @@ int ginn_b200_attention_backward(int device, void* stream, int dtype, int64_t t,
  *   lse[i] = log sum_j exp s[j, i]
  *
  * Query i sees key j when j < k_lengths[b], with `causal` also j <= i + offset, and i < q_lengths[b].
- * A query that sees nothing gives o = 0 and lse = -inf.  What k, v, q and d_o hold behind the lengths
- * is not looked at (NaN included); o and the gradients are zero there.
+ * A query that sees nothing gives o = 0 and lse = -inf.  What q and d_o hold behind the lengths, and k
+ * and v in keys that no query of their sequence sees (behind the length, or with `causal` behind the last
+ * query's position), is not looked at, NaN included; o and the gradients are zero there.  An infinity or
+ * NaN elsewhere may reach any result of its sequence.  No result shares memory with an operand or
+ * with another result.
  *   table      buckets x heads of type `dtype`, leading dimension ldt; NULL = no bias
  *   map        2 * reach + 1 ints on the device: bucket of distance -reach .. reach (see
  *              ginn_b200_relative_buckets); an entry outside [0, buckets) gives no bias
@@ -436,7 +439,7 @@ int ginn_b200_layer_norm_forward(int device, void* stream, int dtype, int64_t ro
  *   dx_j (+)= r (G - mean(G) - xh mean(G (.) xh))  with  xh = (x_j - mu) r,  G = gain (.) dy_j;
  *   dgain (+)= sum_j dy_j (.) xh_j;   dbias (+)= sum_j dy_j   (type `dtype`, summed in fp32 in a
  * fixed order).  The weight gradients take at most 2 * rows * 148 floats of stream-ordered scratch.
- * dx may be dy itself. */
+ * dx may be dy itself (same leading dimension). */
 int ginn_b200_layer_norm_backward(int device, void* stream, int dtype, int64_t rows, int64_t cols,
                                   const void* x, int64_t ldx, const void* gain, const float* mean,
                                   const float* rstd, const void* dy, int64_t lddy, void* dx,
@@ -459,7 +462,7 @@ typedef struct {
 
 /* y = residual + drop(x); residual may be NULL.  The work of ginn's Dropout node
  * (ginn/node/common.h), which draws and keeps a mask tensor, and of the Add behind it.
- * y may be x or residual. */
+ * y may be x or residual (same leading dimension). */
 int ginn_b200_dropout_forward(int device, void* stream, int dtype, int64_t rows, int64_t cols,
                               const void* x, int64_t ldx, const void* residual, int64_t ldr,
                               const ginn_b200_dropout* drop, void* y, int64_t ldy);
@@ -470,7 +473,8 @@ int ginn_b200_dropout_backward(int device, void* stream, int dtype, int64_t rows
 
 /* Both in one pass, the seam between two sublayers of a transformer block:
  *   h = residual + drop(x)  (stored, rounded to `dtype`),   y = normalisation of h as above.
- * residual may be NULL.  h may be residual or x; y must be storage of its own. */
+ * residual may be NULL.  h may be residual or x (same leading dimension); y must be storage of its
+ * own. */
 int ginn_b200_residual_norm_forward(int device, void* stream, int dtype, int64_t rows, int64_t cols,
                                     const void* x, int64_t ldx, const void* residual, int64_t ldr,
                                     const ginn_b200_dropout* drop, const void* gain,
@@ -479,7 +483,8 @@ int ginn_b200_residual_norm_forward(int device, void* stream, int dtype, int64_t
 /* Its gradients: with g = (gradient of the normalisation's input) + dh, dh (may be NULL) being what
  * reaches h along the residual connection:
  *   dres (+)= g,   dx (+)= g on the kept elements times their factor,   dgain, dbias as above.
- * Each result may be NULL.  dres or dx may be dh or dy, but not each other. */
+ * Each result may be NULL.  dres or dx may be dh or dy (same leading dimension), but not
+ * each other. */
 int ginn_b200_residual_norm_backward(int device, void* stream, int dtype, int64_t rows,
                                      int64_t cols, const void* h, int64_t ldh, const void* gain,
                                      const float* mean, const float* rstd, const void* dy,

@@ -86,6 +86,12 @@ def drop(p=0.1):
     (lambda: B.lib().ginn_b200_dropout_backward(0, None, 0, 8, 4, P, 8, drop(), None, 8, 0), BAD),
     (lambda: B.lib().ginn_b200_residual_norm_forward(0, None, 0, 8, 4, P, 8, P + 64, 8, drop(), None, None, 1e-5, P, 8, P, 8, None, None), BAD),
     (lambda: B.lib().ginn_b200_residual_norm_backward(0, None, 0, 8, 4, P, 8, None, P, P, P, 8, None, 0, drop(), P, 8, P, 8, None, None, 0), BAD),
+    (lambda: norm_fwd(ldx=9), BAD), (lambda: norm_bwd(x=P + 64, lddy=9), BAD),  # in place with another leading dimension
+    (lambda: B.lib().ginn_b200_dropout_forward(0, None, 0, 8, 4, P, 9, None, 0, drop(), P, 8), BAD),
+    (lambda: B.lib().ginn_b200_dropout_forward(0, None, 0, 8, 4, P, 8, 2 * P, 9, drop(), 2 * P, 8), BAD),
+    (lambda: B.lib().ginn_b200_dropout_backward(0, None, 0, 8, 4, P, 9, drop(), P, 8, 0), BAD),
+    (lambda: B.lib().ginn_b200_residual_norm_forward(0, None, 0, 8, 4, P, 8, 2 * P, 9, drop(), None, None, 1e-5, 2 * P, 8, 3 * P, 8, None, None), BAD),
+    (lambda: B.lib().ginn_b200_residual_norm_backward(0, None, 0, 8, 4, P, 8, None, P, P, 2 * P, 8, 3 * P, 9, drop(), 4 * P, 8, 3 * P, 8, None, None, 0), BAD),
 ])
 def test_refusals(call, status):
     assert call() == status
@@ -151,7 +157,7 @@ def described(**change):
     """A valid description of 3 sequences, 4 heads over 2, 5 queries, 6 keys of size 8, changed."""
     d = dict(tq=5, tk=6, head_size=8, heads=4, kv_heads=2, batch=3, q=P, ldq=8, stride_q_head=40, stride_q_batch=160, k=P, ldk=8,
              stride_k_head=48, stride_k_batch=96, v=P, ldv=8, stride_v_head=48, stride_v_batch=96, table=P, ldt=32, buckets=32, map=P,
-             reach=16, scale=1.0, causal=0, q_offset=0, o=P, ldo=8, stride_o_head=40, stride_o_batch=160, lse=P)
+             reach=16, scale=1.0, causal=0, q_offset=0, o=2 * P, ldo=8, stride_o_head=40, stride_o_batch=160, lse=P)
     return B._RelativeAttention(**{**d, **change})
 
 
@@ -165,7 +171,7 @@ def forward(dtype=0, **change):
     (dict(head_size=257), UNSUPPORTED), (dict(kv_heads=3), BAD), (dict(kv_heads=0), BAD), (dict(scale=float("inf")), BAD),
     (dict(scale=float("nan")), BAD), (dict(q_offset=1 << 31), BAD), (dict(buckets=0), BAD), (dict(ldt=31), BAD), (dict(map=None), BAD),
     (dict(reach=-1), BAD), (dict(q=None), BAD), (dict(k=None), BAD), (dict(v=None), BAD), (dict(o=None), BAD), (dict(lse=None), BAD),
-    (dict(ldq=-8), BAD), (dict(ldo=7), BAD), (dict(stride_o_head=39), BAD), (dict(stride_o_batch=0), BAD), (dict(batch=1 << 20, heads=1 << 12, kv_heads=1), BAD),
+    (dict(ldq=-8), BAD), (dict(ldo=7), BAD), (dict(stride_o_head=39), BAD), (dict(stride_o_batch=0), BAD), (dict(o=P), BAD), (dict(batch=1 << 20, heads=1 << 12, kv_heads=1), BAD),
 ])
 def test_refused_attention(change, status):
     assert forward(**change) == status
@@ -174,11 +180,11 @@ def test_refused_attention(change, status):
 
 @pytest.mark.parametrize("change,grad", [
     ({}, dict(d_o=None)), (dict(table=None), dict(dtable=P, lddt=32)), ({}, dict(dtable=P, lddt=31)), ({}, dict(dk=P, lddk=8, stride_dk_head=47)),
-    ({}, dict(lddo=-1)),
+    ({}, dict(lddo=-1)), ({}, dict(dq=P)), ({}, dict(dq=2 * P)), ({}, dict(dq=3 * P)), ({}, dict(dk=4 * P, lddk=8, stride_dk_head=48, stride_dk_batch=96)),
 ])
 def test_refused_attention_gradient(change, grad):
     import ctypes
-    g = dict(d_o=P, lddo=8, stride_do_head=40, stride_do_batch=160, dq=P, lddq=8, stride_dq_head=40, stride_dq_batch=160)
+    g = dict(d_o=3 * P, lddo=8, stride_do_head=40, stride_do_batch=160, dq=4 * P, lddq=8, stride_dq_head=40, stride_dq_batch=160)
     call = lambda g: B.lib().ginn_b200_relative_attention_backward(  # noqa: E731
         0, None, 0, ctypes.byref(described(**change)), None if g is None else ctypes.byref(B._RelativeAttentionGrad(**g)))
     assert call({**g, **grad}) == BAD

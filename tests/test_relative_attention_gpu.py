@@ -270,6 +270,22 @@ def test_what_lies_behind_the_lengths_is_not_looked_at(gpu, dt):
 
 
 @pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("hs,tq,tk,offsets", [(64, 40, 300, [100, 3, -20]), (128, 1, 700, [500, 0, -1]), (192, 20, 50, [10, 25, 0]),
+                                              (128, 130, 200, 50)])
+def test_keys_that_no_query_sees_yet_are_not_looked_at(gpu, dt, hs, tq, tk, offsets):
+    """A causal pass over a cache that is filled so far: what lies behind the last query's position may be
+    anything, and takes no gradient."""
+    c = Case(dt, hs, tq, tk, batch=3, heads=4, kv=2, causal=True, offsets=offsets)
+    last = [max(0, min(tk, o + tq)) for o in ([offsets] * 3 if isinstance(offsets, int) else offsets)]
+    for b, n in enumerate(last):
+        c.k[:, n:, :, b] = np.nan
+        c.v[:, n:, :, b] = -np.inf
+    check(gpu, c)
+    for b, n in enumerate(last):
+        assert (c.DK[:, n:, :, b] == 0).all() and (c.DV[:, n:, :, b] == 0).all()
+
+
+@pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("hs,tq,tk", [(64, 40, 300), (128, 1, 700), (192, 20, 50)])
 def test_what_is_not_a_number_stays_one(gpu, dt, hs, tq, tk):
     """A key that is not a number reaches every query that sees it, in o, lse and dq; a query that is not one
