@@ -802,16 +802,15 @@ template <typename T, bool VEC>
 cudaError_t backward_tv(const NormBwd<T>& p, const NormGradArgs& a, int parts, cudaStream_t stream) {
   if (a.rows > kNormRegisterRows) {
     if (p.cols > 0x7fffffffLL) return cudaErrorInvalidValue;
-    if (p.dres != nullptr || p.dx != nullptr) {
-      cudaError_t e = launch_kernel(norm_backward_long_kernel<T, VEC>, dim3(static_cast<unsigned>(p.cols)),
-                                    dim3(512), 0, stream, pdl_enabled(), p);
+    if (p.partial != nullptr) {  // first: dx or dres may be written over dy
+      const long long per = (p.cols + parts - 1) / parts;
+      const cudaError_t e = launch_kernel(norm_weight_grad_kernel<T>,
+                                          dim3(static_cast<unsigned>((p.rows + 255) / 256), static_cast<unsigned>(parts)), dim3(256),
+                                          0, stream, pdl_enabled(), p, per);
       if (e != cudaSuccess) return e;
     }
-    if (p.partial == nullptr) return cudaSuccess;
-    const long long per = (p.cols + parts - 1) / parts;
-    return launch_kernel(norm_weight_grad_kernel<T>,
-                         dim3(static_cast<unsigned>((p.rows + 255) / 256), static_cast<unsigned>(parts)), dim3(256), 0,
-                         stream, pdl_enabled(), p, per);
+    if (p.dres == nullptr && p.dx == nullptr) return cudaSuccess;
+    return launch_kernel(norm_backward_long_kernel<T, VEC>, dim3(static_cast<unsigned>(p.cols)), dim3(512), 0, stream, pdl_enabled(), p);
   }
   const int nv = backward_pieces(p.rows, sizeof(T));
   const int G = group_size(p.rows, nv);

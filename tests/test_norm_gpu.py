@@ -146,6 +146,20 @@ def test_without_gain_bias_and_statistics(gpu, dt):
 
 
 @pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("rows,cols", [(1024, 40), (1001, 9), (5000, 9), (9000, 7), (9001, 7), (16384, 3), (70000, 3)])
+def test_gradient_over_the_upstream_one(gpu, dt, rows, cols):
+    """dx in dy's place, the weight gradients from the dy that was there."""
+    rng = np.random.default_rng(rows)
+    x, dy, gain = data(rng, rows, cols, dt), data(rng, rows, cols, dt), rng.standard_normal(rows).astype(dt)
+    X, G = B.from_host(x), B.from_host(gain)
+    Y, M, R = B.colmajor(rows, cols, X.dtype), torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+    gpu.layer_norm_forward(X, G, None, Y, M, R)
+    D, DG, DB = B.from_host(dy), torch.empty(rows, dtype=X.dtype, device="cuda"), torch.empty(rows, dtype=X.dtype, device="cuda")
+    gpu.layer_norm_backward(X, G, M, R, D, D, DG, DB, accumulate=False)
+    check_backward(x, gain, host(M), host(R), dy, dict(dres=host(D), dgain=host(DG), dbias=host(DB)), dt)
+
+
+@pytest.mark.parametrize("dt", DT)
 def test_constant_column_and_large_offset(gpu, dt):
     """A column without variance gives the bias and a finite gradient; a mean a thousand times the
     spread does not cancel the spread away."""
