@@ -1646,16 +1646,16 @@ int norm_backward(int device, void* stream_, int dtype, const gb::NormGradArgs& 
   DevCtx* ctx;
   if (int s = get_ctx(device, &ctx)) return s;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  const int parts = gb::norm_backward_parts(dtype, a.rows, a.cols, ctx->num_sms);
+  int launches = 0;
+  const int parts = gb::norm_backward_parts(dtype, a, ctx->num_sms, &launches);
   void* partial = nullptr;
   if (weights && parts > 0)
     CU_TRY(cudaMallocAsync(&partial, static_cast<size_t>(parts) * 2 * a.rows * sizeof(float), stream));
-  const cudaError_t e = gb::launch_norm_backward(dtype, a, parts, static_cast<float*>(partial), stream);
+  const cudaError_t e = gb::launch_norm_backward(dtype, a, static_cast<float*>(partial), ctx->num_sms, stream, ctx->d_status);
   if (partial) cudaFreeAsync(partial, stream);
   if (e != cudaSuccess)
     return fail(GINN_B200_CUDA_ERROR, "layer norm backward launch failed: %s", cudaGetErrorString(e));
-  g_launches.fetch_add((a.cols > 0 && (a.rows <= gb::kNormRegisterRows || a.dres || a.dx)) +
-                       (weights && a.cols > 0 && a.rows > gb::kNormRegisterRows) + weights);
+  g_launches.fetch_add(launches);
   return GINN_B200_OK;
 }
 }  // namespace

@@ -52,7 +52,9 @@ struct Philox {
   // x[i] of element 8 * block + i: times `factor` when it is kept, 0 otherwise.  Both halves of a word
   // are compared in its upper sixteen bits.
   __device__ __forceinline__ void drop8(unsigned long long block, float factor, float (&x)[8]) const {
-    const uint4 r = words(block);
+    apply(words(block), factor, x);
+  }
+  __device__ __forceinline__ void apply(const uint4 r, float factor, float (&x)[8]) const {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w}, limit = threshold << 16;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -28,20 +28,35 @@ int walk_kblocks();
 // Launch with the programmatic-stream-serialization attribute when `pdl` is set: the kernel may
 // begin while its predecessor in the stream drains; it must call pdl_wait() before it touches
 // global memory.  Kernel arguments must have the kernel's exact parameter types.
+// `cluster` CTAs in a row of the grid form a cluster.
 template <typename... KArgs>
-cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                          cudaStream_t stream, bool pdl, KArgs... args) {
+cudaError_t launch_cluster_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, unsigned cluster,
+                                  size_t smem, cudaStream_t stream, bool pdl, KArgs... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+template <typename... KArgs>
+cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                          cudaStream_t stream, bool pdl, KArgs... args) {
+  return launch_cluster_kernel(kern, grid, block, 1u, smem, stream, pdl, args...);
 }
 
 // Raises a kernel's dynamic shared-memory limit once per device instead of on every launch (the
@@ -183,14 +198,13 @@ struct NormGradArgs {
   int accumulate;
   Dropout drop;
 };
-// Longest column whose backward pass keeps it in registers.
-constexpr long long kNormRegisterRows = 8192;
-// Partial vectors (2 x rows floats each) the weight gradients of a backward pass need.
-int norm_backward_parts(int dtype, long long rows, long long cols, int num_sms);
+// Partial vectors (2 x rows floats each) the weight gradients of a backward pass need, and how many
+// kernels it launches.
+int norm_backward_parts(int dtype, const NormGradArgs& a, int num_sms, int* launches);
 cudaError_t launch_norm_forward(int dtype, const NormArgs& a, int num_sms, cudaStream_t stream);
 // `partial`: norm_backward_parts(...) x 2 x rows floats, null when neither dgain nor dbias is set.
-cudaError_t launch_norm_backward(int dtype, const NormGradArgs& a, int parts, float* partial,
-                                 cudaStream_t stream);
+cudaError_t launch_norm_backward(int dtype, const NormGradArgs& a, float* partial, int num_sms,
+                                 cudaStream_t stream, int* status);
 // y = drop(x) (+ add); `add` may be y itself.
 cudaError_t launch_dropout(int dtype, const void* x, long long ldx, const void* add, long long lda,
                            void* y, long long ldy, long long rows, long long cols,

@@ -150,23 +150,28 @@ __device__ __forceinline__ float group_sum(float v, int G, int t, float* slot) {
   for (int o = n >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return __shfl_sync(0xffffffffu, v, 0);
 }
-// Two sums at once.
+// Two sums at once: half of a warp's lanes reduce the one, half the other, within the warp and, behind the
+// barrier, over the warps' values (a float2 per warp in `slot`).  The kernels that need it for every column
+// are bound by what they issue, so it is held to eleven shuffles; every thread adding up the sixteen
+// values itself takes fewer steps one after the other, but a quarter more instructions in all.
 __device__ __forceinline__ float2 group_sum2(float2 v, int G, int t, float2* slot) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool upper = lane >= 16;
+  float a = (upper ? v.y : v.x) + __shfl_xor_sync(0xffffffffu, upper ? v.x : v.y, 16);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  for (int o = 8; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  if (G > 32) {
+    float* s = reinterpret_cast<float*>(slot + (warp - (t >> 5))) + (upper ? 1 : 0);
+    const int n = G >> 5, k = lane & 15;
+    if (k == 0) s[2 * (t >> 5)] = a;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / G), "r"(G) : "memory");
+    a = k < n ? s[2 * k] : 0.f;
+    if (n > 8) a += __shfl_xor_sync(0xffffffffu, a, 8);
+    if (n > 4) a += __shfl_xor_sync(0xffffffffu, a, 4);
+    if (n > 2) a += __shfl_xor_sync(0xffffffffu, a, 2);
+    a += __shfl_xor_sync(0xffffffffu, a, 1);
   }
-  if (G == 32) return v;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = G >> 5;
-  if (lane == 0) slot[warp] = v;
-  asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / G), "r"(G) : "memory");
-  v = lane < n ? slot[warp - (t >> 5) + lane] : make_float2(0.f, 0.f);
-  for (int o = n >> 1; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-  }
-  return make_float2(__shfl_sync(0xffffffffu, v.x, 0), __shfl_sync(0xffffffffu, v.y, 0));
+  return make_float2(__shfl_sync(0xffffffffu, a, 0), __shfl_sync(0xffffffffu, a, 16));
 }
 
 template <typename T>
@@ -227,9 +232,35 @@ __device__ __forceinline__ void write_y(const NormFwd<T>& p, long long col, long
   store_piece<VEC>(p.y + col * p.ldy, r0, p.rows, v);
 }
 
+// Eight elements on their way from memory, in either order of rows.
+template <typename T, bool VEC>
+struct Piece {
+  Raw8<T> x;
+  __device__ __forceinline__ void load(const T* col, long long r0, long long rows) {
+    if (r0 < rows) x.load(col + r0);
+    else x.zero();
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const { x.get(v); }
+};
+template <typename T>
+struct Piece<T, false> {
+  T x[8];
+  __device__ __forceinline__ void load(const T* col, long long r0, long long rows) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = r0 + 32 * e < rows ? col[r0 + 32 * e] : from_f<T>(0.f);
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = to_f(x[e]);
+  }
+};
+
 // One group of G threads per column, the column in registers (8 NV elements per thread): the
-// variance is formed from the differences to the mean, not from a difference of squares.
-template <typename T, bool VEC, int NV>
+// variance is formed from the differences to the mean, not from a difference of squares.  RES: behind
+// dropout and a residual connection.  The column's loads are all issued before its first store (which
+// might overwrite what they read, as far as the compiler knows), and the random numbers, which need
+// nothing, are formed while they are on their way.
+template <typename T, bool VEC, int NV, bool RES>
 __global__ void __launch_bounds__(512)
 norm_forward_kernel(const NormFwd<T> p, int G) {
   __shared__ float slot[2][16];
@@ -238,12 +269,49 @@ norm_forward_kernel(const NormFwd<T> p, int G) {
   const int t = threadIdx.x % G, lane = threadIdx.x & 31;
   const long long col = static_cast<long long>(blockIdx.x) * (blockDim.x / G) + threadIdx.x / G;
   if (col >= p.cols) return;  // uniform over the group
-  const Philox gen(p.drop);
   float v[NV][8];
   float s = 0.f;
+  Piece<T, VEC> x[NV], q8[RES ? NV : 1];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) x[i].load(p.x + col * p.ldx, first_row<VEC>(i, G, t), p.rows);
+  if (RES && p.res != nullptr) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) q8[RES ? i : 0].load(p.res + col * p.ldres, first_row<VEC>(i, G, t), p.rows);
+  }
+  uint4 words[RES && VEC ? NV : 1];
+  uint32_t keep[RES && !VEC ? NV : 1];
+  const Philox gen(p.drop);
+  if (RES && p.drop.threshold != 0) {
+    const unsigned long long e0 = static_cast<unsigned long long>(col) * p.rows;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const long long r0 = first_row<VEC>(i, G, t);
+      if (VEC) words[RES && VEC ? i : 0] = gen.words((e0 + r0) >> 3);
+      else keep[RES && !VEC ? i : 0] = gen.keep_strided(e0 + (r0 - lane), lane);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    form_h<VEC>(p, gen, col, first_row<VEC>(i, G, t), lane, v[i]);
+    x[i].get(v[i]);
+    if (RES) {
+      if (p.drop.threshold != 0) {
+        if (VEC) {
+          gen.apply(words[RES && VEC ? i : 0], p.drop.factor, v[i]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[i][e] = (keep[RES && !VEC ? i : 0] >> e) & 1u ? v[i][e] * p.drop.factor : 0.f;
+        }
+      }
+      if (p.res != nullptr) {
+        float q[8];
+        q8[RES ? i : 0].get(q);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] += q[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = to_f(from_f<T>(v[i][e]));  // as it is stored
+      store_piece<VEC>(p.h + col * p.ldh, first_row<VEC>(i, G, t), p.rows, v[i]);
+    }
     s += ((v[i][0] + v[i][1]) + (v[i][2] + v[i][3])) + ((v[i][4] + v[i][5]) + (v[i][6] + v[i][7]));
   }
   const float mean = group_sum(s, G, t, slot[0]) / static_cast<float>(p.rows);
@@ -401,11 +469,12 @@ __device__ __forceinline__ void leave_partial(const NormBwd<T>& p, int G, int t,
 // Groups of G threads walk the columns; a thread meets the same rows in every column, so the
 // weight gradients stay in its registers until the end, where the groups of the CTA add theirs
 // through shared memory (2 x rows floats).
-// Columns off the 16-byte grid, and fp32 columns too long to hold twice, are loaded when their turn comes.
-template <typename T, bool VEC, int NV>
+// Columns off the 16-byte grid take it; they are loaded when their turn comes.
+template <typename T, int NV>
 __global__ void __launch_bounds__(512, 1)
 norm_backward_kernel(const NormBwd<T> p, int G) {
-  __shared__ float2 slot[2][16];
+  constexpr bool VEC = false;
+  __shared__ __align__(16) float2 slot[2][16];
   extern __shared__ float sums[];
   pdl_wait();
   pdl_launch_dependents();
@@ -464,69 +533,143 @@ norm_backward_kernel(const NormBwd<T> p, int G) {
   leave_partial<VEC, NV>(p, G, t, group, groups, sums, dg, db);
 }
 
-// The same with the next column's operands on their way while this one is worked on: a column's reduction
-// (a barrier behind two shuffles trees) waits for all of its loads, so without them the memory idles
-// between columns.  What is kept of a column is packed as it lies in memory.
-// The gain lies in shared memory as fp32 (behind the place of the weight sums).  DH: there is a gradient
-// from elsewhere.
+// The same for columns on the 16-byte grid, through a ring in shared memory: a column's reduction (a barrier
+// behind two shuffle trees) waits for all of its loads, so without the next columns on their way the memory
+// idles between two.  Every group has a ring of its own, filled by its first thread with one bulk copy per
+// operand; a stage is free once the group is through the barrier of the reduction, since what it holds is
+// in registers by then.  No registers are spent on what is still to come, and the bytes in flight are what
+// shared memory holds (two to eight columns).
+// Columns longer than 512 threads hold are shared by the CTAs of a cluster, each with a run of rows; they
+// exchange their column sums through each other's shared memory.
+// The gain lies in shared memory as fp32.  Places behind the last row are zeros that no copy overwrites, so
+// that reading takes no bounds.  DH: there is a gradient from elsewhere.
+// Shared memory serves a 16-byte access eight lanes at a time, and eight lanes 32 bytes apart meet in the same
+// banks.  fp32 pieces are therefore read with the two halves exchanged in every second four lanes, and stay in
+// that order in the registers; the gain lies as two arrays, the first and the second halves of the pieces.
+template <typename T>
+struct Order {  // Half: eight elements are one access
+  __device__ __forceinline__ explicit Order(int) {}
+  __device__ __forceinline__ int gain_part() const { return 0; }
+  template <typename P>
+  __device__ __forceinline__ void load(const P* p, float (&x)[8]) const { load8(p, x); }
+  template <typename P>
+  __device__ __forceinline__ void store(P* p, const float (&x)[8]) const { store8(p, x); }
+  __device__ __forceinline__ void read(const T* p, Raw8<T>& x) const { x.load(p); }
+  __device__ __forceinline__ uint4 words(const uint4 w) const { return w; }
+};
+template <>
+struct Order<float> {
+  int a;  // the half this lane holds first: offset 0 or 4
+  __device__ __forceinline__ explicit Order(int lane) : a(lane & 4) {}
+  __device__ __forceinline__ int gain_part() const { return a >> 2; }
+  __device__ __forceinline__ void load(const float* p, float (&x)[8]) const {
+    const float4 u = *reinterpret_cast<const float4*>(p + a), v = *reinterpret_cast<const float4*>(p + (a ^ 4));
+    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+    x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+  }
+  __device__ __forceinline__ void store(float* p, const float (&x)[8]) const {
+    *reinterpret_cast<float4*>(p + a) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + (a ^ 4)) = make_float4(x[4], x[5], x[6], x[7]);
+  }
+  __device__ __forceinline__ void read(const float* p, Raw8<float>& x) const {
+    x.a = *reinterpret_cast<const float4*>(p + a);
+    x.b = *reinterpret_cast<const float4*>(p + (a ^ 4));
+  }
+  __device__ __forceinline__ uint4 words(const uint4 w) const { return a ? make_uint4(w.z, w.w, w.x, w.y) : w; }
+};
+constexpr int kMaxBars = 64;
+struct NormRing {
+  int G, stages, cluster, run;  // run: rows per CTA of a cluster
+};
 template <typename T, int NV, bool DH>
 __global__ void __launch_bounds__(512, 1)
-norm_backward_ahead_kernel(const NormBwd<T> p, int G) {
-  __shared__ float2 slot[2][16];
-  extern __shared__ __align__(16) float sums[];
+norm_backward_ring_kernel(const NormBwd<T> p, const NormRing ring, int* __restrict__ status) {
+  __shared__ __align__(16) float2 slot[2][16], peers[2][8];
+  __shared__ __align__(8) uint64_t full[kMaxBars];
+  extern __shared__ __align__(16) float gain[];  // then the groups' rings, in the end the weight sums of several groups
+  constexpr int OPS = DH ? 3 : 2;
+  const int G = ring.G, groups = blockDim.x / G, group = threadIdx.x / G;
+  const int t = threadIdx.x % G, lane = threadIdx.x & 31;
+  const int rank = ring.cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int row0 = rank * ring.run, left = static_cast<int>(p.rows) - row0, rows = left < ring.run ? left : ring.run;
+  const int places = NV * kEl * G;  // rows a group holds
+  const uint32_t bytes = rows * static_cast<uint32_t>(sizeof(T)), pitch = places * static_cast<uint32_t>(sizeof(T));
+  T* mine = reinterpret_cast<T*>(gain + places) + static_cast<size_t>(group) * ring.stages * OPS * places;
+  uint64_t* bars = full + group * ring.stages;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < groups * ring.stages; ++i) mbar_init(smem_u32(&full[i]), 1);
+    fence_mbar_init();
+  }
+  for (int k = 0; k < ring.stages * OPS; ++k)
+    for (int r = rows + t; r < places; r += G) mine[static_cast<size_t>(k) * places + r] = from_f<T>(0.f);
   pdl_wait();
   pdl_launch_dependents();
-  const int groups = blockDim.x / G, group = threadIdx.x / G;
-  const int t = threadIdx.x % G, lane = threadIdx.x & 31, rows = static_cast<int>(p.rows);
-  const Philox gen(p.drop);
-  float* gain = sums + (p.partial != nullptr ? 2 * rows : 0);
-  for (int r = threadIdx.x; r < rows; r += blockDim.x) gain[r] = p.gain != nullptr ? to_f(p.gain[r]) : 1.f;
+  for (int r = threadIdx.x; r < places; r += blockDim.x)
+    gain[(r >> 3) * 4 + (r & 3) + ((r >> 2) & 1) * (places / 2)] = r < rows ? (p.gain != nullptr ? to_f(p.gain[row0 + r]) : 1.f) : 0.f;
   __syncthreads();
+  if (ring.cluster > 1) cluster_sync_all();  // every CTA of the cluster is there before one writes to it
+  const Philox gen(p.drop);
+  const Order<T> order(lane);
+  const long long first = static_cast<long long>(blockIdx.x / ring.cluster) * groups + group;
+  const long long step = static_cast<long long>(gridDim.x / ring.cluster) * groups;
+  auto issue = [&](long long col, int s) {
+    const uint32_t bar = smem_u32(&bars[s]), dst = smem_u32(mine + static_cast<size_t>(s) * OPS * places);
+    mbar_arrive_expect_tx(bar, OPS * bytes);
+    bulk_load(dst, p.h + col * p.ldh + row0, bytes, bar);
+    bulk_load(dst + pitch, p.dy + col * p.lddy + row0, bytes, bar);
+    if (DH) bulk_load(dst + 2 * pitch, p.dh + col * p.lddh + row0, bytes, bar);
+  };
+  if (t == 0)
+    for (int s = 0; s < ring.stages; ++s)
+      if (first + s * step < p.cols) issue(first + s * step, s);
+  // this thread's places in the results, moving on with the columns
+  T* dres = p.dres != nullptr ? p.dres + first * p.lddres + row0 + t * kEl : nullptr;
+  T* dx = p.dx != nullptr ? p.dx + first * p.lddx + row0 + t * kEl : nullptr;
+  const long long dres_step = p.dres != nullptr ? step * p.lddres : 0, dx_step = p.dx != nullptr ? step * p.lddx : 0;
   F2 dg[NV][4], db[NV][4];
-  Raw8<T> x[NV], y[NV], z[DH ? NV : 1];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) dg[i][e] = db[i][e] = F2(0.f);
   const float inv = 1.f / static_cast<float>(p.rows);
-  const long long step = static_cast<long long>(gridDim.x) * groups;
   float mean = 0.f, rstd = 0.f;
-  auto fetch = [&](long long col) {
-    if (col >= p.cols) return;
-    mean = p.mean[col];
-    rstd = p.rstd[col];
-    const T* h = p.h + col * p.ldh;
-    const T* dy = p.dy + col * p.lddy;
-    const T* dh = p.dh + col * p.lddh;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int r0 = (i * G + t) * kEl;
-      if (r0 < rows) {
-        x[i].load(h + r0);
-        y[i].load(dy + r0);
-        if (DH) z[i].load(dh + r0);
-      } else {
-        x[i].zero();
-        y[i].zero();
-        if (DH) z[i].zero();
-      }
+  if (first < p.cols) {
+    mean = p.mean[first];
+    rstd = p.rstd[first];
+  }
+  bool ok = true;
+  int s = 0, phase = 0, turn = 0;
+  for (long long col = first; col < p.cols; col += step, turn ^= 1) {
+    const float mean1 = mean, rstd1 = rstd;
+    if (col + step < p.cols) {
+      mean = p.mean[col + step];
+      rstd = p.rstd[col + step];
     }
-  };
-  long long col = static_cast<long long>(blockIdx.x) * groups + group;
-  fetch(col);
-  for (int turn = 0; col < p.cols; col += step, turn ^= 1) {
-    const F2 rs(rstd), shift(-mean * rstd);
-    const float rstd1 = rstd;
+    uint4 words[NV];
+    if (p.dx != nullptr && p.drop.threshold != 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        words[i] = order.words(gen.words((static_cast<unsigned long long>(col) * p.rows + row0 + (i * G + t) * kEl) >> 3));
+    }
+    // the kernel's waits have an end: a group that gave up goes on without its data
+    ok = ok && mbar_wait(smem_u32(&bars[s]), phase, status, DEV_TIMEOUT_FULL, 0x100);
+    const T* stage = mine + static_cast<size_t>(s) * OPS * places;
+    const F2 rs(rstd1), shift(-mean1 * rstd1);
     F2 xh[NV][4], g[NV][4], sx(0.f), sy(0.f);
-    Raw8<T> cz[DH ? NV : 1];
+    Raw8<T> z[DH ? NV : 1];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float a[8], b[8];
-      x[i].get(a);
-      y[i].get(b);
-      if (DH) cz[i] = z[i];
       const int r0 = (i * G + t) * kEl;
-      const float4* w = reinterpret_cast<const float4*>(gain + (r0 < rows ? r0 : 0));
+      Raw8<T> x, y;
+      order.read(stage + r0, x);
+      order.read(stage + places + r0, y);
+      if (DH) order.read(stage + 2 * places + r0, z[i]);
+      float a[8], b[8];
+      x.get(a);
+      y.get(b);
+      const float4* w = reinterpret_cast<const float4*>(gain) + (i * G + t);
+      const int half = places / 8, part = order.gain_part();
+      const float4 k[2] = {w[part * half], w[(part ^ 1) * half]};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         // (x - mean) rstd as one multiply-add: off by 2^-24 of |mean| rstd, as the subtraction's
@@ -535,45 +678,103 @@ norm_backward_ahead_kernel(const NormBwd<T> p, int G) {
         const F2 d(b[2 * e], b[2 * e + 1]);  // zero behind the last row
         dg[i][e] = fma2(d, xh[i][e], dg[i][e]);
         db[i][e] = add2(db[i][e], d);
-        const float4 k = w[e >> 1];
-        g[i][e] = mul2(d, e & 1 ? F2(k.z, k.w) : F2(k.x, k.y));
+        g[i][e] = mul2(d, e & 1 ? F2(k[e >> 1].z, k[e >> 1].w) : F2(k[e >> 1].x, k[e >> 1].y));
         sx = add2(sx, g[i][e]);
         sy = fma2(g[i][e], xh[i][e], sy);
       }
     }
-    fetch(col + step);
-    const float2 s = group_sum2(make_float2(sx.sum(), sy.sum()), G, t, slot[turn]);
-    // rstd (g - s.x / rows - xh s.y / rows)
-    const F2 c0(-rstd1 * s.x * inv), c1(-rstd1 * s.y * inv);
+    float2 sum = group_sum2(make_float2(sx.sum(), sy.sum()), G, t, slot[turn]);
+    if (t == 0 && ok && col + ring.stages * step < p.cols) issue(col + ring.stages * step, s);
+    if (++s == ring.stages) {
+      s = 0;
+      phase ^= 1;
+    }
+    if (ring.cluster > 1) {
+      if (threadIdx.x < ring.cluster) {
+        const uint32_t to = mapa_shared(smem_u32(&peers[turn][rank]), threadIdx.x);
+        st_shared_remote(to, __float_as_uint(sum.x));
+        st_shared_remote(to + 4, __float_as_uint(sum.y));
+      }
+      __syncwarp();
+      cluster_sync_all();
+      sum = make_float2(0.f, 0.f);
+      for (int k = 0; k < ring.cluster; ++k) {
+        sum.x += peers[turn][k].x;
+        sum.y += peers[turn][k].y;
+      }
+    }
+    // rstd (g - sum.x / rows - xh sum.y / rows)
+    const F2 c0(-rstd1 * sum.x * inv), c1(-rstd1 * sum.y * inv);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      const int r0 = (i * G + t) * kEl;
       float d[8], q[8];
-      if (DH) cz[i].get(q);
+      if (DH) z[i].get(q);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         F2 v = fma2(g[i][e], rs, fma2(xh[i][e], c1, c0));
         if (DH) v = add2(v, F2(q[2 * e], q[2 * e + 1]));
         v.get(d[2 * e], d[2 * e + 1]);
       }
-      write_out<true>(p, gen, col, (i * G + t) * kEl, lane, d);
+      if (r0 >= rows) continue;
+      if (dres != nullptr) {
+        T* to = dres + i * G * kEl;
+        if (p.accumulate) {
+          order.load(to, q);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) q[e] += d[e];
+          order.store(to, q);
+        } else {
+          order.store(to, d);
+        }
+      }
+      if (dx != nullptr) {
+        T* to = dx + i * G * kEl;
+        if (p.drop.threshold != 0) gen.apply(words[i], p.drop.factor, d);
+        if (p.accumulate) {
+          order.load(to, q);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[e] += q[e];
+        }
+        order.store(to, d);
+      }
+    }
+    dres += dres_step;
+    dx += dx_step;
+  }
+  if (p.partial == nullptr) return;
+  float* out = p.partial + static_cast<long long>(blockIdx.x / ring.cluster) * 2 * p.rows;
+  float* sums = gain + places;
+  // one group leaves its weight gradients directly, several add theirs in order first
+  for (int k = 0; k < groups; ++k) {
+    if (groups > 1) __syncthreads();  // the first time: the rings are done with
+    if (group != k) continue;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int r0 = (i * G + t) * kEl;
+      if (r0 >= rows) continue;
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        float v[8], q[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) (part ? db : dg)[i][e].get(v[2 * e], v[2 * e + 1]);
+        if (k > 0) {
+          order.load(sums + part * rows + r0, q);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += q[e];
+        }
+        order.store(k + 1 == groups ? out + part * p.rows + row0 + r0 : sums + part * rows + r0, v);
+      }
     }
   }
-  float sum_g[NV][8], sum_b[NV][8];
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      dg[i][e].get(sum_g[i][2 * e], sum_g[i][2 * e + 1]);
-      db[i][e].get(sum_b[i][2 * e], sum_b[i][2 * e + 1]);
-    }
-  leave_partial<true, NV>(p, G, t, group, groups, sums, sum_g, sum_b);
 }
 
 // Long columns: the column sums and the input's gradient in two sweeps, one CTA per column.
-template <typename T, bool VEC>
+template <typename T>
 __global__ void __launch_bounds__(512)
 norm_backward_long_kernel(const NormBwd<T> p) {
-  __shared__ float2 slot[16];
+  constexpr bool VEC = false;
+  __shared__ __align__(16) float2 slot[16];
   pdl_wait();
   pdl_launch_dependents();
   const int G = blockDim.x, t = threadIdx.x, lane = t & 31;
@@ -752,9 +953,51 @@ int group_size(long long rows, int nv) {
   return 0;
 }
 
-// Sweeps of eight rows per thread in the backward pass.  Half: two from 257 rows on; fp32: one as long as
-// 512 threads cover the column, since only then a second column fits in the registers beside the first.
-int backward_pieces(long long rows, int es) { return rows <= (es == 2 ? 256 : 4096) ? 1 : 2; }
+// How a backward pass is laid out.  Columns on the 16-byte grid go through the ring kernel, those longer
+// than 512 threads hold (16 rows each) on clusters of two to eight CTAs; other columns are loaded when their
+// turn comes, and longer ones take the kernels of two sweeps.
+struct NormPlan {
+  bool ring = false, two_sweeps = false;
+  int nv = 1, G = 0, cluster = 1, run = 0, stages = 0, parts = 0, smem = 0;
+};
+constexpr int kNormSmem = 225 * 1024;
+NormPlan plan_backward(const NormGradArgs& a, int es, int num_sms) {
+  NormPlan w;
+  const bool vec = a.rows % 8 == 0 && cols16(a.h, a.ldh, es, a.cols) && cols16(a.dy, a.lddy, es, a.cols) &&
+                   cols16(a.dh, a.lddh, es, a.cols) && cols16(a.dres, a.lddres, es, a.cols) &&
+                   cols16(a.dx, a.lddx, es, a.cols);
+  constexpr long long kHeld = 8192;  // rows that 512 threads hold, 16 each
+  while (vec && w.cluster < 8 && a.rows > kHeld * w.cluster) w.cluster *= 2;
+  if (a.rows > kHeld * w.cluster) {
+    w.two_sweeps = true;
+    // weight gradients: enough CTAs to fill the device with 256 rows each, at most 64 partial vectors
+    const long long row_blocks = (a.rows + 255) / 256;
+    long long parts = (4LL * num_sms + row_blocks - 1) / row_blocks;
+    parts = parts > 64 ? 64 : parts;
+    parts = parts > a.cols ? a.cols : parts;
+    const long long per = (a.cols + parts - 1) / parts;
+    w.parts = static_cast<int>((a.cols + per - 1) / per);
+    return w;
+  }
+  w.ring = vec;
+  w.run = static_cast<int>((a.rows / 8 + w.cluster - 1) / w.cluster * 8);
+  w.nv = a.rows <= (es == 2 ? 256 : 512) ? 1 : 2;
+  w.G = group_size(vec ? w.run : a.rows, w.nv);
+  const int groups = 512 / w.G;
+  const long long want = (a.cols + groups - 1) / groups, most = num_sms / w.cluster;
+  w.parts = static_cast<int>(want < most ? want : most);
+  if (!vec) {
+    w.smem = a.dgain != nullptr || a.dbias != nullptr ? static_cast<int>(2 * a.rows * sizeof(float)) : 0;
+    return w;
+  }
+  const int places = 8 * w.nv * w.G, stage = (a.dh != nullptr ? 3 : 2) * places * es * groups;
+  const int fixed = places * static_cast<int>(sizeof(float));
+  w.stages = (kNormSmem - fixed) / stage;
+  w.stages = w.stages > 8 ? 8 : w.stages;
+  w.stages = w.stages * groups > kMaxBars ? kMaxBars / groups : w.stages;
+  w.smem = fixed + w.stages * stage;
+  return w;
+}
 
 template <typename T, bool VEC>
 cudaError_t forward_tv(const NormFwd<T>& p, int num_sms, cudaStream_t stream) {
@@ -772,7 +1015,8 @@ cudaError_t forward_tv(const NormFwd<T>& p, int num_sms, cudaStream_t stream) {
   const int threads = G > 256 ? G : 256;
   const long long per = threads / G, grid = (p.cols + per - 1) / per;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
-  auto kern = nv == 1 ? norm_forward_kernel<T, VEC, 1> : nv == 2 ? norm_forward_kernel<T, VEC, 2> : norm_forward_kernel<T, VEC, 4>;
+  auto kern = nv == 1 ? norm_forward_kernel<T, VEC, 1, false> : nv == 2 ? norm_forward_kernel<T, VEC, 2, false> : norm_forward_kernel<T, VEC, 4, false>;
+  if (p.h != nullptr) kern = nv == 1 ? norm_forward_kernel<T, VEC, 1, true> : nv == 2 ? norm_forward_kernel<T, VEC, 2, true> : norm_forward_kernel<T, VEC, 4, true>;
   return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(threads), 0, stream, pdl_enabled(), p, G);
 }
 
@@ -798,37 +1042,8 @@ cudaError_t forward_t(const NormArgs& a, int num_sms, cudaStream_t stream) {
   return vec ? forward_tv<T, true>(p, num_sms, stream) : forward_tv<T, false>(p, num_sms, stream);
 }
 
-template <typename T, bool VEC>
-cudaError_t backward_tv(const NormBwd<T>& p, const NormGradArgs& a, int parts, cudaStream_t stream) {
-  if (a.rows > kNormRegisterRows) {
-    if (p.cols > 0x7fffffffLL) return cudaErrorInvalidValue;
-    if (p.partial != nullptr) {  // first: dx or dres may be written over dy
-      const long long per = (p.cols + parts - 1) / parts;
-      const cudaError_t e = launch_kernel(norm_weight_grad_kernel<T>,
-                                          dim3(static_cast<unsigned>((p.rows + 255) / 256), static_cast<unsigned>(parts)), dim3(256),
-                                          0, stream, pdl_enabled(), p, per);
-      if (e != cudaSuccess) return e;
-    }
-    if (p.dres == nullptr && p.dx == nullptr) return cudaSuccess;
-    return launch_kernel(norm_backward_long_kernel<T, VEC>, dim3(static_cast<unsigned>(p.cols)), dim3(512), 0, stream, pdl_enabled(), p);
-  }
-  const int nv = backward_pieces(p.rows, sizeof(T));
-  const int G = group_size(p.rows, nv);
-  auto kern = nv == 1 ? norm_backward_kernel<T, VEC, 1> : norm_backward_kernel<T, VEC, 2>;
-  constexpr int kTwo = sizeof(T) == 2 ? 2 : 1;  // fp32 columns of two sweeps do not fit twice
-  const bool ahead = VEC && nv <= kTwo, dh = p.dh != nullptr;
-  if (ahead && nv == 1) kern = dh ? norm_backward_ahead_kernel<T, 1, true> : norm_backward_ahead_kernel<T, 1, false>;
-  if (ahead && nv == 2) kern = dh ? norm_backward_ahead_kernel<T, kTwo, true> : norm_backward_ahead_kernel<T, kTwo, false>;
-  const int smem = static_cast<int>(((p.partial != nullptr ? 2 : 0) + (ahead ? 1 : 0)) * p.rows * sizeof(float));
-  static unsigned long long smem_set[8] = {};  // one per kernel of this template instantiation
-  cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern), 3 * kNormRegisterRows * static_cast<int>(sizeof(float)),
-                                      &smem_set[(nv - 1) * 4 + ahead * 2 + dh]);
-  if (e != cudaSuccess) return e;
-  return launch_kernel(kern, dim3(static_cast<unsigned>(parts)), dim3(512), smem, stream, pdl_enabled(), p, G);
-}
-
 template <typename T>
-cudaError_t backward_t(const NormGradArgs& a, int parts, float* partial, cudaStream_t stream) {
+cudaError_t backward_t(const NormGradArgs& a, float* partial, int num_sms, cudaStream_t stream, int* status) {
   NormBwd<T> p;
   p.h = static_cast<const T*>(a.h);
   p.gain = static_cast<const T*>(a.gain);
@@ -843,18 +1058,39 @@ cudaError_t backward_t(const NormGradArgs& a, int parts, float* partial, cudaStr
   p.rows = a.rows; p.cols = a.cols;
   p.accumulate = a.accumulate;
   p.drop = a.drop;
-  const int es = sizeof(T);
-  const bool vec = a.rows % 8 == 0 && cols16(a.h, a.ldh, es, a.cols) && cols16(a.dy, a.lddy, es, a.cols) &&
-                   cols16(a.dh, a.lddh, es, a.cols) && cols16(a.dres, a.lddres, es, a.cols) &&
-                   cols16(a.dx, a.lddx, es, a.cols) && cols16(a.gain, 0, es, 1);
-  if (a.cols > 0) {
-    cudaError_t e = vec ? backward_tv<T, true>(p, a, parts, stream) : backward_tv<T, false>(p, a, parts, stream);
+  const NormPlan w = plan_backward(a, sizeof(T), num_sms);
+  const bool weights = a.dgain != nullptr || a.dbias != nullptr;
+  cudaError_t e = cudaSuccess;
+  if (p.cols == 0) {
+    // weight gradients that are sums of nothing
+  } else if (w.two_sweeps) {
+    if (p.cols > 0x7fffffffLL) return cudaErrorInvalidValue;
+    if (weights)  // first: dx or dres may be written over dy
+      e = launch_kernel(norm_weight_grad_kernel<T>, dim3(static_cast<unsigned>((p.rows + 255) / 256), static_cast<unsigned>(w.parts)),
+                        dim3(256), 0, stream, pdl_enabled(), p, (p.cols + w.parts - 1) / w.parts);
+    if (e == cudaSuccess && (p.dres != nullptr || p.dx != nullptr))
+      e = launch_kernel(norm_backward_long_kernel<T>, dim3(static_cast<unsigned>(p.cols)), dim3(512), 0, stream, pdl_enabled(), p);
+  } else if (w.ring) {
+    const bool dh = p.dh != nullptr;
+    auto kern = w.nv == 1 ? (dh ? norm_backward_ring_kernel<T, 1, true> : norm_backward_ring_kernel<T, 1, false>)
+                          : (dh ? norm_backward_ring_kernel<T, 2, true> : norm_backward_ring_kernel<T, 2, false>);
+    static unsigned long long smem_set[4] = {};  // one per kernel of this template instantiation
+    e = set_smem_limit_once(reinterpret_cast<const void*>(kern), kNormSmem, &smem_set[(w.nv - 1) * 2 + dh]);
     if (e != cudaSuccess) return e;
+    const NormRing ring = {w.G, w.stages, w.cluster, w.run};
+    e = launch_cluster_kernel(kern, dim3(static_cast<unsigned>(w.parts * w.cluster)), dim3(512), static_cast<unsigned>(w.cluster), w.smem,
+                              stream, pdl_enabled(), p, ring, status);
+  } else {
+    auto kern = w.nv == 1 ? norm_backward_kernel<T, 1> : norm_backward_kernel<T, 2>;
+    static unsigned long long smem_set[2] = {};
+    e = set_smem_limit_once(reinterpret_cast<const void*>(kern), 2 * 8192 * static_cast<int>(sizeof(float)), &smem_set[w.nv - 1]);
+    if (e != cudaSuccess) return e;
+    e = launch_kernel(kern, dim3(static_cast<unsigned>(w.parts)), dim3(512), w.smem, stream, pdl_enabled(), p, w.G);
   }
-  if (a.dgain == nullptr && a.dbias == nullptr) return cudaSuccess;
+  if (e != cudaSuccess || !weights) return e;
   return launch_kernel(norm_weight_sum_kernel<T>, dim3(static_cast<unsigned>((a.rows + 31) / 32), 2), dim3(1024), 0, stream,
-                       pdl_enabled(), static_cast<const float*>(partial), a.cols > 0 ? parts : 0, a.rows,
-                       static_cast<T*>(a.dgain), static_cast<T*>(a.dbias), a.accumulate);
+                       pdl_enabled(), static_cast<const float*>(partial), w.parts, a.rows, static_cast<T*>(a.dgain),
+                       static_cast<T*>(a.dbias), a.accumulate);
 }
 
 template <typename T>
@@ -884,29 +1120,21 @@ cudaError_t dropout_t(const void* x, long long ldx, const void* add, long long l
 
 }  // namespace
 
-int norm_backward_parts(int dtype, long long rows, long long cols, int num_sms) {
-  if (cols <= 0) return 0;
-  if (rows > kNormRegisterRows) {
-    // enough CTAs to fill the device with 256 rows each, at most 64 partial vectors
-    const long long row_blocks = (rows + 255) / 256;
-    long long parts = (4LL * num_sms + row_blocks - 1) / row_blocks;
-    parts = parts > 64 ? 64 : parts;
-    parts = parts > cols ? cols : parts;
-    const long long per = (cols + parts - 1) / parts;
-    return static_cast<int>((cols + per - 1) / per);
-  }
-  const int groups = 512 / group_size(rows, backward_pieces(rows, dtype == 0 ? 4 : 2));
-  const long long want = (cols + groups - 1) / groups;
-  return static_cast<int>(want < num_sms ? want : num_sms);
+int norm_backward_parts(int dtype, const NormGradArgs& a, int num_sms, int* launches) {
+  const NormPlan w = plan_backward(a, dtype == 0 ? 4 : 2, num_sms);
+  const bool weights = a.dgain != nullptr || a.dbias != nullptr;
+  *launches = weights;
+  if (a.cols > 0) *launches += w.two_sweeps ? weights + (a.dres != nullptr || a.dx != nullptr) : 1;
+  return w.parts;
 }
 
 cudaError_t launch_norm_forward(int dtype, const NormArgs& a, int num_sms, cudaStream_t stream) {
   return dtype == 0 ? forward_t<float>(a, num_sms, stream) : forward_t<__half>(a, num_sms, stream);
 }
 
-cudaError_t launch_norm_backward(int dtype, const NormGradArgs& a, int parts, float* partial,
-                                 cudaStream_t stream) {
-  return dtype == 0 ? backward_t<float>(a, parts, partial, stream) : backward_t<__half>(a, parts, partial, stream);
+cudaError_t launch_norm_backward(int dtype, const NormGradArgs& a, float* partial, int num_sms, cudaStream_t stream,
+                                 int* status) {
+  return dtype == 0 ? backward_t<float>(a, partial, num_sms, stream, status) : backward_t<__half>(a, partial, num_sms, stream, status);
 }
 
 cudaError_t launch_dropout(int dtype, const void* x, long long ldx, const void* add, long long lda, void* y,
