@@ -1001,10 +1001,12 @@ NormPlan plan_backward(const NormGradArgs& a, int es, int num_sms) {
 
 template <typename T, bool VEC>
 cudaError_t forward_tv(const NormFwd<T>& p, int num_sms, cudaStream_t stream) {
-  // Rows per thread: 32 as long as one CTA covers the column that way; 16 off the 16-byte grid, where 32
-  // hold twice the registers (1001 x 5003 fp32: 28 us with 32).  Fewer where the columns alone would
-  // leave SMs idle: then a column's latency counts.
-  int nv = p.rows <= 256 ? 1 : p.rows <= 512 || (!VEC && p.rows <= 8192) ? 2 : 4;
+  // Rows per thread: 32 as long as one CTA covers the column that way; 16 off the 16-byte grid (1001 x 5003
+  // fp32: 28 us with 32) and for fp32 behind a residual connection (4096 x 8192: 95 us with 32, 86 with 16),
+  // where 32 hold too many registers.  Fewer where the columns alone would leave SMs idle: then a column's
+  // latency counts.
+  const bool many = !VEC || (sizeof(T) == 4 && p.h != nullptr);
+  int nv = p.rows <= 256 ? 1 : p.rows <= 512 || (many && p.rows <= 8192) ? 2 : 4;
   while (nv > 1 && p.rows <= 2048 * nv && p.cols * group_size(p.rows, nv) < 256LL * num_sms) nv /= 2;
   const int G = group_size(p.rows, nv);
   if (G == 0) {
