@@ -1,14 +1,15 @@
-// Half attention with a relative position bias whose scores never leave the SM.
+// Attention with a relative position bias whose scores never leave the SM: Half operands, and fp32 ones as
+// two Half planes each.
 //
-// Forward: one CTA serves two tiles of 128 queries of one head and walks that head's keys in tiles
-// of 128, once.  Query tile t has its scores S_t and its result O_t in tensor memory (128 lanes =
-// queries; 4 x 128 columns of fp32 in all); a group of 128 threads, one per query, turns S_t into
-// probabilities -- a row belongs to one thread, so the running maximum and sum need no exchange --
-// and writes them over S_t as the fp16 left operand of O_t += P_t V.  While one tile's threads
-// work, the tensor cores work on the other's products.
+// Forward: one CTA serves one or two tiles of 128 queries of one head and walks that head's keys in tiles
+// of 128, once.  Query tile t has its scores S_t and its result O_t in tensor memory (128 lanes = queries,
+// fp32); a group of 256 threads, two per query with half of the keys each, turns S_t into
+// probabilities -- a row's maximum takes one exchange between two threads -- and writes them over S_t as the
+// fp16 left operand of O_t += P_t V.  While one tile's (or another CTA's) threads work, the tensor cores
+// work on the other's products.
 //   warp 0        TMA: Q once, K and V tiles through rings of NST stages
 //   warp 1        tcgen05.mma: S_t = Q_t K^T (operands in shared memory), O_t += P_t V (P in tensor memory)
-//   warps 4-7     softmax of query tile 0,  warps 8-11  of query tile 1
+//   warps 4-11    softmax of query tile 0,  warps 12-19  of query tile 1
 // Products issued by one thread run in order, so S_t of the next key tile may be issued right
 // behind O_t += P_t V although it overwrites P_t.
 //
@@ -19,6 +20,10 @@
 // Bias: within a tile of 128 x 128 pairs the distances fall in a window of 255; when the whole
 // window lies beyond the reach (most tiles of a long sequence) its bias is one number, otherwise
 // the threads lay the window out in shared memory, where neighbouring rows read neighbouring words.
+//
+// What bounds it: the threads between the two products (16 heads of 4096 x 4096 x 128, causal: 68.7 GFLOP in
+// 90 us, 0.77 PFLOP/s, of 1.65 measured for a plain product), a row's exponentials, conversions and
+// tensor-memory traffic against 2 x 128 x 128 x head size operations of the tensor core.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cstring>
@@ -156,14 +161,19 @@ struct TileBias {
   }
 };
 
-// SPLIT: fp32 operands as two Half planes each (see split_planes_kernel).  NQ: query tiles per CTA, one
-// where two would not fit (128-wide split operands: 64 KB a tile); then K and V have one stage each,
-// which is loaded again while the other's product and the softmax run.
+// SPLIT: fp32 operands as two Half planes each (see split_planes_kernel).  NQ: query tiles per CTA.  One tile
+// of a 64-wide head leaves room for a second CTA on the SM (TWICE), whose start, loads and end then pass while
+// the first computes; a thread has 80 registers there, so it reads its scores twice, 32 at a time, once
+// for the maximum and once for the probabilities.  128-wide split operands (64 KB a tile) leave no room for
+// two tiles either way: K and V have one stage each, which is loaded again while the other's product and the
+// softmax run.
 template <int HS, int NST, int NQ, bool SPLIT>
-__global__ void __launch_bounds__(128 + 256 * NQ, 1)
+__global__ void __launch_bounds__(128 + 256 * NQ, NQ == 1 && HS == 64 ? 2 : 1)
 flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ status) {
   constexpr int WIDE = HS / 64;                  // 64-wide chunks of a plane
   constexpr int CHUNKS = (SPLIT ? 2 : 1) * WIDE;
+  constexpr bool TWICE = NQ == 1 && HS == 64;
+  constexpr int COLS = TWICE ? 256 : 512;
   constexpr int CROSS = NQ * HS;                 // tensor memory: from a tile's result to its cross terms
   constexpr int TILE = FCHUNK * CHUNKS;  // bytes of one operand tile
   constexpr float PSHIFT = SPLIT ? 7.f : 0.f;  // probabilities are formed times 2^PSHIFT: their low parts stay normal
@@ -201,7 +211,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
       fence_mbar_init();
     }
     __syncwarp();
-    tmem_alloc(smem_u32(&tmem_slot), 512);
+    tmem_alloc(smem_u32(&tmem_slot), COLS);
     tmem_relinquish();
     tc_fence_before();
   }
@@ -294,14 +304,14 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
           const uint32_t b = v_s + s * TILE;
 #pragma unroll
           for (int ks = 0; ks < FT / 16; ++ks) {
-            const uint32_t o = tmem + 2 * FT + t * HS, a = tmem + t * FT + (ks / 4) * 64 + (ks % 4) * 8;
+            const uint32_t o = tmem + NQ * FT + t * HS, a = tmem + t * FT + (ks / 2) * 32 + (ks % 2) * 8;
             const uint32_t add = (j > 0 || ks > 0) ? 1u : 0u;
             mma_f16_ts(o, a, make_smem_desc(b + ks * 2048, FCHUNK, 1024), IDESC_O, add);
             if (SPLIT) {
               // The cross terms have an accumulator of their own: the tensor core truncates when it adds, so
               // the long chain of the main one should be as short as it can be.
               mma_f16_ts(o + CROSS, a, make_smem_desc(b + WIDE * FCHUNK + ks * 2048, FCHUNK, 1024), IDESC_O, add);
-              mma_f16_ts(o + CROSS, a + 32, make_smem_desc(b + ks * 2048, FCHUNK, 1024), IDESC_O, 1u);
+              mma_f16_ts(o + CROSS, a + 16, make_smem_desc(b + ks * 2048, FCHUNK, 1024), IDESC_O, 1u);
             }
           }
           if (j == nt - 1) tc_commit(smem_u32(&o_full[t]));
@@ -327,7 +337,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
     const int i = i0 + t * FT + r;
     const int vis = hd.visible(p, i);
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t s_col = lanes + t * FT + half * 64, o_col = lanes + 2 * FT + t * HS + half * (HS / 2);
+    const uint32_t s_col = lanes + t * FT + half * 64, o_col = lanes + NQ * FT + t * HS + half * (HS / 2);
     const float* bias = p.bias != nullptr ? p.bias + hd.head * (2 * p.reach + 1) : nullptr;
     const int unit = hd.batch * p.kv_heads + hd.kv;
     const float c1 = SPLIT ? p.c1 * p.iq[unit] * p.ik[unit] : p.c1;
@@ -340,29 +350,34 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
       // a group that gave up still meets its barriers
       ok = ok && warp_wait(&s_full[t], j & 1, status, DEV_TIMEOUT_ACCUM, 0xc00 + t);
       float mn = -INFINITY;
-      uint32_t v[64];
+      const float* row = win + (FT - 1) - r + 64 * half;
+      const int lim = vis - j * FT - 64 * half;  // columns below it are seen
+      // 32 scores from column `from` on: raw ones with a flat bias, finished ones with a window
+      auto read = [&](int from, uint32_t* v) {
+        tmem_ld32(s_col + from, *reinterpret_cast<uint32_t(*)[32]>(v));
+        tmem_ld_wait();
+        if (tb.near) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(fmaf(__uint_as_float(v[c]), c1, row[from + c]));
+        }
+        if (__any_sync(0xffffffffu, lim < from + 32)) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) v[c] = from + c < lim ? v[c] : 0xff800000u;  // -inf
+        }
+      };
+      uint32_t v[TWICE ? 32 : 64];
       if (ok) {
         tc_fence_after();
-        tmem_ld32(s_col, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-        tmem_ld32(s_col + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-        tmem_ld_wait();
-        // raw scores with a flat bias, finished ones with a window
-        if (tb.near) {
-          const float* row = win + (FT - 1) - r + 64 * half;
-#pragma unroll
-          for (int c = 0; c < 64; ++c) v[c] = __float_as_uint(fmaf(__uint_as_float(v[c]), c1, row[c]));
-        }
-        const int lim = vis - j * FT - 64 * half;  // columns below it are seen
-        if (__any_sync(0xffffffffu, lim < 64)) {
-#pragma unroll
-          for (int c = 0; c < 64; ++c) v[c] = c < lim ? v[c] : 0xff800000u;  // -inf
-        }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 64; c += 8)
+        for (int part = 0; part < 2; ++part) {
+          uint32_t* x = v + (TWICE ? 0 : 32 * part);
+          read(32 * part, x);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            top[e] = fmaxf(top[e], fmaxf(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])));
+          for (int c = 0; c < 32; c += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])));
+        }
         mn = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         if (!tb.near && mn > -INFINITY) mn = fmaf(mn, c1, tb.value);
       }
@@ -395,18 +410,20 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         uint32_t w[16], low[16];
+        uint32_t* z = v + (TWICE ? 0 : c);
+        if (TWICE) read(c, z);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           float x, y;
-          fma2(F2(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])), ca2, cb2).get(x, y);
+          fma2(F2(__uint_as_float(z[2 * e]), __uint_as_float(z[2 * e + 1])), ca2, cb2).get(x, y);
           x = ex2(x);
           y = ex2(y);
           sum[e & 1] = add2(sum[e & 1], F2(x, y));
           if (SPLIT) split_pair(x, y, w[e], low[e]);
           else w[e] = pack_half2(x, y);
         }
-        tmem_st16(s_col + c / 2, w);  // over scores this thread has read
-        if (SPLIT) tmem_st16(s_col + 32 + c / 2, low);
+        tmem_st16(s_col + c, w);  // over scores this thread is done with
+        if (SPLIT) tmem_st16(s_col + c + 16, low);
       }
       float sa, sb;
       add2(sum[0], sum[1]).get(sa, sb);
@@ -453,7 +470,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, COLS);
   }
 }
 
@@ -1816,9 +1833,13 @@ bool flash_supported(const FlashArgs& a) {
 cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* status) {
   FlashParams p;
   if (!fill_params(a, &p)) return cudaErrorInvalidValue;
-  if (a.inverse != nullptr)
-    return a.hs <= 64 ? forward_hs<64, 2, 2, true>(p, stream, status) : forward_hs<128, 1, 1, true>(p, stream, status);
-  return a.hs <= 64 ? forward_hs<64, 3, 2, false>(p, stream, status) : forward_hs<128, 2, 2, false>(p, stream, status);
+  if (a.inverse != nullptr)  // 64 wide, two tiles with two stages each: 16 heads of 2048 x 2048, causal, 103 us; one tile 85
+    return a.hs <= 64 ? forward_hs<64, 1, 1, true>(p, stream, status) : forward_hs<128, 1, 1, true>(p, stream, status);
+  if (a.hs > 64) return forward_hs<128, 2, 2, false>(p, stream, status);
+  // Half, 64 wide: CTAs of one query tile where their work is uneven or short (16 heads of 2048 x 2048, causal:
+  // 42 us with two tiles, 36 with one; 512 of 128 x 128: 25 and 21), of two where every tile walks all keys,
+  // which are then read half as often (16 of 2048 x 2048, not causal: 43 and 46).
+  return a.causal || a.tq <= FT ? forward_hs<64, 2, 1, false>(p, stream, status) : forward_hs<64, 3, 2, false>(p, stream, status);
 }
 
 long long flash_packed(int hs, long long t, long long heads, long long batch) {
