@@ -1163,6 +1163,7 @@ struct FlashBwdParams {
   const float *iq, *ik, *iv, *ido;  // split operands: inverse scales, [batch][kv heads]
   int tq, tk, hs, heads, kv_heads, group, batch, tq_pad, row_tiles, width;
   int vec_dq, vec_dk, vec_dv;       // the results' rows allow 16-byte accesses
+  int delta_keys;                   // Half: most keys a tile sees whose delta is corrected
   long long reach, q_offset;
   const int* q_offsets;
   const int* q_lengths;
@@ -1280,9 +1281,11 @@ flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long lon
 // as large as v, in queries that see few keys (two keys: 5.1e-4 of dq instead of 2.9e-4; 500 keys: 3.0e-4);
 // for fp32 it is the truncation of o's long accumulation, which the table's gradient, whose terms all
 // but cancel, shows several times enlarged (1313 keys: 6.6e-6).  So Half tiles that see at most
-// kDeltaHalf keys and fp32 tiles that see more than kDeltaSplit take the two extra products.
+// kDeltaHalf keys, kDeltaTable where the table's gradient is wanted (500 keys: up to 3.3e-4 instead of the
+// 2.0e-4 of its own rounding), and fp32 tiles that see more than kDeltaSplit take the two extra products
+// (8 x 16 heads of 500 x 500: 18 us of 135).
 enum FlashMode { KEYS_BOTH = 0, QUERIES = 1, KEYS_DK = 2, KEYS_DV = 3, DELTA = 4 };
-constexpr int kDeltaHalf = 256, kDeltaSplit = 512;
+constexpr int kDeltaHalf = 256, kDeltaTable = 512, kDeltaSplit = 512;
 
 // What a CTA works on: 128 rows of one head of one sequence, and the streamed tiles first .. first + per - 1
 // of every query head of the group.
@@ -1315,7 +1318,7 @@ struct FlashBwdTile {
     } else if (r0 < qlen) {
       const int last = r0 + FT - 1 < qlen - 1 ? r0 + FT - 1 : qlen - 1;
       per = (rel_visible(p.causal, last + off, klen) + BN - 1) / BN;
-      if (MODE == DELTA && (SPLIT ? per <= kDeltaSplit / BN : per > kDeltaHalf / BN)) per = 0;
+      if (MODE == DELTA && (SPLIT ? per <= kDeltaSplit / BN : per > p.delta_keys / BN)) per = 0;
     }
   }
 };
@@ -2042,12 +2045,13 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
   // query tiles, from the first on, that may qualify for the correction of delta
   p.delta = reinterpret_cast<float2*>(stats);
   p.row_tiles = qtiles;
+  p.delta_keys = dist != nullptr ? kDeltaTable : kDeltaHalf;
   if (split) {
     if (a.tk <= kDeltaSplit) p.row_tiles = 0;
-  } else if (a.k_lengths == nullptr && a.tk > kDeltaHalf) {
+  } else if (a.k_lengths == nullptr && a.tk > p.delta_keys) {
     if (!a.causal) p.row_tiles = 0;
     if (a.causal && a.q_offsets == nullptr) {
-      const long long tiles = (kDeltaHalf - a.q_offset + FT - 1) / FT;
+      const long long tiles = (p.delta_keys - a.q_offset + FT - 1) / FT;
       p.row_tiles = tiles < 0 ? 0 : tiles < qtiles ? static_cast<int>(tiles) : qtiles;
     }
   }
