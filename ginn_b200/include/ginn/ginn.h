@@ -3,8 +3,11 @@
 #define GINN_B200_HOST_GINN_H
 #include <ginn/autobatch.h>
 #include <ginn/node/affine.h>
+#include <ginn/node/attention.h>
 #include <ginn/node/conv.h>
 #include <ginn/node/data.h>
+#include <ginn/node/dropout.h>
+#include <ginn/node/layernorm.h>
 #include <ginn/node/lstmcell.h>
 #include <ginn/node/nlnode.h>
 #include <ginn/node/pick.h>
