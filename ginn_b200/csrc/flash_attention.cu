@@ -112,7 +112,7 @@ struct FlashParams {
   const float *iq, *ik, *iv;  // split operands: inverse scales, [batch][kv heads]
   int tq, tk, hs, heads, kv_heads, group, batch, qblocks;
   int vec;                    // the result's rows allow 16-byte accesses
-  long long reach, q_offset;
+  int reach, q_offset;
   const int* q_offsets;
   const int* q_lengths;
   const int* k_lengths;
@@ -122,8 +122,7 @@ struct FlashParams {
 
 // What one (sequence, head) looks like to every role of a CTA.
 struct FlashHead {
-  int batch, head, kv, qlen, klen;
-  long long off;
+  int batch, head, kv, qlen, klen, off;
   __device__ __forceinline__ FlashHead(const FlashParams& p, int hb) {
     batch = hb / p.heads;
     head = hb - batch * p.heads;
@@ -148,13 +147,13 @@ struct FlashHead {
 struct TileBias {
   float value = 0.f;
   bool near = false;
-  __device__ __forceinline__ TileBias(const float* bias, long long reach, long long dlo, int gt, float* window,
+  __device__ __forceinline__ TileBias(const float* bias, int reach, int dlo, int gt, float* window,
                                       bool flat_ok) {
     if (flat_ok && (bias == nullptr || dlo >= reach || dlo + 254 <= -reach)) {
       if (bias != nullptr) value = __ldg(bias + (dlo >= reach ? 2 * reach : 0));
     } else {
       near = true;
-      long long d = dlo + gt;
+      int d = dlo + gt;
       d = d > reach ? reach : d < -reach ? -reach : d;
       window[gt] = bias != nullptr ? __ldg(bias + d + reach) : 0.f;
     }
@@ -338,14 +337,14 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
     const int vis = hd.visible(p, i);
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_col = lanes + t * FT + half * 64, o_col = lanes + NQ * FT + t * HS + half * (HS / 2);
-    const float* bias = p.bias != nullptr ? p.bias + hd.head * (2 * p.reach + 1) : nullptr;
+    const float* bias = p.bias != nullptr ? p.bias + static_cast<long long>(hd.head) * (2 * p.reach + 1) : nullptr;
     const int unit = hd.batch * p.kv_heads + hd.kv;
     const float c1 = SPLIT ? p.c1 * p.iq[unit] * p.ik[unit] : p.c1;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nt; ++j) {
       float* win = window[t][j & 1];
-      const TileBias tb(bias, p.reach, static_cast<long long>(j) * FT - (i0 + t * FT + FT - 1 + hd.off), gt, win, c1 > 0.f);
+      const TileBias tb(bias, p.reach, j * FT - (i0 + t * FT + FT - 1 + hd.off), gt, win, c1 > 0.f);
       if (tb.near) group_barrier(1 + t);
       // a group that gave up still meets its barriers
       ok = ok && warp_wait(&s_full[t], j & 1, status, DEV_TIMEOUT_ACCUM, 0xc00 + t);
@@ -690,7 +689,7 @@ struct TokenParams {
   const float* bias;
   int tq, tk, hs, heads, kv_heads, group, batch, rows, splits, chunk;
   int vec_q, vec_k, vec_v;  // fp32: rows allow 16-byte accesses
-  long long reach, q_offset;
+  int reach, q_offset;
   const int* q_offsets;
   const int* q_lengths;
   const int* k_lengths;
@@ -725,9 +724,8 @@ __device__ __forceinline__ void token_store(const TokenParams& p, int batch, int
 // What a lane knows of its two rows of the scores, g and g + 8, and of its CTA's keys.
 struct TokenLane {
   int warp, lane, g, c, split, batch, kv, begin, end;
-  long long unit, first_pos;
-  int vis[2];
-  long long pos[2];
+  long long unit;
+  int first_pos, vis[2], pos[2];
   const float* bias[2];
   float far_lo[2];
   float m[2], l[2];
@@ -751,7 +749,7 @@ struct TokenLane {
       bias[x] = nullptr;
       far_lo[x] = 0.f;
       if (p.bias != nullptr && real) {
-        bias[x] = p.bias + head * (2 * p.reach + 1) + p.reach;
+        bias[x] = p.bias + static_cast<long long>(head) * (2 * p.reach + 1) + p.reach;
         far_lo[x] = bias[x][-p.reach];
       }
       m[x] = -INFINITY;
@@ -783,7 +781,7 @@ struct TokenLane {
           const int key = j + 8 * t + 2 * c + y;
           float b = far_lo[x];
           if (!flat && bias[x] != nullptr) {
-            long long d = key - pos[x];
+            int d = key - pos[x];
             d = d > p.reach ? p.reach : d < -p.reach ? -p.reach : d;
             b = bias[x][d];
           }
@@ -1164,7 +1162,7 @@ struct FlashBwdParams {
   int tq, tk, hs, heads, kv_heads, group, batch, tq_pad, row_tiles, width;
   int vec_dq, vec_dk, vec_dv;       // the results' rows allow 16-byte accesses
   int delta_keys;                   // Half: most keys a tile sees whose delta is corrected
-  long long reach, q_offset;
+  int reach, q_offset;
   const int* q_offsets;
   const int* q_lengths;
   const int* k_lengths;
@@ -1291,8 +1289,7 @@ constexpr int kDeltaHalf = 256, kDeltaTable = 512, kDeltaSplit = 512;
 // of every query head of the group.
 template <int MODE, bool SPLIT>
 struct FlashBwdTile {
-  int tile, batch, head, kv, r0, qlen, klen, first = 0, per = 0;
-  long long off;
+  int tile, batch, head, kv, r0, qlen, klen, off, first = 0, per = 0;
   __device__ __forceinline__ explicit FlashBwdTile(const FlashBwdParams& p) {
     constexpr bool KEYS = MODE != QUERIES && MODE != DELTA;
     // the CTAs with the most work first: under a causal mask the first keys and the last queries
@@ -1308,10 +1305,10 @@ struct FlashBwdTile {
     off = rel_offset(p.q_offset, p.q_offsets, batch);
     if (KEYS) {
       if (r0 < klen && qlen > 0) {
-        long long i = p.causal ? r0 - off : 0;  // the first query that sees key r0
+        int i = p.causal ? r0 - off : 0;  // the first query that sees key r0
         i = i < 0 ? 0 : i;
         if (i < qlen) {
-          first = static_cast<int>(i / BN);
+          first = i / BN;
           per = (qlen + BN - 1) / BN - first;
         }
       }
@@ -1319,6 +1316,19 @@ struct FlashBwdTile {
       const int last = r0 + FT - 1 < qlen - 1 ? r0 + FT - 1 : qlen - 1;
       per = (rel_visible(p.causal, last + off, klen) + BN - 1) / BN;
       if (MODE == DELTA && (SPLIT ? per <= kDeltaSplit / BN : per > p.delta_keys / BN)) per = 0;
+    }
+  }
+};
+
+// Number `it` of the streamed tiles as (query head of the group, tile), without a division per tile.
+struct StreamWalk {
+  int tile, head = 0, per;
+  __device__ __forceinline__ StreamWalk(int it, int per_head) : tile(it), per(per_head) { next(0); }
+  __device__ __forceinline__ void next(int by) {
+    tile += by;
+    while (per > 0 && tile >= per) {
+      tile -= per;
+      ++head;
     }
   }
 };
@@ -1381,8 +1391,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
 
   const FlashBwdTile<MODE, SPLIT> w(p);
   const int tile = w.tile, batch = w.batch, head = w.head, kv = w.kv, r0 = w.r0, qlen = w.qlen, klen = w.klen;
-  const int first = w.first, per = w.per;
-  const long long off = w.off;
+  const int first = w.first, per = w.per, off = w.off;
   const int n = per * (KEYS ? p.group : 1);
 
   if (warp == 0) {
@@ -1394,11 +1403,12 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
         tma_load_4d(a1_s + c * FCHUNK, KEYS ? &p.tmK : &p.tmQ, smem_u32(&rows_full), x, r0, head, plane);
         tma_load_4d(a2_s + c * FCHUNK, KEYS ? &p.tmV : &p.tmDO, smem_u32(&rows_full), x, r0, head, plane);
       }
-      for (int it = 0; it < n; ++it) {
+      StreamWalk walk(0, per);
+      for (int it = 0; it < n; ++it, walk.next(1)) {
         const int s = it % BSTAGES;
         if (!mbar_wait(smem_u32(&b_empty[s]), ((it / BSTAGES) & 1) ^ 1u, status, DEV_TIMEOUT_EMPTY, 0xd00)) break;
         const uint32_t bar = smem_u32(&b_full[s]), dst = b_s + s * 2 * TILE;
-        const int at = (first + it % per) * BN, h = KEYS ? head * p.group + it / per : kv;
+        const int at = (first + walk.tile) * BN, h = KEYS ? head * p.group + walk.head : kv;
         mbar_arrive_expect_tx(bar, 2 * TILE);
         for (int c = 0; c < CHUNKS; ++c) {
           const int x = 64 * (c % WIDE), plane = batch + c / WIDE * p.batch;
@@ -1415,8 +1425,10 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     const bool leader = elect_one();
     const int blen = KEYS ? qlen : klen, bt = KEYS ? p.tq : p.tk;
     bool ok = n == 0 || warp_wait(&rows_full, 0, status, DEV_TIMEOUT_FULL, 0xe00);
-    auto scores = [&](int it) {
-      const int s = it % BSTAGES, at = (first + it % per) * BN;
+    StreamWalk walk(0, per);
+    auto scores = [&](int it) {  // called for one tile after the other
+      const int s = it % BSTAGES, at = (first + walk.tile) * BN;
+      walk.next(1);
       ok = warp_wait(&b_full[s], (it / BSTAGES) & 1, status, DEV_TIMEOUT_FULL, 0xe01);
       if (!ok) return;
       tc_fence_after();
@@ -1497,7 +1509,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       mine = p.stats[(static_cast<long long>(batch) * p.heads + head) * p.tq_pad + row];
       vis = row < qlen ? rel_visible(p.causal, row + off, klen) : 0;
     }
-    const long long low = KEYS ? 0 : rel_dist_low(p.reach, r0 + FT - 1 + off);
+    const int low = KEYS ? 0 : static_cast<int>(rel_dist_low(p.reach, r0 + FT - 1 + off));
     float* dist = nullptr;
     float far_lo = 0.f, far_hi = 0.f;
     if (dist_on) {
@@ -1507,12 +1519,13 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       group_barrier(1 + g);
     }
     bool ok = true;
-    for (int it = g; it < n; it += 2) {
-      const int at = (first + it % per) * BN, turn = (it >> 1) & 1;
-      const int h = KEYS ? head * p.group + it / per : head;
-      const float* bias = p.bias != nullptr ? p.bias + h * (2 * p.reach + 1) : nullptr;
+    StreamWalk walk(g, per);
+    for (int it = g; it < n; it += 2, walk.next(2)) {
+      const int at = (first + walk.tile) * BN, turn = (it >> 1) & 1;
+      const int h = KEYS ? head * p.group + walk.head : head;
+      const float* bias = p.bias != nullptr ? p.bias + static_cast<long long>(h) * (2 * p.reach + 1) : nullptr;
       // distances of the tile's pairs: dlo .. dlo + 190
-      const long long dlo = KEYS ? r0 - (at + BN - 1 + off) : at - (r0 + FT - 1 + off);
+      const int dlo = KEYS ? r0 - (at + BN - 1 + off) : at - (r0 + FT - 1 + off);
       // one number for the whole tile (a masked score is -inf before it is scaled: c1 > 0), or a window
       const bool beyond = dlo >= p.reach || dlo + FT + BN - 2 <= -p.reach;
       const bool flat = c1 > 0.f && (bias == nullptr || beyond);
@@ -1521,7 +1534,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       if (flat) {
         if (bias != nullptr) value = __ldg(bias + (dlo >= p.reach ? 2 * p.reach : 0));
       } else {
-        long long d = dlo + gt;
+        int d = dlo + gt;
         d = d > p.reach ? p.reach : d < -p.reach ? -p.reach : d;
         win[gt] = bias != nullptr ? __ldg(bias + d + p.reach) : 0.f;
       }
@@ -1541,8 +1554,8 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       if (KEYS) {
         hi = row < klen ? 32 : 0;
         if (p.causal) {
-          const long long from = row - off - at - 32 * half;
-          lo = from < 0 ? 0 : from > 32 ? 32 : static_cast<int>(from);
+          const int from = row - off - at - 32 * half;
+          lo = from < 0 ? 0 : from > 32 ? 32 : from;
         }
       } else {
         hi = vis - at - 32 * half;
@@ -1647,7 +1660,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
               const int dg = w - (FT - 1) + 32 * (q & 3) - 32 * (q >> 2);  // e - lane
               if (dg >= -31 && dg <= 31) sum += diag[KEYS ? 0 : g * 8 + q][dg <= 0 ? dg + 31 : 32 + 31 - dg];
             }
-            const long long d = dlo + w;
+            const int d = dlo + w;
             if (d >= p.reach) far_hi += sum;
             else if (d <= -p.reach) far_lo += sum;
             else if (d - low < p.width) dist[d - low] += sum;  // behind the last key: nothing, and no place

@@ -28,13 +28,16 @@ __device__ __forceinline__ int rel_length(const int* lengths, int batch, int t) 
   const int n = lengths[batch];
   return n < 0 ? 0 : n < t ? n : t;
 }
-__device__ __forceinline__ long long rel_offset(long long offset, const int* offsets, int batch) {
-  return offsets != nullptr ? offsets[batch] : offset;
+// Offsets are held within +-2^30, whatever the device array says, and tensors end before 2^29: positions and
+// distances are ints.
+__device__ __forceinline__ int rel_offset(long long offset, const int* offsets, int batch) {
+  const int x = offsets != nullptr ? offsets[batch] : static_cast<int>(offset);
+  return x > (1 << 30) ? 1 << 30 : x < -(1 << 30) ? -(1 << 30) : x;
 }
 // Number of keys 0 .. n - 1 the query at position `pos` sees.
-__device__ __forceinline__ int rel_visible(int causal, long long pos, int klen) {
+__device__ __forceinline__ int rel_visible(int causal, int pos, int klen) {
   if (!causal || pos >= klen - 1) return klen;
-  return pos < 0 ? 0 : static_cast<int>(pos) + 1;
+  return pos < 0 ? 0 : pos + 1;
 }
 
 // Keys 0 .. n - 1 of a sequence that some query sees: under a causal mask those behind the last query's
@@ -43,8 +46,8 @@ template <typename P>
 __device__ __forceinline__ int rel_keys(const P& p, int batch) {
   const int klen = rel_length(p.k_lengths, batch, p.tk);
   if (!p.causal) return klen;
-  const long long last = rel_length(p.q_lengths, batch, p.tq) + rel_offset(p.q_offset, p.q_offsets, batch);
-  return last >= klen ? klen : last < 0 ? 0 : static_cast<int>(last);
+  const int last = rel_length(p.q_lengths, batch, p.tq) + rel_offset(p.q_offset, p.q_offsets, batch);
+  return last >= klen ? klen : last < 0 ? 0 : last;
 }
 // What rel_keys reads, for the passes that need nothing else of the attention.
 struct RelExtent {
@@ -80,7 +83,7 @@ inline int rel_dist_width(long long reach, long long tk, int rows) {
 struct RelQuery {
   long long matrix, local;  // within the scores of this call
   int batch, head, query, visible;
-  long long pos;            // its position in keys
+  int pos;                  // its position in keys
   __device__ __forceinline__ RelQuery(const RelScores& s, long long col) {
     matrix = col / s.nq;
     local = col - matrix * s.nq;
