@@ -1520,6 +1520,12 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     }
     bool ok = true;
     StreamWalk walk(g, per);
+    // statistics of a streamed query, loaded a tile ahead: the group's barrier waits for them
+    auto stat = [&](const StreamWalk& w) {
+      return p.stats[(static_cast<long long>(batch) * p.heads + head * p.group + w.head) * p.tq_pad + (first + w.tile) * BN + gt];
+    };
+    float2 ahead = make_float2(0.f, 0.f);
+    if (KEYS && gt < BN && g < n) ahead = stat(walk);
     for (int it = g; it < n; it += 2, walk.next(2)) {
       const int at = (first + walk.tile) * BN, turn = (it >> 1) & 1;
       const int h = KEYS ? head * p.group + walk.head : head;
@@ -1540,7 +1546,12 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       }
       if (KEYS && gt < BN) {
         // per column: what is added to the scaled score, and to Y times f
-        const float2 st = p.stats[(static_cast<long long>(batch) * p.heads + h) * p.tq_pad + at + gt];
+        const float2 st = ahead;
+        if (it + 2 < n) {
+          StreamWalk then = walk;
+          then.next(2);
+          ahead = stat(then);
+        }
         const bool alone = rel_visible(p.causal, at + gt + off, klen) <= 1;
         colx[KEYS ? g : 0][turn][gt] = (flat ? value : 0.f) + PSHIFT - st.x;
         coly[KEYS ? g : 0][turn][gt] = alone ? 0.f : -st.y * f;
