@@ -325,6 +325,41 @@ def test_captured_step_draws_a_new_mask_at_every_replay(gpu):
                            np.float32, mask=mask)
 
 
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("rows", [9000, 40000, 70000])
+def test_long_columns_in_place_and_captured(gpu, dt, rows):
+    """Columns shared by the CTAs of a cluster and those of two sweeps: y over x, and the backward pass in a graph
+    beside an eager one, same bits."""
+    rng = np.random.default_rng(rows)
+    cols = 90
+    x, dy, gain, bias = data(rng, rows, cols, dt), data(rng, rows, cols, dt), rng.standard_normal(rows).astype(dt), rng.standard_normal(rows).astype(dt)
+    X, DY, G, Bi = B.from_host(x), B.from_host(dy), B.from_host(gain), B.from_host(bias)
+    Y, M, R = B.from_host(x), torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+    gpu.layer_norm_forward(Y, G, Bi, Y, M, R)
+    check_forward(x, gain, bias, host(Y), host(M), host(R), dt)
+
+    def results():
+        return B.colmajor(rows, cols, X.dtype), torch.empty(rows, dtype=X.dtype, device="cuda"), torch.empty(rows, dtype=X.dtype, device="cuda")
+
+    eager, captured = results(), results()
+    gpu.layer_norm_backward(X, G, M, R, DY, *eager, accumulate=False)
+    check_backward(x, gain, host(M), host(R), dy, dict(dres=host(eager[0]), dgain=host(eager[1]), dbias=host(eager[2])), dt)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gpu.layer_norm_backward(X, G, M, R, DY, *captured, accumulate=False)
+    other = torch.cuda.Stream()
+    again = results()
+    for _ in range(3):
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(other):
+            gpu.layer_norm_backward(X, G, M, R, DY, *again, accumulate=False)
+    torch.cuda.synchronize()
+    for a, b, c in zip(eager, captured, again):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
 def test_two_streams_at_once(gpu):
     """Calls on two streams share no scratch."""
     rng = np.random.default_rng(10)

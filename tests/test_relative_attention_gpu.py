@@ -286,6 +286,27 @@ def test_keys_that_no_query_sees_yet_are_not_looked_at(gpu, dt, hs, tq, tk, offs
 
 
 @pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("hs,tq,tk", [(64, 200, 300), (128, 150, 150), (64, 1, 500), (160, 20, 30)])
+def test_negative_and_zero_scale(gpu, dt, hs, tq, tk):
+    """A negative scale is the positive one with q negated, which is exact; a scale of zero leaves the bias."""
+    c = Case(dt, hs, tq, tk, causal=True, offsets=tk - tq)
+    ref, tol = c.reference()
+    c.q = -c.q
+    c.upload()
+    c.kw["scale"] = -c.scale
+    c.forward(gpu)
+    c.backward(gpu)
+    compare("o", c.O, ref["o"], tol["o"])
+    compare("dq", c.DQ, -ref["dq"], tol["dq"])
+    for n, got in (("dk", c.DK), ("dv", c.DV), ("dtable", c.DT)):
+        compare(n, got, ref[n], tol[n])
+    c = Case(dt, hs, tq, tk, causal=True, offsets=tk - tq)
+    c.scale = 0.0
+    check(gpu, c)
+    assert (c.DQ == 0).all() and (c.DK == 0).all()
+
+
+@pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("hs,tq,tk", [(64, 40, 300), (128, 1, 700), (192, 20, 50)])
 def test_what_is_not_a_number_stays_one(gpu, dt, hs, tq, tk):
     """A key that is not a number reaches every query that sees it, in o, lse and dq; a query that is not one
