@@ -1167,6 +1167,7 @@ struct FlashBwdParams {
   const float *iq, *ik, *iv, *ido;  // split operands: inverse scales, [batch][kv heads]
   int tq, tk, hs, heads, kv_heads, group, batch, tq_pad, row_tiles, width;
   int vec_dq, vec_dk, vec_dv;       // the results' rows allow 16-byte accesses
+  int wait_late;                    // the launch before this one is another of the same pass, see the kernel
   int delta_keys;                   // Half: most keys a tile sees whose delta is corrected
   int reach, q_offset;
   const int* q_offsets;
@@ -1339,6 +1340,9 @@ struct StreamWalk {
   }
 };
 
+// The launches of one pass behind the first are independent of it: dQ needs nothing of dK and dV.  They begin when
+// the CTAs of the one before have all begun (which wait for what both read), fill the SMs that its last wave leaves
+// idle, and wait for its end at theirs (wait_late), so that whoever waits for the last launch waits for all.
 template <int HS, int MODE, int BSTAGES, bool SPLIT>
 __global__ void __launch_bounds__(FTHREADS, 1)
 flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict__ status) {
@@ -1392,7 +1396,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  pdl_wait();
+  if (!p.wait_late) pdl_wait();
   pdl_launch_dependents();
 
   const FlashBwdTile<MODE, SPLIT> w(p);
@@ -1758,6 +1762,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (p.wait_late) pdl_wait();
 }
 
 bool heads_aligned(const FlashOperand& x, long long t, long long heads, long long batch) {
@@ -1837,6 +1842,11 @@ cudaError_t backward_any(const FlashBwdParams& p, bool split, cudaStream_t strea
   }
   if (split) return backward_hs<64, MODE, 4, true>(p, stream, status);
   return p.hs <= 64 ? backward_hs<64, MODE, 4, false>(p, stream, status) : backward_hs<128, MODE, 4, false>(p, stream, status);
+}
+
+template <int MODE>
+cudaError_t backward_wide(const FlashBwdParams& p, bool, cudaStream_t stream, int* status) {
+  return backward_hs<128, MODE, 1, true>(p, stream, status);
 }
 
 cudaError_t prepare(const FlashArgs& a, const FlashGradArgs& g, const FlashBwdParams& p, float* stats, float* norms, int qparts,
@@ -2093,26 +2103,17 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
     if (e != cudaSuccess) return e;
   }
   const bool wide = split && a.hs > 64;
-  if (!wide && (p.dk != nullptr || p.dv != nullptr)) {
-    e = backward_any<KEYS_BOTH>(p, split, stream, status);
+  auto launch = [&](cudaError_t (*kernel)(const FlashBwdParams&, bool, cudaStream_t, int*)) {
+    const cudaError_t e = kernel(p, split, stream, status);
     ++*launches;
-    if (e != cudaSuccess) return e;
-  }
-  if (wide && p.dk != nullptr) {
-    e = backward_hs<128, KEYS_DK, 1, true>(p, stream, status);
-    ++*launches;
-    if (e != cudaSuccess) return e;
-  }
-  if (wide && p.dv != nullptr) {
-    e = backward_hs<128, KEYS_DV, 1, true>(p, stream, status);
-    ++*launches;
-    if (e != cudaSuccess) return e;
-  }
-  if (p.dq != nullptr || dist != nullptr) {
-    e = backward_any<QUERIES>(p, split, stream, status);
-    ++*launches;
-    if (e != cudaSuccess) return e;
-  }
+    p.wait_late = 1;
+    return e;
+  };
+  if (!wide && (p.dk != nullptr || p.dv != nullptr)) e = launch(backward_any<KEYS_BOTH>);
+  if (wide && p.dk != nullptr) e = launch(backward_wide<KEYS_DK>);
+  if (e == cudaSuccess && wide && p.dv != nullptr) e = launch(backward_wide<KEYS_DV>);
+  if (e == cudaSuccess && (p.dq != nullptr || dist != nullptr)) e = launch(backward_any<QUERIES>);
+  if (e != cudaSuccess) return e;
   if (dist == nullptr) return cudaSuccess;
   RelDist d;
   d.dist = dist;
