@@ -1995,7 +1995,7 @@ int relative_composed(int device, cudaStream_t stream, int dtype, const ginn_b20
   float* bias = nullptr;
   if (a.table) {
     CU_TRY(scratch.take(&bias, (2 * a.reach + 1) * a.heads));
-    CU_TRY(gb::launch_rel_bias_expand(dtype, a.table, a.ldt, a.map, (int)a.buckets, a.reach, (int)a.heads, 1.f, bias, stream));
+    CU_TRY(gb::launch_rel_bias_expand(dtype, a.table, a.ldt, a.map, (int)a.buckets, a.reach, (int)a.heads, 1.f, bias, nullptr, 0, stream));
     g_launches.fetch_add(1);
   }
   gb::RelScores sc;
@@ -2141,12 +2141,10 @@ gb::FlashArgs flash_args(const ginn_b200_relative_attention& a) {
   f.causal = a.causal ? 1 : 0;
   return f;
 }
-long long split_work(const gb::FlashArgs& f) { return 8LL * f.batch * f.kv_heads; }
 long long bias_floats(const ginn_b200_relative_attention& a) { return a.table ? (2 * a.reach + 1) * a.heads : 0; }
 // Planes of fp32 operands for the flash kernels.
-int flash_split(Scratch* scratch, gb::FlashArgs* f, gb::FlashOperand* d_o, float* stats, float* norms) {
-  float *work, *q, *k, *v, *d = nullptr;
-  CU_TRY(scratch->take(&work, split_work(*f)));
+int flash_split(Scratch* scratch, gb::FlashArgs* f, gb::FlashOperand* d_o, float* work, float* stats, float** norms) {
+  float *q, *k, *v, *d = nullptr;
   CU_TRY(scratch->take(&q, gb::flash_planes(f->hs, f->tq, f->heads, f->batch)));
   CU_TRY(scratch->take(&k, gb::flash_planes(f->hs, f->tk, f->kv_heads, f->batch)));
   CU_TRY(scratch->take(&v, gb::flash_planes(f->hs, f->tk, f->kv_heads, f->batch)));
@@ -2178,13 +2176,16 @@ int flash_pack(Scratch* scratch, DevCtx* ctx, gb::FlashArgs* f, gb::FlashOperand
   g_launches.fetch_add(d_o ? 5 : 3);
   return GINN_B200_OK;
 }
-// Bias of every distance and head, times log2(e), for the flash kernels.
-int flash_bias(Scratch* scratch, int dtype, const ginn_b200_relative_attention& a, gb::FlashArgs* f) {
-  if (!a.table) return GINN_B200_OK;
+// Bias of every distance and head, times log2(e), for the flash kernels, and zeros in `clear`.
+int flash_bias(Scratch* scratch, int dtype, const ginn_b200_relative_attention& a, gb::FlashArgs* f, float* clear, long long nclear) {
+  if (!a.table) {
+    if (nclear > 0) CU_TRY(cudaMemsetAsync(clear, 0, static_cast<size_t>(nclear) * sizeof(float), scratch->stream));
+    return GINN_B200_OK;
+  }
   float* bias;
   CU_TRY(scratch->take(&bias, (2 * a.reach + 1) * a.heads));
-  CU_TRY(gb::launch_rel_bias_expand(dtype, a.table, a.ldt, a.map, (int)a.buckets, a.reach, (int)a.heads, 1.44269504f, bias,
-                                    scratch->stream));
+  CU_TRY(gb::launch_rel_bias_expand(dtype, a.table, a.ldt, a.map, (int)a.buckets, a.reach, (int)a.heads, 1.44269504f, bias, clear,
+                                    nclear, scratch->stream));
   g_launches.fetch_add(1);
   f->bias = bias;
   return GINN_B200_OK;
@@ -2216,8 +2217,10 @@ int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, c
   const bool split = !half && splits == 0;
   const long long queries = split ? gb::flash_planes(f.hs, f.tq, f.heads, f.batch) : 0, keys = split ? gb::flash_planes(f.hs, f.tk, f.kv_heads, f.batch) : 0;
   if (a->table || floats > 0 || split)
-    CU_TRY(scratch.reserve({bias_floats(*a), floats, split ? split_work(f) : 0, queries, keys, keys}));
-  if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
+    CU_TRY(scratch.reserve({bias_floats(*a), floats, split ? gb::flash_split_work(f) : 0, queries, keys, keys}));
+  float* work = nullptr;
+  if (split) CU_TRY(scratch.take(&work, gb::flash_split_work(f)));
+  if (int s = flash_bias(&scratch, dtype, *a, &f, work, split ? gb::flash_split_clear(f) : 0)) return s;
   int launches = 1;
   if (splits > 0) {
     float* parts = nullptr;
@@ -2225,7 +2228,7 @@ int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, c
     CU_TRY(gb::launch_flash_token(dtype, f, splits, parts, &launches, stream));
   } else {
     if (split)
-      if (int s = flash_split(&scratch, &f, nullptr, nullptr, nullptr)) return s;
+      if (int s = flash_split(&scratch, &f, nullptr, work, nullptr, nullptr)) return s;
     CU_TRY(gb::launch_flash_forward(f, stream, ctx->d_status));
   }
   g_launches.fetch_add(launches);
@@ -2283,13 +2286,15 @@ int ginn_b200_relative_attention_backward(int device, void* stream_, int dtype, 
       if (int s = flash_pack(&scratch, ctx, &f, &fg.d_o)) return s;
     const gb::FlashScratch need = gb::flash_backward_scratch(f, g->dtable != nullptr);
     const long long queries = half ? 0 : gb::flash_planes(f.hs, f.tq, f.heads, f.batch), keys = half ? 0 : gb::flash_planes(f.hs, f.tk, f.kv_heads, f.batch);
-    CU_TRY(scratch.reserve({bias_floats(*a), need.stats, need.norms, need.dist, need.sums, split_work(f), queries, queries, keys, keys}));
-    if (int s = flash_bias(&scratch, dtype, *a, &f)) return s;
-    float *stats, *norms, *dist = nullptr, *sums = nullptr;
+    const long long clear = half ? need.norms : gb::flash_split_clear(f), work_floats = half ? need.norms : gb::flash_split_work(f);
+    CU_TRY(scratch.reserve({bias_floats(*a), need.stats, work_floats, need.dist, need.sums, queries, queries, keys, keys}));
+    float *work, *stats, *dist = nullptr, *sums = nullptr;
+    CU_TRY(scratch.take(&work, work_floats));
     CU_TRY(scratch.take(&stats, need.stats));
-    CU_TRY(scratch.take(&norms, need.norms));
+    float* norms = work;  // of Half operands; others have them within `work`
+    if (int s = flash_bias(&scratch, dtype, *a, &f, work, clear)) return s;
     if (!half)
-      if (int s = flash_split(&scratch, &f, &fg.d_o, stats, norms)) return s;
+      if (int s = flash_split(&scratch, &f, &fg.d_o, work, stats, &norms)) return s;
     if (g->dtable) {
       CU_TRY(scratch.take(&dist, need.dist));
       CU_TRY(scratch.take(&sums, need.sums));

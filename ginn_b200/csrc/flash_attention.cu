@@ -1913,7 +1913,11 @@ bool flash_split_supported(const FlashArgs& a, bool backward) {
 }
 long long flash_planes(int hs, long long t, long long heads, long long batch) { return flash_width(hs) * t * heads * batch; }
 
-cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, float* stats, float* norms, cudaStream_t stream) {
+// work: largest magnitudes of four operands, norms of d_o's and v's rows, inverse scales of four operands.
+long long flash_split_work(const FlashArgs& a) { return 10LL * a.batch * a.kv_heads; }
+long long flash_split_clear(const FlashArgs& a) { return 6LL * a.batch * a.kv_heads; }
+
+cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, float* stats, float** norms, cudaStream_t stream) {
   SplitParams p;
   std::memset(&p, 0, sizeof(p));
   const long long units = static_cast<long long>(a->batch) * a->kv_heads;
@@ -1921,10 +1925,11 @@ cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, flo
   p.count = d_o != nullptr ? 4 : 3;
   p.hs = a->hs; p.batch = a->batch; p.kv_heads = a->kv_heads;
   p.most = reinterpret_cast<unsigned*>(work);
-  p.inverse = work + 4 * units;
+  p.inverse = work + 6 * units;
   a->inverse = p.inverse;
   if (d_o != nullptr) {
-    p.norms = reinterpret_cast<unsigned*>(norms);
+    *norms = work + 4 * units;
+    p.norms = reinterpret_cast<unsigned*>(*norms);
     p.o = static_cast<const float*>(a->o.p);
     p.ldo = a->o.ld; p.sho = a->o.head; p.sbo = a->o.batch;
     p.vec_o = rows16(a->o, 4);
@@ -1949,11 +1954,8 @@ cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, flo
     o.block0 = blocks;
     blocks += static_cast<long long>((o.t + kSplitRows - 1) / kSplitRows) * o.heads * a->batch;
   }
-  cudaError_t e = cudaMemsetAsync(p.most, 0, sizeof(unsigned) * 4 * units, stream);
-  if (e == cudaSuccess && d_o != nullptr) e = cudaMemsetAsync(norms, 0, sizeof(unsigned) * 2 * units, stream);
-  if (e != cudaSuccess) return e;
   const bool narrow = a->hs <= 64;
-  e = launch_kernel(narrow ? split_most_kernel<64> : split_most_kernel<128>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
+  const cudaError_t e = launch_kernel(narrow ? split_most_kernel<64> : split_most_kernel<128>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
                     pdl_enabled(), p);
   if (e != cudaSuccess) return e;
   return launch_kernel(narrow ? split_planes_kernel<64> : split_planes_kernel<128>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, pdl_enabled(), p);
@@ -2079,8 +2081,7 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
   cudaError_t e = cudaSuccess;
   *launches = 0;
   if (!split) {  // split operands came with their statistics
-    e = cudaMemsetAsync(norms, 0, sizeof(unsigned) * 2 * a.batch * a.kv_heads, stream);
-    if (e == cudaSuccess) e = prepare(a, g, p, stats, norms, qtiles * 2, stream);
+    e = prepare(a, g, p, stats, norms, qtiles * 2, stream);
     *launches = 1;
     if (e != cudaSuccess) return e;
   }

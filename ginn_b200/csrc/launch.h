@@ -211,10 +211,11 @@ cudaError_t launch_dropout(int dtype, const void* x, long long ldx, const void* 
                            const Dropout& drop, int num_sms, cudaStream_t stream);
 
 // --- attention with a relative position bias: passes of the composed path (relative_attention.cu) ---
-// out[head][reach + d] = factor * table[map[reach + d], head] (0 where the bucket does not exist).
+// out[head][reach + d] = factor * table[map[reach + d], head] (0 where the bucket does not exist), and
+// clear[0 .. nclear) = 0.
 cudaError_t launch_rel_bias_expand(int dtype, const void* table, long long ldt, const int* map,
                                    int buckets, long long reach, int heads, float factor, float* out,
-                                   cudaStream_t stream);
+                                   float* clear, long long nclear, cudaStream_t stream);
 // dst[b][head][t][hsp] = src(h, t, head, b) in fp32, zero behind hs, in queries behind the lengths and
 // in keys that no query sees.
 cudaError_t launch_rel_pack(int dtype, const void* src, long long ld, long long sh, long long sb,
@@ -267,11 +268,14 @@ cudaError_t launch_flash_pack(FlashOperand* x, int hs, int t, int heads, int bat
                               int num_sms, cudaStream_t stream);
 cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* status);
 // fp32 operands of the same kernels: split into two Half planes each, two kernels.  `work`:
-// 8 * batch * kv heads floats; d_o null: forward only, else also the backward pass's stats and norms.
+// flash_split_work(...) floats, of which the first flash_split_clear(...) are zero; d_o null: forward only,
+// else also the backward pass's stats, and its norms within `work`.
 bool flash_split_supported(const FlashArgs& a, bool backward);
+long long flash_split_work(const FlashArgs& a);
+long long flash_split_clear(const FlashArgs& a);
 long long flash_planes(int hs, long long t, long long heads, long long batch);
-cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, float* stats,
-                               float* norms, cudaStream_t stream);
+cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, float* stats, float** norms,
+                               cudaStream_t stream);
 // Few queries against a long cache (at most 16 rows share a key head): number of parts the keys are
 // split into, 0 when the shape does not qualify, and the scratch the parts need.
 int flash_token_splits(const FlashArgs& a, int num_sms, long long* floats);
@@ -286,7 +290,7 @@ struct FlashGradArgs {
 };
 bool flash_backward_supported(const FlashArgs& a, const FlashGradArgs& g);
 // Scratch of the backward pass, in floats: stats and norms filled by launch_flash_split for fp32
-// operands and by launch_flash_backward for Half ones; dist and sums only when the table's gradient is wanted.
+// operands and by launch_flash_backward for Half ones, whose norms start as zero; dist and sums only when the table's gradient is wanted.
 struct FlashScratch {
   long long stats, norms, dist, sums;
 };

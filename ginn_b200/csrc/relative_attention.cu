@@ -28,14 +28,17 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// Bias of every distance, head by head, in fp32: out[head][reach + d].
+// Bias of every distance, head by head, in fp32: out[head][reach + d].  `clear`: words of the call's scratch that
+// start as zero (a memset between two kernels would keep the second from being launched ahead).
 template <typename T>
 __global__ void __launch_bounds__(256)
 rel_bias_expand_kernel(const T* __restrict__ table, long long ldt, const int* __restrict__ map, int buckets,
-                       long long reach, int heads, float factor, float* __restrict__ out) {
+                       long long reach, int heads, float factor, float* __restrict__ out, float* __restrict__ clear,
+                       long long nclear) {
   pdl_wait();
   pdl_launch_dependents();
   const long long n = 2 * reach + 1, at = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (at < nclear) clear[at] = 0.f;
   if (at >= n * heads) return;
   const long long head = at / n;
   const int b = map[at - head * n];
@@ -353,14 +356,15 @@ unsigned blocks_for(long long n) {
 }  // namespace
 
 cudaError_t launch_rel_bias_expand(int dtype, const void* table, long long ldt, const int* map, int buckets,
-                                   long long reach, int heads, float factor, float* out, cudaStream_t stream) {
-  const long long n = (2 * reach + 1) * heads;
-  const dim3 grid(static_cast<unsigned>((n + 255) / 256));
+                                   long long reach, int heads, float factor, float* out, float* clear, long long nclear,
+                                   cudaStream_t stream) {
+  const long long n = (2 * reach + 1) * heads, most = n > nclear ? n : nclear;
+  const dim3 grid(static_cast<unsigned>((most + 255) / 256));
   if (dtype == 0)
     return launch_kernel(rel_bias_expand_kernel<float>, grid, dim3(256), 0, stream, pdl_enabled(),
-                         static_cast<const float*>(table), ldt, map, buckets, reach, heads, factor, out);
+                         static_cast<const float*>(table), ldt, map, buckets, reach, heads, factor, out, clear, nclear);
   return launch_kernel(rel_bias_expand_kernel<__half>, grid, dim3(256), 0, stream, pdl_enabled(),
-                       static_cast<const __half*>(table), ldt, map, buckets, reach, heads, factor, out);
+                       static_cast<const __half*>(table), ldt, map, buckets, reach, heads, factor, out, clear, nclear);
 }
 
 cudaError_t launch_rel_pack(int dtype, const void* src, long long ld, long long sh, long long sb, int hs, int hsp,
