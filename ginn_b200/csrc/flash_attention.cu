@@ -1147,8 +1147,8 @@ flash_token_join_kernel(const TokenParams p) {
 // and key head) to 2^14, so neither large nor small upstream gradients leave a Half's range.
 //
 // What bounds it: the way of a tile from its products through the threads and back.  A streamed tile takes
-// about 2900 cycles (16 heads of 4096 x 4096 x 128, causal: keys 190 us for 137 GFLOP, queries 173 us for
-// 103, 0.72 and 0.60 PFLOP/s), its four products 1280 of them; two tiles are on that way at a time, and
+// about 2800 cycles (16 heads of 4096 x 4096 x 128, causal: keys 185 us for 137 GFLOP, queries 167 us for
+// 103, 0.74 and 0.62 PFLOP/s), its four products 1280 of them; two tiles are on that way at a time, and
 // tensor memory has no room for a third beside the results.
 constexpr int BN = 64;             // rows of a streamed tile
 constexpr int BCHUNK = BN * 128;   // bytes of 64 rows x 64 halves
