@@ -1288,7 +1288,7 @@ flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long lon
 // but cancel, shows several times enlarged (1313 keys: 6.6e-6).  So Half tiles that see at most
 // kDeltaHalf keys, kDeltaTable where the table's gradient is wanted (500 keys: up to 3.3e-4 instead of the
 // 2.0e-4 of its own rounding), and fp32 tiles that see more than kDeltaSplit take the two extra products
-// (8 x 16 heads of 500 x 500: 18 us of 135).
+// (8 x 16 heads of 500 x 500: 18 us of 123).
 enum FlashMode { KEYS_BOTH = 0, QUERIES = 1, KEYS_DK = 2, KEYS_DV = 3, DELTA = 4 };
 constexpr int kDeltaHalf = 256, kDeltaTable = 512, kDeltaSplit = 512;
 
