@@ -675,7 +675,7 @@ flash_pack_kernel(const __half* __restrict__ src, long long ld, long long sh, lo
 // fragments, and the values of two neighbouring keys, interleaved by byte permutes, as those of the second
 // product.  (A tcgen05 tile would be 128 rows high for these 1 to 16, with the cache passing through
 // shared memory.)  32 sequences of up to 8192 keys, four key heads of 128 with four queries each: 336 MB in
-// 77 us, 4.4 TB/s of 6.5 copied; 370 us on the tiles above.
+// 73 us, 4.6 TB/s of 6.5 copied; 370 us on the tiles above.
 constexpr int kTokenRows = 16;
 constexpr int kTokenWarps = 4;  // two CTAs on an SM: one loads while the other starts or joins its warps
 
@@ -1104,26 +1104,58 @@ flash_token32_kernel(const TokenParams p) {
   w.join<HS, float>(p, res, mx, sm);
 }
 
-// The splits' results together, in order: one CTA per row of a (sequence, key head).
+// The splits' results together: one CTA per row of a (sequence, key head).  Every split's weight first, by
+// all threads side by side, then the results, four threads to a head element with every fourth split each, joined
+// in order.  (Two sequences of 16384 keys have 148 splits each: 60 us with one thread per element walking them, 27
+// so.)
+constexpr int kJoinParts = 4;
 template <int HS, typename T>
-__global__ void __launch_bounds__(HS)
+__global__ void __launch_bounds__(kJoinParts * HS)
 flash_token_join_kernel(const TokenParams p) {
+  extern __shared__ float weight[];  // [split]; -1: no keys, its result was not written
+  __shared__ float red[2][32], parts[kJoinParts][HS];
   pdl_wait();
   pdl_launch_dependents();
   const long long unit = blockIdx.x / p.rows;
-  const int row = static_cast<int>(blockIdx.x % p.rows), h = threadIdx.x;
+  const int row = static_cast<int>(blockIdx.x % p.rows), h = threadIdx.x % HS, q = threadIdx.x / HS;
   const int batch = static_cast<int>(unit / p.kv_heads), kv = static_cast<int>(unit % p.kv_heads);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = kJoinParts * HS / 32;
+  const float2* stat = p.stat + unit * p.splits * p.rows + row;
   float m = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.stat[(unit * p.splits + s) * p.rows + row].x);
-  float l = 0.f, v = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const long long at = (unit * p.splits + s) * p.rows + row;
-    const float2 st = p.stat[at];
-    if (st.x == -INFINITY && st.y == 0.f) continue;  // no keys; its result was not written
-    const float a = st.x == -INFINITY ? 0.f : ex2(st.x - m);
-    l += st.y * a;
-    v += p.part[at * HS + h] * a;
+  for (int s = threadIdx.x; s < p.splits; s += kJoinParts * HS) m = fmaxf(m, stat[static_cast<long long>(s) * p.rows].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) red[0][warp] = m;
+  __syncthreads();
+  for (int w = 0; w < warps; ++w) m = fmaxf(m, red[0][w]);
+  float l = 0.f;
+  for (int s = threadIdx.x; s < p.splits; s += kJoinParts * HS) {
+    const float2 st = stat[static_cast<long long>(s) * p.rows];
+    const float a = st.x == -INFINITY ? (st.y == 0.f ? -1.f : 0.f) : ex2(st.x - m);
+    weight[s] = a;
+    if (a >= 0.f) l += st.y * a;
+    else if (!(a < 0.f)) l = a;  // not a number
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if (lane == 0) red[1][warp] = l;
+  __syncthreads();
+  l = 0.f;
+  for (int w = 0; w < warps; ++w) l += red[1][w];
+  const float* part = p.part + (unit * p.splits * p.rows + row) * HS + h;
+  const long long step = static_cast<long long>(p.rows) * HS;
+  float v = 0.f;
+#pragma unroll 8
+  for (int s = q; s < p.splits; s += kJoinParts) {
+    const float a = weight[s];
+    if (!(a < 0.f)) v += part[s * step] * a;
+  }
+  parts[q][h] = v;
+  __syncthreads();
+  if (q != 0) return;
+  v = 0.f;
+#pragma unroll
+  for (int k = 0; k < kJoinParts; ++k) v += parts[k][h];
   token_store<T>(p, batch, kv, row, h, v, m, l);
 }
 
@@ -2021,7 +2053,8 @@ cudaError_t launch_flash_token(int dtype, const FlashArgs& a, int splits, float*
   *launches = 2;
   auto join = half ? (narrow ? flash_token_join_kernel<64, __half> : flash_token_join_kernel<128, __half>)
                    : (narrow ? flash_token_join_kernel<64, float> : flash_token_join_kernel<128, float>);
-  return launch_kernel(join, dim3(static_cast<unsigned>(units * p.rows)), dim3(narrow ? 64 : 128), 0, stream, pdl_enabled(), p);
+  return launch_kernel(join, dim3(static_cast<unsigned>(units * p.rows)), dim3(kJoinParts * (narrow ? 64 : 128)), splits * sizeof(float), stream,
+                       pdl_enabled(), p);
 }
 
 bool flash_backward_supported(const FlashArgs& a, const FlashGradArgs& g) {

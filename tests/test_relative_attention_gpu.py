@@ -191,6 +191,15 @@ def test_lengths_and_offsets(gpu, dt, causal):
 
 
 @pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("hs", [64, 128])
+def test_one_sequence_against_a_long_cache(gpu, dt, hs):
+    """More parts of the cache than one round of the join's threads, most of them behind the sequence's end in the
+    second case."""
+    check(gpu, Case(dt, hs, 1, 20000, heads=2, kv=1, batch=1, causal=True, offsets=19999))
+    check(gpu, Case(dt, hs, 2, 9000, heads=4, kv=1, batch=1, k_lengths=[100]))
+
+
+@pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("pad,order", [(0, (3, 1, 2)), (8, (3, 2, 1)), (0, (2, 3, 1)), (3, (3, 2, 1)), (1, (1, 2, 3))])
 def test_orders_and_strides(gpu, dt, pad, order):
     """Heads side by side within a token, padded tokens (aligned and not), batch inside the heads, time
