@@ -972,6 +972,7 @@ struct NormPlan {
 constexpr int kNormSmem = 225 * 1024;
 NormPlan plan_backward(const NormGradArgs& a, int es, int num_sms) {
   NormPlan w;
+  if (a.cols == 0) return w;  // no columns, no parts: weight gradients are sums of nothing
   const bool vec = a.rows % 8 == 0 && cols16(a.h, a.ldh, es, a.cols) && cols16(a.dy, a.lddy, es, a.cols) &&
                    cols16(a.dh, a.lddh, es, a.cols) && cols16(a.dres, a.lddres, es, a.cols) &&
                    cols16(a.dx, a.lddx, es, a.cols);
