@@ -545,7 +545,7 @@ norm_backward_kernel(const NormBwd<T> p, int G) {
 // The same for columns on the 16-byte grid, through a ring in shared memory: a column's reduction (a barrier
 // behind two shuffle trees) waits for all of its loads, so without the next columns on their way the memory
 // idles between two.  Every group has a ring of its own, filled by its first thread with one bulk copy per
-// operand; a stage is free once the group is through the barrier of the reduction, since what it holds is
+// operand; a stage is free once the group is through the barrier behind the reduction, since what it holds is
 // in registers by then.  No registers are spent on what is still to come, and the bytes in flight are what
 // shared memory holds (two to eight columns).
 // Columns longer than 512 threads hold are shared by the CTAs of a cluster, each with a run of rows; they
@@ -693,6 +693,7 @@ norm_backward_ring_kernel(const NormBwd<T> p, const NormRing ring, int* __restri
       }
     }
     float2 sum = group_sum2(make_float2(sx.sum(), sy.sum()), G, t, slot[turn]);
+    __syncwarp();  // groups of one warp meet no barrier in the reduction: their reads of the stage end here
     if (t == 0 && ok && col + ring.stages * step < p.cols) issue(col + ring.stages * step, s);
     if (++s == ring.stages) {
       s = 0;
