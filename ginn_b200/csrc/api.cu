@@ -2208,7 +2208,7 @@ int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, c
   gb::FlashArgs f = flash_args(*a);
   const bool half = dtype == GINN_B200_F16;
   long long floats = 0;
-  const int splits = t_force_path == PATH_AUTO ? gb::flash_token_splits(f, ctx->num_sms, &floats) : 0;
+  const int splits = t_force_path == PATH_AUTO ? gb::flash_token_splits(dtype, f, ctx->num_sms, &floats) : 0;
   if (t_force_path != PATH_AUTO || !(splits > 0 || (half ? gb::flash_fits(f) : gb::flash_split_supported(f, false))))
     return relative_composed(device, stream, dtype, *a, nullptr);
   Scratch scratch(stream);

@@ -278,7 +278,7 @@ cudaError_t launch_flash_split(FlashArgs* a, FlashOperand* d_o, float* work, flo
                                cudaStream_t stream);
 // Few queries against a long cache (at most 16 rows share a key head): number of parts the keys are
 // split into, 0 when the shape does not qualify, and the scratch the parts need.
-int flash_token_splits(const FlashArgs& a, int num_sms, long long* floats);
+int flash_token_splits(int dtype, const FlashArgs& a, int num_sms, long long* floats);
 cudaError_t launch_flash_token(int dtype, const FlashArgs& a, int splits, float* scratch,
                                int* launches, cudaStream_t stream);
 struct FlashGradArgs {
