@@ -93,6 +93,20 @@ __device__ __forceinline__ void store_row8(float* to, int n, int vec, const floa
       if (e < n) to[e] = add ? to[e] + x[e] : x[e];
   }
 }
+// x += factor * what lies there, for the first n of eight elements of an fp32 row.
+__device__ __forceinline__ void add_row8(const float* from, int n, int vec, float factor, float (&x)[8]) {
+  if (vec && n >= 8) {
+    const float4 a = *reinterpret_cast<const float4*>(from), b = *reinterpret_cast<const float4*>(from + 4);
+    const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fmaf(y[e], factor, x[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) x[e] = fmaf(from[e], factor, x[e]);
+  }
+}
+__device__ __forceinline__ void add_row8(const __half*, int, int, float, float (&)[8]) {}  // Half results have no chains
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -160,6 +174,14 @@ struct TileBias {
   }
 };
 
+// The tensor core truncates each time it adds to an accumulator, once per 16 terms of a contraction.  Terms of one
+// sign make that a bias that grows with the chain: fp32 results are off by 1.2e-6 of their size after 256 terms,
+// 5.8e-6 after 1024, 2.5e-5 after 4096 (a Half result is rounded to 4.9e-4).  The kernels for fp32 operands
+// therefore start a new chain every 1024 terms and add the chains up with rounded additions, in the result's own
+// place: every result keeps 2^-17 of its terms' magnitudes.  The end of a chain costs the forward kernel 9 us (4 heads of
+// 4096 x 4096 x 64, three of them: 126 -> 152 us; chains of 512 terms, 2.7e-6: 180).
+constexpr int kChain = 1024;
+
 // SPLIT: fp32 operands as two Half planes each (see split_planes_kernel).  NQ: query tiles per CTA.  One tile
 // of a 64-wide head leaves room for a second CTA on the SM (TWICE), whose start, loads and end then pass while
 // the first computes; a thread has 80 registers there, so it reads its scores twice, 32 at a time, once
@@ -176,6 +198,8 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
   constexpr int CROSS = NQ * HS;                 // tensor memory: from a tile's result to its cross terms
   constexpr int TILE = FCHUNK * CHUNKS;  // bytes of one operand tile
   constexpr float PSHIFT = SPLIT ? 7.f : 0.f;  // probabilities are formed times 2^PSHIFT: their low parts stay normal
+  constexpr int CUT = kChain / FT;       // split operands: key tiles to a chain
+  using Out = typename std::conditional<SPLIT, float, __half>::type;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t q_full[2], k_full[NST], k_empty[NST], v_full[NST], v_empty[NST];
   __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2];
@@ -304,7 +328,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
 #pragma unroll
           for (int ks = 0; ks < FT / 16; ++ks) {
             const uint32_t o = tmem + NQ * FT + t * HS, a = tmem + t * FT + (ks / 2) * 32 + (ks % 2) * 8;
-            const uint32_t add = (j > 0 || ks > 0) ? 1u : 0u;
+            const uint32_t add = ((SPLIT ? j % CUT : j) > 0 || ks > 0) ? 1u : 0u;
             mma_f16_ts(o, a, make_smem_desc(b + ks * 2048, FCHUNK, 1024), IDESC_O, add);
             if (SPLIT) {
               // The cross terms have an accumulator of their own: the tensor core truncates when it adds, so
@@ -342,6 +366,18 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
     const float c1 = SPLIT ? p.c1 * p.iq[unit] * p.ik[unit] : p.c1;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
+    float md = -INFINITY;  // split operands: the maximum that the chains which ended are relative to
+    auto place = [&] { return static_cast<Out*>(p.O) + i * p.ldo + hd.head * p.sho + hd.batch * p.sbo + half * (HS / 2); };
+    // Elements c .. c + 7 of the chain in tensor memory and, where there are any, `old` times those before it.
+    auto chain8 = [&](int c, bool before, float old, const Out* out, float (&x)[8]) {
+      uint32_t w[8], cross[8];
+      tmem_ld8(o_col + c, w);
+      if (SPLIT) tmem_ld8(o_col + CROSS + c, cross);
+      tmem_ld_wait();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = SPLIT ? __uint_as_float(w[e]) + __uint_as_float(cross[e]) : __uint_as_float(w[e]);
+      if (SPLIT && before) add_row8(out + c, i < p.tq ? p.hs - half * (HS / 2) - c : 0, p.vec, old, x);
+    };
     for (int j = 0; j < nt; ++j) {
       float* win = window[t][j & 1];
       const TileBias tb(bias, p.reach, j * FT - (i0 + t * FT + FT - 1 + hd.off), gt, win, c1 > 0.f);
@@ -367,6 +403,17 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
       uint32_t v[TWICE ? 32 : 64];
       if (ok) {
         tc_fence_after();
+        if (SPLIT && j > 0 && j % CUT == 0) {  // a chain ends: the products of the tiles before it are done
+          const float old = md == m ? 1.f : ex2(md - m);
+          Out* out = place();
+#pragma unroll
+          for (int c = 0; c < HS / 2; c += 8) {
+            float x[8];
+            chain8(c, j > CUT, old, out, x);
+            if (i < p.tq) store_row8(out + c, p.hs - half * (HS / 2) - c, p.vec, x, false);
+          }
+          md = m;
+        }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
@@ -389,7 +436,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
         const float a = mn == -INFINITY ? 1.f : ex2(m - mn);
         l *= a;
         m = mn;
-        if (j > 0) {  // O exists from the second tile on
+        if ((SPLIT ? j % CUT : j) > 0) {  // O exists from the second tile of a chain on
 #pragma unroll
           for (int c = 0; c < (SPLIT ? HS : HS / 2); c += 16) {
             const uint32_t col = o_col + c + (c >= HS / 2 ? CROSS - HS / 2 : 0);  // behind the main result: the cross terms
@@ -442,23 +489,15 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
     }
     if (ok) {
       const bool real = i < p.tq, some = nt > 0 && vis > 0 && l != 0.f;  // (not a number stays one)
-      const float inv = some ? (SPLIT ? p.iv[unit] : 1.f) / l : 0.f;
-      using Out = typename std::conditional<SPLIT, float, __half>::type;
-      Out* out = static_cast<Out*>(p.O) + i * p.ldo + hd.head * p.sho + hd.batch * p.sbo;
+      const float inv = some ? (SPLIT ? p.iv[unit] : 1.f) / l : 0.f, old = md == m ? 1.f : ex2(md - m);
+      Out* out = place();
 #pragma unroll
       for (int c = 0; c < HS / 2; c += 8) {
-        uint32_t w[8], x[8];
-        if (nt > 0) {
-          tmem_ld8(o_col + c, w);
-          if (SPLIT) tmem_ld8(o_col + CROSS + c, x);
-          tmem_ld_wait();
-        }
-        float res[8];
+        float x[8];
+        if (nt > 0) chain8(c, nt > CUT, old, out, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          res[e] = some ? (SPLIT ? __uint_as_float(w[e]) + __uint_as_float(x[e]) : __uint_as_float(w[e])) * inv : 0.f;
-        const int at = half * (HS / 2) + c;
-        if (real) store_row8(out + at, p.hs - at, p.vec, res, false);
+        for (int e = 0; e < 8; ++e) x[e] = some ? x[e] * inv : 0.f;
+        if (real) store_row8(out + c, p.hs - half * (HS / 2) - c, p.vec, x, false);
       }
       if (real && half == 0)
         p.lse[(static_cast<long long>(hd.batch) * p.heads + hd.head) * p.tq + i] = some ? (m + log2f(l) - PSHIFT) * kLn2 : -INFINITY;

@@ -40,3 +40,88 @@ def test_fp32_tokens_of_many_sequences(gpu, tk, batch):
         off = (o[b, 0, 0].double() - ref).abs() / ref
         assert (off <= E + 2.0 ** -19).all(), float(off.max())
         assert abs(float(lse[b]) - float(torch.logsumexp(s, 0))) <= E * math.log(tk)
+
+
+class Operands:
+    """Heads of hs elements with a mean of `shift`, and what the definition makes of them in 64 bits."""
+
+    def __init__(self, dtype, hs, tq, tk, heads=2, kv=2, batch=1, causal=False, shift=1.0, small=1.0, pad=0, seed=0):
+        gen = torch.Generator(device="cuda").manual_seed(seed + hs + tq + tk)
+        new = lambda n, t, s: (s * (randn(gen, batch, n, t, hs + pad) + shift)).to(dtype)[..., :hs]  # noqa: E731
+        self.q, self.k, self.v, self.d_o = new(heads, tq, small), new(kv, tk, 1), new(kv, tk, 1), new(heads, tq, 1)
+        self.o, self.dq = torch.empty_like(self.q), torch.empty_like(self.q)
+        self.dk, self.dv = torch.empty_like(self.k), torch.empty_like(self.v)
+        self.lse = torch.empty(batch, heads, tq, device="cuda")
+        self.scale = float(torch.tensor(hs ** -0.5))
+        self.causal, self.offset = causal, tk - tq if causal else 0
+
+    def forward(self, gb):
+        gb.relative_attention_forward(heads(self.q), heads(self.k), heads(self.v), None, None, heads(self.o), self.lse, scale=self.scale,
+                                      causal=self.causal, q_offset=self.offset)
+
+    def backward(self, gb, accumulate=False):
+        gb.relative_attention_backward(heads(self.q), heads(self.k), heads(self.v), None, None, heads(self.o), self.lse, heads(self.d_o),
+                                       heads(self.dq), heads(self.dk), heads(self.dv), scale=self.scale, causal=self.causal,
+                                       q_offset=self.offset, accumulate=accumulate)
+
+    def reference(self):
+        """(results, products of the magnitudes); the probabilities are taken as they are."""
+        q, k, v, g = (x.double() for x in (self.q, self.k, self.v, self.d_o))
+        n = q.shape[1] // k.shape[1]
+        K, V = k.repeat_interleave(n, 1), v.repeat_interleave(n, 1)
+        s = self.scale * (q @ K.transpose(2, 3))
+        if self.causal:
+            i, j = torch.arange(q.shape[2], device="cuda")[:, None], torch.arange(k.shape[2], device="cuda")
+            s = s.masked_fill(j > i + self.offset, -math.inf)
+        p = torch.softmax(s, 3)
+        dp = g @ V.transpose(2, 3)
+        ds = p * (dp - (p * dp).sum(3, keepdim=True))
+        shared = lambda x: x.unflatten(1, (k.shape[1], n)).sum(2)  # noqa: E731
+        return (dict(o=p @ V, dq=self.scale * ds @ K, dk=self.scale * shared(ds.transpose(2, 3) @ q), dv=shared(p.transpose(2, 3) @ g)),
+                dict(o=p @ V.abs(), dv=shared(p.transpose(2, 3) @ g.abs())))
+
+
+def elementwise(name, got, ref, size, bound):
+    off = ((got.double() - ref).abs() / size).max()
+    assert off <= bound, (name, float(off), bound)
+
+
+# scores below 1/2 as above: 2^-19 for the probabilities
+SMALL = E + 2.0 ** -19
+
+
+@pytest.mark.parametrize("hs,tq,tk,heads,kv,causal,pad", [
+    (64, 100, 512, 2, 2, False, 0), (64, 40, 513, 2, 2, False, 0), (64, 300, 1024, 4, 2, True, 0), (57, 20, 1537, 2, 1, True, 0), (64, 130, 4096, 2, 2, False, 4),
+    (61, 33, 2050, 1, 1, False, 1), (128, 200, 3000, 2, 2, False, 0), (128, 140, 1100, 2, 1, True, 0), (16, 1500, 1500, 1, 1, True, 0)])
+def test_fp32_sums_of_values_of_one_sign(gpu, hs, tq, tk, heads, kv, causal, pad):
+    c = Operands(torch.float32, hs, tq, tk, heads, kv, causal=causal, shift=0.0, small=0.05, pad=pad)
+    c.v.abs_().add_(0.5)
+    c.forward(gpu)
+    ref, size = c.reference()
+    elementwise("o", c.o, ref["o"], size["o"], SMALL)
+
+
+@pytest.mark.parametrize("hs,tq,tk", [(64, 70, 1500), (128, 40, 2100), (40, 200, 1024)])
+def test_fp32_rows_that_see_little_of_the_first_keys(gpu, hs, tq, tk):
+    """A bias of -inf behind a distance: whole chains of keys in which a row sees nothing, then some, its maximum
+    moving in every tile; rows that see nothing at all."""
+    c = Operands(torch.float32, hs, tq, tk, shift=0.0)
+    c.v.abs_().add_(0.5)
+    reach, near = 1200, 300
+    d = torch.arange(-reach, reach + 1, device="cuda")
+    bucket = torch.where(d < -near, 1, 0).to(torch.int32)
+    table = torch.tensor([[0.25, 0.5], [-math.inf, -math.inf]], device="cuda").t().contiguous().t()
+    ramp = torch.linspace(0, 30, tk, device="cuda")[None, None, :, None]
+    c.k = c.k + ramp * 0.2 * c.q[:, :, :1].sign()
+    for offset in (tk - tq, tk + near - tq // 2):
+        gpu.relative_attention_forward(heads(c.q), heads(c.k), heads(c.v), table, bucket, heads(c.o), c.lse, scale=c.scale, q_offset=offset)
+        s = c.scale * (c.q.double() @ c.k.double().transpose(2, 3))
+        size = c.scale * (c.q.double().abs() @ c.k.double().abs().transpose(2, 3))
+        far = torch.arange(tk, device="cuda")[None, :] - torch.arange(tq, device="cuda")[:, None] - offset < -near
+        s = torch.where(far, -math.inf, s + table[0].double()[None, :, None, None])
+        seen = ~far.all(1)
+        assert bool(seen.any()) and bool(seen.all()) == (offset == tk - tq)
+        p = torch.softmax(s[:, :, seen], 3)
+        es = E * (size.max() + 1)  # of a score, relative of a probability; its sum's error as much again
+        elementwise("o", c.o[:, :, seen], p @ c.v.double(), p @ c.v.double(), 2 * es + E)
+        assert (c.o[:, :, ~seen] == 0).all() and torch.isneginf(c.lse[:, :, ~seen]).all()
