@@ -1430,8 +1430,11 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
   constexpr int TILE = BCHUNK * CHUNKS;   // bytes of a streamed tile
   constexpr float PSHIFT = SPLIT ? 14.f : 12.f;  // P is formed times 2^PSHIFT
   constexpr float PINV = SPLIT ? 1.f / 16384.f : 1.f / 4096.f;
+  constexpr bool CHAINS = SPLIT && MODE != DELTA;  // results are added up from chains of CUT streamed tiles
+  constexpr int CUT = kChain / BN;
+  static_assert(CUT % 2 == 0, "both groups have as many tiles in a chain");
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t rows_full, b_full[BSTAGES], b_empty[BSTAGES], x_full[2], p_full[2], acc_full;
+  __shared__ __align__(8) uint64_t rows_full, b_full[BSTAGES], b_empty[BSTAGES], x_full[2], p_full[2], acc_full, acc_empty;
   __shared__ uint32_t tmem_slot;
   __shared__ float window[2][2][256];
   __shared__ __align__(16) float colx[KEYS ? 2 : 1][2][BN], coly[KEYS ? 2 : 1][2][BN];
@@ -1453,6 +1456,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     if (lane == 0) {
       mbar_init(smem_u32(&rows_full), 1);
       mbar_init(smem_u32(&acc_full), 1);
+      mbar_init(smem_u32(&acc_empty), 512);
       for (int s = 0; s < BSTAGES; ++s) {
         mbar_init(smem_u32(&b_full[s]), 1);
         mbar_init(smem_u32(&b_empty[s]), 1);
@@ -1550,6 +1554,8 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       // overwrites P and dS of tile it - 1, whose products are issued; a single stage is still in use
       if (BSTAGES > 1 && it + 1 < n) scores(it + 1);
       ok = ok && warp_wait(&p_full[g], (it >> 1) & 1, status, DEV_TIMEOUT_FULL, 0xe02);
+      if (CHAINS && it > 0 && it % CUT == 0)  // the chain before has left its place
+        ok = ok && warp_wait(&acc_empty, (it / CUT - 1) & 1, status, DEV_TIMEOUT_EMPTY, 0xe03);
       if (!ok) break;
       tc_fence_after();
       if (leader) {
@@ -1558,7 +1564,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
         auto product = [&](uint32_t d, uint32_t left, uint32_t right) {
 #pragma unroll
           for (int ks = 0; ks < BN / 16; ++ks) {
-            const uint32_t l = left + (ks / 2) * 32 + (ks % 2) * 8, add = (it > 0 || ks > 0) ? 1u : 0u;
+            const uint32_t l = left + (ks / 2) * 32 + (ks % 2) * 8, add = ((CHAINS ? it % CUT : it) > 0 || ks > 0) ? 1u : 0u;
             mma_f16_ts(d, l, make_smem_desc(right + ks * 2048, BCHUNK, 1024), IDESC_ACC, add);
             if (SPLIT) {
               mma_f16_ts(d + HS, l, make_smem_desc(right + WIDE * BCHUNK + ks * 2048, BCHUNK, 1024), IDESC_ACC, add);
@@ -1569,7 +1575,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
         if (WANT_P) product(tmem + 2 * FT + PV_COL, a, b + TILE);  // dV += P dO
         if (WANT_D && MODE != DELTA) product(tmem + 2 * FT, a + BN, b);  // dK += dS Q,  dQ += dS K
         tc_commit(smem_u32(&b_empty[s]));
-        if (it == n - 1) tc_commit(smem_u32(&acc_full));
+        if (it == n - 1 || (CHAINS && (it + 1) % CUT == 0)) tc_commit(smem_u32(&acc_full));
       }
       __syncwarp();
       if (BSTAGES == 1 && it + 1 < n) scores(it + 1);
@@ -1611,159 +1617,199 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     };
     float2 ahead = make_float2(0.f, 0.f);
     if (KEYS && gt < BN && g < n) ahead = stat(walk);
-    for (int it = g; it < n; it += 2, walk.next(2)) {
-      const int at = (first + walk.tile) * BN, turn = (it >> 1) & 1;
-      const int h = KEYS ? head * p.group + walk.head : head;
-      const float* bias = p.bias != nullptr ? p.bias + static_cast<long long>(h) * (2 * p.reach + 1) : nullptr;
-      // distances of the tile's pairs: dlo .. dlo + 190
-      const int dlo = KEYS ? r0 - (at + BN - 1 + off) : at - (r0 + FT - 1 + off);
-      // one number for the whole tile (a masked score is -inf before it is scaled: c1 > 0), or a window
-      const bool beyond = dlo >= p.reach || dlo + FT + BN - 2 <= -p.reach;
-      const bool flat = c1 > 0.f && (bias == nullptr || beyond);
-      float value = 0.f;
-      float* win = window[g][turn];
-      if (flat) {
-        if (bias != nullptr) value = __ldg(bias + (dlo >= p.reach ? 2 * p.reach : 0));
-      } else {
-        int d = dlo + gt;
-        d = d > p.reach ? p.reach : d < -p.reach ? -p.reach : d;
-        win[gt] = bias != nullptr ? __ldg(bias + d + p.reach) : 0.f;
-      }
-      if (KEYS && gt < BN) {
-        // per column: what is added to the scaled score, and to Y times f
-        const float2 st = ahead;
-        if (it + 2 < n) {
-          StreamWalk then = walk;
-          then.next(2);
-          ahead = stat(then);
-        }
-        const bool alone = rel_visible(p.causal, at + gt + off, klen) <= 1;
-        colx[KEYS ? g : 0][turn][gt] = (flat ? value : 0.f) + PSHIFT - st.x;
-        coly[KEYS ? g : 0][turn][gt] = alone ? 0.f : -st.y * f;
-      }
-      if (KEYS || !flat) group_barrier(1 + g);
-      // window[c - r + 127] for query rows, window[r - c + 63] for key rows
-      const float* wrow = KEYS ? win + (BN - 1) + r - 32 * half : win + (FT - 1) - r + 32 * half;
-      ok = ok && warp_wait(&x_full[g], turn, status, DEV_TIMEOUT_ACCUM, 0xf00 + g);
-      // of this thread's columns those from lo to hi - 1 take part
-      int lo = 0, hi = 32;
-      if (KEYS) {
-        hi = row < klen ? 32 : 0;
-        if (p.causal) {
-          const int from = row - off - at - 32 * half;
-          lo = from < 0 ? 0 : from > 32 ? 32 : from;
-        }
-      } else {
-        hi = vis - at - 32 * half;
-      }
-      const bool sweep = !KEYS && !beyond && p.reach > 0;  // sums along the diagonals
-      F2 all(0.f, 0.f);
-      if (ok) {
-        tc_fence_after();
-        const bool alone = !KEYS && vis <= 1;
-        const float rx = (flat ? value : 0.f) + PSHIFT - mine.x, ry = alone ? 0.f : -mine.y * f;
-        uint32_t x[32], y[32];
-        tmem_ld32(x_col, x);
-        if (WANT_D) tmem_ld32(y_col, y);
-        tmem_ld_wait();
-        if (!flat) {  // the window's bias joins the scores here, everything else below
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), c1, KEYS ? wrow[-e] : wrow[e]));
-        }
-        if (__any_sync(0xffffffffu, lo > 0 || hi < 32)) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (e < lo || e >= hi) {
-              x[e] = 0xff800000u;  // -inf
-              if (WANT_D) y[e] = 0u;
-            }
-        }
-        // A query that sees one key gives it all its weight whatever the score: dS is zero, not what is
-        // left of two roundings.  The first query of a causal sequence, or every one over a single key.
-        if (WANT_D && (KEYS ? klen <= 1 || (p.causal && at + off <= 0) : __any_sync(0xffffffffu, alone))) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (KEYS ? klen <= 1 || at + 32 * half + e + off <= 0 : alone) y[e] = 0u;
-        }
-        const float cx1 = flat ? c1 : 1.f;
-        const F2 cx(cx1, cx1), f2(fy, fy);
-        uint32_t pw[16], dw[16], plow[16], dlow[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          F2 sx(rx, rx), sy(ry, ry);
-          if (KEYS) {
-            const float2 ax = *reinterpret_cast<const float2*>(&colx[KEYS ? g : 0][turn][32 * half + e]);
-            const float2 ay = *reinterpret_cast<const float2*>(&coly[KEYS ? g : 0][turn][32 * half + e]);
-            sx = F2(ax.x, ax.y);
-            sy = F2(ay.x, ay.y);
-          }
-          float p0, p1;
-          fma2(F2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), cx, sx).get(p0, p1);
-          p0 = ex2(p0);
-          p1 = ex2(p1);
-          if (WANT_P) {
-            if (SPLIT) split_pair(p0, p1, pw[e / 2], plow[e / 2]);
-            else pw[e / 2] = pack_half2(p0, p1);
-          }
-          if (WANT_D) {
-            const F2 ds = mul2(F2(p0, p1), fma2(F2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), f2, sy));
-            float d0, d1;
-            ds.get(d0, d1);
-            if (SPLIT) split_pair(d0, d1, dw[e / 2], dlow[e / 2]);
-            else dw[e / 2] = pack_half2(d0, d1);
-            if (!KEYS) {
-              all = add2(all, ds);
-              y[e] = __float_as_uint(d0);
-              y[e + 1] = __float_as_uint(d1);
-            }
-          }
-        }
-        if (WANT_P) tmem_st16(x_col, pw);
-        if (WANT_P && SPLIT) tmem_st16(x_col + 16, plow);
-        if (WANT_D && MODE != DELTA) tmem_st16(y_col, dw);
-        if (WANT_D && MODE != DELTA && SPLIT) tmem_st16(y_col + 16, dlow);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(smem_u32(&p_full[g]));
-        if (sweep && dist_on) {
-          // the running sum of a diagonal moves down one lane per column; lane 31 ends it
-          float run = 0.f;
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            run = __shfl_up_sync(0xffffffffu, run, 1);
-            run = (lane == 0 ? 0.f : run) + __uint_as_float(y[e]);
-            if (lane == 31) diag[KEYS ? 0 : warp - 4][e] = run;  // diagonal e - 31
-          }
-          if (lane < 31) diag[KEYS ? 0 : warp - 4][32 + lane] = run;  // diagonal 31 - lane
-        }
-      }
-      if (MODE == DELTA) far_lo += all.sum();
-      if (dist_on) {
-        if (!sweep) {  // one side of the reach
-          float a0, a1;
-          all.get(a0, a1);
-          if (dlo >= p.reach) far_hi += a0 + a1;
-          else far_lo += a0 + a1;
+    int it = g;
+    for (int chain = 0;; ++chain) {
+      const int stop = CHAINS && n > (chain + 1) * CUT ? (chain + 1) * CUT : n;
+      for (; it < stop; it += 2, walk.next(2)) {
+        const int at = (first + walk.tile) * BN, turn = (it >> 1) & 1;
+        const int h = KEYS ? head * p.group + walk.head : head;
+        const float* bias = p.bias != nullptr ? p.bias + static_cast<long long>(h) * (2 * p.reach + 1) : nullptr;
+        // distances of the tile's pairs: dlo .. dlo + 190
+        const int dlo = KEYS ? r0 - (at + BN - 1 + off) : at - (r0 + FT - 1 + off);
+        // one number for the whole tile (a masked score is -inf before it is scaled: c1 > 0), or a window
+        const bool beyond = dlo >= p.reach || dlo + FT + BN - 2 <= -p.reach;
+        const bool flat = c1 > 0.f && (bias == nullptr || beyond);
+        float value = 0.f;
+        float* win = window[g][turn];
+        if (flat) {
+          if (bias != nullptr) value = __ldg(bias + (dlo >= p.reach ? 2 * p.reach : 0));
         } else {
-          group_barrier(1 + g);
-          if (gt < FT + BN - 1) {
-            const int w = gt;
-            float sum = 0.f;
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              // column - row = w - 127; warp q of the group: rows 32 (q % 4) + lane, columns 32 (q / 4) + e
-              const int dg = w - (FT - 1) + 32 * (q & 3) - 32 * (q >> 2);  // e - lane
-              if (dg >= -31 && dg <= 31) sum += diag[KEYS ? 0 : g * 8 + q][dg <= 0 ? dg + 31 : 32 + 31 - dg];
-            }
-            const int d = dlo + w;
-            if (d >= p.reach) far_hi += sum;
-            else if (d <= -p.reach) far_lo += sum;
-            else if (d - low < p.width) dist[d - low] += sum;  // behind the last key: nothing, and no place
+          int d = dlo + gt;
+          d = d > p.reach ? p.reach : d < -p.reach ? -p.reach : d;
+          win[gt] = bias != nullptr ? __ldg(bias + d + p.reach) : 0.f;
+        }
+        if (KEYS && gt < BN) {
+          // per column: what is added to the scaled score, and to Y times f
+          const float2 st = ahead;
+          if (it + 2 < n) {
+            StreamWalk then = walk;
+            then.next(2);
+            ahead = stat(then);
           }
-          group_barrier(1 + g);
+          const bool alone = rel_visible(p.causal, at + gt + off, klen) <= 1;
+          colx[KEYS ? g : 0][turn][gt] = (flat ? value : 0.f) + PSHIFT - st.x;
+          coly[KEYS ? g : 0][turn][gt] = alone ? 0.f : -st.y * f;
+        }
+        if (KEYS || !flat) group_barrier(1 + g);
+        // window[c - r + 127] for query rows, window[r - c + 63] for key rows
+        const float* wrow = KEYS ? win + (BN - 1) + r - 32 * half : win + (FT - 1) - r + 32 * half;
+        ok = ok && warp_wait(&x_full[g], turn, status, DEV_TIMEOUT_ACCUM, 0xf00 + g);
+        // of this thread's columns those from lo to hi - 1 take part
+        int lo = 0, hi = 32;
+        if (KEYS) {
+          hi = row < klen ? 32 : 0;
+          if (p.causal) {
+            const int from = row - off - at - 32 * half;
+            lo = from < 0 ? 0 : from > 32 ? 32 : from;
+          }
+        } else {
+          hi = vis - at - 32 * half;
+        }
+        const bool sweep = !KEYS && !beyond && p.reach > 0;  // sums along the diagonals
+        F2 all(0.f, 0.f);
+        if (ok) {
+          tc_fence_after();
+          const bool alone = !KEYS && vis <= 1;
+          const float rx = (flat ? value : 0.f) + PSHIFT - mine.x, ry = alone ? 0.f : -mine.y * f;
+          uint32_t x[32], y[32];
+          tmem_ld32(x_col, x);
+          if (WANT_D) tmem_ld32(y_col, y);
+          tmem_ld_wait();
+          if (!flat) {  // the window's bias joins the scores here, everything else below
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), c1, KEYS ? wrow[-e] : wrow[e]));
+          }
+          if (__any_sync(0xffffffffu, lo > 0 || hi < 32)) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (e < lo || e >= hi) {
+                x[e] = 0xff800000u;  // -inf
+                if (WANT_D) y[e] = 0u;
+              }
+          }
+          // A query that sees one key gives it all its weight whatever the score: dS is zero, not what is
+          // left of two roundings.  The first query of a causal sequence, or every one over a single key.
+          if (WANT_D && (KEYS ? klen <= 1 || (p.causal && at + off <= 0) : __any_sync(0xffffffffu, alone))) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (KEYS ? klen <= 1 || at + 32 * half + e + off <= 0 : alone) y[e] = 0u;
+          }
+          const float cx1 = flat ? c1 : 1.f;
+          const F2 cx(cx1, cx1), f2(fy, fy);
+          uint32_t pw[16], dw[16], plow[16], dlow[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            F2 sx(rx, rx), sy(ry, ry);
+            if (KEYS) {
+              const float2 ax = *reinterpret_cast<const float2*>(&colx[KEYS ? g : 0][turn][32 * half + e]);
+              const float2 ay = *reinterpret_cast<const float2*>(&coly[KEYS ? g : 0][turn][32 * half + e]);
+              sx = F2(ax.x, ax.y);
+              sy = F2(ay.x, ay.y);
+            }
+            float p0, p1;
+            fma2(F2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), cx, sx).get(p0, p1);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            if (WANT_P) {
+              if (SPLIT) split_pair(p0, p1, pw[e / 2], plow[e / 2]);
+              else pw[e / 2] = pack_half2(p0, p1);
+            }
+            if (WANT_D) {
+              const F2 ds = mul2(F2(p0, p1), fma2(F2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), f2, sy));
+              float d0, d1;
+              ds.get(d0, d1);
+              if (SPLIT) split_pair(d0, d1, dw[e / 2], dlow[e / 2]);
+              else dw[e / 2] = pack_half2(d0, d1);
+              if (!KEYS) {
+                all = add2(all, ds);
+                y[e] = __float_as_uint(d0);
+                y[e + 1] = __float_as_uint(d1);
+              }
+            }
+          }
+          if (WANT_P) tmem_st16(x_col, pw);
+          if (WANT_P && SPLIT) tmem_st16(x_col + 16, plow);
+          if (WANT_D && MODE != DELTA) tmem_st16(y_col, dw);
+          if (WANT_D && MODE != DELTA && SPLIT) tmem_st16(y_col + 16, dlow);
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(smem_u32(&p_full[g]));
+          if (sweep && dist_on) {
+            // the running sum of a diagonal moves down one lane per column; lane 31 ends it
+            float run = 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              run = __shfl_up_sync(0xffffffffu, run, 1);
+              run = (lane == 0 ? 0.f : run) + __uint_as_float(y[e]);
+              if (lane == 31) diag[KEYS ? 0 : warp - 4][e] = run;  // diagonal e - 31
+            }
+            if (lane < 31) diag[KEYS ? 0 : warp - 4][32 + lane] = run;  // diagonal 31 - lane
+          }
+        }
+        if (MODE == DELTA) far_lo += all.sum();
+        if (dist_on) {
+          if (!sweep) {  // one side of the reach
+            float a0, a1;
+            all.get(a0, a1);
+            if (dlo >= p.reach) far_hi += a0 + a1;
+            else far_lo += a0 + a1;
+          } else {
+            group_barrier(1 + g);
+            if (gt < FT + BN - 1) {
+              const int w = gt;
+              float sum = 0.f;
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                // column - row = w - 127; warp q of the group: rows 32 (q % 4) + lane, columns 32 (q / 4) + e
+                const int dg = w - (FT - 1) + 32 * (q & 3) - 32 * (q >> 2);  // e - lane
+                if (dg >= -31 && dg <= 31) sum += diag[KEYS ? 0 : g * 8 + q][dg <= 0 ? dg + 31 : 32 + 31 - dg];
+              }
+              const int d = dlo + w;
+              if (d >= p.reach) far_hi += sum;
+              else if (d <= -p.reach) far_lo += sum;
+              else if (d - low < p.width) dist[d - low] += sum;  // behind the last key: nothing, and no place
+            }
+            group_barrier(1 + g);
+          }
         }
       }
+      // ---- results, chain by chain: of two, group 0 writes dK and group 1 dV; a single one's columns are shared ----
+      if (MODE != DELTA && n > 0 && ok) {
+        ok = warp_wait(&acc_full, chain & 1, status, DEV_TIMEOUT_ACCUM, 0xf10 + g);
+        tc_fence_after();
+      }
+      using Out = typename std::conditional<SPLIT, float, __half>::type;
+      const bool values = MODE == KEYS_DV || (MODE == KEYS_BOTH && g == 1);  // this thread writes dV
+      Out* out = static_cast<Out*>(KEYS ? (values ? p.dv : p.dk) : p.dq);
+      const bool real = row < (KEYS ? p.tk : p.tq);
+      if (MODE != DELTA && ok && out != nullptr && (n > 0 || !p.accumulate)) {
+        const long long ld = KEYS ? (values ? p.lddv : p.lddk) : p.lddq, sh = KEYS ? (values ? p.shdv : p.shdk) : p.shdq,
+                        sb = KEYS ? (values ? p.sbdv : p.sbdk) : p.sbdq;
+        const int vec = KEYS ? (values ? p.vec_dv : p.vec_dk) : p.vec_dq;
+        out += row * ld + head * sh + batch * sb;
+        float factor = values ? PINV : p.scale / up;
+        if (SPLIT) factor *= KEYS ? (values ? p.ido[unit] : p.iq[unit]) : p.ik[unit];
+        const uint32_t col0 = lanes + 2 * FT + (values ? PV_COL : 0);
+        constexpr bool SHARED = MODE != KEYS_BOTH;
+        const int c_from = SHARED ? (2 * g + half) * (HS / 4) : half * (HS / 2), c_to = c_from + (SHARED ? HS / 4 : HS / 2);
+        for (int c = c_from; c < c_to; c += 8) {
+          uint32_t w[8], x[8];
+          if (n > 0) {
+            tmem_ld8(col0 + c, w);
+            if (SPLIT) tmem_ld8(col0 + HS + c, x);
+            tmem_ld_wait();
+          }
+          float res[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            res[e] = n > 0 ? (SPLIT ? __uint_as_float(w[e]) + __uint_as_float(x[e]) : __uint_as_float(w[e])) * factor : 0.f;
+          if (real) store_row8(out + c, p.hs - c, vec, res, p.accumulate != 0 || chain > 0);
+        }
+      }
+      if (!CHAINS || stop == n) break;
+      tc_fence_before();
+      mbar_arrive(smem_u32(&acc_empty));
     }
     // ---- sums by distance ----
     if (dist_on) {
@@ -1792,39 +1838,6 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
       }
     }
     if (MODE == DELTA) delta_s[2 * g + half][r] = ok ? far_lo / up : 0.f;
-    // ---- results: of two, group 0 writes dK and group 1 dV; a single one's columns are shared ----
-    if (MODE != DELTA && n > 0 && ok) {
-      ok = warp_wait(&acc_full, 0, status, DEV_TIMEOUT_ACCUM, 0xf10 + g);
-      tc_fence_after();
-    }
-    using Out = typename std::conditional<SPLIT, float, __half>::type;
-    const bool values = MODE == KEYS_DV || (MODE == KEYS_BOTH && g == 1);  // this thread writes dV
-    Out* out = static_cast<Out*>(KEYS ? (values ? p.dv : p.dk) : p.dq);
-    const bool real = row < (KEYS ? p.tk : p.tq);
-    if (MODE != DELTA && ok && out != nullptr && (n > 0 || !p.accumulate)) {
-      const long long ld = KEYS ? (values ? p.lddv : p.lddk) : p.lddq, sh = KEYS ? (values ? p.shdv : p.shdk) : p.shdq,
-                      sb = KEYS ? (values ? p.sbdv : p.sbdk) : p.sbdq;
-      const int vec = KEYS ? (values ? p.vec_dv : p.vec_dk) : p.vec_dq;
-      out += row * ld + head * sh + batch * sb;
-      float factor = values ? PINV : p.scale / up;
-      if (SPLIT) factor *= KEYS ? (values ? p.ido[unit] : p.iq[unit]) : p.ik[unit];
-      const uint32_t col0 = lanes + 2 * FT + (values ? PV_COL : 0);
-      constexpr bool SHARED = MODE != KEYS_BOTH;
-      const int c_from = SHARED ? (2 * g + half) * (HS / 4) : half * (HS / 2), c_to = c_from + (SHARED ? HS / 4 : HS / 2);
-      for (int c = c_from; c < c_to; c += 8) {
-        uint32_t w[8], x[8];
-        if (n > 0) {
-          tmem_ld8(col0 + c, w);
-          if (SPLIT) tmem_ld8(col0 + HS + c, x);
-          tmem_ld_wait();
-        }
-        float res[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          res[e] = n > 0 ? (SPLIT ? __uint_as_float(w[e]) + __uint_as_float(x[e]) : __uint_as_float(w[e])) * factor : 0.f;
-        if (real) store_row8(out + c, p.hs - c, vec, res, p.accumulate != 0);
-      }
-    }
   }
 
   tc_fence_before();

@@ -125,3 +125,33 @@ def test_fp32_rows_that_see_little_of_the_first_keys(gpu, hs, tq, tk):
         es = E * (size.max() + 1)  # of a score, relative of a probability; its sum's error as much again
         elementwise("o", c.o[:, :, seen], p @ c.v.double(), p @ c.v.double(), 2 * es + E)
         assert (c.o[:, :, ~seen] == 0).all() and torch.isneginf(c.lse[:, :, ~seen]).all()
+
+
+def frobenius(name, got, ref, bound):
+    off = float((got.double() - ref).norm() / ref.norm())
+    assert off <= bound, (name, off, bound)
+
+
+@pytest.mark.parametrize("hs,tq,tk,heads,kv,causal,pad", [
+    (64, 1024, 200, 1, 1, False, 0), (64, 1025, 200, 2, 2, False, 0), (64, 300, 300, 8, 2, True, 0), (57, 2100, 130, 1, 1, True, 0), (64, 4096, 150, 1, 1, False, 4),
+    (64, 130, 2500, 2, 1, False, 0), (61, 700, 1100, 3, 1, True, 1), (128, 1500, 300, 2, 2, False, 0), (128, 150, 2049, 2, 1, True, 0), (128, 500, 500, 4, 1, False, 0)])
+def test_fp32_sums_of_gradients_of_one_sign(gpu, hs, tq, tk, heads, kv, causal, pad):
+    """d_o of one sign against dv, and random ones over more terms than a chain holds, the results taken anew and added
+    to."""
+    c = Operands(torch.float32, hs, tq, tk, heads, kv, causal=causal, shift=0.0, small=0.05, pad=pad)
+    if causal:  # a first row that sees one key, rather than the last ones only
+        c.offset = 0 if tk <= tq else c.offset
+    c.d_o.abs_().add_(0.5)
+    c.forward(gpu)
+    c.backward(gpu)
+    ref, size = c.reference()
+    elementwise("dv", c.dv, ref["dv"], size["dv"] + 1e-30, SMALL)
+    c.d_o.copy_(randn(torch.Generator(device="cuda").manual_seed(2), *c.d_o.shape))
+    ref, _ = c.reference()
+    old = {}
+    for accumulate in (False, True):
+        c.backward(gpu, accumulate)
+        for n in ("dq", "dk", "dv"):
+            got = getattr(c, n)
+            frobenius(n, got - old[n] if accumulate else got, ref[n], 1e-5)
+            old[n] = got.clone()
