@@ -1358,14 +1358,16 @@ flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long lon
 //
 // DELTA runs before the others and adds sum_j P (Y - delta) to delta, which is what delta is off by.  delta
 // from the stored o carries o's rounding: for Half that is the largest error of a gradient where o is
-// as large as v, in queries that see few keys (two keys: 5.1e-4 of dq instead of 2.9e-4; 500 keys: 3.0e-4);
-// for fp32 it is the truncation of o's long accumulation, which the table's gradient, whose terms all
-// but cancel, shows several times enlarged (1313 keys: 6.6e-6).  So Half tiles that see at most
-// kDeltaHalf keys, kDeltaTable where the table's gradient is wanted (500 keys: up to 3.3e-4 instead of the
-// 2.0e-4 of its own rounding), and fp32 tiles that see more than kDeltaSplit take the two extra products
-// (8 x 16 heads of 500 x 500: 18 us of 123).
+// as large as v, in queries that see few keys (two keys: 5.1e-4 of dq instead of 2.9e-4; 500 keys: 3.0e-4).
+// For fp32 it is the truncation of o's accumulation, in tiles that see more than kDeltaSplit keys.  A row's
+// score gradients add up to zero; what delta is off by, they add up to, and keys with a mean of their own make that
+// an error of dq (operands of mean 1: 4.6e-5 at 256 keys, 1.5e-4 at 512; corrected 1.8e-6 and 2.4e-6, where plain
+// fp32 sums give 3.7e-6 and 5.0e-6; 64 keys: 2.4e-6 as it is).  The two extra products are a fifth of
+// a backward pass (256 heads of 256 x 256 x 64: 152 -> 184 us).  Half tiles take them up to kDeltaHalf keys,
+// kDeltaTable where the table's gradient is wanted (500 keys: up to 3.3e-4 instead of the 2.0e-4 of its own rounding;
+// 8 x 16 heads of 500 x 500: 18 us of 123).
 enum FlashMode { KEYS_BOTH = 0, QUERIES = 1, KEYS_DK = 2, KEYS_DV = 3, DELTA = 4 };
-constexpr int kDeltaHalf = 256, kDeltaTable = 512, kDeltaSplit = 512;
+constexpr int kDeltaHalf = 256, kDeltaTable = 512, kDeltaSplit = 64;
 
 // What a CTA works on: 128 rows of one head of one sequence, and the streamed tiles first .. first + per - 1
 // of every query head of the group.

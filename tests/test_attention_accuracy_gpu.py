@@ -155,3 +155,16 @@ def test_fp32_sums_of_gradients_of_one_sign(gpu, hs, tq, tk, heads, kv, causal, 
             got = getattr(c, n)
             frobenius(n, got - old[n] if accumulate else got, ref[n], 1e-5)
             old[n] = got.clone()
+
+
+@pytest.mark.parametrize("hs,tq,tk,heads,kv,causal", [
+    (64, 64, 64, 2, 2, False), (64, 128, 128, 2, 2, False), (64, 256, 256, 8, 8, True), (64, 300, 512, 4, 2, False), (128, 256, 256, 2, 2, False),
+    (128, 500, 500, 2, 1, True), (57, 90, 200, 3, 3, False), (16, 40, 1024, 2, 2, True)])
+def test_fp32_gradients_of_operands_with_a_mean(gpu, hs, tq, tk, heads, kv, causal):
+    """A row's score gradients add up to zero; keys with a mean show what is left of that."""
+    c = Operands(torch.float32, hs, tq, tk, heads, kv, causal=causal, shift=1.0)
+    c.forward(gpu)
+    c.backward(gpu)
+    ref, _ = c.reference()
+    for n in ("o", "dq", "dk", "dv"):
+        frobenius(n, getattr(c, n), ref[n], 1e-5)
