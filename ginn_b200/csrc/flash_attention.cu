@@ -1243,7 +1243,6 @@ struct FlashBwdParams {
   int tq, tk, hs, heads, kv_heads, group, batch, tq_pad, row_tiles, width;
   int vec_dq, vec_dk, vec_dv;       // the results' rows allow 16-byte accesses
   int wait_late;                    // the launch before this one is another of the same pass, see the kernel
-  int delta_keys;                   // Half: most keys a tile sees whose delta is corrected
   int reach, q_offset;
   const int* q_offsets;
   const int* q_lengths;
@@ -1356,18 +1355,18 @@ flash_prepare_kernel(const __half* d_o, long long lddo, long long shdo, long lon
 // MODE: what a launch forms.  128-wide split operands leave room in tensor memory for one result (with its
 // cross terms) beside X and Y, and in shared memory for one stage: dK and dV are then two launches.
 //
-// DELTA runs before the others and adds sum_j P (Y - delta) to delta, which is what delta is off by.  delta
-// from the stored o carries o's rounding: for Half that is the largest error of a gradient where o is
-// as large as v, in queries that see few keys (two keys: 5.1e-4 of dq instead of 2.9e-4; 500 keys: 3.0e-4).
-// For fp32 it is the truncation of o's accumulation, in tiles that see more than kDeltaSplit keys.  A row's
-// score gradients add up to zero; what delta is off by, they add up to, and keys with a mean of their own make that
-// an error of dq (operands of mean 1: 4.6e-5 at 256 keys, 1.5e-4 at 512; corrected 1.8e-6 and 2.4e-6, where plain
-// fp32 sums give 3.7e-6 and 5.0e-6; 64 keys: 2.4e-6 as it is).  The two extra products are a fifth of
-// a backward pass (256 heads of 256 x 256 x 64: 152 -> 184 us).  Half tiles take them up to kDeltaHalf keys,
-// kDeltaTable where the table's gradient is wanted (500 keys: up to 3.3e-4 instead of the 2.0e-4 of its own rounding;
-// 8 x 16 heads of 500 x 500: 18 us of 123).
+// DELTA runs before the others and adds sum_j P (Y - delta) to delta, which is what delta is off by: delta from the
+// stored o carries o's rounding for Half and the truncation of o's accumulation for fp32.  A row's score gradients
+// add up to zero; what delta is off by, they add up to, and keys with a mean of their own make that an error of dq,
+// one that does not average out over the keys.  Relative to the gradient, operands of mean 1, as it is and corrected:
+//   Half  dq 1.6e-3 and 3.8e-4 at 64 keys, 3.4e-3 and 3.6e-4 at 512, 9.9e-3 and 3.6e-4 at 4096
+//   fp32  dq 2.4e-6 and 1.1e-6 at 64 keys, 4.6e-5 and 1.8e-6 at 256, 1.5e-4 and 2.4e-6 at 512 (plain sums 5.0e-6)
+// and the table's gradient, whose terms all but cancel, shows it with operands of mean zero: Half, 2048 keys 4.5e-4
+// and 2.2e-4.  So every pass that forms a score gradient takes the two extra products, except fp32 tiles that
+// see at most kDeltaSplit keys.  They are a fifth to a third of it (backward pass, as it would be and is: Half 8 x 8 heads of
+// 512 x 512 x 64 54 and 72 us, 4 heads of 4096 x 4096 x 64 117 and 159; fp32 256 heads of 256 x 256 x 64 152 and 186).
 enum FlashMode { KEYS_BOTH = 0, QUERIES = 1, KEYS_DK = 2, KEYS_DV = 3, DELTA = 4 };
-constexpr int kDeltaHalf = 256, kDeltaTable = 512, kDeltaSplit = 64;
+constexpr int kDeltaSplit = 64;
 
 // What a CTA works on: 128 rows of one head of one sequence, and the streamed tiles first .. first + per - 1
 // of every query head of the group.
@@ -1399,7 +1398,7 @@ struct FlashBwdTile {
     } else if (r0 < qlen) {
       const int last = r0 + FT - 1 < qlen - 1 ? r0 + FT - 1 : qlen - 1;
       per = (rel_visible(p.causal, last + off, klen) + BN - 1) / BN;
-      if (MODE == DELTA && (SPLIT ? per <= kDeltaSplit / BN : per > p.delta_keys / BN)) per = 0;
+      if (MODE == DELTA && SPLIT && per <= kDeltaSplit / BN) per = 0;
     }
   }
 };
@@ -1450,7 +1449,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
   uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t a1_s = base, a2_s = base + ROWS, b_s = base + 2 * ROWS;  // stage: B1, B2
 
-  if (MODE == DELTA) {  // most of its CTAs have nothing to do
+  if (MODE == DELTA) {  // some of its CTAs have nothing to do
     pdl_wait();
     if (FlashBwdTile<MODE, SPLIT>(p).per == 0) return;
   }
@@ -1921,7 +1920,7 @@ cudaError_t backward_hs(const FlashBwdParams& p, cudaStream_t stream, int* statu
   if (e != cudaSuccess) return e;
   FlashBwdParams q = p;
   constexpr bool keys = MODE != QUERIES && MODE != DELTA;
-  q.row_tiles = MODE == DELTA ? p.row_tiles : ((keys ? p.tk : p.tq) + FT - 1) / FT;
+  q.row_tiles = ((keys ? p.tk : p.tq) + FT - 1) / FT;
   const long long grid = static_cast<long long>(q.row_tiles) * (keys ? p.kv_heads : p.heads) * p.batch;
   return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(FTHREADS), smem, stream, pdl_enabled(), q, status);
 }
@@ -2177,20 +2176,8 @@ cudaError_t launch_flash_backward(const FlashArgs& a, const FlashGradArgs& g, fl
     *launches = 1;
     if (e != cudaSuccess) return e;
   }
-  // query tiles, from the first on, that may qualify for the correction of delta
   p.delta = reinterpret_cast<float2*>(stats);
-  p.row_tiles = qtiles;
-  p.delta_keys = dist != nullptr ? kDeltaTable : kDeltaHalf;
-  if (split) {
-    if (a.tk <= kDeltaSplit) p.row_tiles = 0;
-  } else if (a.k_lengths == nullptr && a.tk > p.delta_keys) {
-    if (!a.causal) p.row_tiles = 0;
-    if (a.causal && a.q_offsets == nullptr) {
-      const long long tiles = (p.delta_keys - a.q_offset + FT - 1) / FT;
-      p.row_tiles = tiles < 0 ? 0 : tiles < qtiles ? static_cast<int>(tiles) : qtiles;
-    }
-  }
-  if (p.row_tiles > 0 && (p.dk != nullptr || p.dq != nullptr || dist != nullptr)) {
+  if (!(split && a.tk <= kDeltaSplit) && (p.dk != nullptr || p.dq != nullptr || dist != nullptr)) {
     e = backward_any<DELTA>(p, split, stream, status);
     ++*launches;
     if (e != cudaSuccess) return e;

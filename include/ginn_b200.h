@@ -396,8 +396,7 @@ typedef struct {
   float* lse;
 } ginn_b200_relative_attention;
 
-/* Upstream gradient and results of the backward pass; each result may be NULL (for Half sequences of 257 to
- * 512 keys the others' last bits depend on whether dtable is).  `+=` when accumulate
+/* Upstream gradient and results of the backward pass; each result may be NULL.  `+=` when accumulate
  * != 0, `=` otherwise.  dk and dv are summed over the query heads that share them; dtable (buckets x
  * heads, type `dtype`) over all sequences, in a fixed order. */
 typedef struct {

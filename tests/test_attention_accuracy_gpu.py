@@ -15,7 +15,7 @@ pytestmark = pytest.mark.gpu
 E = 2.0 ** -17
 
 
-def heads(x):
+def heads_of(x):
     """(batch, heads, t, hs) in memory as the calls' (hs, t, heads, batch)."""
     return x.permute(3, 2, 1, 0)
 
@@ -33,7 +33,7 @@ def test_fp32_tokens_of_many_sequences(gpu, tk, batch):
     hs = 16
     q, k, v = 0.05 * randn(gen, batch, 1, 1, hs), randn(gen, batch, 1, tk, hs), randn(gen, batch, 1, tk, hs).abs_() + 0.5
     o, lse = torch.empty_like(q), torch.empty(batch, device="cuda")
-    gpu.relative_attention_forward(heads(q), heads(k), heads(v), None, None, heads(o), lse, scale=0.125)
+    gpu.relative_attention_forward(heads_of(q), heads_of(k), heads_of(v), None, None, heads_of(o), lse, scale=0.125)
     for b in (0, batch // 2, batch - 1):
         s = 0.125 * (k[b, 0].double() @ q[b, 0, 0].double())
         ref = torch.softmax(s, 0) @ v[b, 0].double()
@@ -56,12 +56,12 @@ class Operands:
         self.causal, self.offset = causal, tk - tq if causal else 0
 
     def forward(self, gb):
-        gb.relative_attention_forward(heads(self.q), heads(self.k), heads(self.v), None, None, heads(self.o), self.lse, scale=self.scale,
+        gb.relative_attention_forward(heads_of(self.q), heads_of(self.k), heads_of(self.v), None, None, heads_of(self.o), self.lse, scale=self.scale,
                                       causal=self.causal, q_offset=self.offset)
 
     def backward(self, gb, accumulate=False):
-        gb.relative_attention_backward(heads(self.q), heads(self.k), heads(self.v), None, None, heads(self.o), self.lse, heads(self.d_o),
-                                       heads(self.dq), heads(self.dk), heads(self.dv), scale=self.scale, causal=self.causal,
+        gb.relative_attention_backward(heads_of(self.q), heads_of(self.k), heads_of(self.v), None, None, heads_of(self.o), self.lse, heads_of(self.d_o),
+                                       heads_of(self.dq), heads_of(self.dk), heads_of(self.dv), scale=self.scale, causal=self.causal,
                                        q_offset=self.offset, accumulate=accumulate)
 
     def reference(self):
@@ -114,7 +114,7 @@ def test_fp32_rows_that_see_little_of_the_first_keys(gpu, hs, tq, tk):
     ramp = torch.linspace(0, 30, tk, device="cuda")[None, None, :, None]
     c.k = c.k + ramp * 0.2 * c.q[:, :, :1].sign()
     for offset in (tk - tq, tk + near - tq // 2):
-        gpu.relative_attention_forward(heads(c.q), heads(c.k), heads(c.v), table, bucket, heads(c.o), c.lse, scale=c.scale, q_offset=offset)
+        gpu.relative_attention_forward(heads_of(c.q), heads_of(c.k), heads_of(c.v), table, bucket, heads_of(c.o), c.lse, scale=c.scale, q_offset=offset)
         s = c.scale * (c.q.double() @ c.k.double().transpose(2, 3))
         size = c.scale * (c.q.double().abs() @ c.k.double().abs().transpose(2, 3))
         far = torch.arange(tk, device="cuda")[None, :] - torch.arange(tq, device="cuda")[:, None] - offset < -near
@@ -168,3 +168,21 @@ def test_fp32_gradients_of_operands_with_a_mean(gpu, hs, tq, tk, heads, kv, caus
     ref, _ = c.reference()
     for n in ("o", "dq", "dk", "dv"):
         frobenius(n, getattr(c, n), ref[n], 1e-5)
+
+
+@pytest.mark.parametrize("hs,tq,tk,heads,kv,causal", [
+    (64, 64, 64, 2, 2, False), (64, 300, 300, 4, 2, False), (64, 200, 600, 4, 4, True), (128, 512, 512, 2, 1, True), (57, 90, 900, 3, 3, False),
+    (64, 2048, 2048, 2, 2, False), (128, 300, 4096, 1, 1, False)])
+def test_half_gradients_of_operands_with_a_mean(gpu, hs, tq, tk, heads, kv, causal):
+    c = Operands(torch.float16, hs, tq, tk, heads, kv, causal=causal, shift=1.0)
+    c.forward(gpu)
+    c.backward(gpu)
+    ref, _ = c.reference()
+    for n in ("o", "dq", "dk", "dv"):
+        frobenius(n, getattr(c, n), ref[n], 4 * 2.0 ** -11)
+    dq, dk = c.dq.clone(), c.dk.clone()
+    for out in ("dq", "dk"):  # a result does not depend on which others are wanted
+        new = torch.empty_like(getattr(c, out))
+        gpu.relative_attention_backward(heads_of(c.q), heads_of(c.k), heads_of(c.v), None, None, heads_of(c.o), c.lse, heads_of(c.d_o), scale=c.scale,
+                                        causal=c.causal, q_offset=c.offset, accumulate=False, **{out: heads_of(new)})
+        assert torch.equal(new, dq if out == "dq" else dk)
