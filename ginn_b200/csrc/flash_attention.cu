@@ -93,20 +93,6 @@ __device__ __forceinline__ void store_row8(float* to, int n, int vec, const floa
       if (e < n) to[e] = add ? to[e] + x[e] : x[e];
   }
 }
-// x += factor * what lies there, for the first n of eight elements of an fp32 row.
-__device__ __forceinline__ void add_row8(const float* from, int n, int vec, float factor, float (&x)[8]) {
-  if (vec && n >= 8) {
-    const float4 a = *reinterpret_cast<const float4*>(from), b = *reinterpret_cast<const float4*>(from + 4);
-    const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = fmaf(y[e], factor, x[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < n) x[e] = fmaf(from[e], factor, x[e]);
-  }
-}
-__device__ __forceinline__ void add_row8(const __half*, int, int, float, float (&)[8]) {}  // Half results have no chains
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -177,10 +163,11 @@ struct TileBias {
 // The tensor core truncates each time it adds to an accumulator, once per 16 terms of a contraction.  Terms of one
 // sign make that a bias that grows with the chain: fp32 results are off by 1.2e-6 of their size after 256 terms,
 // 5.8e-6 after 1024, 2.5e-5 after 4096 (a Half result is rounded to 4.9e-4).  The kernels for fp32 operands
-// therefore start a new chain every 1024 terms and add the chains up with rounded additions, in the result's own
-// place: every result keeps 2^-17 of its terms' magnitudes.  The end of a chain costs the forward kernel 9 us (4 heads of
-// 4096 x 4096 x 64, three of them: 126 -> 152 us; chains of 512 terms, 2.7e-6: 180).
-constexpr int kChain = 1024;
+// therefore start a new chain every 512 terms and add the chains up with rounded additions: a result keeps 2^-17 of
+// its terms' magnitudes (one sign 2.7e-6, the largest terms first 5.7e-6; chains of 1024 terms: 1.2e-5).  What ended lies
+// in local memory, where a warp's accesses are neighbours: in the result's own place, rows apart, the end of a
+// chain took 8 us of a CTA's time instead of 2.6 (4 heads of 4096 x 4096 x 64, seven of them: 126 us without, 144, and 180).
+constexpr int kChain = 512;
 
 // SPLIT: fp32 operands as two Half planes each (see split_planes_kernel).  NQ: query tiles per CTA.  One tile
 // of a 64-wide head leaves room for a second CTA on the SM (TWICE), whose start, loads and end then pass while
@@ -367,16 +354,21 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     float md = -INFINITY;  // split operands: the maximum that the chains which ended are relative to
-    auto place = [&] { return static_cast<Out*>(p.O) + i * p.ldo + hd.head * p.sho + hd.batch * p.sbo + half * (HS / 2); };
+    // What they add up to.  Indexed in loops that stay loops, so that it lies in local memory and not among the
+    // registers of every tile; a warp's accesses there are neighbours.
+    float part[SPLIT ? HS / 2 : 1];
     // Elements c .. c + 7 of the chain in tensor memory and, where there are any, `old` times those before it.
-    auto chain8 = [&](int c, bool before, float old, const Out* out, float (&x)[8]) {
+    auto chain8 = [&](int c, bool before, float old, float (&x)[8]) {
       uint32_t w[8], cross[8];
       tmem_ld8(o_col + c, w);
       if (SPLIT) tmem_ld8(o_col + CROSS + c, cross);
       tmem_ld_wait();
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = SPLIT ? __uint_as_float(w[e]) + __uint_as_float(cross[e]) : __uint_as_float(w[e]);
-      if (SPLIT && before) add_row8(out + c, i < p.tq ? p.hs - half * (HS / 2) - c : 0, p.vec, old, x);
+      if (SPLIT && before) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = fmaf(part[SPLIT ? c + e : 0], old, x[e]);
+      }
     };
     for (int j = 0; j < nt; ++j) {
       float* win = window[t][j & 1];
@@ -405,12 +397,12 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
         tc_fence_after();
         if (SPLIT && j > 0 && j % CUT == 0) {  // a chain ends: the products of the tiles before it are done
           const float old = md == m ? 1.f : ex2(md - m);
-          Out* out = place();
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < HS / 2; c += 8) {
             float x[8];
-            chain8(c, j > CUT, old, out, x);
-            if (i < p.tq) store_row8(out + c, p.hs - half * (HS / 2) - c, p.vec, x, false);
+            chain8(c, j > CUT, old, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) part[SPLIT ? c + e : 0] = x[e];
           }
           md = m;
         }
@@ -490,14 +482,21 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
     if (ok) {
       const bool real = i < p.tq, some = nt > 0 && vis > 0 && l != 0.f;  // (not a number stays one)
       const float inv = some ? (SPLIT ? p.iv[unit] : 1.f) / l : 0.f, old = md == m ? 1.f : ex2(md - m);
-      Out* out = place();
-#pragma unroll
-      for (int c = 0; c < HS / 2; c += 8) {
+      Out* out = static_cast<Out*>(p.O) + i * p.ldo + hd.head * p.sho + hd.batch * p.sbo;
+      auto eight = [&](int c) {
         float x[8];
-        if (nt > 0) chain8(c, nt > CUT, old, out, x);
+        if (nt > 0) chain8(c, nt > CUT, old, x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = some ? x[e] * inv : 0.f;
-        if (real) store_row8(out + c, p.hs - half * (HS / 2) - c, p.vec, x, false);
+        const int at = half * (HS / 2) + c;
+        if (real) store_row8(out + at, p.hs - at, p.vec, x, false);
+      };
+      if (SPLIT) {
+#pragma unroll 1
+        for (int c = 0; c < HS / 2; c += 8) eight(c);
+      } else {
+#pragma unroll
+        for (int c = 0; c < HS / 2; c += 8) eight(c);
       }
       if (real && half == 0)
         p.lse[(static_cast<long long>(hd.batch) * p.heads + hd.head) * p.tq + i] = some ? (m + log2f(l) - PSHIFT) * kLn2 : -INFINITY;
@@ -1618,6 +1617,8 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
     };
     float2 ahead = make_float2(0.f, 0.f);
     if (KEYS && gt < BN && g < n) ahead = stat(walk);
+    // What the chains that ended add up to, in local memory (see the forward kernel).
+    float part[CHAINS ? HS / 2 : 1];
     int it = g;
     for (int chain = 0;; ++chain) {
       const int stop = CHAINS && n > (chain + 1) * CUT ? (chain + 1) * CUT : n;
@@ -1775,26 +1776,28 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
           }
         }
       }
-      // ---- results, chain by chain: of two, group 0 writes dK and group 1 dV; a single one's columns are shared ----
+      // ---- results: of two, group 0 writes dK and group 1 dV; a single one's columns are shared ----
+      const bool last = !CHAINS || stop == n;
       if (MODE != DELTA && n > 0 && ok) {
         ok = warp_wait(&acc_full, chain & 1, status, DEV_TIMEOUT_ACCUM, 0xf10 + g);
         tc_fence_after();
       }
       using Out = typename std::conditional<SPLIT, float, __half>::type;
-      const bool values = MODE == KEYS_DV || (MODE == KEYS_BOTH && g == 1);  // this thread writes dV
+      constexpr bool SHARED = MODE != KEYS_BOTH;
+      constexpr int COUNT = SHARED ? HS / 4 : HS / 2;                         // columns of this thread
+      const bool values = MODE == KEYS_DV || (MODE == KEYS_BOTH && g == 1);  // it writes dV
+      const int c_from = SHARED ? (2 * g + half) * COUNT : half * COUNT;
       Out* out = static_cast<Out*>(KEYS ? (values ? p.dv : p.dk) : p.dq);
-      const bool real = row < (KEYS ? p.tk : p.tq);
       if (MODE != DELTA && ok && out != nullptr && (n > 0 || !p.accumulate)) {
         const long long ld = KEYS ? (values ? p.lddv : p.lddk) : p.lddq, sh = KEYS ? (values ? p.shdv : p.shdk) : p.shdq,
                         sb = KEYS ? (values ? p.sbdv : p.sbdk) : p.sbdq;
         const int vec = KEYS ? (values ? p.vec_dv : p.vec_dk) : p.vec_dq;
-        out += row * ld + head * sh + batch * sb;
+        const bool real = row < (KEYS ? p.tk : p.tq);
+        out += row * ld + head * sh + batch * sb + c_from;
         float factor = values ? PINV : p.scale / up;
         if (SPLIT) factor *= KEYS ? (values ? p.ido[unit] : p.iq[unit]) : p.ik[unit];
-        const uint32_t col0 = lanes + 2 * FT + (values ? PV_COL : 0);
-        constexpr bool SHARED = MODE != KEYS_BOTH;
-        const int c_from = SHARED ? (2 * g + half) * (HS / 4) : half * (HS / 2), c_to = c_from + (SHARED ? HS / 4 : HS / 2);
-        for (int c = c_from; c < c_to; c += 8) {
+        const uint32_t col0 = lanes + 2 * FT + (values ? PV_COL : 0) + c_from;
+        auto eight = [&](int c) {
           uint32_t w[8], x[8];
           if (n > 0) {
             tmem_ld8(col0 + c, w);
@@ -1803,12 +1806,22 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
           }
           float res[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            res[e] = n > 0 ? (SPLIT ? __uint_as_float(w[e]) + __uint_as_float(x[e]) : __uint_as_float(w[e])) * factor : 0.f;
-          if (real) store_row8(out + c, p.hs - c, vec, res, p.accumulate != 0 || chain > 0);
+          for (int e = 0; e < 8; ++e) {
+            res[e] = n > 0 ? (SPLIT ? __uint_as_float(w[e]) + __uint_as_float(x[e]) : __uint_as_float(w[e])) : 0.f;
+            if (CHAINS && chain > 0) res[e] += part[CHAINS ? c + e : 0];
+            if (!last) part[CHAINS ? c + e : 0] = res[e];
+            res[e] *= factor;
+          }
+          if (last && real) store_row8(out + c, p.hs - c_from - c, vec, res, p.accumulate != 0);
+        };
+        if (CHAINS) {
+#pragma unroll 1
+          for (int c = 0; c < COUNT; c += 8) eight(c);
+        } else {
+          for (int c = 0; c < COUNT; c += 8) eight(c);
         }
       }
-      if (!CHAINS || stop == n) break;
+      if (last) break;
       tc_fence_before();
       mbar_arrive(smem_u32(&acc_empty));
     }
@@ -1992,9 +2005,7 @@ cudaError_t launch_flash_pack(FlashOperand* x, int hs, int t, int heads, int bat
   return e;
 }
 
-// fp32 through Half planes: contractions of at most 4096, since an accumulator is added to once per 16
-// of them and the tensor core truncates each time, about 2^-25 of the running sum (measured: 4e-7 of the
-// result at 256, 2.5e-6 at 2048; longer ones run on the composed path, whose products cut the chain).
+// fp32 through Half planes: contractions of at most 4096; longer ones run on the composed path.
 bool flash_split_supported(const FlashArgs& a, bool backward) {
   const long long group = a.heads / a.kv_heads, parts = (a.tq + 63) / 64 + (a.tk + 63) / 64;
   return tmap_encoder_available() && a.hs <= 128 && a.tk <= 4096 && (!backward || group * a.tq <= 4096) &&

@@ -186,3 +186,15 @@ def test_half_gradients_of_operands_with_a_mean(gpu, hs, tq, tk, heads, kv, caus
         gpu.relative_attention_backward(heads_of(c.q), heads_of(c.k), heads_of(c.v), None, None, heads_of(c.o), c.lse, heads_of(c.d_o), scale=c.scale,
                                         causal=c.causal, q_offset=c.offset, accumulate=False, **{out: heads_of(new)})
         assert torch.equal(new, dq if out == "dq" else dk)
+
+
+@pytest.mark.parametrize("hs,t,heads", [(64, 900, 2), (64, 2100, 1), (128, 1500, 1)])
+def test_fp32_sums_that_begin_with_their_largest_terms(gpu, hs, t, heads):
+    """The first keys of a causal sequence get 1, 1/2, 1/3 .. of its rows' gradients: nearly every addition of a chain is
+    made to a sum of its full size."""
+    c = Operands(torch.float32, hs, t, t, heads, heads, causal=True, shift=0.0, small=0.05)
+    c.d_o.abs_().add_(0.5)
+    c.forward(gpu)
+    c.backward(gpu)
+    ref, size = c.reference()
+    elementwise("dv", c.dv, ref["dv"], size["dv"], SMALL)
