@@ -2209,7 +2209,7 @@ int ginn_b200_relative_attention_forward(int device, void* stream_, int dtype, c
   const bool half = dtype == GINN_B200_F16;
   long long floats = 0;
   const int splits = t_force_path == PATH_AUTO ? gb::flash_token_splits(dtype, f, ctx->num_sms, &floats) : 0;
-  if (t_force_path != PATH_AUTO || !(splits > 0 || (half ? gb::flash_fits(f) : gb::flash_split_supported(f, false))))
+  if (t_force_path != PATH_AUTO || !(splits > 0 || (half ? gb::flash_fits(f) : gb::flash_split_supported(f))))
     return relative_composed(device, stream, dtype, *a, nullptr);
   Scratch scratch(stream);
   if (half && !gb::flash_supported(f))
@@ -2279,7 +2279,7 @@ int ginn_b200_relative_attention_backward(int device, void* stream_, int dtype, 
     fg.buckets = (int)a->buckets;
     fg.accumulate = g->accumulate ? 1 : 0;
     const bool half = dtype == GINN_B200_F16;
-    if (t_force_path != PATH_AUTO || !(half ? gb::flash_fits(f) : gb::flash_split_supported(f, true)))
+    if (t_force_path != PATH_AUTO || !(half ? gb::flash_fits(f) : gb::flash_split_supported(f)))
       return relative_composed(device, stream, dtype, *a, g);
     Scratch scratch(stream);
     if (half && !gb::flash_backward_supported(f, fg))

@@ -270,7 +270,7 @@ cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* s
 // fp32 operands of the same kernels: split into two Half planes each, two kernels.  `work`:
 // flash_split_work(...) floats, of which the first flash_split_clear(...) are zero; d_o null: forward only,
 // else also the backward pass's stats, and its norms within `work`.
-bool flash_split_supported(const FlashArgs& a, bool backward);
+bool flash_split_supported(const FlashArgs& a);
 long long flash_split_work(const FlashArgs& a);
 long long flash_split_clear(const FlashArgs& a);
 long long flash_planes(int hs, long long t, long long heads, long long batch);

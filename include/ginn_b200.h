@@ -16,8 +16,8 @@
  * every distance and head ((2 * reach + 1) * heads floats), for fp32 operands their planes (as many bytes
  * as q, k, v and, backward, d_o with heads of 64 or 128), for Half operands off the 16-byte grid a dense copy,
  * the parts of a split cache, and backward two floats a query and, with dtable,
- * 2 * min(2 * reach + 1, tk + 127) floats per 128 queries of a head; heads beyond 128 and fp32
- * contractions beyond 4096 keep the scores of as many heads as fit 64 MiB.
+ * 2 * min(2 * reach + 1, tk + 127) floats per 128 queries of a head; heads beyond 128 keep the scores of
+ * as many heads as fit 64 MiB.
  * On the first call for a device the library gives that pool a release threshold of 4 GiB, so
  * that freed scratch stays cached instead of going back to the driver at every synchronisation.
  * ginn_b200_grouped_static is the entry point that allocates nothing.

@@ -198,3 +198,24 @@ def test_fp32_sums_that_begin_with_their_largest_terms(gpu, hs, t, heads):
     c.backward(gpu)
     ref, size = c.reference()
     elementwise("dv", c.dv, ref["dv"], size["dv"], SMALL)
+
+
+@pytest.mark.parametrize("hs,tq,tk,heads,kv,causal", [(64, 100, 8192, 2, 1, False), (128, 40, 5000, 1, 1, True), (64, 4097, 100, 1, 1, False),
+                                                      (57, 2100, 150, 4, 2, True), (128, 4500, 4500, 1, 1, True)])
+def test_fp32_sums_of_long_sequences(gpu, hs, tq, tk, heads, kv, causal):
+    c = Operands(torch.float32, hs, tq, tk, heads, kv, causal=causal, shift=0.0, small=0.05)
+    c.offset = 0 if tk <= tq else c.offset
+    c.v.abs_().add_(0.5)
+    c.d_o.abs_().add_(0.5)
+    c.forward(gpu)
+    c.backward(gpu)
+    ref, size = c.reference()
+    elementwise("o", c.o, ref["o"], size["o"], SMALL)
+    elementwise("dv", c.dv, ref["dv"], size["dv"] + 1e-30, SMALL)
+    for x in (c.v, c.d_o):
+        x.copy_(randn(torch.Generator(device="cuda").manual_seed(3), *x.shape))
+    c.forward(gpu)
+    c.backward(gpu)
+    ref, _ = c.reference()
+    for n in ("o", "dq", "dk", "dv"):
+        frobenius(n, getattr(c, n), ref[n], 1e-5)
