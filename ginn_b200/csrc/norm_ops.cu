@@ -663,7 +663,7 @@ norm_backward_ring_kernel(const NormBwd<T> p, const NormRing ring, int* __restri
     // the kernel's waits have an end: a group that gave up goes on without its data
     ok = ok && mbar_wait(smem_u32(&bars[s]), phase, status, DEV_TIMEOUT_FULL, 0x100);
     const T* stage = mine + static_cast<size_t>(s) * OPS * places;
-    const F2 rs(rstd1), shift(-mean1 * rstd1);
+    const F2 rs(rstd1), shift(-mean1);
     F2 xh[NV][4], g[NV][4], sx(0.f), sy(0.f);
     Raw8<T> z[DH ? NV : 1];
 #pragma unroll
@@ -681,9 +681,9 @@ norm_backward_ring_kernel(const NormBwd<T> p, const NormRing ring, int* __restri
       const float4 k[2] = {w[part * half], w[(part ^ 1) * half]};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        // (x - mean) rstd as one multiply-add: off by 2^-24 of |mean| rstd, as the subtraction's
-        // operands are
-        xh[i][e] = fma2(F2(a[2 * e], a[2 * e + 1]), rs, shift);
+        // the mean is subtracted first, as in the forward pass: the difference of close values is exact, where
+        // x rstd - mean rstd is off by 2^-24 of |mean| rstd (a constant column would not give zero)
+        xh[i][e] = mul2(add2(F2(a[2 * e], a[2 * e + 1]), shift), rs);
         const F2 d(b[2 * e], b[2 * e + 1]);  // zero behind the last row
         dg[i][e] = fma2(d, xh[i][e], dg[i][e]);
         db[i][e] = add2(db[i][e], d);
