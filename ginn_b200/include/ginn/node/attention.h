@@ -27,6 +27,7 @@ class RelativeAttentionNode : public BaseDataNode<Scalar> {
   RelativeAttentionOptions opt_;
   Tensor<Real> lse_;
   Tensor<Int> map_;
+  Size mapped_ = 0;  // rows of the table that map_ was made for
 
   ginn_b200_relative_attention describe() {
     const Shape q = Tensor<Scalar>::reduce(q_->shape(), 4), k = Tensor<Scalar>::reduce(k_->shape(), 4);
@@ -55,12 +56,13 @@ class RelativeAttentionNode : public BaseDataNode<Scalar> {
     GINN_ASSERT(this->dev()->kind() == GPU, "ginn_b200 serves GPU devices only");
     this->value().resize(q_->shape());
     lse_.resize({this->value().size() / this->value().rows()});
-    if (table_ && map_.size() == 0) {
+    if (table_ && mapped_ != table_->value().rows()) {
       std::vector<Int> map(2 * opt_.max_distance + 1);
       internal::b200_check(ginn_b200_relative_buckets(static_cast<int>(table_->value().rows()), opt_.max_distance,
                                                       !opt_.causal, opt_.max_distance, map.data()));
       map_.resize({static_cast<Size>(map.size())});
       map_.set(map);
+      mapped_ = table_->value().rows();
     }
     const ginn_b200_relative_attention a = describe();
     internal::b200_check(ginn_b200_relative_attention_forward(internal::b200_device(this->dev()), stream_of(*this->dev()),
