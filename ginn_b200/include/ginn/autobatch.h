@@ -777,8 +777,17 @@ class BatchedGraph {
     GINN_CUDA_CALL(cudaStreamSynchronize(st));
     reset_forwarded();
     GINN_CUDA_CALL(cudaStreamBeginCapture(st, cudaStreamCaptureModeThreadLocal));
-    forward().reset_grad().backward(loss_coeff);
     cudaGraph_t g = nullptr;
+    try {
+      forward().reset_grad().backward(loss_coeff);
+    } catch (...) {  // a node that cannot be captured: the stream goes back to running what it is given
+      cudaStreamEndCapture(st, &g);
+      if (g) cudaGraphDestroy(g);
+      cudaGetLastError();
+      side_used_ = false;
+      reset_forwarded();
+      throw;
+    }
     GINN_CUDA_CALL(cudaStreamEndCapture(st, &g));
     GINN_CUDA_CALL(cudaGraphInstantiate(&pass_exec_, g, 0));
     GINN_CUDA_CALL(cudaGraphDestroy(g));
