@@ -515,8 +515,8 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
 //
 // An fp32 matrix times a power of two that brings its largest magnitude (per sequence and key head) to
 // [2^14, 2^15) is written as the sum of two Half matrices, high = rn(x), low = rn(x - high): 22 bits of
-// every element down to 2^-18 of the largest, and an absolute error of 2^-40 of the largest below
-// that.  A product is then three Half products, high x high + high x low + low x high, at twice the
+// every element down to 2^-18 of the largest, and an absolute error of 2^-39 of the largest at most below
+// that (half a step of a subnormal, 2^-25, against 2^14).  A product is then three Half products, high x high + high x low + low x high, at twice the
 // rate of three TF32 products and with the same 2^-22 left out.  The planes are dense,
 // [plane][sequence][head][t][64 or 128], zero behind the head size, in queries behind the
 // lengths and in keys that no query sees.

@@ -372,7 +372,12 @@ int ginn_b200_attention_backward(int device, void* stream, int dtype, int64_t t,
  *              ints, within +-2^30) when that is not NULL
  *   *_lengths  device ints, one per sequence, NULL = all of tq / tk; clamped to the tensor
  *   lse        tq x heads x batch floats, dense (i + tq * (head + heads * b)); the backward pass reads it
- * head_size 1 .. 256; tq, tk < 2^29. */
+ * head_size 1 .. 256; tq, tk < 2^29.
+ * Precision.  Statistics and sums are fp32; each result is rounded once.  Half: the probabilities and the scores'
+ * gradient are rounded to Half for the products they enter.  fp32 with more than 16 queries per key head and heads
+ * to 128: elements keep 22 bits down to 2^-18 of the largest of their sequence and key head and 2^-39 of that largest
+ * below, probabilities 22 bits down to 2^-10 of their row's largest and 2^-32 of it below: where tokens differ by more
+ * than that in size, results that come from the small ones alone have fewer bits. */
 typedef struct {
   int64_t tq, tk, head_size, heads, kv_heads, batch;
   const void* q;

@@ -219,3 +219,47 @@ def test_fp32_sums_of_long_sequences(gpu, hs, tq, tk, heads, kv, causal):
     ref, _ = c.reference()
     for n in ("o", "dq", "dk", "dv"):
         frobenius(n, getattr(c, n), ref[n], 1e-5)
+
+
+@pytest.mark.parametrize("hs,t,tk,heads,kv,causal,span", [(64, 40, 40, 2, 2, True, 30), (64, 200, 200, 4, 2, True, 24), (128, 130, 300, 2, 2, False, 24),
+                                                          (57, 70, 70, 1, 1, True, 40)])
+def test_fp32_tokens_of_very_different_size(gpu, hs, t, tk, heads, kv, causal, span):
+    """Values and gradients of sizes over 2^span, in random order.  What the header promises: an element keeps 2^-39 of
+    the largest of its sequence and key head at least, a probability 2^-32 of its row's largest, P in the backward pass 2^-38 and
+    a score's gradient 2^-38 of 2 max|d_o row| max|v row|; above that 2^-17 of the terms' magnitudes."""
+    c = Operands(torch.float32, hs, t, tk, heads, kv, causal=causal, shift=0.0, small=0.5)
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    for x in (c.v, c.d_o):
+        x.mul_(2.0 ** torch.randint(0, span + 1, x.shape[:3] + (1,), generator=gen, device="cuda"))
+    c.forward(gpu)
+    c.backward(gpu)
+    ref, size = c.reference()
+    q, k, v, g = (x.double() for x in (c.q, c.k, c.v, c.d_o))
+    n = heads // kv
+    K, V = k.repeat_interleave(n, 1), v.repeat_interleave(n, 1)
+    s = c.scale * (q @ K.transpose(2, 3))
+    if causal:
+        seen = torch.arange(tk, device="cuda") <= torch.arange(t, device="cuda")[:, None] + c.offset
+        s = s.masked_fill(~seen, -math.inf)
+    p = torch.softmax(s, 3)
+    see = (p > 0).double()
+    es = E * (c.scale * (q.abs() @ K.abs().transpose(2, 3)) + 1)
+    ep = p * 2 * (es * see).amax(3, keepdim=True)  # the exponential and the sum it is divided by
+    top = lambda x: x.abs().amax((2, 3), keepdim=True)  # noqa: E731
+    shared = lambda x: x.unflatten(1, (kv, n)).sum(2)  # noqa: E731
+    most_v, most_g = top(V), top(g).unflatten(1, (kv, n)).amax(2, keepdim=True).expand(-1, -1, n, -1, -1).flatten(1, 2)
+    eo = (ep + E * p + 2.0 ** -32 * p.amax(3, keepdim=True) * see) @ V.abs() + 2.0 ** -39 * most_v
+    assert ((c.o.double() - ref["o"]).abs() <= eo).all()
+    dp = g @ V.transpose(2, 3)
+    delta = (p * dp).sum(3, keepdim=True)
+    ey = E * (g.abs() @ V.abs().transpose(2, 3)) + 2.0 ** -39 * (most_v * g.abs().sum(3, keepdim=True) + (most_g * V.abs().sum(3, keepdim=True)).transpose(2, 3))
+    norm = lambda x: (x ** 2).sum(3).amax(2)[..., None, None].sqrt()  # noqa: E731
+    bound = 2 * norm(g).unflatten(1, (kv, n)).amax(2, keepdim=True).expand(-1, -1, n, -1, -1).flatten(1, 2) * norm(V)
+    eds = ep * (dp - delta).abs() + p * (ey + (p * ey + ep * dp.abs()).sum(3, keepdim=True)) + 2.0 ** -38 * bound * see
+    eds = eds + E * (p * (dp - delta)).abs()
+    ds = (p * (dp - delta)).abs()
+    for name, ref_, tol in (("dq", ref["dq"], c.scale * (eds + E * ds) @ K.abs()), ("dk", ref["dk"], shared(c.scale * (eds + E * ds).transpose(2, 3) @ q.abs())),
+                            ("dv", ref["dv"], shared((ep + E * p + 2.0 ** -38 * see).transpose(2, 3) @ g.abs() + 2.0 ** -39 * most_g * p.sum(2)[..., None]))):
+        got = getattr(c, name).double()
+        bad = ~((got - ref_).abs() <= tol)
+        assert not bad.any(), (name, int(bad.sum()), float(((got - ref_).abs() / tol).max()))
