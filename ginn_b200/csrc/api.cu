@@ -1641,6 +1641,8 @@ int norm_forward(int device, void* stream, int dtype, const gb::NormArgs& a) {
 
 int norm_backward(int device, void* stream_, int dtype, const gb::NormGradArgs& a) {
   const bool weights = a.dgain != nullptr || a.dbias != nullptr;
+  if (a.dgain && a.dgain == a.dbias)  // two CTAs would write it at once
+    return fail(GINN_B200_BAD_ARGUMENT, "dgain and dbias are the same tensor");
   if (!a.dres && !a.dx && !weights) return GINN_B200_OK;
   if (a.rows == 0 || (a.cols == 0 && (!weights || a.accumulate))) return GINN_B200_OK;
   DevCtx* ctx;

@@ -50,7 +50,10 @@ class LayerNormNode : public BaseDataNode<Scalar> {
  public:
   LayerNormNode(const NodePtr<Scalar>& in, const NodePtr<Scalar>& gain, const NodePtr<Scalar>& bias, float eps)
       : BaseDataNode<Scalar>(inputs(in, gain, bias)), in_(in), gain_(gain), bias_(bias), eps_(eps),
-        mean_(this->value_.dev()), rstd_(this->value_.dev()) {}
+        mean_(this->value_.dev()), rstd_(this->value_.dev()) {
+    // one tensor as two operands would have both gradients added to one place by one call
+    GINN_ASSERT(!gain || gain != bias, "LayerNorm expects gain and bias to be different nodes!");
+  }
   std::string name() const override { return "LayerNorm"; }
 };
 

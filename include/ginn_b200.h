@@ -450,7 +450,7 @@ int ginn_b200_layer_norm_forward(int device, void* stream, int dtype, int64_t ro
  *   dx_j (+)= r (G - mean(G) - xh mean(G (.) xh))  with  xh = (x_j - mu) r,  G = gain (.) dy_j;
  *   dgain (+)= sum_j dy_j (.) xh_j;   dbias (+)= sum_j dy_j   (type `dtype`, summed in fp32 in a
  * fixed order).  The weight gradients take at most 2 * rows * 148 floats of stream-ordered scratch.
- * dx may be dy itself (same leading dimension). */
+ * dx may be dy itself (same leading dimension); dgain and dbias are different tensors. */
 int ginn_b200_layer_norm_backward(int device, void* stream, int dtype, int64_t rows, int64_t cols,
                                   const void* x, int64_t ldx, const void* gain, const float* mean,
                                   const float* rstd, const void* dy, int64_t lddy, void* dx,

@@ -94,8 +94,20 @@ static void test_captured_dropout() {
   CHECK(none->value().vector() == x->value().vector());
 }
 
+static void test_one_node_as_two_weights() {
+  auto x = Random<Real>(gpu(), {8, 4}, 30), w = Random<Real>(gpu(), {8}, 31);
+  bool refused = false;
+  try {
+    LayerNorm(x, w, w);
+  } catch (const RuntimeError&) {
+    refused = true;
+  }
+  CHECK(refused);
+}
+
 int main() {
   test_table_of_another_size();
+  test_one_node_as_two_weights();
   test_captured_dropout();
   cudaDeviceSynchronize();
   CHECK(ginn_b200_device_status(0, 1) == 0);
