@@ -2264,6 +2264,12 @@ int ginn_b200_relative_attention_backward(int device, void* stream_, int dtype, 
     for (const void* x : in) own = own && (out[i] == nullptr || out[i] != x);
     if (!own) return fail(GINN_B200_BAD_ARGUMENT, "d%c must be storage of its own", "qkv"[i]);
   }
+  if (g->dtable) {
+    bool own = g->dtable != a->table;
+    for (const void* x : out) own = own && g->dtable != x;
+    for (const void* x : in) own = own && (none || g->dtable != x);
+    if (!own) return fail(GINN_B200_BAD_ARGUMENT, "dtable must be storage of its own");
+  }
   if (none && g->accumulate) return GINN_B200_OK;
   DevCtx* ctx;
   if (int s = get_ctx(device, &ctx)) return s;
