@@ -167,6 +167,8 @@ struct TileBias {
 // its terms' magnitudes (one sign 2.7e-6, the largest terms first 5.7e-6; chains of 1024 terms: 1.2e-5).  What ended lies
 // in local memory, where a warp's accesses are neighbours: in the result's own place, rows apart, the end of a
 // chain took 8 us of a CTA's time instead of 2.6 (4 heads of 4096 x 4096 x 64, seven of them: 126 us without, 144, and 180).
+// Contractions of one chain have kernels without the code for its end (CHAINS), which they would pay registers for
+// (256 heads of 256 x 256 x 64, a step: 255 us, and 247).
 constexpr int kChain = 512;
 
 // SPLIT: fp32 operands as two Half planes each (see split_planes_kernel).  NQ: query tiles per CTA.  One tile
@@ -175,7 +177,7 @@ constexpr int kChain = 512;
 // for the maximum and once for the probabilities.  128-wide split operands (64 KB a tile) leave no room for
 // two tiles either way: K and V have one stage each, which is loaded again while the other's product and the
 // softmax run.
-template <int HS, int NST, int NQ, bool SPLIT>
+template <int HS, int NST, int NQ, bool SPLIT, bool CHAINS>
 __global__ void __launch_bounds__(128 + 256 * NQ, NQ == 1 && HS == 64 ? 2 : 1)
 flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ status) {
   constexpr int WIDE = HS / 64;                  // 64-wide chunks of a plane
@@ -185,7 +187,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
   constexpr int CROSS = NQ * HS;                 // tensor memory: from a tile's result to its cross terms
   constexpr int TILE = FCHUNK * CHUNKS;  // bytes of one operand tile
   constexpr float PSHIFT = SPLIT ? 7.f : 0.f;  // probabilities are formed times 2^PSHIFT: their low parts stay normal
-  constexpr int CUT = kChain / FT;       // split operands: key tiles to a chain
+  constexpr int CUT = kChain / FT;       // key tiles to a chain
   using Out = typename std::conditional<SPLIT, float, __half>::type;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t q_full[2], k_full[NST], k_empty[NST], v_full[NST], v_empty[NST];
@@ -315,7 +317,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
 #pragma unroll
           for (int ks = 0; ks < FT / 16; ++ks) {
             const uint32_t o = tmem + NQ * FT + t * HS, a = tmem + t * FT + (ks / 2) * 32 + (ks % 2) * 8;
-            const uint32_t add = ((SPLIT ? j % CUT : j) > 0 || ks > 0) ? 1u : 0u;
+            const uint32_t add = ((CHAINS ? j % CUT : j) > 0 || ks > 0) ? 1u : 0u;
             mma_f16_ts(o, a, make_smem_desc(b + ks * 2048, FCHUNK, 1024), IDESC_O, add);
             if (SPLIT) {
               // The cross terms have an accumulator of their own: the tensor core truncates when it adds, so
@@ -353,10 +355,10 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
     const float c1 = SPLIT ? p.c1 * p.iq[unit] * p.ik[unit] : p.c1;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    float md = -INFINITY;  // split operands: the maximum that the chains which ended are relative to
+    float md = -INFINITY;  // the maximum that the chains which ended are relative to
     // What they add up to.  Indexed in loops that stay loops, so that it lies in local memory and not among the
     // registers of every tile; a warp's accesses there are neighbours.
-    float part[SPLIT ? HS / 2 : 1];
+    float part[CHAINS ? HS / 2 : 1];
     // Elements c .. c + 7 of the chain in tensor memory and, where there are any, `old` times those before it.
     auto chain8 = [&](int c, bool before, float old, float (&x)[8]) {
       uint32_t w[8], cross[8];
@@ -365,9 +367,9 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
       tmem_ld_wait();
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = SPLIT ? __uint_as_float(w[e]) + __uint_as_float(cross[e]) : __uint_as_float(w[e]);
-      if (SPLIT && before) {
+      if (CHAINS && before) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fmaf(part[SPLIT ? c + e : 0], old, x[e]);
+        for (int e = 0; e < 8; ++e) x[e] = fmaf(part[CHAINS ? c + e : 0], old, x[e]);
       }
     };
     for (int j = 0; j < nt; ++j) {
@@ -395,14 +397,14 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
       uint32_t v[TWICE ? 32 : 64];
       if (ok) {
         tc_fence_after();
-        if (SPLIT && j > 0 && j % CUT == 0) {  // a chain ends: the products of the tiles before it are done
+        if (CHAINS && j > 0 && j % CUT == 0) {  // a chain ends: the products of the tiles before it are done
           const float old = md == m ? 1.f : ex2(md - m);
 #pragma unroll 1
           for (int c = 0; c < HS / 2; c += 8) {
             float x[8];
             chain8(c, j > CUT, old, x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) part[SPLIT ? c + e : 0] = x[e];
+            for (int e = 0; e < 8; ++e) part[CHAINS ? c + e : 0] = x[e];
           }
           md = m;
         }
@@ -428,7 +430,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
         const float a = mn == -INFINITY ? 1.f : ex2(m - mn);
         l *= a;
         m = mn;
-        if ((SPLIT ? j % CUT : j) > 0) {  // O exists from the second tile of a chain on
+        if ((CHAINS ? j % CUT : j) > 0) {  // O exists from the second tile of a chain on
 #pragma unroll
           for (int c = 0; c < (SPLIT ? HS : HS / 2); c += 16) {
             const uint32_t col = o_col + c + (c >= HS / 2 ? CROSS - HS / 2 : 0);  // behind the main result: the cross terms
@@ -491,7 +493,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
         const int at = half * (HS / 2) + c;
         if (real) store_row8(out + at, p.hs - at, p.vec, x, false);
       };
-      if (SPLIT) {
+      if (CHAINS) {
 #pragma unroll 1
         for (int c = 0; c < HS / 2; c += 8) eight(c);
       } else {
@@ -1418,7 +1420,7 @@ struct StreamWalk {
 // The launches of one pass behind the first are independent of it: dQ needs nothing of dK and dV.  They begin when
 // the CTAs of the one before have all begun (which wait for what both read), fill the SMs that its last wave leaves
 // idle, and wait for its end at theirs (wait_late), so that whoever waits for the last launch waits for all.
-template <int HS, int MODE, int BSTAGES, bool SPLIT>
+template <int HS, int MODE, int BSTAGES, bool SPLIT, bool CHAINS>
 __global__ void __launch_bounds__(FTHREADS, 1)
 flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict__ status) {
   constexpr bool KEYS = MODE != QUERIES && MODE != DELTA;
@@ -1430,8 +1432,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
   constexpr int TILE = BCHUNK * CHUNKS;   // bytes of a streamed tile
   constexpr float PSHIFT = SPLIT ? 14.f : 12.f;  // P is formed times 2^PSHIFT
   constexpr float PINV = SPLIT ? 1.f / 16384.f : 1.f / 4096.f;
-  constexpr bool CHAINS = SPLIT && MODE != DELTA;  // results are added up from chains of CUT streamed tiles
-  constexpr int CUT = kChain / BN;
+  constexpr int CUT = kChain / BN;  // streamed tiles to a chain
   static_assert(CUT % 2 == 0, "both groups have as many tiles in a chain");
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t rows_full, b_full[BSTAGES], b_empty[BSTAGES], x_full[2], p_full[2], acc_full, acc_empty;
@@ -1911,11 +1912,11 @@ bool fill_params(const FlashArgs& a, FlashParams* p) {
   return true;
 }
 
-template <int HS, int NST, int NQ, bool SPLIT>
+template <int HS, int NST, int NQ, bool SPLIT, bool CHAINS = false>
 cudaError_t forward_hs(FlashParams& p, cudaStream_t stream, int* status) {
   const int smem = (NQ + 2 * NST) * FCHUNK * (SPLIT ? 2 : 1) * (HS / 64) + 1024;
   static unsigned long long smem_set = 0;  // per template instantiation
-  auto kern = flash_forward_kernel<HS, NST, NQ, SPLIT>;
+  auto kern = flash_forward_kernel<HS, NST, NQ, SPLIT, CHAINS>;
   cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern), smem, &smem_set);
   if (e != cudaSuccess) return e;
   p.qblocks = (p.tq + NQ * FT - 1) / (NQ * FT);
@@ -1924,15 +1925,19 @@ cudaError_t forward_hs(FlashParams& p, cudaStream_t stream, int* status) {
   return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(128 + 256 * NQ), smem, stream, pdl_enabled(), p, status);
 }
 
-template <int HS, int MODE, int BSTAGES, bool SPLIT>
+template <int HS, int MODE, int BSTAGES, bool SPLIT, bool CHAINS = false>
 cudaError_t backward_hs(const FlashBwdParams& p, cudaStream_t stream, int* status) {
+  constexpr bool keys = MODE != QUERIES && MODE != DELTA;
+  if constexpr (SPLIT && !CHAINS && MODE != DELTA) {
+    const long long tiles = keys ? (p.tq + BN - 1LL) / BN * p.group : (p.tk + BN - 1) / BN;
+    if (tiles * BN > kChain) return backward_hs<HS, MODE, BSTAGES, SPLIT, true>(p, stream, status);
+  }
   const int smem = (2 * FCHUNK + BSTAGES * 2 * BCHUNK) * (SPLIT ? 2 : 1) * (HS / 64) + 1024;
   static unsigned long long smem_set = 0;  // per template instantiation
-  auto kern = flash_backward_kernel<HS, MODE, BSTAGES, SPLIT>;
+  auto kern = flash_backward_kernel<HS, MODE, BSTAGES, SPLIT, CHAINS>;
   cudaError_t e = set_smem_limit_once(reinterpret_cast<const void*>(kern), smem, &smem_set);
   if (e != cudaSuccess) return e;
   FlashBwdParams q = p;
-  constexpr bool keys = MODE != QUERIES && MODE != DELTA;
   q.row_tiles = ((keys ? p.tk : p.tq) + FT - 1) / FT;
   const long long grid = static_cast<long long>(q.row_tiles) * (keys ? p.kv_heads : p.heads) * p.batch;
   return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(FTHREADS), smem, stream, pdl_enabled(), q, status);
@@ -1980,8 +1985,11 @@ bool flash_supported(const FlashArgs& a) {
 cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* status) {
   FlashParams p;
   if (!fill_params(a, &p)) return cudaErrorInvalidValue;
-  if (a.inverse != nullptr)  // 64 wide, two tiles with two stages each: 16 heads of 2048 x 2048, causal, 103 us; one tile 85
+  if (a.inverse != nullptr) {  // 64 wide, two tiles with two stages each: 16 heads of 2048 x 2048, causal, 103 us; one tile 85
+    if (a.tk > kChain)
+      return a.hs <= 64 ? forward_hs<64, 1, 1, true, true>(p, stream, status) : forward_hs<128, 1, 1, true, true>(p, stream, status);
     return a.hs <= 64 ? forward_hs<64, 1, 1, true>(p, stream, status) : forward_hs<128, 1, 1, true>(p, stream, status);
+  }
   if (a.hs > 64) return forward_hs<128, 2, 2, false>(p, stream, status);
   // Half, 64 wide: CTAs of one query tile where their work is uneven or short (16 heads of 2048 x 2048, causal:
   // 42 us with two tiles, 36 with one; 512 of 128 x 128: 25 and 21), of two where every tile walks all keys,
