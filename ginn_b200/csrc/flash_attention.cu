@@ -162,14 +162,15 @@ struct TileBias {
 
 // The tensor core truncates each time it adds to an accumulator, once per 16 terms of a contraction.  Terms of one
 // sign make that a bias that grows with the chain: fp32 results are off by 1.2e-6 of their size after 256 terms,
-// 5.8e-6 after 1024, 2.5e-5 after 4096 (a Half result is rounded to 4.9e-4).  The kernels for fp32 operands
-// therefore start a new chain every 512 terms and add the chains up with rounded additions: a result keeps 2^-17 of
-// its terms' magnitudes (one sign 2.7e-6, the largest terms first 5.7e-6; chains of 1024 terms: 1.2e-5).  What ended lies
+// 5.8e-6 after 1024, 2.5e-5 after 4096.  The kernels for fp32 operands therefore start a new chain every 512 terms
+// and add the chains up with rounded additions: a result keeps 2^-17 of its terms' magnitudes (one sign 2.7e-6, the largest terms first 5.7e-6; chains of 1024 terms: 1.2e-5).  What ended lies
 // in local memory, where a warp's accesses are neighbours: in the result's own place, rows apart, the end of a
 // chain took 8 us of a CTA's time instead of 2.6 (4 heads of 4096 x 4096 x 64, seven of them: 126 us without, 144, and 180).
 // Contractions of one chain have kernels without the code for its end (CHAINS), which they would pay registers for
 // (256 heads of 256 x 256 x 64, a step: 255 us, and 247).
-constexpr int kChain = 512;
+// Half results, which are rounded to 4.9e-4, take chains of 8192 terms (5.5e-5 of one sign; 131072 terms in one
+// chain: 8.4e-4).
+constexpr int kChain = 512, kChainHalf = 8192;
 
 // SPLIT: fp32 operands as two Half planes each (see split_planes_kernel).  NQ: query tiles per CTA.  One tile
 // of a 64-wide head leaves room for a second CTA on the SM (TWICE), whose start, loads and end then pass while
@@ -187,7 +188,7 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
   constexpr int CROSS = NQ * HS;                 // tensor memory: from a tile's result to its cross terms
   constexpr int TILE = FCHUNK * CHUNKS;  // bytes of one operand tile
   constexpr float PSHIFT = SPLIT ? 7.f : 0.f;  // probabilities are formed times 2^PSHIFT: their low parts stay normal
-  constexpr int CUT = kChain / FT;       // key tiles to a chain
+  constexpr int CUT = (SPLIT ? kChain : kChainHalf) / FT;  // key tiles to a chain
   using Out = typename std::conditional<SPLIT, float, __half>::type;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t q_full[2], k_full[NST], k_empty[NST], v_full[NST], v_empty[NST];
@@ -1432,7 +1433,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
   constexpr int TILE = BCHUNK * CHUNKS;   // bytes of a streamed tile
   constexpr float PSHIFT = SPLIT ? 14.f : 12.f;  // P is formed times 2^PSHIFT
   constexpr float PINV = SPLIT ? 1.f / 16384.f : 1.f / 4096.f;
-  constexpr int CUT = kChain / BN;  // streamed tiles to a chain
+  constexpr int CUT = (SPLIT ? kChain : kChainHalf) / BN;  // streamed tiles to a chain
   static_assert(CUT % 2 == 0, "both groups have as many tiles in a chain");
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t rows_full, b_full[BSTAGES], b_empty[BSTAGES], x_full[2], p_full[2], acc_full, acc_empty;
@@ -1928,9 +1929,9 @@ cudaError_t forward_hs(FlashParams& p, cudaStream_t stream, int* status) {
 template <int HS, int MODE, int BSTAGES, bool SPLIT, bool CHAINS = false>
 cudaError_t backward_hs(const FlashBwdParams& p, cudaStream_t stream, int* status) {
   constexpr bool keys = MODE != QUERIES && MODE != DELTA;
-  if constexpr (SPLIT && !CHAINS && MODE != DELTA) {
+  if constexpr (!CHAINS && MODE != DELTA) {
     const long long tiles = keys ? (p.tq + BN - 1LL) / BN * p.group : (p.tk + BN - 1) / BN;
-    if (tiles * BN > kChain) return backward_hs<HS, MODE, BSTAGES, SPLIT, true>(p, stream, status);
+    if (tiles * BN > (SPLIT ? kChain : kChainHalf)) return backward_hs<HS, MODE, BSTAGES, SPLIT, true>(p, stream, status);
   }
   const int smem = (2 * FCHUNK + BSTAGES * 2 * BCHUNK) * (SPLIT ? 2 : 1) * (HS / 64) + 1024;
   static unsigned long long smem_set = 0;  // per template instantiation
@@ -1990,11 +1991,14 @@ cudaError_t launch_flash_forward(const FlashArgs& a, cudaStream_t stream, int* s
       return a.hs <= 64 ? forward_hs<64, 1, 1, true, true>(p, stream, status) : forward_hs<128, 1, 1, true, true>(p, stream, status);
     return a.hs <= 64 ? forward_hs<64, 1, 1, true>(p, stream, status) : forward_hs<128, 1, 1, true>(p, stream, status);
   }
-  if (a.hs > 64) return forward_hs<128, 2, 2, false>(p, stream, status);
+  const bool chains = a.tk > kChainHalf;
+  if (a.hs > 64) return chains ? forward_hs<128, 2, 2, false, true>(p, stream, status) : forward_hs<128, 2, 2, false>(p, stream, status);
   // Half, 64 wide: CTAs of one query tile where their work is uneven or short (16 heads of 2048 x 2048, causal:
   // 42 us with two tiles, 36 with one; 512 of 128 x 128: 25 and 21), of two where every tile walks all keys,
   // which are then read half as often (16 of 2048 x 2048, not causal: 43 and 46).
-  return a.causal || a.tq <= FT ? forward_hs<64, 2, 1, false>(p, stream, status) : forward_hs<64, 3, 2, false>(p, stream, status);
+  if (a.causal || a.tq <= FT)
+    return chains ? forward_hs<64, 2, 1, false, true>(p, stream, status) : forward_hs<64, 2, 1, false>(p, stream, status);
+  return chains ? forward_hs<64, 3, 2, false, true>(p, stream, status) : forward_hs<64, 3, 2, false>(p, stream, status);
 }
 
 long long flash_packed(int hs, long long t, long long heads, long long batch) {

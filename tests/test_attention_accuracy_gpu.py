@@ -263,3 +263,25 @@ def test_fp32_tokens_of_very_different_size(gpu, hs, t, tk, heads, kv, causal, s
         got = getattr(c, name).double()
         bad = ~((got - ref_).abs() <= tol)
         assert not bad.any(), (name, int(bad.sum()), float(((got - ref_).abs() / tol).max()))
+
+
+@pytest.mark.parametrize("hs,t,heads,kv,causal", [(64, 40000, 2, 1, False), (128, 36000, 1, 1, False), (64, 33000, 1, 1, True), (57, 20000, 4, 2, False)])
+def test_half_sums_of_one_sign_have_no_bias(gpu, hs, t, heads, kv, causal):
+    """Roundings average out, truncation does not: 512 additions to a chain of 8192 terms truncate less than 2^-22 of its
+    sum each, 2^-13 in all.  150 queries over t keys for o, 150 keys under t queries for dv.  Element by element three
+    roundings of 2^-11 (P, the result and a margin) and, for results below a Half's normal range, 2^-14, half of the
+    step of 2^-24 that they are rounded to: a key that one query among 33000 keys sees has a dv of 3e-5."""
+    for tq, tk in ((150, t), (t, 150)):
+        c = Operands(torch.float16, hs, tq, tk, heads, kv, causal=causal and tk > tq, shift=0.0, small=0.05)
+        c.v.abs_().add_(0.5)
+        c.d_o.abs_().add_(0.5)
+        c.forward(gpu)
+        c.backward(gpu)
+        ref, size = c.reference()
+        for n in ("o", "dv"):
+            off = (getattr(c, n).double() - ref[n]) / size[n]
+            assert abs(float(off.mean())) <= 2.0 ** -13, (n, float(off.mean()))
+            left = (getattr(c, n).double() - ref[n]).abs() - 3 * 2.0 ** -11 * size[n]
+            assert float(left.max()) <= 2.0 ** -25, (n, float(left.max()))
+        for n in ("dq", "dk"):
+            frobenius(n, getattr(c, n), ref[n], 4 * 2.0 ** -11)
