@@ -719,10 +719,10 @@ flash_pack_kernel(const __half* __restrict__ src, long long ld, long long sh, lo
 // 73 us, 4.6 TB/s of 6.5 copied; 370 us on the tiles above.
 constexpr int kTokenRows = 16;
 constexpr int kTokenWarps = 4;  // two CTAs on an SM: one loads while the other starts or joins its warps
-// Keys of a part of an fp32 cache.  The tensor core truncates each time it adds to an accumulator, eight keys at a
-// time, and values of one sign make that a bias that grows with the chain: a part of 16384 keys is off by 4.8e-5
-// of the result, one of 2048 by 5.9e-6.  The parts' results are joined with rounded additions.
-constexpr int kTokenChain = 1024;
+// Most keys of a part of a cache.  The tensor core truncates each time it adds to an accumulator, eight keys of a warp at
+// a time (Half: sixteen), and values of one sign make that a bias that grows with the chain: an fp32 part of 16384 keys is
+// off by 4.8e-5 of the result, one of 2048 by 5.9e-6.  The parts' results are joined with rounded additions.
+constexpr int kTokenChain = 1024, kTokenChainHalf = 32768;
 
 struct TokenParams {
   const void *q, *k, *v;
@@ -2077,11 +2077,12 @@ int flash_token_splits(int dtype, const FlashArgs& a, int num_sms, long long* fl
   *floats = 0;
   if (rows > kTokenRows || a.hs > 128) return 0;
   // Eight CTAs' worth of work per SM, so that ragged lengths even out; a CTA takes at least 64 keys (one
-  // block per warp) and in multiples of that.  fp32: at most kTokenChain, whatever the number of sequences.
+  // block per warp), in multiples of that, and at most a chain, whatever the number of sequences.
   const long long units = static_cast<long long>(a.kv_heads) * a.batch, step = 16 * kTokenWarps;
   long long chunk = (a.tk * units + 8LL * num_sms - 1) / (8LL * num_sms);
   chunk = (chunk + step - 1) / step * step;
-  if (dtype == 0 && chunk > kTokenChain) chunk = kTokenChain;
+  const long long most = dtype == 0 ? kTokenChain : kTokenChainHalf;
+  chunk = chunk < most ? chunk : most;
   const long long splits = (a.tk + chunk - 1) / chunk;
   if (splits * units > 0x7fffffffLL || units * rows > 0x7fffffffLL) return 0;
   if (splits > 1) *floats = units * splits * rows * ((a.hs <= 64 ? 64 : 128) + 2);

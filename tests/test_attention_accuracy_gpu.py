@@ -285,3 +285,21 @@ def test_half_sums_of_one_sign_have_no_bias(gpu, hs, t, heads, kv, causal):
             assert float(left.max()) <= 2.0 ** -25, (n, float(left.max()))
         for n in ("dq", "dk"):
             frobenius(n, getattr(c, n), ref[n], 4 * 2.0 ** -11)
+
+
+def test_half_tokens_of_many_long_sequences_have_no_bias(gpu):
+    """1184 caches of 131072 keys: parts of 32768 keys, 8192 to a warp."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    batch, tk, hs = 1184, 131072, 8
+    q = (0.05 * randn(gen, batch, 1, 1, hs)).half()
+    k, v = (torch.empty(batch, 1, tk, hs, dtype=torch.float16, device="cuda").normal_(generator=gen) for _ in "kv")
+    v.abs_().add_(0.5)
+    o, lse = torch.empty_like(q), torch.empty(batch, device="cuda")
+    gpu.relative_attention_forward(heads_of(q), heads_of(k), heads_of(v), None, None, heads_of(o), lse, scale=0.25)
+    off = []
+    for b in range(0, batch, 9):
+        ref = torch.softmax(0.25 * (k[b, 0].double() @ q[b, 0, 0].double()), 0) @ v[b, 0].double()
+        off.append((o[b, 0, 0].double() - ref) / ref)
+    off = torch.stack(off)  # 1056 results, rounded by 2^-11 at most: their mean by 2^-11 / sqrt(1056) = 2^-16
+    assert abs(float(off.mean())) <= 2.0 ** -13 + 2.0 ** -15, float(off.mean())
+    assert float(off.abs().max()) <= 3 * 2.0 ** -11
