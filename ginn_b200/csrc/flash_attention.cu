@@ -336,8 +336,9 @@ flash_forward_kernel(const __grid_constant__ FlashParams p, int* __restrict__ st
         }
       }
       if (leader) {
-        tc_commit(smem_u32(&v_empty[s]));
-        if (j + 1 < n) tc_commit(smem_u32(&k_empty[s2]));
+        // only where the producer waits for it: behind the last o_full nothing else keeps the CTA until it has arrived
+        if (j + NST < n) tc_commit(smem_u32(&v_empty[s]));
+        if (j + 1 + NST < n) tc_commit(smem_u32(&k_empty[s2]));
       }
       __syncwarp();
     }
@@ -1576,7 +1577,7 @@ flash_backward_kernel(const __grid_constant__ FlashBwdParams p, int* __restrict_
         };
         if (WANT_P) product(tmem + 2 * FT + PV_COL, a, b + TILE);  // dV += P dO
         if (WANT_D && MODE != DELTA) product(tmem + 2 * FT, a + BN, b);  // dK += dS Q,  dQ += dS K
-        tc_commit(smem_u32(&b_empty[s]));
+        if (it + BSTAGES < n) tc_commit(smem_u32(&b_empty[s]));  // only where the producer waits for it
         if (it == n - 1 || (CHAINS && (it + 1) % CUT == 0)) tc_commit(smem_u32(&acc_full));
       }
       __syncwarp();
